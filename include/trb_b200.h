@@ -263,6 +263,34 @@ int trb_gemm_launch_noalloc(int dtype, int m, int n, int k, const void* a, const
 int trb_gemm_host(int dtype, int m, int n, int k, const void* a_host, const void* b_host, void* c_host,
                   float scale_a, float scale_b, int device_id, trb_result* out);
 
+/* ---- products grouped by expert ----------------------------------------- */
+
+/* Conventions of the grouped entry points: rows are sorted by group and
+ * offsets (groups + 1 int32 on the device, not read by the host) says that
+ * group e owns rows [offsets[e], offsets[e + 1]); groups may be empty, and
+ * rows outside every group are neither read nor written.  Offsets that
+ * decrease or leave [0, rows] are found on the device: the call computes
+ * nothing and sets the device error word to 7 (trb_device_error).  At most
+ * 1024 groups.  Asynchronous on `stream`; no workspace, so calls on several
+ * streams may overlap.  No reference counterpart: its GEMM takes one matrix
+ * per operand (src/teamredbench/benchmarks/mfu.py:229-234). */
+
+/* out[r] = a[r] * b[e] for the rows r of group e: a rows x k, out rows x n,
+ * b one matrix per group, k x n row-major (TRB_B_ROW_MAJOR) or n x k
+ * (TRB_B_K_MAJOR, b[e] transposed).  The gradient of a is the same call on the
+ * gradient of out with the other layout of the same b.  bfloat16 or float16
+ * throughout, accumulated in fp32 and rounded once.  n and k must be multiples
+ * of 8 and pointers 16-byte aligned (TMA). */
+int trb_grouped_gemm_launch(int dtype, int groups, int rows, int n, int k, const void* a, const void* b, int b_layout,
+                            const int32_t* offsets, void* out, void* stream);
+
+/* Gradient of the weights: out[e] (k x n row-major) = the sum over the rows r
+ * of group e of a[r]^T g[r], a rows x k, g rows x n; zeros for a group without
+ * rows.  For weights kept n x k, exchange a and g (and k and n).  Types,
+ * accumulation, sizes and alignment as trb_grouped_gemm_launch. */
+int trb_grouped_wgrad_launch(int dtype, int groups, int rows, int n, int k, const void* a, const void* g,
+                             const int32_t* offsets, void* out, void* stream);
+
 /* Round f32 values in place on the device to tf32 (round to nearest, ties
  * away from zero; cvt.rna.tf32.f32).  Used to prepare tf32 GEMM inputs. */
 int trb_round_tf32(void* data, uint64_t count, void* stream);

@@ -45,6 +45,8 @@ EXPORTED_SYMBOLS = (
     "trb_gemm_launch_ex",
     "trb_gemm_launch_noalloc",
     "trb_gemm_host",
+    "trb_grouped_gemm_launch",
+    "trb_grouped_wgrad_launch",
     "trb_round_tf32",
     "trb_selftest_bounded_wait",
 )
@@ -168,6 +170,10 @@ def load() -> ctypes.CDLL:
     lib.trb_gemm_launch_noalloc.restype = i32
     lib.trb_gemm_host.argtypes = [i32, i32, i32, i32, vp, vp, vp, flt, flt, i32, res_p]
     lib.trb_gemm_host.restype = i32
+    lib.trb_grouped_gemm_launch.argtypes = [i32, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp]
+    lib.trb_grouped_gemm_launch.restype = i32
+    lib.trb_grouped_wgrad_launch.argtypes = [i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]
+    lib.trb_grouped_wgrad_launch.restype = i32
     lib.trb_round_tf32.argtypes = [vp, u64, vp]
     lib.trb_round_tf32.restype = i32
     lib.trb_selftest_bounded_wait.argtypes = [ctypes.c_uint32, i32, res_p]
@@ -247,6 +253,17 @@ def gemm_host(dtype: str, m: int, n: int, k: int, a: int, b: int, c: int, scale_
     check(load().trb_gemm_host(DTYPE_CODES[dtype], m, n, k, a, b, c, scale_a, scale_b, device_id,
                                ctypes.byref(result)))
     return result
+
+
+def grouped_gemm_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: int, b: int, b_layout: str,
+                        offsets: int, out: int, stream: int = 0) -> None:
+    check(load().trb_grouped_gemm_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, b, B_LAYOUTS[b_layout], offsets,
+                                         out, stream or None))
+
+
+def grouped_wgrad_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: int, g: int, offsets: int, out: int,
+                         stream: int = 0) -> None:
+    check(load().trb_grouped_wgrad_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, g, offsets, out, stream or None))
 
 
 def round_tf32(data: int, count: int, stream: int = 0) -> None:

@@ -1,0 +1,845 @@
+// gemm_grouped.cu -- matrix products grouped by expert, with ragged numbers of rows.
+//
+//   grouped_gemm   out[r] = a[r] * b[e]                 for the rows r of group e
+//   grouped_wgrad  out[e] = a[rows of e]^T * g[rows of e]
+//
+// Rows are sorted by group; group e owns rows [offsets[e], offsets[e + 1]), and
+// offsets live on the device, so no call waits for the host to read them.  The
+// launch covers the largest possible number of tiles and every CTA derives the
+// real tile list from the offsets.
+//
+// No counterpart in the reference, whose GEMM takes one matrix per operand
+// (src/teamredbench/benchmarks/mfu.py:229-234).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "trb_common.cuh"
+
+namespace trb {
+namespace grouped {
+
+__device__ int g_grouped_error;
+
+constexpr int kMaxGroups = 1024;
+constexpr int kThreads = 192;        // producer warp, MMA warp, 4 epilogue warps
+constexpr int kBK = 64;              // 16-bit elements per 128-byte swizzle row
+constexpr int kInstrK = 16;          // K elements per tcgen05.mma
+constexpr int kStages = 6;
+constexpr int kOperandStage = 128 * 128;  // one CTA's 128 rows (or columns) x 128 bytes of one operand
+constexpr size_t kRingBytes = (size_t)kStages * 2 * kOperandStage;
+constexpr int kNumAcc = 2;
+constexpr int kTmemCols = 512;
+constexpr int kEpiBytes = 32 * 64;   // a 32 x 32 block of 16-bit results
+
+struct GroupTable {
+    int start[kMaxGroups];
+    int rows[kMaxGroups];
+};
+
+// Reads the offsets (all threads of the CTA; ends with a barrier).  Offsets
+// that decrease or leave [0, total_rows] set the device error word; the call
+// then computes nothing (returns 0 groups), so that no offsets, however wrong,
+// reach outside the operands.
+__device__ __forceinline__ int load_groups(const int* offsets, int groups, int total_rows, GroupTable& g) {
+    bool bad = false;
+    for (int e = threadIdx.x; e < groups; e += blockDim.x) {
+        const int lo = offsets[e], hi = offsets[e + 1];
+        bad = bad || lo < 0 || hi < lo || hi > total_rows;
+        g.start[e] = lo;
+        g.rows[e] = hi - lo;
+    }
+    if (!__syncthreads_or(bad)) return groups;
+    if (threadIdx.x == 0) atomicCAS(&g_grouped_error, 0, kErrOffsets);
+    return 0;
+}
+
+// F32 <- BF16 x BF16 or F16 x F16 instruction descriptor; bit 15 / 16: A / B is MN-major.
+template <int DT>
+__host__ __device__ constexpr uint32_t make_idesc(int m, bool a_mn, bool b_mn) {
+    constexpr uint32_t fmt = DT == TRB_BFLOAT16 ? 1u : 0u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+           ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t idesc_n(uint32_t idesc, int n) { return idesc | ((uint32_t)(n >> 3) << 17); }
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
+    if constexpr (DT == TRB_FLOAT16) {
+        __half2 h = __floats2half2_rn(__uint_as_float(lo), __uint_as_float(hi));
+        return *reinterpret_cast<uint32_t*>(&h);
+    } else {
+        __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+}
+
+// Four 8 x 8 blocks of 16-bit values from registers (the fragment order of an m16n8 product: thread t holds
+// row t / 4, columns 2 (t % 4) and + 1) to shared memory, each transposed; thread 8i + j gives the 16-byte
+// row that takes column j of block i.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0),
+                 "r"(r1), "r"(r2), "r"(r3)
+                 : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// ------------------------------------------------------------------ out[r] = a[r] * b[e]
+// A CTA pair (tcgen05.mma.cta_group::2, M = 256) computes the transposed tile
+//   out^T[256 columns n, R rows r] = b[e]^T[n, k] * a[r, k]^T:
+// the 256 TMEM lanes of the pair run along n, the instruction's N side along
+// the R <= 256 rows of one group.  N goes in steps of 32, so a group of r rows
+// costs ceil(r / 32) * 32 rows of products instead of whole 128- or 256-row
+// tiles, and no row of another group ever meets this group's weights.  A group
+// of more than 256 rows is cut into equal chunks.  Rows past the group's end
+// are loaded and multiplied but not stored; each output depends on its own row
+// only, so what stands there (the next group's rows, NaN) does not matter.
+// K past the end is zero in both operands (the tensor maps are per group).
+struct ProductTile {
+    int e, row0, rows, n0;
+};
+
+struct ProductTable : GroupTable {
+    int chunk0[kMaxGroups + 1];  // chunks of the groups before this one
+};
+
+constexpr int kTileN = 256;    // columns of a tile (pair)
+constexpr int kTileRows = 256; // largest chunk
+
+__device__ __forceinline__ int chunks_of(int rows) { return (rows + kTileRows - 1) / kTileRows; }
+
+// Exclusive scan of the groups' chunk counts (one warp).
+__device__ __forceinline__ void scan_chunks(int groups, ProductTable& g, int lane) {
+    int base = 0;
+    for (int e0 = 0; e0 < groups; e0 += 32) {
+        const int e = e0 + lane;
+        const int c = e < groups ? chunks_of(g.rows[e]) : 0;
+        int sum = c;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += up;
+        }
+        if (e < groups) g.chunk0[e] = base + sum - c;
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) g.chunk0[groups] = base;
+}
+
+// Tile t: groups in order; inside a group, runs of 8 chunks walk the columns
+// together (a weight panel is read by the chunks next to each other in time).
+__device__ __forceinline__ ProductTile product_tile(int t, int groups, int num_n, const ProductTable& g) {
+    const int q = t / num_n;
+    int lo = 0, hi = groups - 1;  // the last group whose chunks begin at or before q
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (g.chunk0[mid] <= q) lo = mid;
+        else hi = mid - 1;
+    }
+    const int local = t - g.chunk0[lo] * num_n;
+    const int rows = g.rows[lo];
+    const int chunks = chunks_of(rows);
+    const int run = 8 * num_n;
+    const int first = local / run * 8;
+    const int width = min(8, chunks - first);
+    const int in_run = local - first * num_n;
+    const int chunk = first + in_run % width;
+    const int per = ((rows + chunks - 1) / chunks + 31) & ~31;
+    ProductTile p;
+    p.e = lo;
+    p.row0 = g.start[lo] + chunk * per;
+    p.rows = min(per, rows - chunk * per);
+    p.n0 = in_run / width * kTileN;
+    return p;
+}
+
+constexpr size_t kProductSmem = kRingBytes + 1024 + 4 * kEpiBytes;
+
+template <int DT, bool KB>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX128,
+                        const __grid_constant__ CUtensorMap tmX32, const int* __restrict__ offsets,
+                        uint16_t* __restrict__ out, int groups, int total_rows, int N, int K) {
+    constexpr uint32_t kIdesc = make_idesc<DT>(256, !KB, false);
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ ProductTable table;
+    __shared__ __align__(8) uint64_t full_bar[kStages];   // leader: both CTAs' TMA bytes land here
+    __shared__ __align__(8) uint64_t empty_bar[kStages];  // both: MMA finished reading the stage
+    __shared__ __align__(8) uint64_t accf_bar[kNumAcc];   // both: accumulator ready for the epilogue
+    __shared__ __align__(8) uint64_t acce_bar[kNumAcc];   // leader: both CTAs' epilogues drained it
+    __shared__ __align__(8) uint64_t drain_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sW = smem_base;
+    const uint32_t sX = smem_base + kStages * kOperandStage;
+    const uint32_t sEpi = smem_base + (uint32_t)kRingBytes;
+
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int pair = blockIdx.x >> 1;
+    const int num_pairs = gridDim.x >> 1;
+    const int num_n = (N + kTileN - 1) / kTileN;
+    const int num_kb = (K + kBK - 1) / kBK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        for (int a = 0; a < kNumAcc; ++a) {
+            mbar_init(smem_u32(&accf_bar[a]), 1);
+            mbar_init(smem_u32(&acce_bar[a]), 8);  // 4 epilogue warps x 2 CTAs
+        }
+        mbar_init(smem_u32(&drain_bar), 1);
+        abort_flag = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmX128);
+        tma_prefetch_desc(&tmX32);
+    }
+    if (warp == 0) {
+        tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
+        tmem_relinquish_pair();
+    }
+    grid_launch_dependents();
+    grid_dependency_wait();  // offsets, operands and out may belong to the previous grid until here
+    groups = load_groups(offsets, groups, total_rows, table);
+    if (warp == 0) scan_chunks(groups, table, lane);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // barrier inits of both CTAs visible before any cross-CTA signal
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    const int num_tiles = table.chunk0[groups] * num_n;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer (both CTAs; completion on the leader's full barriers)
+            uint32_t stage = 0, phase = 0;
+            uint32_t issued_mask = 0, issued_phase = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+                const ProductTile p = product_tile(tile, groups, num_n, table);
+                const int half = ((p.rows + 31) & ~31) >> 1;  // rows this CTA loads
+                const int x_row = p.row0 + (int)rank * half;
+                const int x_boxes = (half + 31) / 32;
+                const uint32_t x_bytes = (uint32_t)x_boxes * 32 * 128;
+                const int w_col = p.n0 + (int)rank * 128;
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    if (!mbar_wait_cluster(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
+                        atomicCAS(&g_grouped_error, 0, kErrProducerWait);
+                        abort_flag = 1;
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t fb_local = smem_u32(&full_bar[stage]);
+                    if (leader) mbar_arrive_expect_tx(fb_local, 2 * (kOperandStage + x_bytes));
+                    const uint32_t fb = fb_local & kPeerBitMask;
+                    const uint32_t w = sW + stage * kOperandStage, x = sX + stage * kOperandStage;
+                    if constexpr (KB) {
+                        tma_load_3d_pair(w, &tmW, fb, kb * kBK, w_col, p.e);
+                    } else {
+                        tma_load_3d_pair(w, &tmW, fb, w_col, kb * kBK, p.e);
+                        tma_load_3d_pair(w + kOperandStage / 2, &tmW, fb, w_col + 64, kb * kBK, p.e);
+                    }
+                    if (x_boxes == 4) {
+                        tma_load_2d_pair(x, &tmX128, fb, kb * kBK, x_row);
+                    } else {
+                        for (int i = 0; i < x_boxes; ++i)
+                            tma_load_2d_pair(x + (uint32_t)i * 32 * 128, &tmX32, fb, kb * kBK, x_row + i * 32);
+                    }
+                    issued_mask |= 1u << stage;
+                    issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (leader)  // every armed phase completes only once both CTAs' bytes have landed
+                for (int s = 0; s < kStages; ++s)
+                    if (issued_mask & (1u << s))
+                        if (!mbar_wait_cluster(smem_u32(&full_bar[s]), (issued_phase >> s) & 1u, nullptr))
+                            atomicCAS(&g_grouped_error, 0, kErrDrainWait);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            // ---------------- MMA issuer: the leader CTA only
+            const uint64_t w_desc0 = KB ? make_sdesc(sW, 16, 1024) : make_sdesc(sW, kOperandStage / 2, 1024);
+            const uint64_t x_desc0 = make_sdesc(sX, 16, 1024);
+            constexpr int kWStep = KB ? kInstrK * 2 : kInstrK * 128;  // bytes per instruction K step
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            int t_local = 0;
+            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs, ++t_local) {
+                const ProductTile p = product_tile(tile, groups, num_n, table);
+                const uint32_t idesc = idesc_n(kIdesc, (p.rows + 31) & ~31);
+                const int acc = t_local & 1;
+                if (!mbar_wait_cluster(smem_u32(&acce_bar[acc]), ((uint32_t)(t_local >> 1) & 1u) ^ 1u, &abort_flag)) {
+                    atomicCAS(&g_grouped_error, 0, kErrMmaWait);
+                    abort_flag = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (uint32_t)(acc * kTileRows);
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    if (!mbar_wait_cluster(smem_u32(&full_bar[stage]), phase, &abort_flag)) {
+                        atomicCAS(&g_grouped_error, 0, kErrMmaWait);
+                        abort_flag = 1;
+                        ok = false;
+                        break;
+                    }
+                    const uint64_t off = (uint64_t)((stage * kOperandStage) >> 4);
+#pragma unroll
+                    for (int ks = 0; ks < kBK / kInstrK; ++ks)
+                        mma_pair_f16(d_tmem, w_desc0 + off + (uint64_t)(ks * kWStep >> 4),
+                                     x_desc0 + off + (uint64_t)(ks * kInstrK * 2 >> 4), idesc,
+                                     (kb != 0 || ks != 0) ? 1u : 0u);
+                    tc_commit_pair_multicast(smem_u32(&empty_bar[stage]), 0x3);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (ok) tc_commit_pair_multicast(smem_u32(&accf_bar[acc]), 0x3);
+            }
+            tc_commit_pair_multicast(smem_u32(&drain_bar), 0x1);
+            if (!mbar_wait_cluster(smem_u32(&drain_bar), 0, nullptr)) atomicCAS(&g_grouped_error, 0, kErrDrainWait);
+        }
+    } else {
+        // ---------------- epilogue (both CTAs): warps 2..5, one TMEM lane quarter (32 columns of out) each.
+        // TMEM holds out^T, so 32 x 32 blocks go through shared memory transposed (stmatrix .trans) and leave
+        // as 64-byte runs of a row, 16 bytes a lane.
+        const int q = warp & 3;
+        const uint32_t acce_leader0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
+        const uint32_t acce_leader1 = mapa_shared(smem_u32(&acce_bar[1]), 0);
+        const uint32_t buf = sEpi + (uint32_t)(q * kEpiBytes);
+        // block row j is 64 bytes; its 16-byte piece i stands at i ^ ((j >> 1) & 3), free of bank conflicts both ways
+        const uint32_t st_row = buf + (uint32_t)((lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) * 16));
+        const uint32_t ld_row = buf + (uint32_t)((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) * 16));
+        int t_local = 0;
+        for (int tile = pair; tile < num_tiles; tile += num_pairs, ++t_local) {
+            const ProductTile p = product_tile(tile, groups, num_n, table);
+            const int acc = t_local & 1;
+            bool ok = mbar_wait_cluster(smem_u32(&accf_bar[acc]), (uint32_t)(t_local >> 1) & 1u, &abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+                if (lane == 0) {
+                    atomicCAS(&g_grouped_error, 0, kErrEpilogueWait);
+                    abort_flag = 1;
+                }
+                break;
+            }
+            tc_fence_after();
+            const uint32_t t_tile = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kTileRows);
+            const int col = p.n0 + (int)rank * 128 + q * 32 + (lane & 3) * 8;
+            uint16_t* out_lane = out + (size_t)(p.row0 + (lane >> 2)) * N + col;
+#pragma unroll 1
+            for (int c = 0; c * 32 < p.rows; ++c) {
+                uint32_t lo[16], hi[16];  // TMEM lanes 0..15 and 16..31 of the quarter, 32 rows of out
+                tmem_ld_16x256b_x4(t_tile + (uint32_t)(c * 32), lo);
+                tmem_ld_16x256b_x4(t_tile + (16u << 16) + (uint32_t)(c * 32), hi);
+                tmem_wait_ld();
+                __syncwarp();  // the previous block has been read out of buf
+#pragma unroll
+                for (int j = 0; j < 4; ++j)  // rows 8j .. 8j + 7; columns in octets 0..3
+                    stmatrix_x4_trans(st_row + (uint32_t)(j * 8 * 64), pack2<DT>(lo[4 * j], lo[4 * j + 1]),
+                                      pack2<DT>(lo[4 * j + 2], lo[4 * j + 3]), pack2<DT>(hi[4 * j], hi[4 * j + 1]),
+                                      pack2<DT>(hi[4 * j + 2], hi[4 * j + 3]));
+                __syncwarp();
+                if (col < N) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = c * 32 + i * 8;
+                        if (row + (lane >> 2) < p.rows)
+                            *reinterpret_cast<uint4*>(out_lane + (size_t)row * N) =
+                                ld_shared_v4(ld_row + (uint32_t)(i * 8 * 64));
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc ? acce_leader1 : acce_leader0);
+        }
+    }
+
+    // Teardown: the leader's MMAs read the peer's shared memory and write its
+    // TMEM, so neither CTA releases TMEM or exits before both are done.
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+// ------------------------------------------------------------------ out[e] = a^T * g over the rows of e
+// A CTA pair computes 256 x 256 of one group's K x N gradient; the products run
+// over the group's rows, 64 per stage, both operands MN-major (their rows are
+// the contraction).  The last stage of a group reaches into the next group's
+// rows (or past the end, where TMA gives zeros): products run over whole
+// 16-row steps only as far as the group goes, and the rows between its end and
+// the end of that step are overwritten with zeros in both operands first, so
+// that nothing of the next group, infinities and NaN included, gets in.  Such
+// a stage lands on a barrier of its own CTA; a fixer warp clears the rows and
+// then signals the leader's full barrier.
+// A group without rows has a gradient of zeros, which the epilogue writes.
+struct WgradTile {
+    int e, row0, rows, m0, n0;
+};
+
+__device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, const GroupTable& g) {
+    const int per = num_m * num_n;
+    WgradTile w;
+    w.e = t / per;
+    w.row0 = g.start[w.e];
+    w.rows = g.rows[w.e];
+    const int local = t - w.e * per;
+    const int run = 8 * num_n;
+    const int first = local / run * 8;
+    const int width = min(8, num_m - first);
+    const int in_run = local - first * num_n;
+    w.m0 = (first + in_run % width) * 256;
+    w.n0 = in_run / width * 256;
+    return w;
+}
+
+constexpr int kWgradThreads = kThreads + 32;  // and the fixer warp
+constexpr size_t kWgradSmem = kRingBytes + 1024 + 4 * 2 * kEpiBytes;
+
+template <int DT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
+    grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmG,
+                         const __grid_constant__ CUtensorMap tmOut, const int* __restrict__ offsets, int groups,
+                         int total_rows, int N, int K) {
+    constexpr uint32_t kIdesc = make_idesc<DT>(256, true, true) | ((uint32_t)(256 >> 3) << 17);
+    constexpr uint32_t kBox = 64 * 128;  // 64 rows x 64 columns
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ GroupTable table;
+    __shared__ __align__(8) uint64_t full_bar[kStages];   // leader: the stage is ready in both CTAs
+    __shared__ __align__(8) uint64_t part_bar[kStages];   // both: this CTA's bytes of a stage to be fixed have landed
+    __shared__ __align__(8) uint64_t empty_bar[kStages];  // both: MMA finished reading the stage
+    __shared__ __align__(8) uint64_t accf_bar[kNumAcc];
+    __shared__ __align__(8) uint64_t acce_bar[kNumAcc];
+    __shared__ __align__(8) uint64_t drain_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sA = smem_base;
+    const uint32_t sG = smem_base + kStages * kOperandStage;
+    const uint32_t sEpi = smem_base + (uint32_t)kRingBytes;
+
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int pair = blockIdx.x >> 1;
+    const int num_pairs = gridDim.x >> 1;
+    const int num_m = (K + 255) / 256;
+    const int num_n = (N + 255) / 256;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&full_bar[s]), 2);  // leader's producer twice, or one fixer per CTA
+            mbar_init(smem_u32(&part_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        for (int a = 0; a < kNumAcc; ++a) {
+            mbar_init(smem_u32(&accf_bar[a]), 1);
+            mbar_init(smem_u32(&acce_bar[a]), 8);
+        }
+        mbar_init(smem_u32(&drain_bar), 1);
+        abort_flag = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmG);
+        tma_prefetch_desc(&tmOut);
+    }
+    if (warp == 0) {
+        tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
+        tmem_relinquish_pair();
+    }
+    grid_launch_dependents();
+    grid_dependency_wait();
+    groups = load_groups(offsets, groups, total_rows, table);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    const int num_tiles = groups * num_m * num_n;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer
+            uint32_t stage = 0, phase = 0;
+            uint32_t issued_mask = 0, issued_phase = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+                const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
+                const int a_col = w.m0 + (int)rank * 128, g_col = w.n0 + (int)rank * 128;
+                for (int done = 0; done < w.rows; done += kBK) {
+                    if (!mbar_wait_cluster(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
+                        atomicCAS(&g_grouped_error, 0, kErrProducerWait);
+                        abort_flag = 1;
+                        ok = false;
+                        break;
+                    }
+                    const bool fix = w.rows - done < kBK && (w.rows - done) % kInstrK != 0;
+                    const uint32_t a = sA + stage * kOperandStage, g = sG + stage * kOperandStage;
+                    const int row = w.row0 + done;
+                    if (fix) {
+                        const uint32_t bar = smem_u32(&part_bar[stage]);
+                        mbar_arrive_expect_tx(bar, 4 * kBox);
+                        tma_load_2d(a, &tmA, bar, a_col, row);
+                        tma_load_2d(a + kBox, &tmA, bar, a_col + 64, row);
+                        tma_load_2d(g, &tmG, bar, g_col, row);
+                        tma_load_2d(g + kBox, &tmG, bar, g_col + 64, row);
+                    } else {
+                        const uint32_t fb_local = smem_u32(&full_bar[stage]);
+                        if (leader) {
+                            mbar_arrive_expect_tx(fb_local, 8 * kBox);
+                            mbar_arrive(fb_local);
+                        }
+                        const uint32_t fb = fb_local & kPeerBitMask;
+                        tma_load_2d_pair(a, &tmA, fb, a_col, row);
+                        tma_load_2d_pair(a + kBox, &tmA, fb, a_col + 64, row);
+                        tma_load_2d_pair(g, &tmG, fb, g_col, row);
+                        tma_load_2d_pair(g + kBox, &tmG, fb, g_col + 64, row);
+                    }
+                    issued_mask |= 1u << stage;
+                    issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (leader)  // every armed phase completes only once both CTAs' bytes have landed
+                for (int s = 0; s < kStages; ++s)
+                    if (issued_mask & (1u << s))
+                        if (!mbar_wait_cluster(smem_u32(&full_bar[s]), (issued_phase >> s) & 1u, nullptr))
+                            atomicCAS(&g_grouped_error, 0, kErrDrainWait);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            // ---------------- MMA issuer
+            const uint64_t a_desc0 = make_sdesc(sA, kBox, 1024);
+            const uint64_t g_desc0 = make_sdesc(sG, kBox, 1024);
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            int t_local = 0;
+            for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+                const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
+                if (w.rows == 0) continue;
+                const int acc = t_local & 1;
+                if (!mbar_wait_cluster(smem_u32(&acce_bar[acc]), ((uint32_t)(t_local >> 1) & 1u) ^ 1u, &abort_flag)) {
+                    atomicCAS(&g_grouped_error, 0, kErrMmaWait);
+                    abort_flag = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (uint32_t)(acc * 256);
+                for (int done = 0; done < w.rows; done += kBK) {
+                    if (!mbar_wait_cluster(smem_u32(&full_bar[stage]), phase, &abort_flag)) {
+                        atomicCAS(&g_grouped_error, 0, kErrMmaWait);
+                        abort_flag = 1;
+                        ok = false;
+                        break;
+                    }
+                    const uint64_t off = (uint64_t)((stage * kOperandStage) >> 4);
+                    const int left = w.rows - done;
+#pragma unroll
+                    for (int ks = 0; ks < kBK / kInstrK; ++ks)
+                        if (ks * kInstrK < left)
+                            mma_pair_f16(d_tmem, a_desc0 + off + (uint64_t)(ks * kInstrK * 128 >> 4),
+                                         g_desc0 + off + (uint64_t)(ks * kInstrK * 128 >> 4), kIdesc,
+                                         (done != 0 || ks != 0) ? 1u : 0u);
+                    tc_commit_pair_multicast(smem_u32(&empty_bar[stage]), 0x3);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (ok) tc_commit_pair_multicast(smem_u32(&accf_bar[acc]), 0x3);
+                ++t_local;
+            }
+            tc_commit_pair_multicast(smem_u32(&drain_bar), 0x1);
+            if (!mbar_wait_cluster(smem_u32(&drain_bar), 0, nullptr)) atomicCAS(&g_grouped_error, 0, kErrDrainWait);
+        }
+    } else if (warp == kWgradThreads / 32 - 1) {
+        // ---------------- fixer (both CTAs): zeros behind a group's last row
+        const uint32_t full_leader0 = mapa_shared(smem_u32(&full_bar[0]), 0);
+        uint32_t stage = 0, part_phase = 0;  // part_phase: bit s = parity of part_bar[s]'s next use
+        bool ok = true;
+        for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+            const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
+            const int stages = (w.rows + kBK - 1) / kBK;
+            const int left = w.rows - (stages - 1) * kBK;  // rows of the last stage (of none: > kBK)
+            if (stages > 0 && left % kInstrK != 0) {
+                const uint32_t s = (stage + (uint32_t)(stages - 1)) % kStages;
+                ok = mbar_wait(smem_u32(&part_bar[s]), (part_phase >> s) & 1u, &abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) {
+                    if (lane == 0) {
+                        atomicCAS(&g_grouped_error, 0, kErrProducerWait);
+                        abort_flag = 1;
+                    }
+                    break;
+                }
+                part_phase ^= 1u << s;
+                const int pieces = (((left + kInstrK - 1) & ~(kInstrK - 1)) - left) * 8;  // 16-byte pieces per box
+                const uint32_t first = sA + s * kOperandStage + (uint32_t)left * 128;
+                for (int i = lane; i < pieces; i += 32) {
+                    const uint32_t at = first + (uint32_t)i * 16;
+                    st_shared_v4(at, 0, 0, 0, 0);
+                    st_shared_v4(at + kBox, 0, 0, 0, 0);
+                    st_shared_v4(at + (sG - sA), 0, 0, 0, 0);
+                    st_shared_v4(at + (sG - sA) + kBox, 0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(full_leader0 + s * 8);
+            }
+            stage = (stage + (uint32_t)stages) % kStages;
+        }
+    } else {
+        // ---------------- epilogue (both CTAs): warps 2..5 read this CTA's 128 accumulator rows
+        const int q = warp & 3;
+        const uint32_t acce_leader0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
+        const uint32_t acce_leader1 = mapa_shared(smem_u32(&acce_bar[1]), 0);
+        const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16);
+        int t_local = 0;
+        uint32_t boxes = 0;  // TMA-store boxes this warp has issued (selects its staging buffer)
+        for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+            const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
+            const int acc = t_local & 1;
+            if (w.rows > 0) {
+                bool ok = mbar_wait_cluster(smem_u32(&accf_bar[acc]), (uint32_t)(t_local >> 1) & 1u, &abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) {
+                    if (lane == 0) {
+                        atomicCAS(&g_grouped_error, 0, kErrEpilogueWait);
+                        abort_flag = 1;
+                    }
+                    break;
+                }
+                tc_fence_after();
+            }
+            const int row0 = w.m0 + (int)rank * 128 + q * 32;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                uint32_t r[32];
+                if (w.rows > 0) {
+                    tmem_ld_32x32b_x32(t_quarter + (uint32_t)(acc * 256 + c * 32), r);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) r[i] = 0;
+                }
+                const int col = w.n0 + c * 32;
+                if (row0 >= K || col >= N) continue;  // warp-uniform: the box lies outside the gradient
+                const uint32_t buf = sEpi + (uint32_t)((q * 2 + (int)(boxes & 1u)) * kEpiBytes);
+                if (lane == 0) bulk_wait_read<1>();  // the store issued two boxes ago has read `buf`
+                __syncwarp();
+                // the 64-byte swizzle of the output's tensor map: piece j of row `lane` at j ^ ((lane >> 1) & 3)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    st_shared_v4(buf + (uint32_t)(lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)),
+                                 pack2<DT>(r[8 * j], r[8 * j + 1]), pack2<DT>(r[8 * j + 2], r[8 * j + 3]),
+                                 pack2<DT>(r[8 * j + 4], r[8 * j + 5]), pack2<DT>(r[8 * j + 6], r[8 * j + 7]));
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_3d(&tmOut, buf, col, row0, w.e);
+                    bulk_commit();
+                }
+                ++boxes;
+            }
+            if (w.rows > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(acc ? acce_leader1 : acce_leader0);
+                ++t_local;
+            }
+        }
+        if (lane == 0) bulk_wait_all();  // this warp's TMA stores are complete before teardown
+        __syncwarp();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+template <typename Kernel, typename... Args>
+static int launch_kernel(Kernel kernel, int grid, int threads, size_t smem, int dev, bool (&attr_set)[64],
+                         cudaStream_t stream, Args... args) {
+    if (dev >= 64 || !attr_set[dev]) {
+        TRB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev < 64) attr_set[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    TRB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return TRB_OK;
+}
+
+// Checks shared by both products.
+static int check(const char* what, int dtype, int groups, int rows, int n, int k, const void* p0, const void* p1,
+                 const void* p2, const int* offsets) {
+    if (groups <= 0 || rows < 0 || n <= 0 || k <= 0 || offsets == nullptr ||
+        (rows > 0 && (p0 == nullptr || p1 == nullptr || p2 == nullptr))) {
+        set_error("%s: sizes must be positive (rows may be 0) and pointers non-null", what);
+        return TRB_ERR_ARGS;
+    }
+    if (dtype != TRB_BFLOAT16 && dtype != TRB_FLOAT16) {
+        set_error("%s: unsupported dtype %s (bfloat16 and float16)", what, dtype_name(dtype));
+        return TRB_SKIPPED;
+    }
+    if (groups > kMaxGroups) {
+        set_error("%s: at most %d groups (got %d)", what, kMaxGroups, groups);
+        return TRB_SKIPPED;
+    }
+    if (n % 8 != 0 || k % 8 != 0) {
+        set_error("%s: n and k must be multiples of 8 (n=%d k=%d)", what, n, k);
+        return TRB_ERR_ALIGN;
+    }
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p0) | reinterpret_cast<uintptr_t>(p1) |
+                           reinterpret_cast<uintptr_t>(p2);
+    if ((bits & 15u) != 0 || (reinterpret_cast<uintptr_t>(offsets) & 3u) != 0) {
+        set_error("%s: matrices must be 16-byte aligned and offsets 4-byte aligned", what);
+        return TRB_ERR_ALIGN;
+    }
+    return TRB_OK;
+}
+
+static int pairs_for(int64_t tiles, int dev) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count(dev) / 2));
+}
+
+template <int DT, bool KB>
+static int launch_product(int groups, int rows, int n, int k, const void* a, const void* b, const int* offsets,
+                          void* out, int dev, cudaStream_t stream) {
+    static bool attr_set[64] = {};
+    CUtensorMap tmW, tmX128, tmX32;
+    const uint64_t we[3] = {(uint64_t)(KB ? k : n), (uint64_t)(KB ? n : k), (uint64_t)groups};
+    const uint32_t wb[3] = {64, KB ? 128u : 64u, 1};
+    const uint64_t xe[2] = {(uint64_t)k, (uint64_t)rows};
+    const uint32_t xb128[2] = {64, 128}, xb32[2] = {64, 32};
+    int rc = gemm::encode_tiled(&tmW, b, 2, 3, we, wb, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX128, a, 2, 2, xe, xb128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, xb32, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != TRB_OK) return rc;
+    const int64_t num_n = (n + kTileN - 1) / kTileN;
+    const int64_t tiles = num_n * ((int64_t)rows / kTileRows + std::min(groups, rows));
+    if (tiles > INT32_MAX) {
+        set_error("trb_grouped_gemm_launch: too many tiles (rows=%d n=%d groups=%d)", rows, n, groups);
+        return TRB_SKIPPED;
+    }
+    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, kProductSmem, dev, attr_set,
+                         stream, tmW, tmX128, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
+}
+
+template <int DT>
+static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const void* g, const int* offsets,
+                        void* out, int dev, cudaStream_t stream) {
+    static bool attr_set[64] = {};
+    CUtensorMap tmA, tmG, tmOut;
+    // Without rows no operand is read; the maps then stand on the output, which is there.
+    const uint64_t extent_rows = (uint64_t)std::max(rows, 1);
+    const uint64_t ae[2] = {(uint64_t)k, extent_rows}, ge[2] = {(uint64_t)n, extent_rows};
+    const uint64_t oe[3] = {(uint64_t)n, (uint64_t)k, (uint64_t)groups};
+    const uint32_t box[2] = {64, 64}, obox[3] = {32, 32, 1};
+    int rc = gemm::encode_tiled(&tmA, rows > 0 ? a : out, 2, 2, ae, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmG, rows > 0 ? g : out, 2, 2, ge, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmOut, out, 2, 3, oe, obox, CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc != TRB_OK) return rc;
+    const int64_t tiles = (int64_t)groups * ((k + 255) / 256) * ((n + 255) / 256);
+    if (tiles > INT32_MAX) {
+        set_error("trb_grouped_wgrad_launch: too many tiles (groups=%d n=%d k=%d)", groups, n, k);
+        return TRB_SKIPPED;
+    }
+    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, kWgradSmem, dev, attr_set,
+                         stream, tmA, tmG, tmOut, offsets, groups, rows, n, k);
+}
+
+int read_error(bool clear) {
+    int v = 0;
+    TRB_CUDA(cudaMemcpyFromSymbol(&v, g_grouped_error, sizeof(int)));
+    if (clear) {
+        const int zero = 0;
+        TRB_CUDA(cudaMemcpyToSymbol(g_grouped_error, &zero, sizeof(int)));
+    }
+    return v;
+}
+
+}  // namespace grouped
+}  // namespace trb
+
+extern "C" int trb_grouped_gemm_launch(int dtype, int groups, int rows, int n, int k, const void* a, const void* b,
+                                       int b_layout, const int32_t* offsets, void* out, void* stream) {
+    using namespace trb;
+    clear_error();
+    int rc = grouped::check("trb_grouped_gemm_launch", dtype, groups, rows, n, k, a, b, out, offsets);
+    if (rc != TRB_OK) return rc;
+    if (b_layout != TRB_B_ROW_MAJOR && b_layout != TRB_B_K_MAJOR) {
+        set_error("trb_grouped_gemm_launch: unknown b_layout %d", b_layout);
+        return TRB_ERR_ARGS;
+    }
+    if (rows == 0) return TRB_OK;
+    int dev = 0;
+    TRB_CUDA(cudaGetDevice(&dev));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool kb = b_layout == TRB_B_K_MAJOR;
+    if (dtype == TRB_BFLOAT16)
+        return kb ? grouped::launch_product<TRB_BFLOAT16, true>(groups, rows, n, k, a, b, offsets, out, dev, s)
+                  : grouped::launch_product<TRB_BFLOAT16, false>(groups, rows, n, k, a, b, offsets, out, dev, s);
+    return kb ? grouped::launch_product<TRB_FLOAT16, true>(groups, rows, n, k, a, b, offsets, out, dev, s)
+              : grouped::launch_product<TRB_FLOAT16, false>(groups, rows, n, k, a, b, offsets, out, dev, s);
+}
+
+extern "C" int trb_grouped_wgrad_launch(int dtype, int groups, int rows, int n, int k, const void* a, const void* g,
+                                        const int32_t* offsets, void* out, void* stream) {
+    using namespace trb;
+    clear_error();
+    const int rc = grouped::check("trb_grouped_wgrad_launch", dtype, groups, rows, n, k, a, g, out, offsets);
+    if (rc != TRB_OK) return rc;
+    if (out == nullptr) {
+        set_error("trb_grouped_wgrad_launch: out is null");
+        return TRB_ERR_ARGS;
+    }
+    int dev = 0;
+    TRB_CUDA(cudaGetDevice(&dev));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == TRB_BFLOAT16
+               ? grouped::launch_wgrad<TRB_BFLOAT16>(groups, rows, n, k, a, g, offsets, out, dev, s)
+               : grouped::launch_wgrad<TRB_FLOAT16>(groups, rows, n, k, a, g, offsets, out, dev, s);
+}

@@ -146,19 +146,6 @@ struct Traits<TRB_INT8> {
     static constexpr uint32_t kIdesc = make_idesc(2, 1, 1);  // S32 <- S8 x S8
 };
 
-// Shared-memory matrix descriptor, sm100 version (bit 46), swizzled layout
-// type at [61,64) (2 = 128B swizzle, 1 = 128B swizzle with 32B atoms).
-// Addresses and offsets are in 16-byte units.
-__device__ __forceinline__ uint64_t make_sdesc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes,
-                                               uint32_t layout_type = 2) {
-    uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16;
-    d |= (uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)layout_type << 61;
-    return d;
-}
-
 template <int KIND>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     if constexpr (KIND == 0) mma_f16(d, a, b, idesc, acc);
@@ -1957,8 +1944,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-static int encode_2d(CUtensorMap* map, const void* base, int esize, uint64_t inner, uint64_t outer,
-                     uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
+int encode_tiled(CUtensorMap* map, const void* base, int esize, int rank, const uint64_t* extent, const uint32_t* box,
+                 CUtensorMapSwizzle swizzle) {
     auto fn = encode_fn();
     if (fn == nullptr) {
         set_error("cuTensorMapEncodeTiled entry point unavailable");
@@ -1967,18 +1954,29 @@ static int encode_2d(CUtensorMap* map, const void* base, int esize, uint64_t inn
     const CUtensorMapDataType dt = esize == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
                                                 : CU_TENSOR_MAP_DATA_TYPE_UINT32;
-    cuuint64_t dims[2] = {inner, outer};
-    cuuint64_t strides[1] = {inner * (uint64_t)esize};
-    cuuint32_t box[2] = {box_inner, box_outer};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    cuuint64_t dims[3], strides[2];
+    cuuint32_t boxes[3], estr[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        dims[i] = extent[i];
+        boxes[i] = box[i];
+        if (i > 0) strides[i - 1] = i == 1 ? dims[0] * (uint64_t)esize : strides[i - 2] * dims[i - 1];
+    }
+    CUresult r = fn(map, dt, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, boxes, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        set_error("cuTensorMapEncodeTiled failed (%d) for %llux%llu box %ux%u", (int)r, (unsigned long long)inner,
-                  (unsigned long long)outer, box_inner, box_outer);
+        set_error("cuTensorMapEncodeTiled failed (%d) for %llux%llu box %ux%u", (int)r, (unsigned long long)extent[0],
+                  (unsigned long long)extent[1], box[0], box[1]);
         return TRB_ERR_CUDA;
     }
     return TRB_OK;
+}
+
+static int encode_2d(CUtensorMap* map, const void* base, int esize, uint64_t inner, uint64_t outer,
+                     uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
+    const uint64_t extent[2] = {inner, outer};
+    const uint32_t box[2] = {box_inner, box_outer};
+    return encode_tiled(map, base, esize, 2, extent, box, swizzle);
 }
 
 // Split-K workspace of one device: fp32 partials + per-tile arrival counters.

@@ -220,9 +220,11 @@ extern "C" int trb_device_error(int device_id, int clear) {
     if (rc != TRB_OK) return rc;
     const int e1 = hbm::read_error(clear != 0);
     const int e2 = gemm::read_error(clear != 0);
+    const int e3 = grouped::read_error(clear != 0);
     if (e1 < 0) return e1;
     if (e2 < 0) return e2;
-    return e1 ? e1 : e2;
+    if (e3 < 0) return e3;
+    return e1 ? e1 : e2 ? e2 : e3;
 }
 
 extern "C" int trb_hbm_run(const trb_hbm_args* args, trb_result* out) {

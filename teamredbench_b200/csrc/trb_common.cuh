@@ -67,7 +67,14 @@ int fill_operand(void* data, int dtype, uint64_t n, int k, uint64_t seed, unsign
 int read_error(bool clear);
 // Bounded-wait self-test kernel (see trb_selftest_bounded_wait).
 int wait_probe(uint64_t limit_ns, cudaStream_t stream);
+// Tensor map of a contiguous tensor of rank 2 or 3, extents innermost first.
+int encode_tiled(CUtensorMap* map, const void* base, int esize, int rank, const uint64_t* extent, const uint32_t* box,
+                 CUtensorMapSwizzle swizzle);
 }  // namespace gemm
+
+namespace grouped {
+int read_error(bool clear);
+}  // namespace grouped
 
 namespace dgemm {
 // float64 C = A * B on the DMMA tensor path (no tcgen05 kind takes fp64); any m, n, k.
@@ -88,6 +95,7 @@ enum : int {
     kErrDrainWait = 4,
     kErrBulkWait = 5,
     kErrSelfTestWait = 6,  // the bounded-wait self-test's deliberate give-up
+    kErrOffsets = 7,       // a grouped product's offsets decrease or leave [0, rows]
 };
 
 #if defined(__CUDACC__)
@@ -162,6 +170,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// 3-D tiled TMA load (no multicast) of the box at element coordinates (x, y, z).
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
+            "r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
 // 2-D tiled TMA store of a shared-memory box to global element coordinates
 // (x, y); completion is tracked by this thread's bulk async-groups
 // (bulk_commit / bulk_wait_read / bulk_wait_all below).
@@ -169,6 +186,12 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                      reinterpret_cast<uint64_t>(map)),
                  "r"(src), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -263,6 +286,19 @@ TRB_DEFINE_MMA(mma_f8f6f4, "f8f6f4")
 TRB_DEFINE_MMA(mma_i8, "i8")
 #undef TRB_DEFINE_MMA
 
+// Shared-memory matrix descriptor, sm100 version (bit 46), swizzled layout
+// type at [61,64) (2 = 128B swizzle, 1 = 128B swizzle with 32B atoms).
+// Addresses and offsets are in 16-byte units.
+__device__ __forceinline__ uint64_t make_sdesc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes,
+                                               uint32_t layout_type = 2) {
+    uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)layout_type << 61;
+    return d;
+}
+
 // ---- CTA pairs (clusters of 2) and tcgen05 cta_group::2 ----
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
@@ -340,6 +376,14 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y,
+                                                 int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols)
                  : "memory");
@@ -390,6 +434,17 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
 __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// 16 lanes (taddr's lane field: a multiple of 16 in the warp's quarter) x 32 consecutive 32-bit columns in the
+// fragment order of an m16n8 product: for column octet c, register 4c + 2h + i of thread t holds lane 8h + t / 4,
+// column 8c + 2 (t % 4) + i.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])

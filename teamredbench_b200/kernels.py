@@ -112,3 +112,73 @@ def gemm(a: Any, b: Any, out: Any, *, dtype: str | None = None, scale_a: float =
                            float(scale_b), int(splits), int(cta_pair), "k_major" if b_transposed else "row_major",
                            _stream_handle(a, stream), int(tile_n))
     return out
+
+
+def _check_offsets(offsets: Any, groups: int) -> None:
+    if str(offsets.dtype) != "torch.int32" or offsets.dim() != 1 or offsets.shape[0] != groups + 1:
+        raise ValueError(f"offsets must be {groups + 1} int32 values, got {tuple(offsets.shape)} {offsets.dtype}")
+
+
+def _check_one_device(*tensors: Any) -> None:
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors must share one device, got {t.device} beside {device}")
+
+
+def grouped_gemm(a: Any, b: Any, offsets: Any, out: Any, *, b_transposed: bool = False, stream: Any | None = None) -> Any:
+    """out[r] = a[r] @ b[e] for the rows r of group (expert) e, bf16 or f16.
+
+    a (rows x k) and out (rows x n) are sorted by group; offsets (groups + 1
+    int32 on the device) gives group e the rows [offsets[e], offsets[e + 1]).
+    b is (groups x k x n), or (groups x n x k) with b_transposed=True; the
+    gradient of a is the same call on the gradient of out with the other value
+    of b_transposed.  Groups may be empty; rows outside every group are left as
+    they are.  n and k must be multiples of 8.  Offsets that decrease or leave
+    [0, rows] compute nothing and set the device error word to 7
+    (``_native.device_error``), which the host does not wait for here."""
+    _require_cuda_contiguous(a, b, offsets, out)
+    _check_one_device(a, b, offsets, out)
+    if a.dim() != 2 or b.dim() != 3:
+        raise ValueError(f"grouped_gemm takes a 2-D a and a 3-D b, got {tuple(a.shape)} and {tuple(b.shape)}")
+    rows, k = a.shape
+    groups, bk, n = b.shape
+    if b_transposed:
+        bk, n = n, bk
+    if bk != k:
+        raise ValueError(f"incompatible shapes {tuple(a.shape)} x {tuple(b.shape)} (b_transposed={b_transposed})")
+    if out.shape != (rows, n):
+        raise ValueError(f"out must be {(rows, n)}, got {tuple(out.shape)}")
+    if b.dtype != a.dtype or out.dtype != a.dtype:
+        raise ValueError("a, b and out must share one dtype")
+    _check_offsets(offsets, groups)
+    _native.grouped_gemm_launch(trb_dtype(a), groups, rows, n, k, a.data_ptr(), b.data_ptr(),
+                                "k_major" if b_transposed else "row_major", offsets.data_ptr(), out.data_ptr(),
+                                _stream_handle(a, stream))
+    return out
+
+
+def grouped_gemm_wgrad(a: Any, grad: Any, offsets: Any, out: Any, *, stream: Any | None = None) -> Any:
+    """out[e] = a[rows of e].T @ grad[rows of e]: the gradient of grouped_gemm's
+    (groups x k x n) weights from a (rows x k) and the gradient of its output
+    (rows x n); zeros for a group without rows.  For weights kept
+    (groups x n x k) pass grad first and a second.  offsets, types, sizes and
+    errors as in grouped_gemm."""
+    _require_cuda_contiguous(a, grad, offsets, out)
+    _check_one_device(a, grad, offsets, out)
+    if a.dim() != 2 or grad.dim() != 2 or out.dim() != 3:
+        raise ValueError(f"grouped_gemm_wgrad takes 2-D a and grad and a 3-D out, got {tuple(a.shape)}, "
+                         f"{tuple(grad.shape)} and {tuple(out.shape)}")
+    rows, k = a.shape
+    n = grad.shape[1]
+    groups = out.shape[0]
+    if grad.shape[0] != rows:
+        raise ValueError(f"a and grad must have the same number of rows, got {rows} and {grad.shape[0]}")
+    if out.shape != (groups, k, n):
+        raise ValueError(f"out must be {(groups, k, n)}, got {tuple(out.shape)}")
+    if grad.dtype != a.dtype or out.dtype != a.dtype:
+        raise ValueError("a, grad and out must share one dtype")
+    _check_offsets(offsets, groups)
+    _native.grouped_wgrad_launch(trb_dtype(a), groups, rows, n, k, a.data_ptr(), grad.data_ptr(), offsets.data_ptr(),
+                                 out.data_ptr(), _stream_handle(a, stream))
+    return out
