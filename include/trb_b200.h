@@ -291,6 +291,20 @@ int trb_grouped_gemm_launch(int dtype, int groups, int rows, int n, int k, const
 int trb_grouped_wgrad_launch(int dtype, int groups, int rows, int n, int k, const void* a, const void* g,
                              const int32_t* offsets, void* out, void* stream);
 
+/* Products with 4-bit weights: out[r, n] = the sum over k of
+ * x[r, k] * (q[e, n, k] - z[e, n, k / group_size]) * s[e, n, k / group_size]
+ * for the rows r of group e; meant for few rows a group (each 8 or 16 rows of
+ * a group read its weights once).  x rows x k, out rows x n, s groups x n x
+ * (k / group_size), bfloat16 or float16 alike; q groups x n x (k / 2) bytes,
+ * the even k in the low four bits; zeros bytes shaped as s (the low four bits
+ * count), or NULL for 8 throughout.  offsets as above, or NULL for one group of
+ * all rows.  fp32 sums, the scale applied in fp32 to each group's sum, one
+ * rounding.  group_size: a power of two, at least 32, that divides k; k at most
+ * 65536, any n; x and q 16-byte aligned.  Error word, streams and limits as for
+ * the other grouped entry points. */
+int trb_gemv_w4_launch(int dtype, int groups, int rows, int n, int k, int group_size, const void* x, const void* q,
+                       const void* scales, const void* zeros, const int32_t* offsets, void* out, void* stream);
+
 /* Round f32 values in place on the device to tf32 (round to nearest, ties
  * away from zero; cvt.rna.tf32.f32).  Used to prepare tf32 GEMM inputs. */
 int trb_round_tf32(void* data, uint64_t count, void* stream);

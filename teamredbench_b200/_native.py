@@ -47,6 +47,7 @@ EXPORTED_SYMBOLS = (
     "trb_gemm_host",
     "trb_grouped_gemm_launch",
     "trb_grouped_wgrad_launch",
+    "trb_gemv_w4_launch",
     "trb_round_tf32",
     "trb_selftest_bounded_wait",
 )
@@ -174,6 +175,8 @@ def load() -> ctypes.CDLL:
     lib.trb_grouped_gemm_launch.restype = i32
     lib.trb_grouped_wgrad_launch.argtypes = [i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]
     lib.trb_grouped_wgrad_launch.restype = i32
+    lib.trb_gemv_w4_launch.argtypes = [i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]
+    lib.trb_gemv_w4_launch.restype = i32
     lib.trb_round_tf32.argtypes = [vp, u64, vp]
     lib.trb_round_tf32.restype = i32
     lib.trb_selftest_bounded_wait.argtypes = [ctypes.c_uint32, i32, res_p]
@@ -264,6 +267,12 @@ def grouped_gemm_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: i
 def grouped_wgrad_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: int, g: int, offsets: int, out: int,
                          stream: int = 0) -> None:
     check(load().trb_grouped_wgrad_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, g, offsets, out, stream or None))
+
+
+def gemv_w4_launch(dtype: str, groups: int, rows: int, n: int, k: int, group_size: int, x: int, q: int, scales: int,
+                   zeros: int | None, offsets: int | None, out: int, stream: int = 0) -> None:
+    check(load().trb_gemv_w4_launch(DTYPE_CODES[dtype], groups, rows, n, k, group_size, x, q, scales, zeros, offsets,
+                                    out, stream or None))
 
 
 def round_tf32(data: int, count: int, stream: int = 0) -> None:

@@ -16,13 +16,13 @@
 #include <algorithm>
 
 #include "trb_common.cuh"
+#include "trb_groups.cuh"
 
 namespace trb {
 namespace grouped {
 
 __device__ int g_grouped_error;
 
-constexpr int kMaxGroups = 1024;
 constexpr int kThreads = 192;        // producer warp, MMA warp, 4 epilogue warps
 constexpr int kBK = 64;              // 16-bit elements per 128-byte swizzle row
 constexpr int kInstrK = 16;          // K elements per tcgen05.mma
@@ -32,28 +32,6 @@ constexpr size_t kRingBytes = (size_t)kStages * 2 * kOperandStage;
 constexpr int kNumAcc = 2;
 constexpr int kTmemCols = 512;
 constexpr int kEpiBytes = 32 * 64;   // a 32 x 32 block of 16-bit results
-
-struct GroupTable {
-    int start[kMaxGroups];
-    int rows[kMaxGroups];
-};
-
-// Reads the offsets (all threads of the CTA; ends with a barrier).  Offsets
-// that decrease or leave [0, total_rows] set the device error word; the call
-// then computes nothing (returns 0 groups), so that no offsets, however wrong,
-// reach outside the operands.
-__device__ __forceinline__ int load_groups(const int* offsets, int groups, int total_rows, GroupTable& g) {
-    bool bad = false;
-    for (int e = threadIdx.x; e < groups; e += blockDim.x) {
-        const int lo = offsets[e], hi = offsets[e + 1];
-        bad = bad || lo < 0 || hi < lo || hi > total_rows;
-        g.start[e] = lo;
-        g.rows[e] = hi - lo;
-    }
-    if (!__syncthreads_or(bad)) return groups;
-    if (threadIdx.x == 0) atomicCAS(&g_grouped_error, 0, kErrOffsets);
-    return 0;
-}
 
 // F32 <- BF16 x BF16 or F16 x F16 instruction descriptor; bit 15 / 16: A / B is MN-major.
 template <int DT>
@@ -105,45 +83,17 @@ struct ProductTile {
     int e, row0, rows, n0;
 };
 
-struct ProductTable : GroupTable {
-    int chunk0[kMaxGroups + 1];  // chunks of the groups before this one
-};
-
 constexpr int kTileN = 256;    // columns of a tile (pair)
 constexpr int kTileRows = 256; // largest chunk
 
 __device__ __forceinline__ int chunks_of(int rows) { return (rows + kTileRows - 1) / kTileRows; }
 
-// Exclusive scan of the groups' chunk counts (one warp).
-__device__ __forceinline__ void scan_chunks(int groups, ProductTable& g, int lane) {
-    int base = 0;
-    for (int e0 = 0; e0 < groups; e0 += 32) {
-        const int e = e0 + lane;
-        const int c = e < groups ? chunks_of(g.rows[e]) : 0;
-        int sum = c;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += up;
-        }
-        if (e < groups) g.chunk0[e] = base + sum - c;
-        base += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (lane == 0) g.chunk0[groups] = base;
-}
-
 // Tile t: groups in order; inside a group, runs of 8 chunks walk the columns
 // together (a weight panel is read by the chunks next to each other in time).
-__device__ __forceinline__ ProductTile product_tile(int t, int groups, int num_n, const ProductTable& g) {
-    const int q = t / num_n;
-    int lo = 0, hi = groups - 1;  // the last group whose chunks begin at or before q
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (g.chunk0[mid] <= q) lo = mid;
-        else hi = mid - 1;
-    }
-    const int local = t - g.chunk0[lo] * num_n;
-    const int rows = g.rows[lo];
+__device__ __forceinline__ ProductTile product_tile(int t, int groups, int num_n, const GroupTable& g) {
+    const int e = group_of_chunk(t / num_n, groups, g);
+    const int local = t - g.chunk0[e] * num_n;
+    const int rows = g.rows[e];
     const int chunks = chunks_of(rows);
     const int run = 8 * num_n;
     const int first = local / run * 8;
@@ -152,8 +102,8 @@ __device__ __forceinline__ ProductTile product_tile(int t, int groups, int num_n
     const int chunk = first + in_run % width;
     const int per = ((rows + chunks - 1) / chunks + 31) & ~31;
     ProductTile p;
-    p.e = lo;
-    p.row0 = g.start[lo] + chunk * per;
+    p.e = e;
+    p.row0 = g.start[e] + chunk * per;
     p.rows = min(per, rows - chunk * per);
     p.n0 = in_run / width * kTileN;
     return p;
@@ -169,7 +119,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     constexpr uint32_t kIdesc = make_idesc<DT>(256, !KB, false);
 
     extern __shared__ uint8_t smem_raw[];
-    __shared__ ProductTable table;
+    __shared__ int group_words[3 * kMaxGroups + 1];
     __shared__ __align__(8) uint64_t full_bar[kStages];   // leader: both CTAs' TMA bytes land here
     __shared__ __align__(8) uint64_t empty_bar[kStages];  // both: MMA finished reading the stage
     __shared__ __align__(8) uint64_t accf_bar[kNumAcc];   // both: accumulator ready for the epilogue
@@ -191,6 +141,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int num_pairs = gridDim.x >> 1;
     const int num_n = (N + kTileN - 1) / kTileN;
     const int num_kb = (K + kBK - 1) / kBK;
+    const GroupTable table = {group_words, group_words + kMaxGroups, group_words + 2 * kMaxGroups};
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -214,8 +165,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     grid_launch_dependents();
     grid_dependency_wait();  // offsets, operands and out may belong to the previous grid until here
-    groups = load_groups(offsets, groups, total_rows, table);
-    if (warp == 0) scan_chunks(groups, table, lane);
+    groups = load_groups(offsets, groups, total_rows, table, &g_grouped_error);
+    if (warp == 0) scan_chunks(groups, kTileRows, table, lane);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();  // barrier inits of both CTAs visible before any cross-CTA signal
@@ -428,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     constexpr uint32_t kBox = 64 * 128;  // 64 rows x 64 columns
 
     extern __shared__ uint8_t smem_raw[];
-    __shared__ GroupTable table;
+    __shared__ int group_words[2 * kMaxGroups];
     __shared__ __align__(8) uint64_t full_bar[kStages];   // leader: the stage is ready in both CTAs
     __shared__ __align__(8) uint64_t part_bar[kStages];   // both: this CTA's bytes of a stage to be fixed have landed
     __shared__ __align__(8) uint64_t empty_bar[kStages];  // both: MMA finished reading the stage
@@ -451,6 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     const int num_pairs = gridDim.x >> 1;
     const int num_m = (K + 255) / 256;
     const int num_n = (N + 255) / 256;
+    const GroupTable table = {group_words, group_words + kMaxGroups, nullptr};
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -475,7 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     }
     grid_launch_dependents();
     grid_dependency_wait();
-    groups = load_groups(offsets, groups, total_rows, table);
+    groups = load_groups(offsets, groups, total_rows, table, &g_grouped_error);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();

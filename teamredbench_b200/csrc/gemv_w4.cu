@@ -1,0 +1,466 @@
+// gemv_w4.cu -- few rows times matrices of 4-bit weights with a scale per group of k.
+//
+//   out[r, n] = sum over groups g of k:  s[e, n, g] * sum over k in g of x[r, k] * (q[e, n, k] - z[e, n, g])
+//
+// for the rows r of expert e (one expert: a plain matrix).  q is stored two to
+// a byte along k, the low four bits first.
+//
+// The bytes of q bound it: 1/2 byte per weight, read once for up to 8 (16)
+// rows of x.  The products run on mma.sync m16n8k16, 16 outputs x 8 rows of x
+// per instruction -- at one row the tensor pipe still does with one
+// instruction per 256 weights what would take 256 FMA lanes, and the exact
+// products of small whole numbers with 16-bit x accumulate in fp32.  Weights
+// become 16-bit floats by bit operations: a 4-bit q ORed into the mantissa of
+// 128 (bf16) or 64 (f16) is 128 + q (64 + q) exactly, and subtracting 128 + z
+// is exact too, so nothing is rounded before the product, and the scale is
+// applied in fp32 to each group's sum.
+//
+// Each warp streams its own boxes of 16 * MT outputs x 256 k (128 bytes of q a
+// row) through a private ring filled by TMA: no barrier between warps until
+// the sums of a tile are joined.  WK warps of a CTA share a tile's k, in a
+// fixed order of addition.
+//
+// No counterpart in the reference.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "trb_common.cuh"
+#include "trb_groups.cuh"
+
+namespace trb {
+namespace w4 {
+
+__device__ int g_w4_error;
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kBoxK = 256;   // k of a box: one 128-byte swizzle row
+constexpr int kBlockK = 32;  // k of a block: 16 bytes a row, two products
+
+struct Shape {
+    int groups, rows, n, k;
+    int k_groups;    // scales per output
+    int group_log2;
+    int wk;          // warps that share a tile's k
+    int depth;       // boxes in each warp's ring
+    int tokens;      // rows of x taken at once
+};
+
+template <int DT>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (DT == TRB_BFLOAT16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+            "%2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+            "%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Pair p of a word of eight q: (q[p], q[p + 4]) as two 16-bit floats, each plus 128 (bf16) or 64 (f16).
+template <int DT>
+__device__ __forceinline__ uint32_t biased_pair(uint32_t w, int p) {
+    if constexpr (DT == TRB_BFLOAT16) return ((w >> (4 * p)) & 0x000F000Fu) | 0x43004300u;
+    else return ((p == 0 ? w << 4 : w >> (4 * (p - 1))) & 0x00F000F0u) | 0x54005400u;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t biased_zero(uint32_t z) {
+    if constexpr (DT == TRB_BFLOAT16) return 0x43004300u + z * 0x00010001u;
+    else return 0x54005400u + z * 0x00100010u;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    if constexpr (DT == TRB_BFLOAT16) {
+        __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+        return *reinterpret_cast<uint32_t*>(&r);
+    } else {
+        __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+        return *reinterpret_cast<uint32_t*>(&r);
+    }
+}
+template <int DT>
+__device__ __forceinline__ float scale_of(uint32_t packed) {  // scale in the upper 16 bits
+    if constexpr (DT == TRB_BFLOAT16) return __uint_as_float(packed & 0xFFFF0000u);
+    else return __half2float(__ushort_as_half((unsigned short)(packed >> 16)));
+}
+template <int DT>
+__device__ __forceinline__ uint16_t round16(float v) {
+    if constexpr (DT == TRB_BFLOAT16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    else return __half_as_ushort(__float2half_rn(v));
+}
+
+// A place in a warp's stream of boxes.
+struct Cursor {
+    int tile, box, e, n0;
+};
+
+// MT * 16 outputs x NT * 8 rows of x per warp; a group of k spans GB blocks (8: a box or more).
+template <int DT, int MT, int NT, int GB>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+    gemv_w4_kernel(const __grid_constant__ CUtensorMap tmQ, const uint16_t* __restrict__ x,
+                   const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros,
+                   const int* __restrict__ offsets, uint16_t* __restrict__ out, const Shape sh) {
+    constexpr int kRows = 16 * MT;              // outputs of a warp's box
+    constexpr uint32_t kBoxBytes = kRows * 128;
+    constexpr int kPer = GB == 1 ? 2 : 1;       // groups whose scale a thread holds, per output
+    constexpr int kMaxDepth = 8;
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[kWarps * kMaxDepth];
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int num_box = (sh.k + kBoxK - 1) / kBoxK;
+    const int wk = sh.wk, wr = kWarps / wk;
+    const int kw = warp % wk, rw = warp / wk;
+    const int tile_n = wr * kRows;
+    const int tiles_n = (sh.n + tile_n - 1) / tile_n;
+
+    uint8_t* ring_ptr = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint4* xs = reinterpret_cast<uint4*>(ring_ptr + (size_t)kWarps * sh.depth * kBoxBytes);
+    float* red = reinterpret_cast<float*>(xs + (size_t)num_box * 8 * sh.tokens * 4);
+    int* words = reinterpret_cast<int*>(red + 2 * kWarps * NT * 8 * kRows);
+    const GroupTable table = {words, words + sh.groups, words + 2 * sh.groups};
+    const uint32_t ring = smem_u32(ring_ptr) + (uint32_t)(warp * sh.depth) * kBoxBytes;
+    const uint32_t bars = smem_u32(&full_bar[warp * kMaxDepth]);
+
+    if (lane == 0) {
+        for (int s = 0; s < sh.depth; ++s) mbar_init(bars + s * 8, 1);
+        fence_mbar_init();
+        if (warp == 0) tma_prefetch_desc(&tmQ);
+    }
+    grid_launch_dependents();
+    grid_dependency_wait();
+    int groups = sh.groups;
+    if (offsets != nullptr) {
+        groups = load_groups(offsets, sh.groups, sh.rows, table, &g_w4_error);
+    } else if (threadIdx.x == 0) {
+        table.start[0] = 0;
+        table.rows[0] = sh.rows;
+    }
+    __syncthreads();
+    if (warp == 0) scan_chunks(groups, sh.tokens, table, lane);
+    __syncthreads();
+
+    // This CTA's share of the tiles, contiguous so that x stays in shared memory.
+    const int64_t total = (int64_t)table.chunk0[groups] * tiles_n;
+    const int tile0 = (int)(total * blockIdx.x / gridDim.x);
+    const int tile1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+
+    auto enter = [&](Cursor& c) {  // the first box at or after c.tile that is this warp's
+        for (; c.tile < tile1; ++c.tile) {
+            const int q = c.tile / tiles_n;
+            c.n0 = (c.tile - q * tiles_n) * tile_n + rw * kRows;
+            if (c.n0 < sh.n) {
+                c.e = group_of_chunk(q, groups, table);
+                c.box = kw;
+                return;
+            }
+        }
+    };
+    auto advance = [&](Cursor& c) {
+        c.box += wk;
+        if (c.box >= num_box) {
+            ++c.tile;
+            enter(c);
+        }
+    };
+    auto issue = [&](const Cursor& c, int slot) {
+        mbar_arrive_expect_tx(bars + slot * 8, kBoxBytes);
+        tma_load_3d(ring + slot * kBoxBytes, &tmQ, bars + slot * 8, c.box * 128, c.n0, c.e);
+    };
+    // Scales (upper half) and zero points (lower) of a box, spread over the four threads of an output.
+    auto load_scales = [&](const Cursor& c, uint32_t (&sc)[2 * MT][kPer]) {
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {
+            const int row = c.n0 + i * 8 + g;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int in_box = GB == 1 ? 2 * t + j : GB == 2 ? t : GB == 4 ? (t & 1) : 0;
+                const int kg = GB == 8 ? (c.box * kBoxK) >> sh.group_log2 : c.box * (8 / GB) + in_box;
+                sc[i][j] = 8;
+                if (c.tile < tile1 && row < sh.n && kg < sh.k_groups) {
+                    const size_t at = ((size_t)c.e * sh.n + row) * sh.k_groups + kg;
+                    sc[i][j] = (uint32_t)scales[at] << 16 | (zeros != nullptr ? zeros[at] & 15u : 8u);
+                }
+            }
+        }
+    };
+
+    Cursor ahead = {tile0, 0, 0, 0};  // the next box to request
+    enter(ahead);
+    if (lane == 0) {
+        Cursor c = ahead;
+        for (int s = 0; s < sh.depth && c.tile < tile1; ++s, advance(c)) issue(c, s);
+        ahead = c;
+    }
+    Cursor next = {tile0, 0, 0, 0};  // the next box to multiply
+    enter(next);
+    uint32_t sc_next[2 * MT][kPer];
+    load_scales(next, sc_next);
+
+    int slot = 0, chunk = -1, red_at = 0;
+    uint32_t phase = 0;
+    int tokens = 0, row0 = 0;
+    bool failed = false;
+    for (int tile = tile0; tile < tile1; ++tile) {
+        const int q = tile / tiles_n;
+        if (q != chunk) {  // other rows of x: in shared memory, [block of 32 k][row][t]: the 8 values of thread t
+            chunk = q;     // in the order the pairs of a word of q come in
+            const int e = group_of_chunk(q, groups, table);
+            const int first = (q - table.chunk0[e]) * sh.tokens;
+            row0 = table.start[e] + first;
+            tokens = min(sh.tokens, table.rows[e] - first);
+            __syncthreads();
+            for (int i = threadIdx.x; i < num_box * 8 * tokens * 4; i += kThreads) {
+                const int c = (i >> 2) % tokens, k0 = ((i >> 2) / tokens) * kBlockK + (i & 3) * 8;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (k0 < sh.k) v = *reinterpret_cast<const uint4*>(x + (size_t)(row0 + c) * sh.k + k0);
+                xs[i] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                                   __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+            }
+            __syncthreads();
+        }
+        float sum[MT][NT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[m][c][i] = 0.0f;
+
+        while (next.tile == tile) {
+            uint32_t sc[2 * MT][kPer];
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) sc[i][j] = sc_next[i][j];
+            const int box = next.box;
+            advance(next);
+            load_scales(next, sc_next);
+            if (!failed && !mbar_wait(bars + slot * 8, (phase >> slot) & 1u, nullptr)) {
+                if (lane == 0) atomicCAS(&g_w4_error, 0, kErrBulkWait);
+                failed = true;  // go on without the weights: the other warps wait at the joins
+                for (int s = 0; s < sh.depth; ++s) mbar_wait(bars + s * 8, (phase >> s) & 1u, nullptr);
+            }
+            const uint8_t* q_box = ring_ptr + (size_t)(warp * sh.depth + slot) * kBoxBytes;
+            float acc[MT][NT][4];
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                uint32_t zero[2 * MT];
+                float scale[2 * MT];
+                if (b % GB == 0) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int c = 0; c < NT; ++c)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[m][c][i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * MT; ++i) {
+                    const int in_box = b / GB;
+                    const uint32_t v = GB == 8   ? sc[i][0]
+                                       : GB == 1 ? __shfl_sync(0xffffffffu, sc[i][in_box & (kPer - 1)], in_box >> 1, 4)
+                                                 : __shfl_sync(0xffffffffu, sc[i][0], in_box, 4);
+                    zero[i] = biased_zero<DT>(v & 0xFFu);
+                    scale[i] = scale_of<DT>(v);
+                }
+                uint4 xv[NT];
+#pragma unroll
+                for (int c = 0; c < NT; ++c) {
+                    xv[c] = make_uint4(0, 0, 0, 0);
+                    if (c * 8 + g < tokens) xv[c] = xs[((box * 8 + b) * tokens + c * 8 + g) * 4 + t];
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const uint8_t* at = q_box + (m * 16 + g) * 128 + ((b ^ g) * 16 + t * 4);
+                    const uint32_t lo = *reinterpret_cast<const uint32_t*>(at);
+                    const uint32_t hi = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t a[4] = {sub2<DT>(biased_pair<DT>(lo, 2 * h), zero[2 * m]),
+                                               sub2<DT>(biased_pair<DT>(hi, 2 * h), zero[2 * m + 1]),
+                                               sub2<DT>(biased_pair<DT>(lo, 2 * h + 1), zero[2 * m]),
+                                               sub2<DT>(biased_pair<DT>(hi, 2 * h + 1), zero[2 * m + 1])};
+#pragma unroll
+                        for (int c = 0; c < NT; ++c)
+                            mma_16816<DT>(acc[m][c], a, h ? xv[c].z : xv[c].x, h ? xv[c].w : xv[c].y);
+                    }
+                    if (b % GB == GB - 1) {
+#pragma unroll
+                        for (int c = 0; c < NT; ++c)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                sum[m][c][i] = fmaf(scale[2 * m + (i >> 1)], acc[m][c][i], sum[m][c][i]);
+                    }
+                }
+            }
+            __syncwarp();  // all threads have read the box
+            if (lane == 0 && !failed && ahead.tile < tile1) {
+                issue(ahead, slot);
+                advance(ahead);
+            }
+            phase ^= 1u << slot;
+            if (++slot == sh.depth) slot = 0;
+        }
+
+        // Join the wk partial sums of this row group's outputs.
+        float* mine = red + (size_t)(red_at * kWarps + warp) * (NT * 8 * kRows);
+        red_at ^= 1;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    mine[(c * 8 + 2 * t + (i & 1)) * kRows + m * 16 + (i >> 1) * 8 + g] = sum[m][c][i];
+        named_barrier(1 + rw, wk * 32);
+        const float* parts = mine - (size_t)kw * (NT * 8 * kRows);
+        const int n0 = (tile - q * tiles_n) * tile_n + rw * kRows;
+        for (int i = kw * 32 + lane; i < tokens * kRows; i += wk * 32) {
+            float v = 0.0f;
+            for (int w = 0; w < wk; ++w) v += parts[(size_t)w * (NT * 8 * kRows) + i];
+            const int n = n0 + i % kRows;
+            if (n < sh.n) out[(size_t)(row0 + i / kRows) * sh.n + n] = round16<DT>(v);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+template <int DT, int MT, int NT, int GB>
+static int launch_kernel(const CUtensorMap& tmQ, const void* x, const void* scales, const void* zeros,
+                         const int* offsets, void* out, Shape sh, int dev, cudaStream_t stream) {
+    static bool attr_set[64] = {};
+    constexpr size_t kMaxSmem = 225 * 1024;
+    if (dev >= 64 || !attr_set[dev]) {
+        TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, MT, NT, GB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)kMaxSmem));
+        if (dev < 64) attr_set[dev] = true;
+    }
+    const int num_box = (sh.k + kBoxK - 1) / kBoxK;
+    sh.wk = num_box >= 8 ? 8 : num_box >= 4 ? 4 : num_box >= 2 ? 2 : 1;
+    sh.tokens = std::min({sh.rows, NT * 8, 256 / num_box});
+    const size_t fixed = 1024 + (size_t)num_box * 512 * sh.tokens + 2 * kWarps * NT * 8 * 16 * MT * 4 +
+                         (size_t)(3 * sh.groups + 1) * 4;
+    const size_t slots = (size_t)kWarps * 16 * MT * 128;  // one box for each warp
+    int per_sm = 1;
+    if (NT == 1 && fixed + 4 * slots <= 112 * 1024) {
+        per_sm = 2;
+        sh.depth = 4;
+    } else {
+        sh.depth = (int)std::min<size_t>(8, (kMaxSmem - fixed) / slots);
+    }
+    const size_t smem = fixed + sh.depth * slots;
+    const int tile_n = kWarps / sh.wk * 16 * MT;
+    const int64_t tiles_n = (sh.n + tile_n - 1) / tile_n;
+    const int64_t tiles = tiles_n * ((int64_t)sh.rows / sh.tokens + std::min(sh.groups, sh.rows));
+    if (tiles > INT32_MAX) {
+        set_error("trb_gemv_w4_launch: too many tiles (rows=%d n=%d groups=%d)", sh.rows, sh.n, sh.groups);
+        return TRB_SKIPPED;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles, (int64_t)per_sm * device_sm_count(dev)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemv_w4_kernel<DT, MT, NT, GB>, tmQ, static_cast<const uint16_t*>(x),
+                                static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), offsets,
+                                static_cast<uint16_t*>(out), sh));
+    return TRB_OK;
+}
+
+template <int DT, int MT, int NT>
+static int launch_rows(const void* x, const void* q, const void* scales, const void* zeros, const int* offsets,
+                       void* out, const Shape& sh, int dev, cudaStream_t stream) {
+    CUtensorMap tmQ;
+    const uint64_t extent[3] = {(uint64_t)sh.k / 2, (uint64_t)sh.n, (uint64_t)sh.groups};
+    const uint32_t box[3] = {128, 16 * MT, 1};
+    const int rc = gemm::encode_tiled(&tmQ, q, 1, 3, extent, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != TRB_OK) return rc;
+    switch (sh.group_log2) {
+        case 5: return launch_kernel<DT, MT, NT, 1>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 6: return launch_kernel<DT, MT, NT, 2>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 7: return launch_kernel<DT, MT, NT, 4>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        default: return launch_kernel<DT, MT, NT, 8>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+    }
+}
+
+template <int DT>
+static int launch(const void* x, const void* q, const void* scales, const void* zeros, const int* offsets, void* out,
+                  const Shape& sh, int dev, cudaStream_t stream) {
+    // More than 8 rows a group on average: 16 rows at once read the weights half as often.
+    if (sh.rows > 8 * (int64_t)sh.groups) return launch_rows<DT, 2, 2>(x, q, scales, zeros, offsets, out, sh, dev, stream);
+    return launch_rows<DT, 1, 1>(x, q, scales, zeros, offsets, out, sh, dev, stream);
+}
+
+int read_error(bool clear) {
+    int v = 0;
+    TRB_CUDA(cudaMemcpyFromSymbol(&v, g_w4_error, sizeof(int)));
+    if (clear) {
+        const int zero = 0;
+        TRB_CUDA(cudaMemcpyToSymbol(g_w4_error, &zero, sizeof(int)));
+    }
+    return v;
+}
+
+}  // namespace w4
+}  // namespace trb
+
+extern "C" int trb_gemv_w4_launch(int dtype, int groups, int rows, int n, int k, int group_size, const void* x,
+                                  const void* q, const void* scales, const void* zeros, const int32_t* offsets,
+                                  void* out, void* stream) {
+    using namespace trb;
+    clear_error();
+    if (groups <= 0 || rows < 0 || n <= 0 || k <= 0 || q == nullptr || scales == nullptr ||
+        (rows > 0 && (x == nullptr || out == nullptr)) || (offsets == nullptr && groups != 1)) {
+        set_error("trb_gemv_w4_launch: sizes must be positive (rows may be 0), pointers non-null, and several groups "
+                  "need offsets");
+        return TRB_ERR_ARGS;
+    }
+    if (dtype != TRB_BFLOAT16 && dtype != TRB_FLOAT16) {
+        set_error("trb_gemv_w4_launch: unsupported dtype %s (bfloat16 and float16)", dtype_name(dtype));
+        return TRB_SKIPPED;
+    }
+    if (group_size < 32 || (group_size & (group_size - 1)) != 0 || k % group_size != 0) {
+        set_error("trb_gemv_w4_launch: the group size must be a power of two of at least 32 that divides k (group size "
+                  "%d, k %d)", group_size, k);
+        return TRB_SKIPPED;
+    }
+    if (k > 65536 || groups > kMaxGroups) {
+        set_error("trb_gemv_w4_launch: k at most 65536 and at most %d groups (k=%d groups=%d)", kMaxGroups, k, groups);
+        return TRB_SKIPPED;
+    }
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(q)) & 15u) != 0 ||
+        ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(out)) & 1u) != 0 ||
+        (reinterpret_cast<uintptr_t>(offsets) & 3u) != 0) {
+        set_error("trb_gemv_w4_launch: x and q must be 16-byte aligned, the others as their elements");
+        return TRB_ERR_ALIGN;
+    }
+    if (rows == 0) return TRB_OK;
+    int dev = 0;
+    TRB_CUDA(cudaGetDevice(&dev));
+    w4::Shape sh = {};
+    sh.groups = groups;
+    sh.rows = rows;
+    sh.n = n;
+    sh.k = k;
+    sh.k_groups = k / group_size;
+    while ((1 << sh.group_log2) < group_size) ++sh.group_log2;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == TRB_BFLOAT16 ? w4::launch<TRB_BFLOAT16>(x, q, scales, zeros, offsets, out, sh, dev, s)
+                                 : w4::launch<TRB_FLOAT16>(x, q, scales, zeros, offsets, out, sh, dev, s);
+}

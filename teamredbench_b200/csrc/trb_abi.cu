@@ -221,10 +221,12 @@ extern "C" int trb_device_error(int device_id, int clear) {
     const int e1 = hbm::read_error(clear != 0);
     const int e2 = gemm::read_error(clear != 0);
     const int e3 = grouped::read_error(clear != 0);
+    const int e4 = w4::read_error(clear != 0);
     if (e1 < 0) return e1;
     if (e2 < 0) return e2;
     if (e3 < 0) return e3;
-    return e1 ? e1 : e2 ? e2 : e3;
+    if (e4 < 0) return e4;
+    return e1 ? e1 : e2 ? e2 : e3 ? e3 : e4;
 }
 
 extern "C" int trb_hbm_run(const trb_hbm_args* args, trb_result* out) {

@@ -76,6 +76,10 @@ namespace grouped {
 int read_error(bool clear);
 }  // namespace grouped
 
+namespace w4 {
+int read_error(bool clear);
+}  // namespace w4
+
 namespace dgemm {
 // float64 C = A * B on the DMMA tensor path (no tcgen05 kind takes fp64); any m, n, k.
 int launch(int m, int n, int k, const void* a, const void* b, void* c, int b_kmajor, cudaStream_t stream,

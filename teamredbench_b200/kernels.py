@@ -182,3 +182,44 @@ def grouped_gemm_wgrad(a: Any, grad: Any, offsets: Any, out: Any, *, stream: Any
     _native.grouped_wgrad_launch(trb_dtype(a), groups, rows, n, k, a.data_ptr(), grad.data_ptr(), offsets.data_ptr(),
                                  out.data_ptr(), _stream_handle(a, stream))
     return out
+
+
+def gemv_w4(x: Any, q: Any, scales: Any, out: Any, *, zeros: Any | None = None, offsets: Any | None = None,
+            stream: Any | None = None) -> Any:
+    """out[r] = W[e] @ x[r] for the rows r of group (expert) e, with 4-bit weights
+    W[e, n, k] = (q[e, n, k] - zeros[e, n, k // g]) * scales[e, n, k // g].
+
+    x is (rows x k) and out (rows x n), bf16 or f16; q is uint8 (groups x n x k/2),
+    two weights a byte, the even k in the low four bits; scales (groups x n x k/g),
+    of x's dtype, sets the group size g (a power of two of at least 32); zeros is
+    uint8 of the same shape (values 0 to 15), or None for 8.  A single matrix may
+    be given without the leading dimension, and needs no offsets; otherwise
+    offsets are those of grouped_gemm.  Meant for few rows a group: their weights
+    are read once for each 8 or 16 rows.  k is at most 65536; n is free."""
+    _require_cuda_contiguous(x, q, scales, out, zeros, offsets)
+    _check_one_device(x, q, scales, out, zeros, offsets)
+    if x.dim() != 2 or q.dim() not in (2, 3):
+        raise ValueError(f"gemv_w4 takes a 2-D x and a 2-D or 3-D q, got {tuple(x.shape)} and {tuple(q.shape)}")
+    rows, k = x.shape
+    groups = q.shape[0] if q.dim() == 3 else 1
+    n = q.shape[-2]
+    if 2 * q.shape[-1] != k:
+        raise ValueError(f"q holds {2 * q.shape[-1]} weights a row for k = {k}")
+    if scales.shape[:-1] != q.shape[:-1] or scales.shape[-1] == 0 or k % scales.shape[-1]:
+        raise ValueError(f"scales must be {tuple(q.shape[:-1])} x a divisor of {k}, got {tuple(scales.shape)}")
+    if zeros is not None and zeros.shape != scales.shape:
+        raise ValueError(f"zeros must be {tuple(scales.shape)}, got {tuple(zeros.shape)}")
+    if out.shape != (rows, n):
+        raise ValueError(f"out must be {(rows, n)}, got {tuple(out.shape)}")
+    if scales.dtype != x.dtype or out.dtype != x.dtype:
+        raise ValueError("x, scales and out must share one dtype")
+    if str(q.dtype) != "torch.uint8" or (zeros is not None and zeros.dtype != q.dtype):
+        raise ValueError("q and zeros must be uint8")
+    if offsets is not None:
+        _check_offsets(offsets, groups)
+    elif groups != 1:
+        raise ValueError(f"{groups} groups need offsets")
+    _native.gemv_w4_launch(trb_dtype(x), groups, rows, n, k, k // scales.shape[-1], x.data_ptr(), q.data_ptr(),
+                           scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
+                           None if offsets is None else offsets.data_ptr(), out.data_ptr(), _stream_handle(x, stream))
+    return out

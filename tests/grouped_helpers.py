@@ -59,3 +59,21 @@ def wgrad(a, grad, offsets):
         ref[e] = a[lo:hi].double().T @ grad[lo:hi].double()
         mag[e] = a[lo:hi].double().abs().T @ grad[lo:hi].double().abs()
     return ref, mag
+
+
+def w4_operands(groups, n, k, group, dtype, seed, with_zeros):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randint(0, 256, (groups, n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = randn((groups, n, k // group), dtype, seed + 1, 0.05)
+    zeros = None
+    if with_zeros:
+        zeros = torch.randint(0, 16, scales.shape, generator=g, device="cuda", dtype=torch.uint8)
+    return q, scales, zeros
+
+
+def w4_weights(q, scales, zeros):
+    """The weights that q, scales and zeros stand for, in 64 bits."""
+    w = torch.stack([q & 15, q >> 4], -1).flatten(-2).double()
+    group = w.shape[-1] // scales.shape[-1]
+    z = 8.0 if zeros is None else zeros.double().repeat_interleave(group, -1)
+    return (w - z) * scales.double().repeat_interleave(group, -1)
