@@ -15,10 +15,10 @@
 // is exact too, so nothing is rounded before the product, and the scale is
 // applied in fp32 to each group's sum.
 //
-// Each warp streams its own boxes of 16 * MT outputs x 256 k (128 bytes of q a
-// row) through a private ring filled by TMA: no barrier between warps until
-// the sums of a tile are joined.  WK warps of a CTA share a tile's k, in a
-// fixed order of addition.
+// Each warp streams its own boxes of 16 outputs x 256 k (128 bytes of q a row)
+// through a private ring filled by TMA: no barrier between warps until the
+// sums of a tile are joined.  WK warps of a CTA share a tile's k, a contiguous
+// range each, and their sums are added in a fixed order.
 //
 // No counterpart in the reference.
 #include <cuda_bf16.h>
@@ -34,10 +34,13 @@ namespace w4 {
 
 __device__ int g_w4_error;
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 16;    // outputs of a box
 constexpr int kBoxK = 256;   // k of a box: one 128-byte swizzle row
 constexpr int kBlockK = 32;  // k of a block: 16 bytes a row, two products
+constexpr uint32_t kBoxBytes = kRows * 128;
+constexpr int kMaxDepth = 8;
 
 struct Shape {
     int groups, rows, n, k;
@@ -46,6 +49,8 @@ struct Shape {
     int wk;          // warps that share a tile's k
     int depth;       // boxes in each warp's ring
     int tokens;      // rows of x taken at once
+    int red_rows;    // tokens, as the join's buffer counts them
+    int vector_scales;  // scales and zero points may be read kHeld at a time
 };
 
 template <int DT>
@@ -70,10 +75,14 @@ __device__ __forceinline__ uint32_t biased_pair(uint32_t w, int p) {
     if constexpr (DT == TRB_BFLOAT16) return ((w >> (4 * p)) & 0x000F000Fu) | 0x43004300u;
     else return ((p == 0 ? w << 4 : w >> (4 * (p - 1))) & 0x00F000F0u) | 0x54005400u;
 }
+// Byte i of four zero points (stored by zero_bytes) as two equal 16-bit floats, plus the same 128 or 64.
 template <int DT>
-__device__ __forceinline__ uint32_t biased_zero(uint32_t z) {
-    if constexpr (DT == TRB_BFLOAT16) return 0x43004300u + z * 0x00010001u;
-    else return 0x54005400u + z * 0x00100010u;
+__device__ __forceinline__ uint32_t zero_bytes(uint32_t z) {
+    return DT == TRB_BFLOAT16 ? z & 0x0F0F0F0Fu : (z & 0x0F0F0F0Fu) << 4;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t biased_zero(uint32_t bytes, int i) {
+    return __byte_perm(bytes, DT == TRB_BFLOAT16 ? 0x43u : 0x54u, 0x4040u + 0x0101u * (uint32_t)i);
 }
 template <int DT>
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
@@ -86,9 +95,9 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
     }
 }
 template <int DT>
-__device__ __forceinline__ float scale_of(uint32_t packed) {  // scale in the upper 16 bits
-    if constexpr (DT == TRB_BFLOAT16) return __uint_as_float(packed & 0xFFFF0000u);
-    else return __half2float(__ushort_as_half((unsigned short)(packed >> 16)));
+__device__ __forceinline__ float scale_of(uint32_t pair, int i) {  // the lower or upper 16 bits
+    if constexpr (DT == TRB_BFLOAT16) return __uint_as_float(i ? pair & 0xFFFF0000u : pair << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(i ? pair >> 16 : pair & 0xFFFFu)));
 }
 template <int DT>
 __device__ __forceinline__ uint16_t round16(float v) {
@@ -96,21 +105,20 @@ __device__ __forceinline__ uint16_t round16(float v) {
     else return __half_as_ushort(__float2half_rn(v));
 }
 
-// A place in a warp's stream of boxes.
+// A place in a warp's stream of boxes: tile tile_n of chunk q (group e), box box.
 struct Cursor {
-    int tile, box, e, n0;
+    int tile, q, tile_n, e, box;
 };
 
-// MT * 16 outputs x NT * 8 rows of x per warp; a group of k spans GB blocks (8: a box or more).
-template <int DT, int MT, int NT, int GB>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+// NT * 8 rows of x at once; a group of k spans GB blocks (8: a box or more); Z: zero points given.
+template <int DT, int NT, int GB, bool Z>
+__global__ void __launch_bounds__(kThreads, 1)
     gemv_w4_kernel(const __grid_constant__ CUtensorMap tmQ, const uint16_t* __restrict__ x,
                    const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros,
                    const int* __restrict__ offsets, uint16_t* __restrict__ out, const Shape sh) {
-    constexpr int kRows = 16 * MT;              // outputs of a warp's box
-    constexpr uint32_t kBoxBytes = kRows * 128;
-    constexpr int kPer = GB == 1 ? 2 : 1;       // groups whose scale a thread holds, per output
-    constexpr int kMaxDepth = 8;
+    // Scales travel in units: the groups of kUnit boxes of each output, kHeld of them in each of its four threads.
+    constexpr int kUnit = GB == 1 ? 2 : 4;
+    constexpr int kHeld = GB <= 2 ? 4 : GB == 4 ? 2 : 1;
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kWarps * kMaxDepth];
@@ -119,17 +127,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int num_box = (sh.k + kBoxK - 1) / kBoxK;
-    const int wk = sh.wk, wr = kWarps / wk;
-    const int kw = warp % wk, rw = warp / wk;
-    const int tile_n = wr * kRows;
-    const int tiles_n = (sh.n + tile_n - 1) / tile_n;
+    const int kw = warp & (sh.wk - 1), rw = warp / sh.wk;
+    const int box0 = num_box * kw / sh.wk, box1 = num_box * (kw + 1) / sh.wk;
+    const int tile_rows = kWarps / sh.wk * kRows;
+    const int tiles_n = (sh.n + tile_rows - 1) / tile_rows;
 
     uint8_t* ring_ptr = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint4* xs = reinterpret_cast<uint4*>(ring_ptr + (size_t)kWarps * sh.depth * kBoxBytes);
     float* red = reinterpret_cast<float*>(xs + (size_t)num_box * 8 * sh.tokens * 4);
-    int* words = reinterpret_cast<int*>(red + 2 * kWarps * NT * 8 * kRows);
+    int* words = reinterpret_cast<int*>(red + kWarps * sh.red_rows * kRows);
     const GroupTable table = {words, words + sh.groups, words + 2 * sh.groups};
-    const uint32_t ring = smem_u32(ring_ptr) + (uint32_t)(warp * sh.depth) * kBoxBytes;
+    ring_ptr += (size_t)(warp * sh.depth) * kBoxBytes;
     const uint32_t bars = smem_u32(&full_bar[warp * kMaxDepth]);
 
     if (lane == 0) {
@@ -154,214 +162,236 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     const int64_t total = (int64_t)table.chunk0[groups] * tiles_n;
     const int tile0 = (int)(total * blockIdx.x / gridDim.x);
     const int tile1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+    if (tile0 >= tile1) return;
 
-    auto enter = [&](Cursor& c) {  // the first box at or after c.tile that is this warp's
-        for (; c.tile < tile1; ++c.tile) {
-            const int q = c.tile / tiles_n;
-            c.n0 = (c.tile - q * tiles_n) * tile_n + rw * kRows;
-            if (c.n0 < sh.n) {
-                c.e = group_of_chunk(q, groups, table);
-                c.box = kw;
-                return;
-            }
+    auto row_of = [&](const Cursor& c) { return c.tile_n * tile_rows + rw * kRows; };
+    auto next_tile = [&](Cursor& c) {
+        c.box = box0;
+        ++c.tile;
+        if (++c.tile_n == tiles_n) {
+            c.tile_n = 0;
+            ++c.q;
+            if (c.tile < tile1) c.e = group_of_chunk(c.q, groups, table);
         }
     };
-    auto advance = [&](Cursor& c) {
-        c.box += wk;
-        if (c.box >= num_box) {
-            ++c.tile;
-            enter(c);
-        }
+    // On to the next box (step boxes) whose outputs exist.
+    auto settle = [&](Cursor& c) {
+        while (c.tile < tile1 && (c.box >= box1 || row_of(c) >= sh.n)) next_tile(c);
     };
     auto issue = [&](const Cursor& c, int slot) {
         mbar_arrive_expect_tx(bars + slot * 8, kBoxBytes);
-        tma_load_3d(ring + slot * kBoxBytes, &tmQ, bars + slot * 8, c.box * 128, c.n0, c.e);
+        tma_load_3d(smem_u32(ring_ptr) + slot * kBoxBytes, &tmQ, bars + slot * 8, c.box * 128, row_of(c), c.e);
     };
-    // Scales (upper half) and zero points (lower) of a box, spread over the four threads of an output.
-    auto load_scales = [&](const Cursor& c, uint32_t (&sc)[2 * MT][kPer]) {
+    // Scales and zero points of the unit that begins at box c.box, for outputs g and g + 8.
+    auto load_unit = [&](const Cursor& c, uint32_t (&sc)[2][(kHeld + 1) / 2], uint32_t (&zr)[2]) {
+        const int kg = GB == 1   ? c.box * 8 + 4 * t
+                       : GB == 2 ? (c.box + t) * 4
+                       : GB == 4 ? (c.box + t) * 2
+                                 : ((c.box + t) * kBoxK) >> sh.group_log2;
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            const int row = c.n0 + i * 8 + g;
+        for (int i = 0; i < 2; ++i) {
+            const int row = row_of(c) + i * 8 + g;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int in_box = GB == 1 ? 2 * t + j : GB == 2 ? t : GB == 4 ? (t & 1) : 0;
-                const int kg = GB == 8 ? (c.box * kBoxK) >> sh.group_log2 : c.box * (8 / GB) + in_box;
-                sc[i][j] = 8;
-                if (c.tile < tile1 && row < sh.n && kg < sh.k_groups) {
-                    const size_t at = ((size_t)c.e * sh.n + row) * sh.k_groups + kg;
-                    sc[i][j] = (uint32_t)scales[at] << 16 | (zeros != nullptr ? zeros[at] & 15u : 8u);
+            for (int j = 0; j < (kHeld + 1) / 2; ++j) sc[i][j] = 0;
+            if constexpr (Z) zr[i] = 0;
+            if (c.tile >= tile1 || row >= sh.n || kg >= sh.k_groups) continue;
+            const size_t at = ((size_t)c.e * sh.n + row) * sh.k_groups + kg;
+            if (kHeld == 1) {
+                sc[i][0] = scales[at];
+                if constexpr (Z) zr[i] = zeros[at];
+            } else if (sh.vector_scales) {  // k_groups is a multiple of kHeld
+                if constexpr (kHeld == 4) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(scales + at);
+                    sc[i][0] = v.x;
+                    sc[i][1] = v.y;
+                    if constexpr (Z) zr[i] = *reinterpret_cast<const uint32_t*>(zeros + at);
+                } else if constexpr (kHeld == 2) {
+                    sc[i][0] = *reinterpret_cast<const uint32_t*>(scales + at);
+                    if constexpr (Z) zr[i] = *reinterpret_cast<const uint16_t*>(zeros + at);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kHeld; ++j) {
+                    if (kg + j >= sh.k_groups) break;
+                    sc[i][j >> 1] |= (uint32_t)scales[at + j] << (16 * (j & 1));
+                    if constexpr (Z) zr[i] |= (uint32_t)zeros[at + j] << (8 * j);
                 }
             }
         }
     };
 
-    Cursor ahead = {tile0, 0, 0, 0};  // the next box to request
-    enter(ahead);
+    Cursor next = {tile0, tile0 / tiles_n, tile0 % tiles_n, 0, box0};  // the next unit of scales
+    next.e = group_of_chunk(next.q, groups, table);
+    settle(next);
+    Cursor ahead = next;  // lane 0: the next box to request
     if (lane == 0) {
-        Cursor c = ahead;
-        for (int s = 0; s < sh.depth && c.tile < tile1; ++s, advance(c)) issue(c, s);
-        ahead = c;
+        for (int s = 0; s < sh.depth && ahead.tile < tile1; ++s) {
+            issue(ahead, s);
+            ++ahead.box;
+            settle(ahead);
+        }
     }
-    Cursor next = {tile0, 0, 0, 0};  // the next box to multiply
-    enter(next);
-    uint32_t sc_next[2 * MT][kPer];
-    load_scales(next, sc_next);
+    uint32_t sc_next[2][(kHeld + 1) / 2], zr_next[2];
+    load_unit(next, sc_next, zr_next);
 
-    int slot = 0, chunk = -1, red_at = 0;
+    Cursor now = {tile0, tile0 / tiles_n, tile0 % tiles_n, 0, box0};
+    int slot = 0, chunk = -1;
     uint32_t phase = 0;
     int tokens = 0, row0 = 0;
     bool failed = false;
-    for (int tile = tile0; tile < tile1; ++tile) {
-        const int q = tile / tiles_n;
-        if (q != chunk) {  // other rows of x: in shared memory, [block of 32 k][row][t]: the 8 values of thread t
-            chunk = q;     // in the order the pairs of a word of q come in
-            const int e = group_of_chunk(q, groups, table);
-            const int first = (q - table.chunk0[e]) * sh.tokens;
+    for (; now.tile < tile1; next_tile(now)) {
+        if (now.q != chunk) {  // other rows of x: in shared memory, [block of 32 k][row][t]: the 8 values of thread t
+            chunk = now.q;     // in the order the pairs of a word of q come in
+            const int e = group_of_chunk(chunk, groups, table);
+            const int first = (chunk - table.chunk0[e]) * sh.tokens;
             row0 = table.start[e] + first;
             tokens = min(sh.tokens, table.rows[e] - first);
             __syncthreads();
-            for (int i = threadIdx.x; i < num_box * 8 * tokens * 4; i += kThreads) {
-                const int c = (i >> 2) % tokens, k0 = ((i >> 2) / tokens) * kBlockK + (i & 3) * 8;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (k0 < sh.k) v = *reinterpret_cast<const uint4*>(x + (size_t)(row0 + c) * sh.k + k0);
-                xs[i] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+            for (int c = 0; c < tokens; ++c)
+                for (int j = threadIdx.x; j < num_box * 32; j += kThreads) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (j * 8 < sh.k) v = *reinterpret_cast<const uint4*>(x + (size_t)(row0 + c) * sh.k + j * 8);
+                    xs[((j >> 2) * tokens + c) * 4 + (j & 3)] =
+                        make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                                    __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-            }
+                }
             __syncthreads();
         }
-        float sum[MT][NT][4];
+        float sum[NT][4];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int c = 0; c < NT; ++c)
 #pragma unroll
-            for (int c = 0; c < NT; ++c)
+            for (int i = 0; i < 4; ++i) sum[c][i] = 0.0f;
+        // Columns of the products past the last row of x are computed from that row and not used.
+        const uint4* x_lane[NT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[m][c][i] = 0.0f;
+        for (int c = 0; c < NT; ++c) x_lane[c] = xs + min(c * 8 + g, tokens - 1) * 4 + t;
 
-        while (next.tile == tile) {
-            uint32_t sc[2 * MT][kPer];
+        const int n0 = row_of(now);
+        for (int unit = n0 < sh.n ? box0 : box1; unit < box1; unit += kUnit) {
+            uint32_t sc[2][(kHeld + 1) / 2], zr[2];
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i)
+            for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) sc[i][j] = sc_next[i][j];
-            const int box = next.box;
-            advance(next);
-            load_scales(next, sc_next);
-            if (!failed && !mbar_wait(bars + slot * 8, (phase >> slot) & 1u, nullptr)) {
-                if (lane == 0) atomicCAS(&g_w4_error, 0, kErrBulkWait);
-                failed = true;  // go on without the weights: the other warps wait at the joins
-                for (int s = 0; s < sh.depth; ++s) mbar_wait(bars + s * 8, (phase >> s) & 1u, nullptr);
+                for (int j = 0; j < (kHeld + 1) / 2; ++j) sc[i][j] = sc_next[i][j];
+                zr[i] = Z ? zero_bytes<DT>(zr_next[i]) : 0;
             }
-            const uint8_t* q_box = ring_ptr + (size_t)(warp * sh.depth + slot) * kBoxBytes;
-            float acc[MT][NT][4];
+            next.box += kUnit;
+            settle(next);
+            load_unit(next, sc_next, zr_next);
+            for (int in_unit = 0; in_unit < kUnit && unit + in_unit < box1; ++in_unit) {
+                if (!failed && !mbar_wait(bars + slot * 8, (phase >> slot) & 1u, nullptr)) {
+                    if (lane == 0) atomicCAS(&g_w4_error, 0, kErrBulkWait);
+                    failed = true;  // go on without the weights: the other warps wait at the joins
+                    for (int s = 0; s < sh.depth; ++s) mbar_wait(bars + s * 8, (phase >> s) & 1u, nullptr);
+                }
+                const uint8_t* q_lane = ring_ptr + slot * kBoxBytes + g * 128 + t * 4;
+                const int x_box = (unit + in_unit) * 8 * tokens * 4;
+                float acc[NT][4];
+                uint32_t pair[2], zero[2], zw[2];
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                uint32_t zero[2 * MT];
-                float scale[2 * MT];
-                if (b % GB == 0) {
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
+                for (int b = 0; b < 8; ++b) {
+                    if (b % GB == 0) {
+                        const int src = GB == 1 ? in_unit * 2 + (b >> 2) : in_unit;
+                        const int held = GB == 8 ? 0 : (b / GB) % kHeld;
 #pragma unroll
                         for (int c = 0; c < NT; ++c)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[m][c][i] = 0.0f;
-                }
+                            for (int i = 0; i < 4; ++i) acc[c][i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 2 * MT; ++i) {
-                    const int in_box = b / GB;
-                    const uint32_t v = GB == 8   ? sc[i][0]
-                                       : GB == 1 ? __shfl_sync(0xffffffffu, sc[i][in_box & (kPer - 1)], in_box >> 1, 4)
-                                                 : __shfl_sync(0xffffffffu, sc[i][0], in_box, 4);
-                    zero[i] = biased_zero<DT>(v & 0xFFu);
-                    scale[i] = scale_of<DT>(v);
-                }
-                uint4 xv[NT];
+                        for (int i = 0; i < 2; ++i) {
+                            if (held % 2 == 0) pair[i] = __shfl_sync(0xffffffffu, sc[i][held >> 1], src, 4);
+                            if constexpr (Z) {
+                                if (held == 0) zw[i] = __shfl_sync(0xffffffffu, zr[i], src, 4);
+                                zero[i] = biased_zero<DT>(zw[i], held);
+                            } else {
+                                zero[i] = DT == TRB_BFLOAT16 ? 0x43084308u : 0x54805480u;  // 128 + 8, 64 + 8
+                            }
+                        }
+                    }
+                    uint4 xv[NT];
 #pragma unroll
-                for (int c = 0; c < NT; ++c) {
-                    xv[c] = make_uint4(0, 0, 0, 0);
-                    if (c * 8 + g < tokens) xv[c] = xs[((box * 8 + b) * tokens + c * 8 + g) * 4 + t];
-                }
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const uint8_t* at = q_box + (m * 16 + g) * 128 + ((b ^ g) * 16 + t * 4);
+                    for (int c = 0; c < NT; ++c) xv[c] = x_lane[c][x_box + b * tokens * 4];
+                    const uint8_t* at = q_lane + ((b ^ g) * 16);
                     const uint32_t lo = *reinterpret_cast<const uint32_t*>(at);
                     const uint32_t hi = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t a[4] = {sub2<DT>(biased_pair<DT>(lo, 2 * h), zero[2 * m]),
-                                               sub2<DT>(biased_pair<DT>(hi, 2 * h), zero[2 * m + 1]),
-                                               sub2<DT>(biased_pair<DT>(lo, 2 * h + 1), zero[2 * m]),
-                                               sub2<DT>(biased_pair<DT>(hi, 2 * h + 1), zero[2 * m + 1])};
+                        const uint32_t a[4] = {sub2<DT>(biased_pair<DT>(lo, 2 * h), zero[0]),
+                                               sub2<DT>(biased_pair<DT>(hi, 2 * h), zero[1]),
+                                               sub2<DT>(biased_pair<DT>(lo, 2 * h + 1), zero[0]),
+                                               sub2<DT>(biased_pair<DT>(hi, 2 * h + 1), zero[1])};
 #pragma unroll
                         for (int c = 0; c < NT; ++c)
-                            mma_16816<DT>(acc[m][c], a, h ? xv[c].z : xv[c].x, h ? xv[c].w : xv[c].y);
+                            mma_16816<DT>(acc[c], a, h ? xv[c].z : xv[c].x, h ? xv[c].w : xv[c].y);
                     }
                     if (b % GB == GB - 1) {
+                        const int held = GB == 8 ? 0 : (b / GB) % kHeld;
+                        const float s0 = scale_of<DT>(pair[0], held & 1), s1 = scale_of<DT>(pair[1], held & 1);
 #pragma unroll
                         for (int c = 0; c < NT; ++c)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                sum[m][c][i] = fmaf(scale[2 * m + (i >> 1)], acc[m][c][i], sum[m][c][i]);
+                            for (int i = 0; i < 4; ++i) sum[c][i] = fmaf(i < 2 ? s0 : s1, acc[c][i], sum[c][i]);
                     }
                 }
+                __syncwarp();  // all threads have read the box
+                if (lane == 0 && !failed && ahead.tile < tile1) {
+                    issue(ahead, slot);
+                    ++ahead.box;
+                    settle(ahead);
+                }
+                phase ^= 1u << slot;
+                if (++slot == sh.depth) slot = 0;
             }
-            __syncwarp();  // all threads have read the box
-            if (lane == 0 && !failed && ahead.tile < tile1) {
-                issue(ahead, slot);
-                advance(ahead);
-            }
-            phase ^= 1u << slot;
-            if (++slot == sh.depth) slot = 0;
         }
 
         // Join the wk partial sums of this row group's outputs.
-        float* mine = red + (size_t)(red_at * kWarps + warp) * (NT * 8 * kRows);
-        red_at ^= 1;
+        float* mine = red + (size_t)warp * sh.red_rows * kRows;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int c = 0; c < NT; ++c)
 #pragma unroll
-            for (int c = 0; c < NT; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    mine[(c * 8 + 2 * t + (i & 1)) * kRows + m * 16 + (i >> 1) * 8 + g] = sum[m][c][i];
-        named_barrier(1 + rw, wk * 32);
-        const float* parts = mine - (size_t)kw * (NT * 8 * kRows);
-        const int n0 = (tile - q * tiles_n) * tile_n + rw * kRows;
-        for (int i = kw * 32 + lane; i < tokens * kRows; i += wk * 32) {
+            for (int i = 0; i < 4; ++i) {
+                const int row = c * 8 + 2 * t + (i & 1);
+                if (row < tokens) mine[row * kRows + (i >> 1) * 8 + g] = sum[c][i];
+            }
+        named_barrier(1 + rw, sh.wk * 32);
+        const float* parts = red + (size_t)(warp - kw) * sh.red_rows * kRows;
+        for (int i = kw * 32 + lane; i < tokens * kRows; i += sh.wk * 32) {
             float v = 0.0f;
-            for (int w = 0; w < wk; ++w) v += parts[(size_t)w * (NT * 8 * kRows) + i];
+            for (int w = 0; w < sh.wk; ++w) v += parts[w * sh.red_rows * kRows + i];
             const int n = n0 + i % kRows;
             if (n < sh.n) out[(size_t)(row0 + i / kRows) * sh.n + n] = round16<DT>(v);
         }
+        named_barrier(1 + rw, sh.wk * 32);
     }
 }
 
 // ------------------------------------------------------------------ host side
-template <int DT, int MT, int NT, int GB>
+template <int DT, int NT, int GB, bool Z>
 static int launch_kernel(const CUtensorMap& tmQ, const void* x, const void* scales, const void* zeros,
                          const int* offsets, void* out, Shape sh, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
-    constexpr size_t kMaxSmem = 225 * 1024;
+    constexpr size_t kMaxSmem = 226 * 1024;
     if (dev >= 64 || !attr_set[dev]) {
-        TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, MT, NT, GB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, NT, GB, Z>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)kMaxSmem));
         if (dev < 64) attr_set[dev] = true;
     }
     const int num_box = (sh.k + kBoxK - 1) / kBoxK;
-    sh.wk = num_box >= 8 ? 8 : num_box >= 4 ? 4 : num_box >= 2 ? 2 : 1;
-    sh.tokens = std::min({sh.rows, NT * 8, 256 / num_box});
-    const size_t fixed = 1024 + (size_t)num_box * 512 * sh.tokens + 2 * kWarps * NT * 8 * 16 * MT * 4 +
+    sh.wk = 1;
+    while (sh.wk < kWarps && sh.wk * 2 <= num_box) sh.wk *= 2;
+    sh.tokens = std::min({sh.rows, NT * 8, 256 / num_box});  // x takes at most 128 KiB
+    sh.red_rows = sh.tokens;
+    constexpr int kHeld = GB <= 2 ? 4 : GB == 4 ? 2 : 1;
+    sh.vector_scales = sh.k_groups % kHeld == 0 && reinterpret_cast<uintptr_t>(scales) % (2 * kHeld) == 0 &&
+                       reinterpret_cast<uintptr_t>(zeros) % kHeld == 0;
+    const size_t fixed = 1024 + (size_t)num_box * 512 * sh.tokens + (size_t)kWarps * sh.red_rows * kRows * 4 +
                          (size_t)(3 * sh.groups + 1) * 4;
-    const size_t slots = (size_t)kWarps * 16 * MT * 128;  // one box for each warp
-    int per_sm = 1;
-    if (NT == 1 && fixed + 4 * slots <= 112 * 1024) {
-        per_sm = 2;
-        sh.depth = 4;
-    } else {
-        sh.depth = (int)std::min<size_t>(8, (kMaxSmem - fixed) / slots);
-    }
+    const size_t slots = (size_t)kWarps * kBoxBytes;  // one box for each warp
+    sh.depth = (int)std::min<size_t>(4, (kMaxSmem - fixed) / slots);
     const size_t smem = fixed + sh.depth * slots;
-    const int tile_n = kWarps / sh.wk * 16 * MT;
-    const int64_t tiles_n = (sh.n + tile_n - 1) / tile_n;
+    const int tile_rows = kWarps / sh.wk * kRows;
+    const int64_t tiles_n = (sh.n + tile_rows - 1) / tile_rows;
     const int64_t tiles = tiles_n * ((int64_t)sh.rows / sh.tokens + std::min(sh.groups, sh.rows));
     if (tiles > INT32_MAX) {
         set_error("trb_gemv_w4_launch: too many tiles (rows=%d n=%d groups=%d)", sh.rows, sh.n, sh.groups);
@@ -371,31 +401,31 @@ static int launch_kernel(const CUtensorMap& tmQ, const void* x, const void* scal
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles, (int64_t)per_sm * device_sm_count(dev)));
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles, device_sm_count(dev)));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemv_w4_kernel<DT, MT, NT, GB>, tmQ, static_cast<const uint16_t*>(x),
+    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemv_w4_kernel<DT, NT, GB, Z>, tmQ, static_cast<const uint16_t*>(x),
                                 static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), offsets,
                                 static_cast<uint16_t*>(out), sh));
     return TRB_OK;
 }
 
-template <int DT, int MT, int NT>
-static int launch_rows(const void* x, const void* q, const void* scales, const void* zeros, const int* offsets,
-                       void* out, const Shape& sh, int dev, cudaStream_t stream) {
+template <int DT, int NT, bool Z>
+static int launch_group(const void* x, const void* q, const void* scales, const void* zeros, const int* offsets,
+                        void* out, const Shape& sh, int dev, cudaStream_t stream) {
     CUtensorMap tmQ;
     const uint64_t extent[3] = {(uint64_t)sh.k / 2, (uint64_t)sh.n, (uint64_t)sh.groups};
-    const uint32_t box[3] = {128, 16 * MT, 1};
+    const uint32_t box[3] = {128, kRows, 1};
     const int rc = gemm::encode_tiled(&tmQ, q, 1, 3, extent, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
     switch (sh.group_log2) {
-        case 5: return launch_kernel<DT, MT, NT, 1>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        case 6: return launch_kernel<DT, MT, NT, 2>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        case 7: return launch_kernel<DT, MT, NT, 4>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        default: return launch_kernel<DT, MT, NT, 8>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 5: return launch_kernel<DT, NT, 1, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 6: return launch_kernel<DT, NT, 2, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 7: return launch_kernel<DT, NT, 4, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        default: return launch_kernel<DT, NT, 8, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
     }
 }
 
@@ -403,8 +433,11 @@ template <int DT>
 static int launch(const void* x, const void* q, const void* scales, const void* zeros, const int* offsets, void* out,
                   const Shape& sh, int dev, cudaStream_t stream) {
     // More than 8 rows a group on average: 16 rows at once read the weights half as often.
-    if (sh.rows > 8 * (int64_t)sh.groups) return launch_rows<DT, 2, 2>(x, q, scales, zeros, offsets, out, sh, dev, stream);
-    return launch_rows<DT, 1, 1>(x, q, scales, zeros, offsets, out, sh, dev, stream);
+    if (sh.rows > 8 * (int64_t)sh.groups)
+        return zeros ? launch_group<DT, 2, true>(x, q, scales, zeros, offsets, out, sh, dev, stream)
+                     : launch_group<DT, 2, false>(x, q, scales, zeros, offsets, out, sh, dev, stream);
+    return zeros ? launch_group<DT, 1, true>(x, q, scales, zeros, offsets, out, sh, dev, stream)
+                 : launch_group<DT, 1, false>(x, q, scales, zeros, offsets, out, sh, dev, stream);
 }
 
 int read_error(bool clear) {
