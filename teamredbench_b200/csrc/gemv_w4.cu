@@ -15,10 +15,13 @@
 // is exact too, so nothing is rounded before the product, and the scale is
 // applied in fp32 to each group's sum.
 //
-// Each warp streams its own boxes of 16 outputs x 256 k (128 bytes of q a row)
-// through a private ring filled by TMA: no barrier between warps until the
-// sums of a tile are joined.  WK warps of a CTA share a tile's k, a contiguous
-// range each, and their sums are added in a fixed order.
+// A CTA takes rows of 16 outputs of one group in jobs.  The boxes of a job (16
+// outputs x 256 k, 128 bytes of q a row) are one sequence, cut evenly among the
+// 16 warps, so a warp works through neighbouring boxes of one or two rows
+// whatever k is, with nothing to wait for but its own boxes: they come by TMA
+// through a private ring.  What a warp has summed of a row goes to shared
+// memory when it leaves the row, and at the job's end the parts of each row are
+// added in the order of k.
 //
 // No counterpart in the reference.
 #include <cuda_bf16.h>
@@ -42,14 +45,14 @@ constexpr int kBlockK = 32;  // k of a block: 16 bytes a row, two products
 constexpr uint32_t kBoxBytes = kRows * 128;
 constexpr int kMaxDepth = 8;
 
+constexpr int kJobRows = 16;  // rows of 16 outputs in a job, at most
+
 struct Shape {
     int groups, rows, n, k;
-    int k_groups;    // scales per output
+    int k_groups;       // scales per output
     int group_log2;
-    int wk;          // warps that share a tile's k
-    int depth;       // boxes in each warp's ring
-    int tokens;      // rows of x taken at once
-    int red_rows;    // tokens, as the join's buffer counts them
+    int depth;          // boxes in each warp's ring
+    int tokens;         // rows of x taken at once
     int vector_scales;  // scales and zero points may be read kHeld at a time
 };
 
@@ -105,9 +108,16 @@ __device__ __forceinline__ uint16_t round16(float v) {
     else return __half_as_ushort(__float2half_rn(v));
 }
 
-// A place in a warp's stream of boxes: tile tile_n of chunk q (group e), box box.
+// Rows of 16 outputs [row, row + rows) of group e for the rows of x in chunk q.
+struct Job {
+    int first;  // in the count of all rows of outputs of all chunks
+    int rows, row, q, e;
+};
+
+// A warp's place in its share of a job: box `box` of row `row` of the job, `left` boxes to go.
 struct Cursor {
-    int tile, q, tile_n, e, box;
+    Job job;
+    int row, box, left;
 };
 
 // NT * 8 rows of x at once; a group of k spans GB blocks (8: a box or more); Z: zero points given.
@@ -127,17 +137,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int num_box = (sh.k + kBoxK - 1) / kBoxK;
-    const int kw = warp & (sh.wk - 1), rw = warp / sh.wk;
-    const int box0 = num_box * kw / sh.wk, box1 = num_box * (kw + 1) / sh.wk;
-    const int tile_rows = kWarps / sh.wk * kRows;
-    const int tiles_n = (sh.n + tile_rows - 1) / tile_rows;
+    const int rows_n = (sh.n + kRows - 1) / kRows;
 
-    uint8_t* ring_ptr = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint4* xs = reinterpret_cast<uint4*>(ring_ptr + (size_t)kWarps * sh.depth * kBoxBytes);
-    float* red = reinterpret_cast<float*>(xs + (size_t)num_box * 8 * sh.tokens * 4);
-    int* words = reinterpret_cast<int*>(red + kWarps * sh.red_rows * kRows);
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t ring = (uint32_t)(warp * sh.depth) * kBoxBytes;             // offsets into smem
+    const uint32_t xs = (uint32_t)(kWarps * sh.depth) * kBoxBytes;
+    float* red = reinterpret_cast<float*>(smem + xs + (size_t)num_box * 512 * sh.tokens);
+    const int part = sh.tokens * kRows;                                        // one warp's sums of a row
+    int* words = reinterpret_cast<int*>(red + (kWarps + kJobRows) * part);
     const GroupTable table = {words, words + sh.groups, words + 2 * sh.groups};
-    ring_ptr += (size_t)(warp * sh.depth) * kBoxBytes;
+    const uint32_t ring_addr = smem_u32(smem) + ring;
     const uint32_t bars = smem_u32(&full_bar[warp * kMaxDepth]);
 
     if (lane == 0) {
@@ -158,29 +167,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) scan_chunks(groups, sh.tokens, table, lane);
     __syncthreads();
 
-    // This CTA's share of the tiles, contiguous so that x stays in shared memory.
-    const int64_t total = (int64_t)table.chunk0[groups] * tiles_n;
-    const int tile0 = (int)(total * blockIdx.x / gridDim.x);
-    const int tile1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
-    if (tile0 >= tile1) return;
-
-    auto row_of = [&](const Cursor& c) { return c.tile_n * tile_rows + rw * kRows; };
-    auto next_tile = [&](Cursor& c) {
-        c.box = box0;
-        ++c.tile;
-        if (++c.tile_n == tiles_n) {
-            c.tile_n = 0;
-            ++c.q;
-            if (c.tile < tile1) c.e = group_of_chunk(c.q, groups, table);
+    // This CTA's share of the rows of outputs, contiguous so that x stays in shared memory.
+    const int64_t total = (int64_t)table.chunk0[groups] * rows_n;
+    const int end = (int)(total * (blockIdx.x + 1) / gridDim.x);
+    auto job_at = [&](int first) {
+        Job j;
+        j.first = first;
+        j.q = first / rows_n;
+        j.row = first - j.q * rows_n;
+        j.rows = min(min(end - first, rows_n - j.row), kJobRows);
+        j.e = first < end ? group_of_chunk(j.q, groups, table) : 0;
+        return j;
+    };
+    auto first_box = [&](const Job& j, int w) { return j.rows * num_box * w / kWarps; };
+    // A warp's share of jobs from c.job on: at the first box of the first job in which it has one.
+    auto enter = [&](Cursor& c) {
+        while (c.job.first < end) {
+            const int p = first_box(c.job, warp);
+            c.left = first_box(c.job, warp + 1) - p;
+            c.row = p / num_box;
+            c.box = p - c.row * num_box;
+            if (c.left > 0) return;
+            c.job = job_at(c.job.first + c.job.rows);
+        }
+        c.left = 0;
+    };
+    auto step = [&](Cursor& c, int boxes) {  // within a row
+        c.box += boxes;
+        c.left -= boxes;
+        if (c.left == 0) {
+            c.job = job_at(c.job.first + c.job.rows);
+            enter(c);
+        } else if (c.box == num_box) {
+            c.box = 0;
+            ++c.row;
         }
     };
-    // On to the next box (step boxes) whose outputs exist.
-    auto settle = [&](Cursor& c) {
-        while (c.tile < tile1 && (c.box >= box1 || row_of(c) >= sh.n)) next_tile(c);
-    };
+    auto unit_boxes = [&](const Cursor& c) { return min(min(kUnit, c.left), num_box - c.box); };
     auto issue = [&](const Cursor& c, int slot) {
-        mbar_arrive_expect_tx(bars + slot * 8, kBoxBytes);
-        tma_load_3d(smem_u32(ring_ptr) + slot * kBoxBytes, &tmQ, bars + slot * 8, c.box * 128, row_of(c), c.e);
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bars + slot * 8, kBoxBytes);
+            tma_load_3d(ring_addr + slot * kBoxBytes, &tmQ, bars + slot * 8, c.box * 128, (c.job.row + c.row) * kRows,
+                        c.job.e);
+        }
     };
     // Scales and zero points of the unit that begins at box c.box, for outputs g and g + 8.
     auto load_unit = [&](const Cursor& c, uint32_t (&sc)[2][(kHeld + 1) / 2], uint32_t (&zr)[2]) {
@@ -190,12 +219,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                  : ((c.box + t) * kBoxK) >> sh.group_log2;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int row = row_of(c) + i * 8 + g;
+            const int row = (c.job.row + c.row) * kRows + i * 8 + g;
 #pragma unroll
             for (int j = 0; j < (kHeld + 1) / 2; ++j) sc[i][j] = 0;
-            if constexpr (Z) zr[i] = 0;
-            if (c.tile >= tile1 || row >= sh.n || kg >= sh.k_groups) continue;
-            const size_t at = ((size_t)c.e * sh.n + row) * sh.k_groups + kg;
+            zr[i] = 0;
+            if (c.left == 0 || row >= sh.n || kg >= sh.k_groups) continue;
+            const size_t at = ((size_t)c.job.e * sh.n + row) * sh.k_groups + kg;
             if (kHeld == 1) {
                 sc[i][0] = scales[at];
                 if constexpr (Z) zr[i] = zeros[at];
@@ -220,55 +249,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     };
 
-    Cursor next = {tile0, tile0 / tiles_n, tile0 % tiles_n, 0, box0};  // the next unit of scales
-    next.e = group_of_chunk(next.q, groups, table);
-    settle(next);
-    Cursor ahead = next;  // lane 0: the next box to request
-    if (lane == 0) {
-        for (int s = 0; s < sh.depth && ahead.tile < tile1; ++s) {
-            issue(ahead, s);
-            ++ahead.box;
-            settle(ahead);
-        }
+    Job job = job_at((int)(total * blockIdx.x / gridDim.x));
+    Cursor next = {job, 0, 0, 0};  // the next unit of scales
+    enter(next);
+    Cursor ahead = next;  // the next box to request
+    for (int s = 0; s < sh.depth && ahead.left > 0; ++s) {
+        issue(ahead, s);
+        step(ahead, 1);
     }
     uint32_t sc_next[2][(kHeld + 1) / 2], zr_next[2];
     load_unit(next, sc_next, zr_next);
 
-    Cursor now = {tile0, tile0 / tiles_n, tile0 % tiles_n, 0, box0};
     int slot = 0, chunk = -1;
     uint32_t phase = 0;
     int tokens = 0, row0 = 0;
     bool failed = false;
-    for (; now.tile < tile1; next_tile(now)) {
-        if (now.q != chunk) {  // other rows of x: in shared memory, [block of 32 k][row][t]: the 8 values of thread t
-            chunk = now.q;     // in the order the pairs of a word of q come in
-            const int e = group_of_chunk(chunk, groups, table);
-            const int first = (chunk - table.chunk0[e]) * sh.tokens;
-            row0 = table.start[e] + first;
-            tokens = min(sh.tokens, table.rows[e] - first);
-            __syncthreads();
+    for (; job.first < end; job = job_at(job.first + job.rows)) {
+        if (job.q != chunk) {  // other rows of x: in shared memory, [block of 32 k][row][t]: the 8 values of thread t
+            chunk = job.q;     // in the order the pairs of a word of q come in
+            const int first = (chunk - table.chunk0[job.e]) * sh.tokens;
+            row0 = table.start[job.e] + first;
+            tokens = min(sh.tokens, table.rows[job.e] - first);
+            uint4* x_out = reinterpret_cast<uint4*>(smem + xs);
             for (int c = 0; c < tokens; ++c)
+#pragma unroll 2
                 for (int j = threadIdx.x; j < num_box * 32; j += kThreads) {
                     uint4 v = make_uint4(0, 0, 0, 0);
                     if (j * 8 < sh.k) v = *reinterpret_cast<const uint4*>(x + (size_t)(row0 + c) * sh.k + j * 8);
-                    xs[((j >> 2) * tokens + c) * 4 + (j & 3)] =
+                    x_out[((j >> 2) * tokens + c) * 4 + (j & 3)] =
                         make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                                    __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
                 }
             __syncthreads();
         }
+        // Columns of the products past the last row of x are computed from that row and not used.
+        const uint32_t x_block = (uint32_t)tokens * 64;
+        uint32_t x_lane[NT];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) x_lane[c] = xs + (uint32_t)(min(c * 8 + g, tokens - 1) * 64 + t * 16);
+
         float sum[NT][4];
 #pragma unroll
         for (int c = 0; c < NT; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[c][i] = 0.0f;
-        // Columns of the products past the last row of x are computed from that row and not used.
-        const uint4* x_lane[NT];
-#pragma unroll
-        for (int c = 0; c < NT; ++c) x_lane[c] = xs + min(c * 8 + g, tokens - 1) * 4 + t;
-
-        const int n0 = row_of(now);
-        for (int unit = n0 < sh.n ? box0 : box1; unit < box1; unit += kUnit) {
+        while (next.job.first == job.first && next.left > 0) {
+            const int row = next.row, box = next.box, boxes = unit_boxes(next);
             uint32_t sc[2][(kHeld + 1) / 2], zr[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -276,17 +302,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < (kHeld + 1) / 2; ++j) sc[i][j] = sc_next[i][j];
                 zr[i] = Z ? zero_bytes<DT>(zr_next[i]) : 0;
             }
-            next.box += kUnit;
-            settle(next);
+            step(next, boxes);
             load_unit(next, sc_next, zr_next);
-            for (int in_unit = 0; in_unit < kUnit && unit + in_unit < box1; ++in_unit) {
+            uint32_t x_at = (uint32_t)(box * 8) * x_block;
+            for (int in_unit = 0; in_unit < boxes; ++in_unit) {
                 if (!failed && !mbar_wait(bars + slot * 8, (phase >> slot) & 1u, nullptr)) {
                     if (lane == 0) atomicCAS(&g_w4_error, 0, kErrBulkWait);
                     failed = true;  // go on without the weights: the other warps wait at the joins
                     for (int s = 0; s < sh.depth; ++s) mbar_wait(bars + s * 8, (phase >> s) & 1u, nullptr);
                 }
-                const uint8_t* q_lane = ring_ptr + slot * kBoxBytes + g * 128 + t * 4;
-                const int x_box = (unit + in_unit) * 8 * tokens * 4;
+                // 16-byte piece b of row g stands at b ^ g (the tensor map's swizzle)
+                const uint32_t q_lane = ring + slot * kBoxBytes + (uint32_t)(g * 128 + g * 16 + t * 4);
                 float acc[NT][4];
                 uint32_t pair[2], zero[2], zw[2];
 #pragma unroll
@@ -311,8 +337,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     uint4 xv[NT];
 #pragma unroll
-                    for (int c = 0; c < NT; ++c) xv[c] = x_lane[c][x_box + b * tokens * 4];
-                    const uint8_t* at = q_lane + ((b ^ g) * 16);
+                    for (int c = 0; c < NT; ++c)
+                        xv[c] = *reinterpret_cast<const uint4*>(smem + x_lane[c] + x_at);
+                    x_at += x_block;
+                    const uint8_t* at = smem + (q_lane ^ (uint32_t)(b * 16));
                     const uint32_t lo = *reinterpret_cast<const uint32_t*>(at);
                     const uint32_t hi = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
 #pragma unroll
@@ -335,34 +363,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 __syncwarp();  // all threads have read the box
-                if (lane == 0 && !failed && ahead.tile < tile1) {
+                if (!failed && ahead.left > 0) {
                     issue(ahead, slot);
-                    ++ahead.box;
-                    settle(ahead);
+                    step(ahead, 1);
                 }
                 phase ^= 1u << slot;
                 if (++slot == sh.depth) slot = 0;
             }
+            if (next.job.first != job.first || next.row != row) {  // this warp is done with the row
+                // (warp, row) pairs of a job go up one at a time, so their sums are places of their own
+                float* mine = red + (warp + row) * part;
+#pragma unroll
+                for (int c = 0; c < NT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int token = c * 8 + 2 * t + (i & 1);
+                        if (token < tokens) mine[token * kRows + (i >> 1) * 8 + g] = sum[c][i];
+                        sum[c][i] = 0.0f;
+                    }
+            }
         }
 
-        // Join the wk partial sums of this row group's outputs.
-        float* mine = red + (size_t)warp * sh.red_rows * kRows;
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = c * 8 + 2 * t + (i & 1);
-                if (row < tokens) mine[row * kRows + (i >> 1) * 8 + g] = sum[c][i];
-            }
-        named_barrier(1 + rw, sh.wk * 32);
-        const float* parts = red + (size_t)(warp - kw) * sh.red_rows * kRows;
-        for (int i = kw * 32 + lane; i < tokens * kRows; i += sh.wk * 32) {
+        __syncthreads();
+        const int boxes = job.rows * num_box;
+        for (int i = threadIdx.x; i < job.rows * tokens * kRows; i += kThreads) {
+            const int in_row = i % (tokens * kRows), row = i / (tokens * kRows);
+            const int token = in_row / kRows, n = (job.row + row) * kRows + in_row % kRows;
+            // warp w has box p when boxes * w / 16 <= p < boxes * (w + 1) / 16 (whole quotients)
+            const int w0 = (kWarps * (row * num_box + 1) - 1) / boxes, w1 = (kWarps * (row + 1) * num_box - 1) / boxes;
             float v = 0.0f;
-            for (int w = 0; w < sh.wk; ++w) v += parts[w * sh.red_rows * kRows + i];
-            const int n = n0 + i % kRows;
-            if (n < sh.n) out[(size_t)(row0 + i / kRows) * sh.n + n] = round16<DT>(v);
+            for (int w = w0; w <= w1; ++w)
+                if (first_box(job, w) < first_box(job, w + 1)) v += red[(w + row) * part + in_row];
+            if (n < sh.n) out[(size_t)(row0 + token) * sh.n + n] = round16<DT>(v);
         }
-        named_barrier(1 + rw, sh.wk * 32);
+        __syncthreads();
     }
 }
 
@@ -378,23 +412,19 @@ static int launch_kernel(const CUtensorMap& tmQ, const void* x, const void* scal
         if (dev < 64) attr_set[dev] = true;
     }
     const int num_box = (sh.k + kBoxK - 1) / kBoxK;
-    sh.wk = 1;
-    while (sh.wk < kWarps && sh.wk * 2 <= num_box) sh.wk *= 2;
     sh.tokens = std::min({sh.rows, NT * 8, 256 / num_box});  // x takes at most 128 KiB
-    sh.red_rows = sh.tokens;
     constexpr int kHeld = GB <= 2 ? 4 : GB == 4 ? 2 : 1;
     sh.vector_scales = sh.k_groups % kHeld == 0 && reinterpret_cast<uintptr_t>(scales) % (2 * kHeld) == 0 &&
                        reinterpret_cast<uintptr_t>(zeros) % kHeld == 0;
-    const size_t fixed = 1024 + (size_t)num_box * 512 * sh.tokens + (size_t)kWarps * sh.red_rows * kRows * 4 +
-                         (size_t)(3 * sh.groups + 1) * 4;
+    const size_t fixed = 1024 + (size_t)num_box * 512 * sh.tokens +
+                         (size_t)(kWarps + kJobRows) * sh.tokens * kRows * 4 + (size_t)(3 * sh.groups + 1) * 4;
     const size_t slots = (size_t)kWarps * kBoxBytes;  // one box for each warp
     sh.depth = (int)std::min<size_t>(4, (kMaxSmem - fixed) / slots);
     const size_t smem = fixed + sh.depth * slots;
-    const int tile_rows = kWarps / sh.wk * kRows;
-    const int64_t tiles_n = (sh.n + tile_rows - 1) / tile_rows;
-    const int64_t tiles = tiles_n * ((int64_t)sh.rows / sh.tokens + std::min(sh.groups, sh.rows));
+    const int64_t rows_n = (sh.n + kRows - 1) / kRows;
+    const int64_t tiles = rows_n * ((int64_t)sh.rows / sh.tokens + std::min(sh.groups, sh.rows));
     if (tiles > INT32_MAX) {
-        set_error("trb_gemv_w4_launch: too many tiles (rows=%d n=%d groups=%d)", sh.rows, sh.n, sh.groups);
+        set_error("trb_gemv_w4_launch: too many outputs (rows=%d n=%d groups=%d)", sh.rows, sh.n, sh.groups);
         return TRB_SKIPPED;
     }
     cudaLaunchConfig_t cfg = {};
