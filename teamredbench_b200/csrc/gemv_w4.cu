@@ -11,9 +11,9 @@
 // instruction per 256 weights what would take 256 FMA lanes, and the exact
 // products of small whole numbers with 16-bit x accumulate in fp32.  Weights
 // become 16-bit floats by bit operations: a 4-bit q ORed into the mantissa of
-// 128 (bf16) or 64 (f16) is 128 + q (64 + q) exactly, and subtracting 128 + z
-// is exact too, so nothing is rounded before the product, and the scale is
-// applied in fp32 to each group's sum.
+// 128 is 128 + q exactly, and subtracting 128 + z is exact too, so nothing is
+// rounded before the product, and the scale is applied in fp32 to each
+// group's sum.
 //
 // A CTA takes rows of 16 outputs of one group in jobs.  The boxes of a job (16
 // outputs x 256 k, 128 bytes of q a row) are one sequence, cut evenly among the
@@ -72,20 +72,36 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Pair p of a word of eight q: (q[p], q[p + 4]) as two 16-bit floats, each plus 128 (bf16) or 64 (f16).
-template <int DT>
-__device__ __forceinline__ uint32_t biased_pair(uint32_t w, int p) {
-    if constexpr (DT == TRB_BFLOAT16) return ((w >> (4 * p)) & 0x000F000Fu) | 0x43004300u;
-    else return ((p == 0 ? w << 4 : w >> (4 * (p - 1))) & 0x00F000F0u) | 0x54005400u;
-}
-// Byte i of four zero points (stored by zero_bytes) as two equal 16-bit floats, plus the same 128 or 64.
-template <int DT>
-__device__ __forceinline__ uint32_t zero_bytes(uint32_t z) {
-    return DT == TRB_BFLOAT16 ? z & 0x0F0F0F0Fu : (z & 0x0F0F0F0Fu) << 4;
+// Pair p of a word of eight q: (q[p], q[p + 4]) as two 16-bit floats.  bf16: 128 + q each.  f16 has mantissa bits
+// enough to take q where it stands in the word or its upper half: 1024 + q for even p, 64 + q for odd p.
+// One lop3 for the mask and the exponent together (written as & and |, it became two).
+__device__ __forceinline__ uint32_t mask_or(uint32_t v, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
+    return r;
 }
 template <int DT>
-__device__ __forceinline__ uint32_t biased_zero(uint32_t bytes, int i) {
-    return __byte_perm(bytes, DT == TRB_BFLOAT16 ? 0x43u : 0x54u, 0x4040u + 0x0101u * (uint32_t)i);
+__device__ __forceinline__ void biased_pairs(uint32_t w, uint32_t (&pair)[4]) {
+    if constexpr (DT == TRB_BFLOAT16) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) pair[p] = mask_or(w >> (4 * p), 0x000F000Fu, 0x43004300u);
+    } else {
+        pair[0] = mask_or(w, 0x000F000Fu, 0x64006400u);
+        pair[1] = mask_or(w, 0x00F000F0u, 0x54005400u);
+        pair[2] = mask_or(w >> 8, 0x000F000Fu, 0x64006400u);
+        pair[3] = mask_or(w >> 8, 0x00F000F0u, 0x54005400u);
+    }
+}
+// Byte i of four zero points as two equal 16-bit floats with the same bias, for even and odd pairs.
+template <int DT>
+__device__ __forceinline__ void biased_zeros(uint32_t bytes, int i, uint32_t& even, uint32_t& odd) {
+    const uint32_t twice = 0x4040u + 0x0101u * (uint32_t)i;
+    if constexpr (DT == TRB_BFLOAT16) {
+        even = odd = __byte_perm(bytes, 0x43u, twice);
+    } else {
+        even = __byte_perm(bytes, 0x64u, twice);
+        odd = __byte_perm(bytes << 4, 0x54u, twice);
+    }
 }
 template <int DT>
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
@@ -300,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int j = 0; j < (kHeld + 1) / 2; ++j) sc[i][j] = sc_next[i][j];
-                zr[i] = Z ? zero_bytes<DT>(zr_next[i]) : 0;
+                zr[i] = Z ? zr_next[i] & 0x0F0F0F0Fu : 0;
             }
             step(next, boxes);
             load_unit(next, sc_next, zr_next);
@@ -314,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // 16-byte piece b of row g stands at b ^ g (the tensor map's swizzle)
                 const uint32_t q_lane = ring + slot * kBoxBytes + (uint32_t)(g * 128 + g * 16 + t * 4);
                 float acc[NT][4];
-                uint32_t pair[2], zero[2], zw[2];
+                uint32_t pair[2], even[2], odd[2], zw[2];
 #pragma unroll
                 for (int b = 0; b < 8; ++b) {
                     if (b % GB == 0) {
@@ -329,9 +345,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (held % 2 == 0) pair[i] = __shfl_sync(0xffffffffu, sc[i][held >> 1], src, 4);
                             if constexpr (Z) {
                                 if (held == 0) zw[i] = __shfl_sync(0xffffffffu, zr[i], src, 4);
-                                zero[i] = biased_zero<DT>(zw[i], held);
+                                biased_zeros<DT>(zw[i], held, even[i], odd[i]);
                             } else {
-                                zero[i] = DT == TRB_BFLOAT16 ? 0x43084308u : 0x54805480u;  // 128 + 8, 64 + 8
+                                biased_zeros<DT>(8u, 0, even[i], odd[i]);
                             }
                         }
                     }
@@ -343,12 +359,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint8_t* at = smem + (q_lane ^ (uint32_t)(b * 16));
                     const uint32_t lo = *reinterpret_cast<const uint32_t*>(at);
                     const uint32_t hi = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
+                    uint32_t lo_pairs[4], hi_pairs[4];
+                    biased_pairs<DT>(lo, lo_pairs);
+                    biased_pairs<DT>(hi, hi_pairs);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t a[4] = {sub2<DT>(biased_pair<DT>(lo, 2 * h), zero[0]),
-                                               sub2<DT>(biased_pair<DT>(hi, 2 * h), zero[1]),
-                                               sub2<DT>(biased_pair<DT>(lo, 2 * h + 1), zero[0]),
-                                               sub2<DT>(biased_pair<DT>(hi, 2 * h + 1), zero[1])};
+                        const uint32_t a[4] = {sub2<DT>(lo_pairs[2 * h], even[0]), sub2<DT>(hi_pairs[2 * h], even[1]),
+                                               sub2<DT>(lo_pairs[2 * h + 1], odd[0]),
+                                               sub2<DT>(hi_pairs[2 * h + 1], odd[1])};
 #pragma unroll
                         for (int c = 0; c < NT; ++c)
                             mma_16816<DT>(acc[c], a, h ? xv[c].z : xv[c].x, h ? xv[c].w : xv[c].y);
