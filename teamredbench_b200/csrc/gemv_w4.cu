@@ -45,6 +45,8 @@ constexpr int kBlockK = 32;  // k of a block: 16 bytes a row, two products
 constexpr uint32_t kBoxBytes = kRows * 128;
 constexpr int kMaxDepth = 8;
 
+// Scales a thread holds of a unit (see the kernel) for groups that span gb blocks.
+__host__ __device__ constexpr int held_scales(int gb) { return gb <= 2 ? 4 : gb == 4 ? 2 : 1; }
 constexpr int kJobRows = 16;  // rows of 16 outputs in a job, at most
 
 struct Shape {
@@ -53,7 +55,6 @@ struct Shape {
     int group_log2;
     int depth;          // boxes in each warp's ring
     int tokens;         // rows of x taken at once
-    int vector_scales;  // scales and zero points may be read kHeld at a time
 };
 
 template <int DT>
@@ -124,32 +125,29 @@ __device__ __forceinline__ uint16_t round16(float v) {
     else return __half_as_ushort(__float2half_rn(v));
 }
 
-// Rows of 16 outputs [row, row + rows) of group e for the rows of x in chunk q.
+// Rows of 16 outputs [row, row + rows) of group e for the rows of x in chunk q, and a warp's share of their boxes:
+// boxes [p, p_end) of the job's sequence, the first of them box `box` of row `p_row`.
 struct Job {
     int first;  // in the count of all rows of outputs of all chunks
     int rows, row, q, e;
+    int p, p_end, p_row, box;
 };
 
-// A warp's place in its share of a job: box `box` of row `row` of the job, `left` boxes to go.
-struct Cursor {
-    Job job;
-    int row, box, left;
-};
-
-// NT * 8 rows of x at once; a group of k spans GB blocks (8: a box or more); Z: zero points given.
-template <int DT, int NT, int GB, bool Z>
+// NT * 8 rows of x at once; a group of k spans GB blocks (8: a box or more); Z: zero points given; V: scales and zero
+// points may be read kHeld at a time.
+template <int DT, int NT, int GB, bool Z, bool V>
 __global__ void __launch_bounds__(kThreads, 1)
     gemv_w4_kernel(const __grid_constant__ CUtensorMap tmQ, const uint16_t* __restrict__ x,
                    const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros,
                    const int* __restrict__ offsets, uint16_t* __restrict__ out, const Shape sh) {
     // Scales travel in units: the groups of kUnit boxes of each output, kHeld of them in each of its four threads.
     constexpr int kUnit = GB == 1 ? 2 : 4;
-    constexpr int kHeld = GB <= 2 ? 4 : GB == 4 ? 2 : 1;
+    constexpr int kHeld = held_scales(GB);
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kWarps * kMaxDepth];
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int num_box = (sh.k + kBoxK - 1) / kBoxK;
@@ -186,101 +184,89 @@ __global__ void __launch_bounds__(kThreads, 1)
     // This CTA's share of the rows of outputs, contiguous so that x stays in shared memory.
     const int64_t total = (int64_t)table.chunk0[groups] * rows_n;
     const int end = (int)(total * (blockIdx.x + 1) / gridDim.x);
+    auto first_box = [&](int rows, int w) { return rows * num_box * w / kWarps; };
     auto job_at = [&](int first) {
-        Job j;
+        Job j = {};
         j.first = first;
+        if (first >= end) return j;
         j.q = first / rows_n;
         j.row = first - j.q * rows_n;
         j.rows = min(min(end - first, rows_n - j.row), kJobRows);
-        j.e = first < end ? group_of_chunk(j.q, groups, table) : 0;
+        j.e = group_of_chunk(j.q, groups, table);
+        j.p = first_box(j.rows, warp);
+        j.p_end = first_box(j.rows, warp + 1);
+        j.p_row = j.p / num_box;
+        j.box = j.p - j.p_row * num_box;
         return j;
     };
-    auto first_box = [&](const Job& j, int w) { return j.rows * num_box * w / kWarps; };
-    // A warp's share of jobs from c.job on: at the first box of the first job in which it has one.
-    auto enter = [&](Cursor& c) {
-        while (c.job.first < end) {
-            const int p = first_box(c.job, warp);
-            c.left = first_box(c.job, warp + 1) - p;
-            c.row = p / num_box;
-            c.box = p - c.row * num_box;
-            if (c.left > 0) return;
-            c.job = job_at(c.job.first + c.job.rows);
-        }
-        c.left = 0;
-    };
-    auto step = [&](Cursor& c, int boxes) {  // within a row
-        c.box += boxes;
-        c.left -= boxes;
-        if (c.left == 0) {
-            c.job = job_at(c.job.first + c.job.rows);
-            enter(c);
-        } else if (c.box == num_box) {
-            c.box = 0;
-            ++c.row;
-        }
-    };
-    auto unit_boxes = [&](const Cursor& c) { return min(min(kUnit, c.left), num_box - c.box); };
-    auto issue = [&](const Cursor& c, int slot) {
+    auto issue = [&](int box, int row, int e, int slot) {
         if (lane == 0) {
             mbar_arrive_expect_tx(bars + slot * 8, kBoxBytes);
-            tma_load_3d(ring_addr + slot * kBoxBytes, &tmQ, bars + slot * 8, c.box * 128, (c.job.row + c.row) * kRows,
-                        c.job.e);
+            tma_load_3d(ring_addr + slot * kBoxBytes, &tmQ, bars + slot * 8, box * 128, row * kRows, e);
         }
     };
-    // Scales and zero points of the unit that begins at box c.box, for outputs g and g + 8.
-    auto load_unit = [&](const Cursor& c, uint32_t (&sc)[2][(kHeld + 1) / 2], uint32_t (&zr)[2]) {
-        const int kg = GB == 1   ? c.box * 8 + 4 * t
-                       : GB == 2 ? (c.box + t) * 4
-                       : GB == 4 ? (c.box + t) * 2
-                                 : ((c.box + t) * kBoxK) >> sh.group_log2;
+    // Scales and zero points of the unit that begins at box `box`, for outputs g and g + 8 of row `row`.
+    uint32_t sc_next[2][(kHeld + 1) / 2], zr_next[2];
+    auto load_unit = [&](int box, int row, int e) {
+        const int kg = GB == 1   ? box * 8 + 4 * t
+                       : GB == 2 ? (box + t) * 4
+                       : GB == 4 ? (box + t) * 2
+                                 : ((box + t) * kBoxK) >> sh.group_log2;
+        const size_t at0 = ((size_t)e * sh.n + row * kRows + g) * sh.k_groups + kg;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int row = (c.job.row + c.row) * kRows + i * 8 + g;
-#pragma unroll
-            for (int j = 0; j < (kHeld + 1) / 2; ++j) sc[i][j] = 0;
-            zr[i] = 0;
-            if (c.left == 0 || row >= sh.n || kg >= sh.k_groups) continue;
-            const size_t at = ((size_t)c.job.e * sh.n + row) * sh.k_groups + kg;
-            if (kHeld == 1) {
-                sc[i][0] = scales[at];
-                if constexpr (Z) zr[i] = zeros[at];
-            } else if (sh.vector_scales) {  // k_groups is a multiple of kHeld
-                if constexpr (kHeld == 4) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(scales + at);
-                    sc[i][0] = v.x;
-                    sc[i][1] = v.y;
-                    if constexpr (Z) zr[i] = *reinterpret_cast<const uint32_t*>(zeros + at);
-                } else if constexpr (kHeld == 2) {
-                    sc[i][0] = *reinterpret_cast<const uint32_t*>(scales + at);
-                    if constexpr (Z) zr[i] = *reinterpret_cast<const uint16_t*>(zeros + at);
-                }
+            const size_t at = at0 + (size_t)(i * 8 * sh.k_groups);
+            const bool in = row * kRows + i * 8 + g < sh.n && kg < sh.k_groups;
+            if constexpr (kHeld == 1) {
+                sc_next[i][0] = in ? scales[at] : 0;
+                if constexpr (Z) zr_next[i] = in ? zeros[at] : 0;
+            } else if constexpr (V && kHeld == 4) {  // k_groups is a multiple of kHeld
+                const uint2 v = in ? *reinterpret_cast<const uint2*>(scales + at) : make_uint2(0, 0);
+                sc_next[i][0] = v.x;
+                sc_next[i][1] = v.y;
+                if constexpr (Z) zr_next[i] = in ? *reinterpret_cast<const uint32_t*>(zeros + at) : 0;
+            } else if constexpr (V) {
+                sc_next[i][0] = in ? *reinterpret_cast<const uint32_t*>(scales + at) : 0;
+                if constexpr (Z) zr_next[i] = in ? *reinterpret_cast<const uint16_t*>(zeros + at) : 0;
             } else {
+                if constexpr (Z) zr_next[i] = 0;
 #pragma unroll
                 for (int j = 0; j < kHeld; ++j) {
-                    if (kg + j >= sh.k_groups) break;
-                    sc[i][j >> 1] |= (uint32_t)scales[at + j] << (16 * (j & 1));
-                    if constexpr (Z) zr[i] |= (uint32_t)zeros[at + j] << (8 * j);
+                    const bool in_j = in && kg + j < sh.k_groups;
+                    const uint32_t v = (uint32_t)(in_j ? scales[at + j] : 0) << (16 * (j & 1));
+                    sc_next[i][j >> 1] = j & 1 ? sc_next[i][j >> 1] | v : v;
+                    if constexpr (Z) zr_next[i] |= (uint32_t)(in_j ? zeros[at + j] : 0) << (8 * j);
                 }
             }
         }
     };
 
-    Job job = job_at((int)(total * blockIdx.x / gridDim.x));
-    Cursor next = {job, 0, 0, 0};  // the next unit of scales
-    enter(next);
-    Cursor ahead = next;  // the next box to request
-    for (int s = 0; s < sh.depth && ahead.left > 0; ++s) {
-        issue(ahead, s);
-        step(ahead, 1);
-    }
-    uint32_t sc_next[2][(kHeld + 1) / 2], zr_next[2];
-    load_unit(next, sc_next, zr_next);
-
     int slot = 0, chunk = -1;
     uint32_t phase = 0;
     int tokens = 0, row0 = 0;
     bool failed = false;
-    for (; job.first < end; job = job_at(job.first + job.rows)) {
+    // The place behind the last box requested of the job at hand.
+    int a_box = 0, a_row = 0, a_left = 0;
+    auto begin = [&](const Job& j) {  // request a job's first boxes (the ring is empty) and scales
+        a_box = j.box;
+        a_row = j.row + j.p_row;
+        a_left = j.p_end - j.p;
+        if (a_left == 0) return;
+        load_unit(a_box, a_row, j.e);
+        for (int s = slot, i = 0; i < sh.depth && a_left > 0; ++i) {
+            if (!failed) issue(a_box, a_row, j.e, s);
+            if (++s == sh.depth) s = 0;
+            --a_left;
+            if (++a_box == num_box) {
+                a_box = 0;
+                ++a_row;
+            }
+        }
+    };
+
+    Job job = job_at((int)(total * blockIdx.x / gridDim.x));
+    begin(job);
+    while (job.first < end) {
         if (job.q != chunk) {  // other rows of x: in shared memory, [block of 32 k][row][t]: the 8 values of thread t
             chunk = job.q;     // in the order the pairs of a word of q come in
             const int first = (chunk - table.chunk0[job.e]) * sh.tokens;
@@ -298,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             __syncthreads();
         }
-        // Columns of the products past the last row of x are computed from that row and not used.
+    // Columns of the products past the last row of x are computed from that row and not used.
         const uint32_t x_block = (uint32_t)tokens * 64;
         uint32_t x_lane[NT];
 #pragma unroll
@@ -309,18 +295,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < NT; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[c][i] = 0.0f;
-        while (next.job.first == job.first && next.left > 0) {
-            const int row = next.row, box = next.box, boxes = unit_boxes(next);
-            uint32_t sc[2][(kHeld + 1) / 2], zr[2];
+        int box = job.box, row = job.p_row;
+        for (int left = job.p_end - job.p; left > 0;) {
+            const int boxes = min(min(kUnit, left), num_box - box);
+            uint32_t sc[2][(kHeld + 1) / 2], zr[2] = {};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int j = 0; j < (kHeld + 1) / 2; ++j) sc[i][j] = sc_next[i][j];
-                zr[i] = Z ? zr_next[i] & 0x0F0F0F0Fu : 0;
+                if constexpr (Z) zr[i] = zr_next[i] & 0x0F0F0F0Fu;
             }
-            step(next, boxes);
-            load_unit(next, sc_next, zr_next);
             uint32_t x_at = (uint32_t)(box * 8) * x_block;
+            left -= boxes;
+            box += boxes;
+            const bool row_done = box == num_box;
+            if (row_done) box = 0;
+            if (left > 0) load_unit(box, job.row + row + row_done, job.e);
             for (int in_unit = 0; in_unit < boxes; ++in_unit) {
                 if (!failed && !mbar_wait(bars + slot * 8, (phase >> slot) & 1u, nullptr)) {
                     if (lane == 0) atomicCAS(&g_w4_error, 0, kErrBulkWait);
@@ -381,14 +371,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 __syncwarp();  // all threads have read the box
-                if (!failed && ahead.left > 0) {
-                    issue(ahead, slot);
-                    step(ahead, 1);
+                if (a_left > 0) {
+                    if (!failed) issue(a_box, a_row, job.e, slot);
+                    --a_left;
+                    if (++a_box == num_box) {
+                        a_box = 0;
+                        ++a_row;
+                    }
                 }
                 phase ^= 1u << slot;
                 if (++slot == sh.depth) slot = 0;
             }
-            if (next.job.first != job.first || next.row != row) {  // this warp is done with the row
+            if (row_done || left == 0) {  // this warp is done with the row
                 // (warp, row) pairs of a job go up one at a time, so their sums are places of their own
                 float* mine = red + (warp + row) * part;
 #pragma unroll
@@ -399,9 +393,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (token < tokens) mine[token * kRows + (i >> 1) * 8 + g] = sum[c][i];
                         sum[c][i] = 0.0f;
                     }
+                ++row;
             }
         }
 
+        const Job next = job_at(job.first + job.rows);
+        begin(next);
         __syncthreads();
         const int boxes = job.rows * num_box;
         for (int i = threadIdx.x; i < job.rows * tokens * kRows; i += kThreads) {
@@ -411,29 +408,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int w0 = (kWarps * (row * num_box + 1) - 1) / boxes, w1 = (kWarps * (row + 1) * num_box - 1) / boxes;
             float v = 0.0f;
             for (int w = w0; w <= w1; ++w)
-                if (first_box(job, w) < first_box(job, w + 1)) v += red[(w + row) * part + in_row];
+                if (first_box(job.rows, w) < first_box(job.rows, w + 1)) v += red[(w + row) * part + in_row];
             if (n < sh.n) out[(size_t)(row0 + token) * sh.n + n] = round16<DT>(v);
         }
         __syncthreads();
+        job = next;
     }
 }
 
 // ------------------------------------------------------------------ host side
-template <int DT, int NT, int GB, bool Z>
+template <int DT, int NT, int GB, bool Z, bool V>
 static int launch_kernel(const CUtensorMap& tmQ, const void* x, const void* scales, const void* zeros,
                          const int* offsets, void* out, Shape sh, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
     constexpr size_t kMaxSmem = 226 * 1024;
     if (dev >= 64 || !attr_set[dev]) {
-        TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, NT, GB, Z>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, NT, GB, Z, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)kMaxSmem));
         if (dev < 64) attr_set[dev] = true;
     }
     const int num_box = (sh.k + kBoxK - 1) / kBoxK;
     sh.tokens = std::min({sh.rows, NT * 8, 256 / num_box});  // x takes at most 128 KiB
-    constexpr int kHeld = GB <= 2 ? 4 : GB == 4 ? 2 : 1;
-    sh.vector_scales = sh.k_groups % kHeld == 0 && reinterpret_cast<uintptr_t>(scales) % (2 * kHeld) == 0 &&
-                       reinterpret_cast<uintptr_t>(zeros) % kHeld == 0;
     const size_t fixed = 1024 + (size_t)num_box * 512 * sh.tokens +
                          (size_t)(kWarps + kJobRows) * sh.tokens * kRows * 4 + (size_t)(3 * sh.groups + 1) * 4;
     const size_t slots = (size_t)kWarps * kBoxBytes;  // one box for each warp
@@ -455,10 +450,22 @@ static int launch_kernel(const CUtensorMap& tmQ, const void* x, const void* scal
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemv_w4_kernel<DT, NT, GB, Z>, tmQ, static_cast<const uint16_t*>(x),
+    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemv_w4_kernel<DT, NT, GB, Z, V>, tmQ, static_cast<const uint16_t*>(x),
                                 static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), offsets,
                                 static_cast<uint16_t*>(out), sh));
     return TRB_OK;
+}
+
+template <int DT, int NT, int GB, bool Z>
+static int launch_scales(const CUtensorMap& tmQ, const void* x, const void* scales, const void* zeros,
+                         const int* offsets, void* out, const Shape& sh, int dev, cudaStream_t stream) {
+    constexpr int kHeld = held_scales(GB);
+    const bool vector = kHeld > 1 && sh.k_groups % kHeld == 0 &&
+                        reinterpret_cast<uintptr_t>(scales) % (2 * kHeld) == 0 &&
+                        reinterpret_cast<uintptr_t>(zeros) % kHeld == 0;
+    if constexpr (kHeld > 1)
+        if (vector) return launch_kernel<DT, NT, GB, Z, true>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+    return launch_kernel<DT, NT, GB, Z, false>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
 }
 
 template <int DT, int NT, bool Z>
@@ -470,10 +477,10 @@ static int launch_group(const void* x, const void* q, const void* scales, const 
     const int rc = gemm::encode_tiled(&tmQ, q, 1, 3, extent, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
     switch (sh.group_log2) {
-        case 5: return launch_kernel<DT, NT, 1, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        case 6: return launch_kernel<DT, NT, 2, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        case 7: return launch_kernel<DT, NT, 4, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        default: return launch_kernel<DT, NT, 8, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 5: return launch_scales<DT, NT, 1, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 6: return launch_scales<DT, NT, 2, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 7: return launch_scales<DT, NT, 4, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        default: return launch_scales<DT, NT, 8, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
     }
 }
 
