@@ -13,15 +13,24 @@
 // become 16-bit floats by bit operations: a 4-bit q ORed into the mantissa of
 // 128 is 128 + q exactly, and subtracting 128 + z is exact too, so nothing is
 // rounded before the product, and the scale is applied in fp32 to each
-// group's sum.
+// group's sum.  Those operations (22 to 26 of some 35 instructions per 512
+// weights) are what the kernel spends its issue slots on.
 //
-// A CTA takes rows of 16 outputs of one group in jobs.  The boxes of a job (16
-// outputs x 256 k, 128 bytes of q a row) are one sequence, cut evenly among the
-// 16 warps, so a warp works through neighbouring boxes of one or two rows
-// whatever k is, with nothing to wait for but its own boxes: they come by TMA
-// through a private ring.  What a warp has summed of a row goes to shared
-// memory when it leaves the row, and at the job's end the parts of each row are
-// added in the order of k.
+// The order of k inside a product is free as long as q and x agree on it, so
+// each of the four threads that share an output takes W consecutive words (8
+// q each) straight from global memory into registers: no shared memory, no
+// barrier between the loads and the products.  One step is 4 W words of an
+// output, 32 W k, with W = 1, 2 or 4 so that a group of 32, 64 or 128 (or
+// more) k covers whole steps; a pack of 512 k is 16 / W steps and 32 registers,
+// and each step's registers take the same step of the next pack as soon as
+// they are used, 64 KiB in flight on an SM.
+//
+// A CTA takes rows of 16 outputs of one group in jobs.  The packs of a job are
+// one sequence, cut evenly among the 16 warps, so a warp works through
+// neighbouring packs of one or two rows whatever k is, with nothing to wait for
+// but its own loads.  What a warp has summed of a row goes to shared memory
+// when it leaves the row, and at the job's end the parts of each row are added
+// in the order of k.
 //
 // No counterpart in the reference.
 #include <cuda_bf16.h>
@@ -39,38 +48,53 @@ __device__ int g_w4_error;
 
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 16;    // outputs of a box
-constexpr int kBoxK = 256;   // k of a box: one 128-byte swizzle row
-constexpr int kBlockK = 32;  // k of a block: 16 bytes a row, two products
-constexpr uint32_t kBoxBytes = kRows * 128;
-constexpr int kMaxDepth = 8;
-
-// Scales a thread holds of a unit (see the kernel) for groups that span gb blocks.
-__host__ __device__ constexpr int held_scales(int gb) { return gb <= 2 ? 4 : gb == 4 ? 2 : 1; }
-constexpr int kJobRows = 16;  // rows of 16 outputs in a job, at most
+constexpr int kRows = 16;      // outputs of a row of a job
+constexpr int kPackK = 512;    // k of a pack
+constexpr int kJobRows = 16;   // rows of 16 outputs in a job, at most
 
 struct Shape {
     int groups, rows, n, k;
-    int k_groups;       // scales per output
+    int k_groups;    // scales per output
     int group_log2;
-    int depth;          // boxes in each warp's ring
-    int tokens;         // rows of x taken at once
+    int tokens;      // rows of x taken at once
 };
 
+// d (+)= a * b on the tensor cores, 16 outputs x 8 rows of x x 16 k; `first` starts from zero.
+#define TRB_MMA_16816(TYPE, C0, C1, C2, C3)                                                                 \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, " \
+                 "{%8, %9}, {%10, %11, %12, %13};"                                                          \
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                           \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(C0), "f"(C1), "f"(C2), "f"(C3))
 template <int DT>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (DT == TRB_BFLOAT16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
-            "%2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+    if constexpr (DT == TRB_BFLOAT16) {
+        if (first) TRB_MMA_16816("bf16", 0.f, 0.f, 0.f, 0.f);
+        else TRB_MMA_16816("bf16", d[0], d[1], d[2], d[3]);
+    } else {
+        if (first) TRB_MMA_16816("f16", 0.f, 0.f, 0.f, 0.f);
+        else TRB_MMA_16816("f16", d[0], d[1], d[2], d[3]);
+    }
+}
+#undef TRB_MMA_16816
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+// W words of q.  A step of W = 1 takes half a 32-byte sector of each output, the next step the other half, which
+// stays in L1 for it; wider steps use whole sectors once.
+template <int W>
+__device__ __forceinline__ void load_words(const uint8_t* p, bool in, uint32_t (&v)[W]) {
+    if (!in) return;
+    if constexpr (W == 4)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                     : "l"(p));
+    else if constexpr (W == 2)
+        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
     else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
-            "%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
 }
 
 // Pair p of a word of eight q: (q[p], q[p + 4]) as two 16-bit floats.  bf16: 128 + q each.  f16 has mantissa bits
@@ -125,66 +149,58 @@ __device__ __forceinline__ uint16_t round16(float v) {
     else return __half_as_ushort(__float2half_rn(v));
 }
 
-// Rows of 16 outputs [row, row + rows) of group e for the rows of x in chunk q, and a warp's share of their boxes:
-// boxes [p, p_end) of the job's sequence, the first of them box `box` of row `p_row`.
+// Rows of 16 outputs [row, row + rows) of group e for the rows of x in chunk q, and a warp's share of their packs:
+// `left` packs from pack `pack` of row `p_row` on.
 struct Job {
     int first;  // in the count of all rows of outputs of all chunks
     int rows, row, q, e;
-    int p, p_end, p_row, box;
+    int p_row, pack, left;
 };
 
-// NT * 8 rows of x at once; a group of k spans GB blocks (8: a box or more); Z: zero points given; V: scales and zero
-// points may be read kHeld at a time.
-template <int DT, int NT, int GB, bool Z, bool V>
+// NT * 8 rows of x at once; W: words of a step; Z: zero points given; V: a thread's scales of a pack are one aligned
+// read.
+template <int DT, int NT, int W, bool Z, bool V>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemv_w4_kernel(const __grid_constant__ CUtensorMap tmQ, const uint16_t* __restrict__ x,
+    gemv_w4_kernel(const uint8_t* __restrict__ weights, const uint16_t* __restrict__ x,
                    const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros,
                    const int* __restrict__ offsets, uint16_t* __restrict__ out, const Shape sh) {
-    // Scales travel in units: the groups of kUnit boxes of each output, kHeld of them in each of its four threads.
-    constexpr int kUnit = GB == 1 ? 2 : 4;
-    constexpr int kHeld = held_scales(GB);
+    constexpr int kSteps = 16 / W;      // of a pack
+    constexpr int kStepK = 32 * W;
+    constexpr int kHeld = kSteps / 4;   // steps of a pack whose scale a thread holds for the four of an output
+    constexpr int kScaleWords = (kHeld + 1) / 2;
 
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[kWarps * kMaxDepth];
+    extern __shared__ __align__(16) uint8_t smem[];
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const int num_box = (sh.k + kBoxK - 1) / kBoxK;
+    const int num_pack = (sh.k + kPackK - 1) / kPackK;
     const int rows_n = (sh.n + kRows - 1) / kRows;
 
-    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    const uint32_t ring = (uint32_t)(warp * sh.depth) * kBoxBytes;             // offsets into smem
-    const uint32_t xs = (uint32_t)(kWarps * sh.depth) * kBoxBytes;
-    float* red = reinterpret_cast<float*>(smem + xs + (size_t)num_box * 512 * sh.tokens);
-    const int part = sh.tokens * kRows;                                        // one warp's sums of a row
+    // x, the parts of the sums, the groups
+    float* red = reinterpret_cast<float*>(smem + (size_t)num_pack * (kPackK * 2) * sh.tokens);
+    const int part = sh.tokens * kRows;  // one warp's sums of a row
     int* words = reinterpret_cast<int*>(red + (kWarps + kJobRows) * part);
     const GroupTable table = {words, words + sh.groups, words + 2 * sh.groups};
-    const uint32_t ring_addr = smem_u32(smem) + ring;
-    const uint32_t bars = smem_u32(&full_bar[warp * kMaxDepth]);
 
-    if (lane == 0) {
-        for (int s = 0; s < sh.depth; ++s) mbar_init(bars + s * 8, 1);
-        fence_mbar_init();
-        if (warp == 0) tma_prefetch_desc(&tmQ);
-    }
     grid_launch_dependents();
     grid_dependency_wait();
     int groups = sh.groups;
     if (offsets != nullptr) {
         groups = load_groups(offsets, sh.groups, sh.rows, table, &g_w4_error);
+        if (warp == 0) scan_chunks(groups, sh.tokens, table, lane);
     } else if (threadIdx.x == 0) {
         table.start[0] = 0;
         table.rows[0] = sh.rows;
+        table.chunk0[0] = 0;
+        table.chunk0[1] = (sh.rows + sh.tokens - 1) / sh.tokens;
     }
-    __syncthreads();
-    if (warp == 0) scan_chunks(groups, sh.tokens, table, lane);
     __syncthreads();
 
     // This CTA's share of the rows of outputs, contiguous so that x stays in shared memory.
     const int64_t total = (int64_t)table.chunk0[groups] * rows_n;
     const int end = (int)(total * (blockIdx.x + 1) / gridDim.x);
-    auto first_box = [&](int rows, int w) { return rows * num_box * w / kWarps; };
+    auto first_pack = [&](int rows, int w) { return rows * num_pack * w / kWarps; };
     auto job_at = [&](int first) {
         Job j = {};
         j.first = first;
@@ -193,30 +209,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         j.row = first - j.q * rows_n;
         j.rows = min(min(end - first, rows_n - j.row), kJobRows);
         j.e = group_of_chunk(j.q, groups, table);
-        j.p = first_box(j.rows, warp);
-        j.p_end = first_box(j.rows, warp + 1);
-        j.p_row = j.p / num_box;
-        j.box = j.p - j.p_row * num_box;
+        const int p = first_pack(j.rows, warp);
+        j.left = first_pack(j.rows, warp + 1) - p;
+        j.p_row = p / num_pack;
+        j.pack = p - j.p_row * num_pack;
         return j;
     };
-    auto issue = [&](int box, int row, int e, int slot) {
-        if (lane == 0) {
-            mbar_arrive_expect_tx(bars + slot * 8, kBoxBytes);
-            tma_load_3d(ring_addr + slot * kBoxBytes, &tmQ, bars + slot * 8, box * 128, row * kRows, e);
-        }
-    };
-    // Scales and zero points of the unit that begins at box `box`, for outputs g and g + 8 of row `row`.
-    uint32_t sc_next[2][(kHeld + 1) / 2], zr_next[2];
-    auto load_unit = [&](int box, int row, int e) {
-        const int kg = GB == 1   ? box * 8 + 4 * t
-                       : GB == 2 ? (box + t) * 4
-                       : GB == 4 ? (box + t) * 2
-                                 : ((box + t) * kBoxK) >> sh.group_log2;
-        const size_t at0 = ((size_t)e * sh.n + row * kRows + g) * sh.k_groups + kg;
+
+    uint32_t lo[kSteps][W], hi[kSteps][W];  // q of outputs g and g + 8
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int w = 0; w < W; ++w) lo[i][w] = hi[i][w] = 0;
+    uint32_t sc_next[2][kScaleWords], zr_next[2];
+    // The pack to load next: this thread's first word for outputs g and g + 8, and its steps.  Outputs past n are
+    // computed from the last one and not stored; steps past k keep old words and meet zeros in x.
+    const uint8_t *q_lo = weights, *q_hi = weights;
+    int steps = 0;
+    auto at_pack = [&](int e, int row, int pack) {
+        const size_t first = (size_t)e * sh.n;
+        const int r_lo = min(row * kRows + g, sh.n - 1), r_hi = min(row * kRows + 8 + g, sh.n - 1);
+        const int byte = pack * (kPackK / 2) + t * 4 * W;
+        q_lo = weights + (first + r_lo) * (size_t)(sh.k / 2) + byte;
+        q_hi = weights + (first + r_hi) * (size_t)(sh.k / 2) + byte;
+        steps = min(kSteps, (sh.k - pack * kPackK) / kStepK);
+        const int step = pack * kSteps + t * kHeld;
+        const int kg = W == 4 ? (step * kStepK) >> sh.group_log2 : step;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const size_t at = at0 + (size_t)(i * 8 * sh.k_groups);
-            const bool in = row * kRows + i * 8 + g < sh.n && kg < sh.k_groups;
+            const size_t at = (first + (i ? r_hi : r_lo)) * sh.k_groups + kg;
+            const bool in = kg < sh.k_groups;
             if constexpr (kHeld == 1) {
                 sc_next[i][0] = in ? scales[at] : 0;
                 if constexpr (Z) zr_next[i] = in ? zeros[at] : 0;
@@ -232,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (Z) zr_next[i] = 0;
 #pragma unroll
                 for (int j = 0; j < kHeld; ++j) {
-                    const bool in_j = in && kg + j < sh.k_groups;
+                    const bool in_j = kg + j < sh.k_groups;
                     const uint32_t v = (uint32_t)(in_j ? scales[at + j] : 0) << (16 * (j & 1));
                     sc_next[i][j >> 1] = j & 1 ? sc_next[i][j >> 1] | v : v;
                     if constexpr (Z) zr_next[i] |= (uint32_t)(in_j ? zeros[at + j] : 0) << (8 * j);
@@ -240,118 +262,96 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     };
-
-    int slot = 0, chunk = -1;
-    uint32_t phase = 0;
-    int tokens = 0, row0 = 0;
-    bool failed = false;
-    // The place behind the last box requested of the job at hand.
-    int a_box = 0, a_row = 0, a_left = 0;
-    auto begin = [&](const Job& j) {  // request a job's first boxes (the ring is empty) and scales
-        a_box = j.box;
-        a_row = j.row + j.p_row;
-        a_left = j.p_end - j.p;
-        if (a_left == 0) return;
-        load_unit(a_box, a_row, j.e);
-        for (int s = slot, i = 0; i < sh.depth && a_left > 0; ++i) {
-            if (!failed) issue(a_box, a_row, j.e, s);
-            if (++s == sh.depth) s = 0;
-            --a_left;
-            if (++a_box == num_box) {
-                a_box = 0;
-                ++a_row;
-            }
-        }
+    auto load_step = [&](int i) {
+        load_words<W>(q_lo + i * 16 * W, i < steps, lo[i]);
+        load_words<W>(q_hi + i * 16 * W, i < steps, hi[i]);
+    };
+    auto begin = [&](const Job& j) {  // a job's first pack
+        if (j.left == 0) return;
+        at_pack(j.e, j.row + j.p_row, j.pack);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) load_step(i);
     };
 
     Job job = job_at((int)(total * blockIdx.x / gridDim.x));
     begin(job);
+    int chunk = -1, tokens = 0, row0 = 0;
     while (job.first < end) {
-        if (job.q != chunk) {  // other rows of x: in shared memory, [block of 32 k][row][t]: the 8 values of thread t
-            chunk = job.q;     // in the order the pairs of a word of q come in
+        if (job.q != chunk) {  // other rows of x: in shared memory, [step][word of a thread][row][t]: 8 values in the
+            chunk = job.q;     // order the pairs of a word of q come in, zeros past k
             const int first = (chunk - table.chunk0[job.e]) * sh.tokens;
             row0 = table.start[job.e] + first;
             tokens = min(sh.tokens, table.rows[job.e] - first);
-            uint4* x_out = reinterpret_cast<uint4*>(smem + xs);
-            for (int c = 0; c < tokens; ++c)
-#pragma unroll 2
-                for (int j = threadIdx.x; j < num_box * 32; j += kThreads) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (j * 8 < sh.k) v = *reinterpret_cast<const uint4*>(x + (size_t)(row0 + c) * sh.k + j * 8);
-                    x_out[((j >> 2) * tokens + c) * 4 + (j & 3)] =
-                        make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                                   __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-                }
+            uint4* x_out = reinterpret_cast<uint4*>(smem);
+            const int pieces = num_pack * (kPackK / 8);
+#pragma unroll 8
+            for (int i = threadIdx.x; i < pieces * tokens; i += kThreads) {
+                const int c = i / pieces, j = i - c * pieces;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (j * 8 < sh.k) v = __ldg(reinterpret_cast<const uint4*>(x + (size_t)(row0 + c) * sh.k + j * 8));
+                const int step = j / (4 * W), of = j / W % 4, w = j % W;
+                x_out[((step * W + w) * tokens + c) * 4 + of] =
+                    make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                               __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+            }
             __syncthreads();
         }
-    // Columns of the products past the last row of x are computed from that row and not used.
+        // Columns of the products past the last row of x are computed from that row and not used.
         const uint32_t x_block = (uint32_t)tokens * 64;
         uint32_t x_lane[NT];
 #pragma unroll
-        for (int c = 0; c < NT; ++c) x_lane[c] = xs + (uint32_t)(min(c * 8 + g, tokens - 1) * 64 + t * 16);
+        for (int c = 0; c < NT; ++c) x_lane[c] = smem_u32(smem) + (uint32_t)(min(c * 8 + g, tokens - 1) * 64 + t * 16);
 
         float sum[NT][4];
 #pragma unroll
         for (int c = 0; c < NT; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[c][i] = 0.0f;
-        int box = job.box, row = job.p_row;
-        for (int left = job.p_end - job.p; left > 0;) {
-            const int boxes = min(min(kUnit, left), num_box - box);
-            uint32_t sc[2][(kHeld + 1) / 2], zr[2] = {};
+        int row = job.p_row, pack = job.pack;
+        for (int left = job.left; left > 0;) {
+            uint32_t sc[2][kScaleWords], zr[2] = {};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int j = 0; j < (kHeld + 1) / 2; ++j) sc[i][j] = sc_next[i][j];
+                for (int j = 0; j < kScaleWords; ++j) sc[i][j] = sc_next[i][j];
                 if constexpr (Z) zr[i] = zr_next[i] & 0x0F0F0F0Fu;
             }
-            uint32_t x_at = (uint32_t)(box * 8) * x_block;
-            left -= boxes;
-            box += boxes;
-            const bool row_done = box == num_box;
-            if (row_done) box = 0;
-            if (left > 0) load_unit(box, job.row + row + row_done, job.e);
-            for (int in_unit = 0; in_unit < boxes; ++in_unit) {
-                if (!failed && !mbar_wait(bars + slot * 8, (phase >> slot) & 1u, nullptr)) {
-                    if (lane == 0) atomicCAS(&g_w4_error, 0, kErrBulkWait);
-                    failed = true;  // go on without the weights: the other warps wait at the joins
-                    for (int s = 0; s < sh.depth; ++s) mbar_wait(bars + s * 8, (phase >> s) & 1u, nullptr);
-                }
-                // 16-byte piece b of row g stands at b ^ g (the tensor map's swizzle)
-                const uint32_t q_lane = ring + slot * kBoxBytes + (uint32_t)(g * 128 + g * 16 + t * 4);
-                float acc[NT][4];
-                uint32_t pair[2], even[2], odd[2], zw[2];
+            uint32_t x_at[NT];
 #pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                    if (b % GB == 0) {
-                        const int src = GB == 1 ? in_unit * 2 + (b >> 2) : in_unit;
-                        const int held = GB == 8 ? 0 : (b / GB) % kHeld;
+            for (int c = 0; c < NT; ++c) x_at[c] = x_lane[c] + (uint32_t)(pack * 16) * x_block;
+            --left;
+            const bool row_done = ++pack == num_pack;
+            if (row_done) pack = 0;
+            steps = 0;
+            if (left > 0) at_pack(job.e, job.row + row + row_done, pack);
+
+            uint32_t pair[2], zw[2];
 #pragma unroll
-                        for (int c = 0; c < NT; ++c)
+            for (int i = 0; i < kSteps; ++i) {
+                const int held = i % kHeld;
+                uint32_t even[2], odd[2];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[c][i] = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            if (held % 2 == 0) pair[i] = __shfl_sync(0xffffffffu, sc[i][held >> 1], src, 4);
-                            if constexpr (Z) {
-                                if (held == 0) zw[i] = __shfl_sync(0xffffffffu, zr[i], src, 4);
-                                biased_zeros<DT>(zw[i], held, even[i], odd[i]);
-                            } else {
-                                biased_zeros<DT>(8u, 0, even[i], odd[i]);
-                            }
-                        }
+                for (int h = 0; h < 2; ++h) {
+                    if (held % 2 == 0) pair[h] = __shfl_sync(0xffffffffu, sc[h][held >> 1], i / kHeld, 4);
+                    if constexpr (Z) {
+                        if (held == 0) zw[h] = __shfl_sync(0xffffffffu, zr[h], i / kHeld, 4);
+                        biased_zeros<DT>(zw[h], held, even[h], odd[h]);
+                    } else {
+                        biased_zeros<DT>(8u, 0, even[h], odd[h]);
                     }
+                }
+                float acc[NT][4];
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
                     uint4 xv[NT];
 #pragma unroll
-                    for (int c = 0; c < NT; ++c)
-                        xv[c] = *reinterpret_cast<const uint4*>(smem + x_lane[c] + x_at);
-                    x_at += x_block;
-                    const uint8_t* at = smem + (q_lane ^ (uint32_t)(b * 16));
-                    const uint32_t lo = *reinterpret_cast<const uint32_t*>(at);
-                    const uint32_t hi = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
+                    for (int c = 0; c < NT; ++c) {
+                        xv[c] = lds128(x_at[c]);
+                        x_at[c] += x_block;
+                    }
                     uint32_t lo_pairs[4], hi_pairs[4];
-                    biased_pairs<DT>(lo, lo_pairs);
-                    biased_pairs<DT>(hi, hi_pairs);
+                    biased_pairs<DT>(lo[i][w], lo_pairs);
+                    biased_pairs<DT>(hi[i][w], hi_pairs);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t a[4] = {sub2<DT>(lo_pairs[2 * h], even[0]), sub2<DT>(hi_pairs[2 * h], even[1]),
@@ -359,28 +359,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                sub2<DT>(hi_pairs[2 * h + 1], odd[1])};
 #pragma unroll
                         for (int c = 0; c < NT; ++c)
-                            mma_16816<DT>(acc[c], a, h ? xv[c].z : xv[c].x, h ? xv[c].w : xv[c].y);
-                    }
-                    if (b % GB == GB - 1) {
-                        const int held = GB == 8 ? 0 : (b / GB) % kHeld;
-                        const float s0 = scale_of<DT>(pair[0], held & 1), s1 = scale_of<DT>(pair[1], held & 1);
-#pragma unroll
-                        for (int c = 0; c < NT; ++c)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) sum[c][i] = fmaf(i < 2 ? s0 : s1, acc[c][i], sum[c][i]);
+                            mma_16816<DT>(acc[c], a, h ? xv[c].z : xv[c].x, h ? xv[c].w : xv[c].y, w == 0 && h == 0);
                     }
                 }
-                __syncwarp();  // all threads have read the box
-                if (a_left > 0) {
-                    if (!failed) issue(a_box, a_row, job.e, slot);
-                    --a_left;
-                    if (++a_box == num_box) {
-                        a_box = 0;
-                        ++a_row;
-                    }
-                }
-                phase ^= 1u << slot;
-                if (++slot == sh.depth) slot = 0;
+                load_step(i);
+                const float s_lo = scale_of<DT>(pair[0], held & 1), s_hi = scale_of<DT>(pair[1], held & 1);
+#pragma unroll
+                for (int c = 0; c < NT; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum[c][j] = fmaf(j < 2 ? s_lo : s_hi, acc[c][j], sum[c][j]);
             }
             if (row_done || left == 0) {  // this warp is done with the row
                 // (warp, row) pairs of a job go up one at a time, so their sums are places of their own
@@ -400,15 +387,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Job next = job_at(job.first + job.rows);
         begin(next);
         __syncthreads();
-        const int boxes = job.rows * num_box;
+        const int packs = job.rows * num_pack;
         for (int i = threadIdx.x; i < job.rows * tokens * kRows; i += kThreads) {
-            const int in_row = i % (tokens * kRows), row = i / (tokens * kRows);
-            const int token = in_row / kRows, n = (job.row + row) * kRows + in_row % kRows;
-            // warp w has box p when boxes * w / 16 <= p < boxes * (w + 1) / 16 (whole quotients)
-            const int w0 = (kWarps * (row * num_box + 1) - 1) / boxes, w1 = (kWarps * (row + 1) * num_box - 1) / boxes;
+            const int in_row = i % (tokens * kRows), r = i / (tokens * kRows);
+            const int token = in_row / kRows, n = (job.row + r) * kRows + in_row % kRows;
+            // warp w has pack p when packs * w / 16 <= p < packs * (w + 1) / 16 (whole quotients)
+            const int w0 = (kWarps * (r * num_pack + 1) - 1) / packs, w1 = (kWarps * (r + 1) * num_pack - 1) / packs;
             float v = 0.0f;
             for (int w = w0; w <= w1; ++w)
-                if (first_box(job.rows, w) < first_box(job.rows, w + 1)) v += red[(w + row) * part + in_row];
+                if (first_pack(job.rows, w) < first_pack(job.rows, w + 1)) v += red[(w + r) * part + in_row];
             if (n < sh.n) out[(size_t)(row0 + token) * sh.n + n] = round16<DT>(v);
         }
         __syncthreads();
@@ -417,23 +404,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------ host side
-template <int DT, int NT, int GB, bool Z, bool V>
-static int launch_kernel(const CUtensorMap& tmQ, const void* x, const void* scales, const void* zeros,
-                         const int* offsets, void* out, Shape sh, int dev, cudaStream_t stream) {
+struct Operands {
+    const void *x, *q, *scales, *zeros;
+    const int* offsets;
+    void* out;
+};
+
+template <int DT, int NT, int W, bool Z, bool V>
+static int launch_kernel(const Operands& op, Shape sh, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
-    constexpr size_t kMaxSmem = 226 * 1024;
+    constexpr size_t kMaxSmem = 226 * 1024, kMaxX = 160 * 1024;
     if (dev >= 64 || !attr_set[dev]) {
-        TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, NT, GB, Z, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, NT, W, Z, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)kMaxSmem));
         if (dev < 64) attr_set[dev] = true;
     }
-    const int num_box = (sh.k + kBoxK - 1) / kBoxK;
-    sh.tokens = std::min({sh.rows, NT * 8, 256 / num_box});  // x takes at most 128 KiB
-    const size_t fixed = 1024 + (size_t)num_box * 512 * sh.tokens +
-                         (size_t)(kWarps + kJobRows) * sh.tokens * kRows * 4 + (size_t)(3 * sh.groups + 1) * 4;
-    const size_t slots = (size_t)kWarps * kBoxBytes;  // one box for each warp
-    sh.depth = (int)std::min<size_t>(4, (kMaxSmem - fixed) / slots);
-    const size_t smem = fixed + sh.depth * slots;
+    const size_t row_bytes = (size_t)(sh.k + kPackK - 1) / kPackK * kPackK * 2;
+    sh.tokens = std::min({sh.rows, NT * 8, (int)(kMaxX / row_bytes)});
+    const size_t smem = row_bytes * sh.tokens + (size_t)(kWarps + kJobRows) * sh.tokens * kRows * 4 +
+                        (size_t)(3 * sh.groups + 1) * 4;
     const int64_t rows_n = (sh.n + kRows - 1) / kRows;
     const int64_t tiles = rows_n * ((int64_t)sh.rows / sh.tokens + std::min(sh.groups, sh.rows));
     if (tiles > INT32_MAX) {
@@ -450,49 +439,35 @@ static int launch_kernel(const CUtensorMap& tmQ, const void* x, const void* scal
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemv_w4_kernel<DT, NT, GB, Z, V>, tmQ, static_cast<const uint16_t*>(x),
-                                static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros), offsets,
-                                static_cast<uint16_t*>(out), sh));
+    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemv_w4_kernel<DT, NT, W, Z, V>, static_cast<const uint8_t*>(op.q),
+                                static_cast<const uint16_t*>(op.x), static_cast<const uint16_t*>(op.scales),
+                                static_cast<const uint8_t*>(op.zeros), op.offsets, static_cast<uint16_t*>(op.out), sh));
     return TRB_OK;
 }
 
-template <int DT, int NT, int GB, bool Z>
-static int launch_scales(const CUtensorMap& tmQ, const void* x, const void* scales, const void* zeros,
-                         const int* offsets, void* out, const Shape& sh, int dev, cudaStream_t stream) {
-    constexpr int kHeld = held_scales(GB);
-    const bool vector = kHeld > 1 && sh.k_groups % kHeld == 0 &&
-                        reinterpret_cast<uintptr_t>(scales) % (2 * kHeld) == 0 &&
-                        reinterpret_cast<uintptr_t>(zeros) % kHeld == 0;
-    if constexpr (kHeld > 1)
-        if (vector) return launch_kernel<DT, NT, GB, Z, true>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-    return launch_kernel<DT, NT, GB, Z, false>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-}
-
 template <int DT, int NT, bool Z>
-static int launch_group(const void* x, const void* q, const void* scales, const void* zeros, const int* offsets,
-                        void* out, const Shape& sh, int dev, cudaStream_t stream) {
-    CUtensorMap tmQ;
-    const uint64_t extent[3] = {(uint64_t)sh.k / 2, (uint64_t)sh.n, (uint64_t)sh.groups};
-    const uint32_t box[3] = {128, kRows, 1};
-    const int rc = gemm::encode_tiled(&tmQ, q, 1, 3, extent, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc != TRB_OK) return rc;
+static int launch_group(const Operands& op, const Shape& sh, int dev, cudaStream_t stream) {
+    auto vector = [&](int held) {
+        return sh.k_groups % held == 0 && reinterpret_cast<uintptr_t>(op.scales) % (2 * held) == 0 &&
+               reinterpret_cast<uintptr_t>(op.zeros) % held == 0;
+    };
     switch (sh.group_log2) {
-        case 5: return launch_scales<DT, NT, 1, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        case 6: return launch_scales<DT, NT, 2, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        case 7: return launch_scales<DT, NT, 4, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
-        default: return launch_scales<DT, NT, 8, Z>(tmQ, x, scales, zeros, offsets, out, sh, dev, stream);
+        case 5:
+            return vector(4) ? launch_kernel<DT, NT, 1, Z, true>(op, sh, dev, stream)
+                             : launch_kernel<DT, NT, 1, Z, false>(op, sh, dev, stream);
+        case 6:
+            return vector(2) ? launch_kernel<DT, NT, 2, Z, true>(op, sh, dev, stream)
+                             : launch_kernel<DT, NT, 2, Z, false>(op, sh, dev, stream);
+        default: return launch_kernel<DT, NT, 4, Z, false>(op, sh, dev, stream);
     }
 }
 
 template <int DT>
-static int launch(const void* x, const void* q, const void* scales, const void* zeros, const int* offsets, void* out,
-                  const Shape& sh, int dev, cudaStream_t stream) {
+static int launch(const Operands& op, const Shape& sh, int dev, cudaStream_t stream) {
     // More than 8 rows a group on average: 16 rows at once read the weights half as often.
     if (sh.rows > 8 * (int64_t)sh.groups)
-        return zeros ? launch_group<DT, 2, true>(x, q, scales, zeros, offsets, out, sh, dev, stream)
-                     : launch_group<DT, 2, false>(x, q, scales, zeros, offsets, out, sh, dev, stream);
-    return zeros ? launch_group<DT, 1, true>(x, q, scales, zeros, offsets, out, sh, dev, stream)
-                 : launch_group<DT, 1, false>(x, q, scales, zeros, offsets, out, sh, dev, stream);
+        return op.zeros ? launch_group<DT, 2, true>(op, sh, dev, stream) : launch_group<DT, 2, false>(op, sh, dev, stream);
+    return op.zeros ? launch_group<DT, 1, true>(op, sh, dev, stream) : launch_group<DT, 1, false>(op, sh, dev, stream);
 }
 
 int read_error(bool clear) {
@@ -549,6 +524,6 @@ extern "C" int trb_gemv_w4_launch(int dtype, int groups, int rows, int n, int k,
     sh.k_groups = k / group_size;
     while ((1 << sh.group_log2) < group_size) ++sh.group_log2;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return dtype == TRB_BFLOAT16 ? w4::launch<TRB_BFLOAT16>(x, q, scales, zeros, offsets, out, sh, dev, s)
-                                 : w4::launch<TRB_FLOAT16>(x, q, scales, zeros, offsets, out, sh, dev, s);
+    const w4::Operands op = {x, q, scales, zeros, offsets, out};
+    return dtype == TRB_BFLOAT16 ? w4::launch<TRB_BFLOAT16>(op, sh, dev, s) : w4::launch<TRB_FLOAT16>(op, sh, dev, s);
 }
