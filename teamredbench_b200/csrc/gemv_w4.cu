@@ -50,7 +50,7 @@ constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;      // outputs of a row of a job
 constexpr int kPackK = 512;    // k of a pack
-constexpr int kJobRows = 16;   // rows of 16 outputs in a job, at most
+constexpr int kJobRows = 32;   // rows of 16 outputs in a job, at most
 
 struct Shape {
     int groups, rows, n, k;
@@ -88,13 +88,13 @@ template <int W>
 __device__ __forceinline__ void load_words(const uint8_t* p, bool in, uint32_t (&v)[W]) {
     if (!in) return;
     if constexpr (W == 4)
-        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+        asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                      : "l"(p));
     else if constexpr (W == 2)
-        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+        asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
     else
-        asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+        asm volatile("ld.global.nc.L2::256B.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
 }
 
 // Pair p of a word of eight q: (q[p], q[p + 4]) as two 16-bit floats.  bf16: 128 + q each.  f16 has mantissa bits
@@ -413,7 +413,7 @@ struct Operands {
 template <int DT, int NT, int W, bool Z, bool V>
 static int launch_kernel(const Operands& op, Shape sh, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
-    constexpr size_t kMaxSmem = 226 * 1024, kMaxX = 160 * 1024;
+    constexpr size_t kMaxSmem = 226 * 1024, kMaxX = 128 * 1024;
     if (dev >= 64 || !attr_set[dev]) {
         TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, NT, W, Z, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)kMaxSmem));
