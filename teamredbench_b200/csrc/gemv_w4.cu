@@ -283,16 +283,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             row0 = table.start[job.e] + first;
             tokens = min(sh.tokens, table.rows[job.e] - first);
             uint4* x_out = reinterpret_cast<uint4*>(smem);
-            const int pieces = num_pack * (kPackK / 8);
-#pragma unroll 8
-            for (int i = threadIdx.x; i < pieces * tokens; i += kThreads) {
-                const int c = i / pieces, j = i - c * pieces;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (j * 8 < sh.k) v = __ldg(reinterpret_cast<const uint4*>(x + (size_t)(row0 + c) * sh.k + j * 8));
+            for (int j = threadIdx.x; j < num_pack * (kPackK / 8); j += kThreads) {
+                const bool in = j * 8 < sh.k;
+                const uint4* src = reinterpret_cast<const uint4*>(x + (size_t)row0 * sh.k) + j;
                 const int step = j / (4 * W), of = j / W % 4, w = j % W;
-                x_out[((step * W + w) * tokens + c) * 4 + of] =
-                    make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                               __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+                uint4* dst = x_out + (step * W + w) * tokens * 4 + of;
+#pragma unroll 8
+                for (int c = 0; c < tokens; ++c) {
+                    const uint4 v = in ? __ldg(src + (size_t)c * (sh.k / 8)) : make_uint4(0, 0, 0, 0);
+                    dst[c * 4] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                                            __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+                }
             }
             __syncthreads();
         }
