@@ -23,7 +23,8 @@ namespace grouped {
 
 __device__ int g_grouped_error;
 
-constexpr int kThreads = 192;        // producer warp, MMA warp, 4 epilogue warps
+constexpr int kEpiWarps = 8;         // two for each quarter of the TMEM lanes
+constexpr int kThreads = 64 + 32 * kEpiWarps;  // producer warp, MMA warp, epilogue warps
 constexpr int kBK = 64;              // 16-bit elements per 128-byte swizzle row
 constexpr int kInstrK = 16;          // K elements per tcgen05.mma
 constexpr int kStages = 6;
@@ -109,7 +110,7 @@ __device__ __forceinline__ ProductTile product_tile(int t, int groups, int num_n
     return p;
 }
 
-constexpr size_t kProductSmem = kRingBytes + 1024 + 4 * kEpiBytes;
+constexpr size_t kProductSmem = kRingBytes + 1024 + kEpiWarps * kEpiBytes;
 
 template <int DT, bool KB>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -150,7 +151,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         for (int a = 0; a < kNumAcc; ++a) {
             mbar_init(smem_u32(&accf_bar[a]), 1);
-            mbar_init(smem_u32(&acce_bar[a]), 8);  // 4 epilogue warps x 2 CTAs
+            mbar_init(smem_u32(&acce_bar[a]), 2 * kEpiWarps);  // of both CTAs
         }
         mbar_init(smem_u32(&drain_bar), 1);
         abort_flag = 0;
@@ -269,13 +270,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!mbar_wait_cluster(smem_u32(&drain_bar), 0, nullptr)) atomicCAS(&g_grouped_error, 0, kErrDrainWait);
         }
     } else {
-        // ---------------- epilogue (both CTAs): warps 2..5, one TMEM lane quarter (32 columns of out) each.
-        // TMEM holds out^T, so 32 x 32 blocks go through shared memory transposed (stmatrix .trans) and leave
+        // ---------------- epilogue (both CTAs): warps 2..9, a TMEM lane quarter (32 columns of out) and every other
+        // block of 32 rows each.  TMEM holds out^T, so 32 x 32 blocks go through shared memory transposed (stmatrix .trans) and leave
         // as 64-byte runs of a row, 16 bytes a lane.
-        const int q = warp & 3;
+        const int q = warp & 3, first_block = (warp - 2) >> 2;
         const uint32_t acce_leader0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
         const uint32_t acce_leader1 = mapa_shared(smem_u32(&acce_bar[1]), 0);
-        const uint32_t buf = sEpi + (uint32_t)(q * kEpiBytes);
+        const uint32_t buf = sEpi + (uint32_t)((warp - 2) * kEpiBytes);
         // block row j is 64 bytes; its 16-byte piece i stands at i ^ ((j >> 1) & 3), free of bank conflicts both ways
         const uint32_t st_row = buf + (uint32_t)((lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) * 16));
         const uint32_t ld_row = buf + (uint32_t)((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) * 16));
@@ -297,7 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int col = p.n0 + (int)rank * 128 + q * 32 + (lane & 3) * 8;
             uint16_t* out_lane = out + (size_t)(p.row0 + (lane >> 2)) * N + col;
 #pragma unroll 1
-            for (int c = 0; c * 32 < p.rows; ++c) {
+            for (int c = first_block; c * 32 < p.rows; c += 2) {
                 uint32_t lo[16], hi[16];  // TMEM lanes 0..15 and 16..31 of the quarter, 32 rows of out
                 tmem_ld_16x256b_x4(t_tile + (uint32_t)(c * 32), lo);
                 tmem_ld_16x256b_x4(t_tile + (16u << 16) + (uint32_t)(c * 32), hi);
@@ -368,18 +369,22 @@ __device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, con
 }
 
 constexpr int kWgradThreads = kThreads + 32;  // and the fixer warp
-constexpr size_t kWgradSmem = kRingBytes + 1024 + 4 * 2 * kEpiBytes;
+constexpr int kWgradBox = 32 * 128;              // 32 rows x 64 results of the gradient
+// Ring, staging, groups.  Six stages up to a few hundred groups, then five.
+constexpr size_t wgrad_smem(int stages, int groups) {
+    return (size_t)stages * 2 * kOperandStage + kEpiWarps * kWgradBox + (size_t)groups * 8;
+}
+constexpr size_t kMaxDynamicSmem = 226 * 1024;
 
 template <int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmG,
                          const __grid_constant__ CUtensorMap tmOut, const int* __restrict__ offsets, int groups,
-                         int total_rows, int N, int K) {
+                         int total_rows, int N, int K, int stages) {
     constexpr uint32_t kIdesc = make_idesc<DT>(256, true, true) | ((uint32_t)(256 >> 3) << 17);
     constexpr uint32_t kBox = 64 * 128;  // 64 rows x 64 columns
 
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ int group_words[2 * kMaxGroups];
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kStages];   // leader: the stage is ready in both CTAs
     __shared__ __align__(8) uint64_t part_bar[kStages];   // both: this CTA's bytes of a stage to be fixed have landed
     __shared__ __align__(8) uint64_t empty_bar[kStages];  // both: MMA finished reading the stage
@@ -389,10 +394,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
 
-    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sA = smem_base;
-    const uint32_t sG = smem_base + kStages * kOperandStage;
-    const uint32_t sEpi = smem_base + (uint32_t)kRingBytes;
+    const uint32_t sA = smem_u32(smem_raw);
+    const uint32_t sG = sA + stages * kOperandStage;
+    const uint32_t sEpi = sG + stages * kOperandStage;
+    int* group_words = reinterpret_cast<int*>(smem_raw + 2 * stages * kOperandStage + kEpiWarps * kWgradBox);
 
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
@@ -402,17 +407,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     const int num_pairs = gridDim.x >> 1;
     const int num_m = (K + 255) / 256;
     const int num_n = (N + 255) / 256;
-    const GroupTable table = {group_words, group_words + kMaxGroups, nullptr};
+    const GroupTable table = {group_words, group_words + groups, nullptr};
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(smem_u32(&full_bar[s]), 2);  // leader's producer twice, or one fixer per CTA
             mbar_init(smem_u32(&part_bar[s]), 1);
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
         for (int a = 0; a < kNumAcc; ++a) {
             mbar_init(smem_u32(&accf_bar[a]), 1);
-            mbar_init(smem_u32(&acce_bar[a]), 8);
+            mbar_init(smem_u32(&acce_bar[a]), 2 * kEpiWarps);
         }
         mbar_init(smem_u32(&drain_bar), 1);
         abort_flag = 0;
@@ -475,14 +480,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                     }
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-                    if (++stage == kStages) {
+                    if (++stage == stages) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
             }
             if (leader)  // every armed phase completes only once both CTAs' bytes have landed
-                for (int s = 0; s < kStages; ++s)
+                for (int s = 0; s < stages; ++s)
                     if (issued_mask & (1u << s))
                         if (!mbar_wait_cluster(smem_u32(&full_bar[s]), (issued_phase >> s) & 1u, nullptr))
                             atomicCAS(&g_grouped_error, 0, kErrDrainWait);
@@ -522,7 +527,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                                          g_desc0 + off + (uint64_t)(ks * kInstrK * 128 >> 4), kIdesc,
                                          (done != 0 || ks != 0) ? 1u : 0u);
                     tc_commit_pair_multicast(smem_u32(&empty_bar[stage]), 0x3);
-                    if (++stage == kStages) {
+                    if (++stage == stages) {
                         stage = 0;
                         phase ^= 1u;
                     }
@@ -540,10 +545,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         bool ok = true;
         for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
             const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
-            const int stages = (w.rows + kBK - 1) / kBK;
-            const int left = w.rows - (stages - 1) * kBK;  // rows of the last stage (of none: > kBK)
-            if (stages > 0 && left % kInstrK != 0) {
-                const uint32_t s = (stage + (uint32_t)(stages - 1)) % kStages;
+            const int blocks = (w.rows + kBK - 1) / kBK;
+            const int left = w.rows - (blocks - 1) * kBK;  // rows of the last block
+            if (blocks > 0 && left % kInstrK != 0) {
+                const uint32_t s = (stage + (uint32_t)(blocks - 1)) % (uint32_t)stages;
                 ok = mbar_wait(smem_u32(&part_bar[s]), (part_phase >> s) & 1u, &abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
@@ -567,16 +572,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(full_leader0 + s * 8);
             }
-            stage = (stage + (uint32_t)stages) % kStages;
+            stage = (stage + (uint32_t)blocks) % (uint32_t)stages;
         }
     } else {
-        // ---------------- epilogue (both CTAs): warps 2..5 read this CTA's 128 accumulator rows
-        const int q = warp & 3;
+        // ---------------- epilogue (both CTAs): warps 2..9 read this CTA's 128 accumulator rows, 32 rows and 128
+        // columns each, and store them in boxes of 32 x 64 by TMA, which clips at K and N
+        const int q = warp & 3, half = (warp - 2) >> 2;
         const uint32_t acce_leader0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
         const uint32_t acce_leader1 = mapa_shared(smem_u32(&acce_bar[1]), 0);
-        const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16);
+        const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
+        const uint32_t buf = sEpi + (uint32_t)((warp - 2) * kWgradBox);
         int t_local = 0;
-        uint32_t boxes = 0;  // TMA-store boxes this warp has issued (selects its staging buffer)
         for (int tile = pair; tile < num_tiles; tile += num_pairs) {
             const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
             const int acc = t_local & 1;
@@ -593,41 +599,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                 tc_fence_after();
             }
             const int row0 = w.m0 + (int)rank * 128 + q * 32;
-#pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-                uint32_t r[32];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t packed[32];
                 if (w.rows > 0) {
-                    tmem_ld_32x32b_x32(t_quarter + (uint32_t)(acc * 256 + c * 32), r);
+                    uint32_t r[64];
+                    tmem_ld_32x32b_x64(t_quarter + (uint32_t)(acc * 256 + c * 64), r);
                     tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) packed[i] = pack2<DT>(r[2 * i], r[2 * i + 1]);
+                    if (c == 1) {  // the accumulator is read out: the next tile but one may have it
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(acc ? acce_leader1 : acce_leader0);
+                    }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) r[i] = 0;
+                    for (int i = 0; i < 32; ++i) packed[i] = 0;
                 }
-                const int col = w.n0 + c * 32;
+                const int col = w.n0 + half * 128 + c * 64;
                 if (row0 >= K || col >= N) continue;  // warp-uniform: the box lies outside the gradient
-                const uint32_t buf = sEpi + (uint32_t)((q * 2 + (int)(boxes & 1u)) * kEpiBytes);
-                if (lane == 0) bulk_wait_read<1>();  // the store issued two boxes ago has read `buf`
+                if (lane == 0) bulk_wait_read<0>();   // the store before this one has read `buf`
                 __syncwarp();
-                // the 64-byte swizzle of the output's tensor map: piece j of row `lane` at j ^ ((lane >> 1) & 3)
+                // the 128-byte swizzle of the output's tensor map: piece j of row `lane` at j ^ (lane & 7)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    st_shared_v4(buf + (uint32_t)(lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)),
-                                 pack2<DT>(r[8 * j], r[8 * j + 1]), pack2<DT>(r[8 * j + 2], r[8 * j + 3]),
-                                 pack2<DT>(r[8 * j + 4], r[8 * j + 5]), pack2<DT>(r[8 * j + 6], r[8 * j + 7]));
+                for (int j = 0; j < 8; ++j)
+                    st_shared_v4(buf + (uint32_t)(lane * 128 + ((j ^ (lane & 7)) * 16)), packed[4 * j],
+                                 packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
                     tma_store_3d(&tmOut, buf, col, row0, w.e);
                     bulk_commit();
                 }
-                ++boxes;
             }
-            if (w.rows > 0) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(acc ? acce_leader1 : acce_leader0);
-                ++t_local;
-            }
+            if (w.rows > 0) ++t_local;
         }
         if (lane == 0) bulk_wait_all();  // this warp's TMA stores are complete before teardown
         __syncwarp();
@@ -644,10 +650,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
 
 // ------------------------------------------------------------------ host side
 template <typename Kernel, typename... Args>
-static int launch_kernel(Kernel kernel, int grid, int threads, size_t smem, int dev, bool (&attr_set)[64],
-                         cudaStream_t stream, Args... args) {
+static int launch_kernel(Kernel kernel, int grid, int threads, size_t smem, size_t max_smem, int dev,
+                         bool (&attr_set)[64], cudaStream_t stream, Args... args) {
     if (dev >= 64 || !attr_set[dev]) {
-        TRB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        TRB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)max_smem));
         if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
@@ -716,8 +722,8 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
         set_error("trb_grouped_gemm_launch: too many tiles (rows=%d n=%d groups=%d)", rows, n, groups);
         return TRB_SKIPPED;
     }
-    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, kProductSmem, dev, attr_set,
-                         stream, tmW, tmX128, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
+    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, kProductSmem, kProductSmem, dev,
+                         attr_set, stream, tmW, tmX128, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
 template <int DT>
@@ -729,18 +735,19 @@ static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const
     const uint64_t extent_rows = (uint64_t)std::max(rows, 1);
     const uint64_t ae[2] = {(uint64_t)k, extent_rows}, ge[2] = {(uint64_t)n, extent_rows};
     const uint64_t oe[3] = {(uint64_t)n, (uint64_t)k, (uint64_t)groups};
-    const uint32_t box[2] = {64, 64}, obox[3] = {32, 32, 1};
+    const uint32_t box[2] = {64, 64}, obox[3] = {64, 32, 1};
     int rc = gemm::encode_tiled(&tmA, rows > 0 ? a : out, 2, 2, ae, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmG, rows > 0 ? g : out, 2, 2, ge, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmOut, out, 2, 3, oe, obox, CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmOut, out, 2, 3, oe, obox, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
     const int64_t tiles = (int64_t)groups * ((k + 255) / 256) * ((n + 255) / 256);
     if (tiles > INT32_MAX) {
         set_error("trb_grouped_wgrad_launch: too many tiles (groups=%d n=%d k=%d)", groups, n, k);
         return TRB_SKIPPED;
     }
-    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, kWgradSmem, dev, attr_set,
-                         stream, tmA, tmG, tmOut, offsets, groups, rows, n, k);
+    const int stages = wgrad_smem(kStages, groups) <= kMaxDynamicSmem ? kStages : kStages - 1;
+    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, wgrad_smem(stages, groups),
+                         kMaxDynamicSmem, dev, attr_set, stream, tmA, tmG, tmOut, offsets, groups, rows, n, k, stages);
 }
 
 int read_error(bool clear) {
