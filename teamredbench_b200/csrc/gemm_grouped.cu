@@ -62,6 +62,12 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t r0, ui
                  "r"(r1), "r"(r2), "r"(r3)
                  : "memory");
 }
+// The same without transposing: thread 8i + j gives the 16-byte row that takes row j of block i.
+__device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0), "r"(r1),
+                 "r"(r2), "r"(r3)
+                 : "memory");
+}
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr)
@@ -369,7 +375,7 @@ __device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, con
 }
 
 constexpr int kWgradThreads = kThreads + 32;  // and the fixer warp
-constexpr int kWgradBox = 32 * 128;              // 32 rows x 64 results of the gradient
+constexpr int kWgradBox = 16 * 256;              // 16 rows x 128 results of the gradient
 // Ring, staging, groups.  Six stages up to a few hundred groups, then five.
 constexpr size_t wgrad_smem(int stages, int groups) {
     return (size_t)stages * 2 * kOperandStage + kEpiWarps * kWgradBox + (size_t)groups * 8;
@@ -379,8 +385,8 @@ constexpr size_t kMaxDynamicSmem = 226 * 1024;
 template <int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmG,
-                         const __grid_constant__ CUtensorMap tmOut, const int* __restrict__ offsets, int groups,
-                         int total_rows, int N, int K, int stages) {
+                         const int* __restrict__ offsets, uint16_t* __restrict__ out, int groups, int total_rows, int N,
+                         int K, int stages) {
     constexpr uint32_t kIdesc = make_idesc<DT>(256, true, true) | ((uint32_t)(256 >> 3) << 17);
     constexpr uint32_t kBox = 64 * 128;  // 64 rows x 64 columns
 
@@ -417,14 +423,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         }
         for (int a = 0; a < kNumAcc; ++a) {
             mbar_init(smem_u32(&accf_bar[a]), 1);
-            mbar_init(smem_u32(&acce_bar[a]), 2 * kEpiWarps);
+            mbar_init(smem_u32(&acce_bar[a]), 8);  // the four warps that read it, of both CTAs
         }
         mbar_init(smem_u32(&drain_bar), 1);
         abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmG);
-        tma_prefetch_desc(&tmOut);
     }
     if (warp == 0) {
         tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
@@ -575,19 +580,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
             stage = (stage + (uint32_t)blocks) % (uint32_t)stages;
         }
     } else {
-        // ---------------- epilogue (both CTAs): warps 2..9 read this CTA's 128 accumulator rows, 32 rows and 128
-        // columns each, and store them in boxes of 32 x 64 by TMA, which clips at K and N
-        const int q = warp & 3, half = (warp - 2) >> 2;
-        const uint32_t acce_leader0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
-        const uint32_t acce_leader1 = mapa_shared(smem_u32(&acce_bar[1]), 0);
-        const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * 128);
+        // ---------------- epilogue (both CTAs): warps 2..5 read the first accumulator, warps 6..9 the second, 32 rows
+        // of the tile each, so that one tile is read out of TMEM while another waits on its stores.  Blocks of 16 x 128
+        // go through shared memory (stmatrix) and leave as 256-byte runs, the two of a row one after the other: where N
+        // is not a multiple of 16, rows begin in the middle of a sector and every end of a run is a part of one.
+        const int q = warp & 3, group = (warp - 2) >> 2;
+        const uint32_t acce_leader = mapa_shared(smem_u32(&acce_bar[group]), 0);
+        const uint32_t t_rows = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(group * 256);
         const uint32_t buf = sEpi + (uint32_t)((warp - 2) * kWgradBox);
-        int t_local = 0;
+        // 16-byte piece i of row r stands at i ^ (r & 7), free of bank conflicts both ways
+        const uint32_t st_row = buf + (uint32_t)((lane & 15) * 256);
+        int t_local = 0, empty = 0;  // tiles with products, and without
         for (int tile = pair; tile < num_tiles; tile += num_pairs) {
             const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
-            const int acc = t_local & 1;
-            if (w.rows > 0) {
-                bool ok = mbar_wait_cluster(smem_u32(&accf_bar[acc]), (uint32_t)(t_local >> 1) & 1u, &abort_flag);
+            const bool products = w.rows > 0;
+            const int count = products ? t_local++ : empty++;
+            if ((count & 1) != group) continue;
+            if (products) {
+                bool ok = mbar_wait_cluster(smem_u32(&accf_bar[group]), (uint32_t)(count >> 1) & 1u, &abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
                     if (lane == 0) {
@@ -600,43 +610,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
             }
             const int row0 = w.m0 + (int)rank * 128 + q * 32;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t packed[32];
-                if (w.rows > 0) {
-                    uint32_t r[64];
-                    tmem_ld_32x32b_x64(t_quarter + (uint32_t)(acc * 256 + c * 64), r);
-                    tmem_wait_ld();
+            for (int b = 0; b < 4; ++b) {  // rows 16 (b / 2), columns 128 (b % 2)
+                const int h = b >> 1, c = b & 1;
+                uint32_t packed[4][8];
+                if (products) {
+                    uint32_t r[4][16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) packed[i] = pack2<DT>(r[2 * i], r[2 * i + 1]);
-                    if (c == 1) {  // the accumulator is read out: the next tile but one may have it
+                    for (int j = 0; j < 4; ++j)
+                        tmem_ld_16x256b_x4(t_rows + ((uint32_t)(h * 16) << 16) + (uint32_t)(c * 128 + j * 32), r[j]);
+                    tmem_wait_ld();
+                    if (b == 3) {  // the accumulator is read out: the next tile but one may have it
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(acc ? acce_leader1 : acce_leader0);
+                        if (lane == 0) mbar_arrive_cluster(acce_leader);
                     }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) packed[j][i] = pack2<DT>(r[j][2 * i], r[j][2 * i + 1]);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) packed[i] = 0;
-                }
-                const int col = w.n0 + half * 128 + c * 64;
-                if (row0 >= K || col >= N) continue;  // warp-uniform: the box lies outside the gradient
-                if (lane == 0) bulk_wait_read<0>();   // the store before this one has read `buf`
-                __syncwarp();
-                // the 128-byte swizzle of the output's tensor map: piece j of row `lane` at j ^ (lane & 7)
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    st_shared_v4(buf + (uint32_t)(lane * 128 + ((j ^ (lane & 7)) * 16)), packed[4 * j],
-                                 packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
-                fence_proxy_async_smem();
+                        for (int i = 0; i < 8; ++i) packed[j][i] = 0;
+                }
+                const int rows_left = K - row0 - h * 16;
+                if (rows_left <= 0 || w.n0 + c * 128 >= N) continue;  // warp-uniform: outside the gradient
+                __syncwarp();  // the block before has been read out of buf
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int o = 0; o < 2; ++o)  // column octets 4j + 2o and the next, rows 0..7 and 8..15 of each
+                        stmatrix_x4(st_row + (uint32_t)(((j * 4 + o * 2 + (lane >> 4)) ^ (lane & 7)) * 16),
+                                    packed[j][4 * o], packed[j][4 * o + 1], packed[j][4 * o + 2], packed[j][4 * o + 3]);
                 __syncwarp();
-                if (lane == 0) {
-                    tma_store_3d(&tmOut, buf, col, row0, w.e);
-                    bulk_commit();
+                const int col = w.n0 + c * 128 + (lane & 15) * 8;
+                uint16_t* dst = out + ((size_t)w.e * K + row0 + h * 16 + (lane >> 4)) * N + col;
+                if (col < N) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int row = i * 2 + (lane >> 4);
+                        if (row < rows_left)
+                            *reinterpret_cast<uint4*>(dst + (size_t)(i * 2) * N) =
+                                ld_shared_v4(buf + (uint32_t)(row * 256 + (((lane & 15) ^ (row & 7)) * 16)));
+                    }
                 }
             }
-            if (w.rows > 0) ++t_local;
         }
-        if (lane == 0) bulk_wait_all();  // this warp's TMA stores are complete before teardown
-        __syncwarp();
     }
 
     tc_fence_before();
@@ -730,15 +750,13 @@ template <int DT>
 static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const void* g, const int* offsets,
                         void* out, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
-    CUtensorMap tmA, tmG, tmOut;
+    CUtensorMap tmA, tmG;
     // Without rows no operand is read; the maps then stand on the output, which is there.
     const uint64_t extent_rows = (uint64_t)std::max(rows, 1);
     const uint64_t ae[2] = {(uint64_t)k, extent_rows}, ge[2] = {(uint64_t)n, extent_rows};
-    const uint64_t oe[3] = {(uint64_t)n, (uint64_t)k, (uint64_t)groups};
-    const uint32_t box[2] = {64, 64}, obox[3] = {64, 32, 1};
+    const uint32_t box[2] = {64, 64};
     int rc = gemm::encode_tiled(&tmA, rows > 0 ? a : out, 2, 2, ae, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmG, rows > 0 ? g : out, 2, 2, ge, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmOut, out, 2, 3, oe, obox, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
     const int64_t tiles = (int64_t)groups * ((k + 255) / 256) * ((n + 255) / 256);
     if (tiles > INT32_MAX) {
@@ -747,7 +765,8 @@ static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const
     }
     const int stages = wgrad_smem(kStages, groups) <= kMaxDynamicSmem ? kStages : kStages - 1;
     return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, wgrad_smem(stages, groups),
-                         kMaxDynamicSmem, dev, attr_set, stream, tmA, tmG, tmOut, offsets, groups, rows, n, k, stages);
+                         kMaxDynamicSmem, dev, attr_set, stream, tmA, tmG, offsets, static_cast<uint16_t*>(out), groups,
+                         rows, n, k, stages);
 }
 
 int read_error(bool clear) {
