@@ -375,7 +375,7 @@ __device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, con
 }
 
 constexpr int kWgradThreads = kThreads + 32;  // and the fixer warp
-constexpr int kWgradBox = 16 * 256;              // 16 rows x 128 results of the gradient
+constexpr int kWgradBox = 8 * 512;               // 8 rows x 256 results of the gradient
 // Ring, staging, groups.  Six stages up to a few hundred groups, then five.
 constexpr size_t wgrad_smem(int stages, int groups) {
     return (size_t)stages * 2 * kOperandStage + kEpiWarps * kWgradBox + (size_t)groups * 8;
@@ -581,15 +581,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         }
     } else {
         // ---------------- epilogue (both CTAs): warps 2..5 read the first accumulator, warps 6..9 the second, 32 rows
-        // of the tile each, so that one tile is read out of TMEM while another waits on its stores.  Blocks of 16 x 128
-        // go through shared memory (stmatrix) and leave as 256-byte runs, the two of a row one after the other: where N
-        // is not a multiple of 16, rows begin in the middle of a sector and every end of a run is a part of one.
+        // of the tile each, so that one tile is read out of TMEM while another waits on its stores.  8 x 256 results at a
+        // time go through shared memory (stmatrix) and leave as whole rows of the tile, 512 bytes a store: where N is not
+        // a multiple of 16, rows begin in the middle of a sector and each end of a run writes a part of one (64 zero
+        // gradients of 2048 x 1544: 133 us in runs of 128 bytes, 100 in runs of 256, 67 us for 2048 x 1536).
         const int q = warp & 3, group = (warp - 2) >> 2;
         const uint32_t acce_leader = mapa_shared(smem_u32(&acce_bar[group]), 0);
         const uint32_t t_rows = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(group * 256);
         const uint32_t buf = sEpi + (uint32_t)((warp - 2) * kWgradBox);
         // 16-byte piece i of row r stands at i ^ (r & 7), free of bank conflicts both ways
-        const uint32_t st_row = buf + (uint32_t)((lane & 15) * 256);
+        const uint32_t st_row = buf + (uint32_t)((lane & 7) * 512);
         int t_local = 0, empty = 0;  // tiles with products, and without
         for (int tile = pair; tile < num_tiles; tile += num_pairs) {
             const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
@@ -609,50 +610,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                 tc_fence_after();
             }
             const int row0 = w.m0 + (int)rank * 128 + q * 32;
+            const int col = w.n0 + lane * 8;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {  // rows 16 (b / 2), columns 128 (b % 2)
-                const int h = b >> 1, c = b & 1;
-                uint32_t packed[4][8];
-                if (products) {
+            for (int b = 0; b < 2; ++b) {  // rows 16 b of the 32
+                uint32_t packed[8][8];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
                     uint32_t r[4][16];
+                    if (products) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        tmem_ld_16x256b_x4(t_rows + ((uint32_t)(h * 16) << 16) + (uint32_t)(c * 128 + j * 32), r[j]);
-                    tmem_wait_ld();
-                    if (b == 3) {  // the accumulator is read out: the next tile but one may have it
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(acce_leader);
+                        for (int j = 0; j < 4; ++j)
+                            tmem_ld_16x256b_x4(t_rows + ((uint32_t)(b * 16) << 16) + (uint32_t)(c * 128 + j * 32), r[j]);
+                        tmem_wait_ld();
+                        if (b == 1 && c == 1) {  // the accumulator is read out: the next tile but one may have it
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive_cluster(acce_leader);
+                        }
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) packed[j][i] = pack2<DT>(r[j][2 * i], r[j][2 * i + 1]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) packed[j][i] = 0;
+                        for (int i = 0; i < 8; ++i)
+                            packed[c * 4 + j][i] = products ? pack2<DT>(r[j][2 * i], r[j][2 * i + 1]) : 0;
                 }
-                const int rows_left = K - row0 - h * 16;
-                if (rows_left <= 0 || w.n0 + c * 128 >= N) continue;  // warp-uniform: outside the gradient
-                __syncwarp();  // the block before has been read out of buf
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int h = 0; h < 2; ++h) {
+                    const int row_h = row0 + b * 16 + h * 8;
+                    if (row_h >= K) continue;  // warp-uniform: outside the gradient
+                    __syncwarp();  // the rows before have been read out of buf
 #pragma unroll
-                    for (int o = 0; o < 2; ++o)  // column octets 4j + 2o and the next, rows 0..7 and 8..15 of each
-                        stmatrix_x4(st_row + (uint32_t)(((j * 4 + o * 2 + (lane >> 4)) ^ (lane & 7)) * 16),
-                                    packed[j][4 * o], packed[j][4 * o + 1], packed[j][4 * o + 2], packed[j][4 * o + 3]);
-                __syncwarp();
-                const int col = w.n0 + c * 128 + (lane & 15) * 8;
-                uint16_t* dst = out + ((size_t)w.e * K + row0 + h * 16 + (lane >> 4)) * N + col;
-                if (col < N) {
+                    for (int j = 0; j < 8; ++j)  // column octets 4j .. 4j + 3
+                        stmatrix_x4(st_row + (uint32_t)(((j * 4 + (lane >> 3)) ^ (lane & 7)) * 16), packed[j][h],
+                                    packed[j][2 + h], packed[j][4 + h], packed[j][6 + h]);
+                    __syncwarp();
+                    uint16_t* dst = out + ((size_t)w.e * K + row_h) * N + col;
+                    if (col < N) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int row = i * 2 + (lane >> 4);
-                        if (row < rows_left)
-                            *reinterpret_cast<uint4*>(dst + (size_t)(i * 2) * N) =
-                                ld_shared_v4(buf + (uint32_t)(row * 256 + (((lane & 15) ^ (row & 7)) * 16)));
+                        for (int i = 0; i < 8; ++i)
+                            if (row_h + i < K)
+                                *reinterpret_cast<uint4*>(dst + (size_t)i * N) =
+                                    ld_shared_v4(buf + (uint32_t)(i * 512 + ((lane ^ i) * 16)));
                     }
                 }
             }
