@@ -27,8 +27,11 @@ constexpr int kEpiWarps = 8;         // two for each quarter of the TMEM lanes
 constexpr int kThreads = 64 + 32 * kEpiWarps;  // producer warp, MMA warp, epilogue warps
 constexpr int kBK = 64;              // 16-bit elements per 128-byte swizzle row
 constexpr int kInstrK = 16;          // K elements per tcgen05.mma
-constexpr int kStages = 6;
-constexpr int kOperandStage = 128 * 128;  // one CTA's 128 rows (or columns) x 128 bytes of one operand
+// Two k-blocks a stage: a stage costs the MMA thread about 260 ns whatever it holds (wait, issue, commit), as long as
+// the four products of one k-block with 128 rows take.
+constexpr int kStages = 3;
+constexpr int kBlockBytes = 128 * 128;    // one CTA's 128 rows (or columns) x 128 bytes of one operand: a k-block
+constexpr int kOperandStage = 2 * kBlockBytes;
 constexpr size_t kRingBytes = (size_t)kStages * 2 * kOperandStage;
 constexpr int kNumAcc = 2;
 constexpr int kTmemCols = 512;
@@ -194,7 +197,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int x_boxes = (half + 31) / 32;
                 const uint32_t x_bytes = (uint32_t)x_boxes * 32 * 128;
                 const int w_col = p.n0 + (int)rank * 128;
-                for (int kb = 0; kb < num_kb; ++kb) {
+                for (int kb = 0; kb < num_kb; kb += 2) {
+                    const int blocks = min(2, num_kb - kb);
                     if (!mbar_wait_cluster(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
                         atomicCAS(&g_grouped_error, 0, kErrProducerWait);
                         abort_flag = 1;
@@ -202,20 +206,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         break;
                     }
                     const uint32_t fb_local = smem_u32(&full_bar[stage]);
-                    if (leader) mbar_arrive_expect_tx(fb_local, 2 * (kOperandStage + x_bytes));
+                    // Row-major weights come in boxes of 128 k (past K: zeros); the other boxes are one k-block each.
+                    const uint32_t w_bytes = KB ? blocks * kBlockBytes : kOperandStage;
+                    if (leader) mbar_arrive_expect_tx(fb_local, 2 * (w_bytes + blocks * x_bytes));
                     const uint32_t fb = fb_local & kPeerBitMask;
                     const uint32_t w = sW + stage * kOperandStage, x = sX + stage * kOperandStage;
-                    if constexpr (KB) {
-                        tma_load_3d_pair(w, &tmW, fb, kb * kBK, w_col, p.e);
-                    } else {
+                    if constexpr (!KB) {
                         tma_load_3d_pair(w, &tmW, fb, w_col, kb * kBK, p.e);
-                        tma_load_3d_pair(w + kOperandStage / 2, &tmW, fb, w_col + 64, kb * kBK, p.e);
+                        tma_load_3d_pair(w + kBlockBytes, &tmW, fb, w_col + 64, kb * kBK, p.e);
                     }
-                    if (x_boxes == 4) {
-                        tma_load_2d_pair(x, &tmX128, fb, kb * kBK, x_row);
-                    } else {
-                        for (int i = 0; i < x_boxes; ++i)
-                            tma_load_2d_pair(x + (uint32_t)i * 32 * 128, &tmX32, fb, kb * kBK, x_row + i * 32);
+                    for (int i = 0; i < blocks; ++i) {
+                        if constexpr (KB) tma_load_3d_pair(w + i * kBlockBytes, &tmW, fb, (kb + i) * kBK, w_col, p.e);
+                        const uint32_t xi = x + i * kBlockBytes;
+                        if (x_boxes == 4) {
+                            tma_load_2d_pair(xi, &tmX128, fb, (kb + i) * kBK, x_row);
+                        } else {
+                            for (int j = 0; j < x_boxes; ++j)
+                                tma_load_2d_pair(xi + (uint32_t)j * 32 * 128, &tmX32, fb, (kb + i) * kBK,
+                                                 x_row + j * 32);
+                        }
                     }
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
@@ -234,9 +243,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         if (lane == 0 && leader) {
             // ---------------- MMA issuer: the leader CTA only
-            const uint64_t w_desc0 = KB ? make_sdesc(sW, 16, 1024) : make_sdesc(sW, kOperandStage / 2, 1024);
+            const uint64_t w_desc0 = KB ? make_sdesc(sW, 16, 1024) : make_sdesc(sW, kBlockBytes, 1024);
             const uint64_t x_desc0 = make_sdesc(sX, 16, 1024);
-            constexpr int kWStep = KB ? kInstrK * 2 : kInstrK * 128;  // bytes per instruction K step
+            constexpr int kWStep = KB ? kInstrK * 2 : kInstrK * 128;           // bytes per instruction K step
+            constexpr int kWBlock = KB ? kBlockBytes : kBlockBytes / 2;        // and per k-block
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             int t_local = 0;
@@ -251,7 +261,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(acc * kTileRows);
-                for (int kb = 0; kb < num_kb; ++kb) {
+                for (int kb = 0; kb < num_kb; kb += 2) {
                     if (!mbar_wait_cluster(smem_u32(&full_bar[stage]), phase, &abort_flag)) {
                         atomicCAS(&g_grouped_error, 0, kErrMmaWait);
                         abort_flag = 1;
@@ -260,10 +270,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     const uint64_t off = (uint64_t)((stage * kOperandStage) >> 4);
 #pragma unroll
-                    for (int ks = 0; ks < kBK / kInstrK; ++ks)
-                        mma_pair_f16(d_tmem, w_desc0 + off + (uint64_t)(ks * kWStep >> 4),
-                                     x_desc0 + off + (uint64_t)(ks * kInstrK * 2 >> 4), idesc,
-                                     (kb != 0 || ks != 0) ? 1u : 0u);
+                    for (int i = 0; i < 2; ++i) {
+                        if (kb + i >= num_kb) break;
+#pragma unroll
+                        for (int ks = 0; ks < kBK / kInstrK; ++ks)
+                            mma_pair_f16(d_tmem, w_desc0 + off + (uint64_t)((i * kWBlock + ks * kWStep) >> 4),
+                                         x_desc0 + off + (uint64_t)((i * kBlockBytes + ks * kInstrK * 2) >> 4), idesc,
+                                         (kb != 0 || i != 0 || ks != 0) ? 1u : 0u);
+                    }
                     tc_commit_pair_multicast(smem_u32(&empty_bar[stage]), 0x3);
                     if (++stage == kStages) {
                         stage = 0;
@@ -345,7 +359,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------ out[e] = a^T * g over the rows of e
 // A CTA pair computes 256 x 256 of one group's K x N gradient; the products run
-// over the group's rows, 64 per stage, both operands MN-major (their rows are
+// over the group's rows, 128 per stage, both operands MN-major (their rows are
 // the contraction).  The last stage of a group reaches into the next group's
 // rows (or past the end, where TMA gives zeros): products run over whole
 // 16-row steps only as far as the group goes, and the rows between its end and
@@ -358,12 +372,12 @@ struct WgradTile {
     int e, row0, rows, m0, n0;
 };
 
-__device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, const GroupTable& g) {
+__device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, const int* offsets) {
     const int per = num_m * num_n;
     WgradTile w;
     w.e = t / per;
-    w.row0 = g.start[w.e];
-    w.rows = g.rows[w.e];
+    w.row0 = offsets[w.e];
+    w.rows = offsets[w.e + 1] - w.row0;
     const int local = t - w.e * per;
     const int run = 8 * num_n;
     const int first = local / run * 8;
@@ -376,21 +390,18 @@ __device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, con
 
 constexpr int kWgradThreads = kThreads + 32;  // and the fixer warp
 constexpr int kWgradBox = 8 * 512;               // 8 rows x 256 results of the gradient
-// Ring, staging, groups.  Six stages up to a few hundred groups, then five.
-constexpr size_t wgrad_smem(int stages, int groups) {
-    return (size_t)stages * 2 * kOperandStage + kEpiWarps * kWgradBox + (size_t)groups * 8;
-}
-constexpr size_t kMaxDynamicSmem = 226 * 1024;
+constexpr size_t kWgradSmem = kRingBytes + 1024 + kEpiWarps * kWgradBox;
+constexpr int kStageRows = 2 * kBK;
 
 template <int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmG,
                          const int* __restrict__ offsets, uint16_t* __restrict__ out, int groups, int total_rows, int N,
-                         int K, int stages) {
+                         int K) {
     constexpr uint32_t kIdesc = make_idesc<DT>(256, true, true) | ((uint32_t)(256 >> 3) << 17);
-    constexpr uint32_t kBox = 64 * 128;  // 64 rows x 64 columns
+    constexpr uint32_t kBox = kBlockBytes / 2;  // 64 rows x 64 columns
 
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kStages];   // leader: the stage is ready in both CTAs
     __shared__ __align__(8) uint64_t part_bar[kStages];   // both: this CTA's bytes of a stage to be fixed have landed
     __shared__ __align__(8) uint64_t empty_bar[kStages];  // both: MMA finished reading the stage
@@ -400,10 +411,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
 
-    const uint32_t sA = smem_u32(smem_raw);
-    const uint32_t sG = sA + stages * kOperandStage;
-    const uint32_t sEpi = sG + stages * kOperandStage;
-    int* group_words = reinterpret_cast<int*>(smem_raw + 2 * stages * kOperandStage + kEpiWarps * kWgradBox);
+    const uint32_t sA = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sG = sA + kStages * kOperandStage;
+    const uint32_t sEpi = sG + kStages * kOperandStage;
 
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
@@ -413,10 +423,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     const int num_pairs = gridDim.x >> 1;
     const int num_m = (K + 255) / 256;
     const int num_n = (N + 255) / 256;
-    const GroupTable table = {group_words, group_words + groups, nullptr};
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_u32(&full_bar[s]), 2);  // leader's producer twice, or one fixer per CTA
             mbar_init(smem_u32(&part_bar[s]), 1);
             mbar_init(smem_u32(&empty_bar[s]), 1);
@@ -437,7 +446,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     }
     grid_launch_dependents();
     grid_dependency_wait();
-    groups = load_groups(offsets, groups, total_rows, table, &g_grouped_error);
+    groups = check_groups(offsets, groups, total_rows, &g_grouped_error);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();
@@ -452,47 +461,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
             uint32_t issued_mask = 0, issued_phase = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-                const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
+                const WgradTile w = wgrad_tile(tile, num_m, num_n, offsets);
                 const int a_col = w.m0 + (int)rank * 128, g_col = w.n0 + (int)rank * 128;
-                for (int done = 0; done < w.rows; done += kBK) {
+                for (int done = 0; done < w.rows; done += kStageRows) {
                     if (!mbar_wait_cluster(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
                         atomicCAS(&g_grouped_error, 0, kErrProducerWait);
                         abort_flag = 1;
                         ok = false;
                         break;
                     }
-                    const bool fix = w.rows - done < kBK && (w.rows - done) % kInstrK != 0;
+                    const int left = w.rows - done;
+                    const int blocks = left > kBK ? 2 : 1;
+                    const bool fix = left < kStageRows && left % kInstrK != 0;
                     const uint32_t a = sA + stage * kOperandStage, g = sG + stage * kOperandStage;
                     const int row = w.row0 + done;
                     if (fix) {
                         const uint32_t bar = smem_u32(&part_bar[stage]);
-                        mbar_arrive_expect_tx(bar, 4 * kBox);
-                        tma_load_2d(a, &tmA, bar, a_col, row);
-                        tma_load_2d(a + kBox, &tmA, bar, a_col + 64, row);
-                        tma_load_2d(g, &tmG, bar, g_col, row);
-                        tma_load_2d(g + kBox, &tmG, bar, g_col + 64, row);
+                        mbar_arrive_expect_tx(bar, blocks * 4 * kBox);
+                        for (int i = 0; i < blocks; ++i) {
+                            const uint32_t o = i * kBlockBytes;
+                            tma_load_2d(a + o, &tmA, bar, a_col, row + i * kBK);
+                            tma_load_2d(a + o + kBox, &tmA, bar, a_col + 64, row + i * kBK);
+                            tma_load_2d(g + o, &tmG, bar, g_col, row + i * kBK);
+                            tma_load_2d(g + o + kBox, &tmG, bar, g_col + 64, row + i * kBK);
+                        }
                     } else {
                         const uint32_t fb_local = smem_u32(&full_bar[stage]);
                         if (leader) {
-                            mbar_arrive_expect_tx(fb_local, 8 * kBox);
+                            mbar_arrive_expect_tx(fb_local, blocks * 8 * kBox);
                             mbar_arrive(fb_local);
                         }
                         const uint32_t fb = fb_local & kPeerBitMask;
-                        tma_load_2d_pair(a, &tmA, fb, a_col, row);
-                        tma_load_2d_pair(a + kBox, &tmA, fb, a_col + 64, row);
-                        tma_load_2d_pair(g, &tmG, fb, g_col, row);
-                        tma_load_2d_pair(g + kBox, &tmG, fb, g_col + 64, row);
+                        for (int i = 0; i < blocks; ++i) {
+                            const uint32_t o = i * kBlockBytes;
+                            tma_load_2d_pair(a + o, &tmA, fb, a_col, row + i * kBK);
+                            tma_load_2d_pair(a + o + kBox, &tmA, fb, a_col + 64, row + i * kBK);
+                            tma_load_2d_pair(g + o, &tmG, fb, g_col, row + i * kBK);
+                            tma_load_2d_pair(g + o + kBox, &tmG, fb, g_col + 64, row + i * kBK);
+                        }
                     }
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-                    if (++stage == stages) {
+                    if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
             }
             if (leader)  // every armed phase completes only once both CTAs' bytes have landed
-                for (int s = 0; s < stages; ++s)
+                for (int s = 0; s < kStages; ++s)
                     if (issued_mask & (1u << s))
                         if (!mbar_wait_cluster(smem_u32(&full_bar[s]), (issued_phase >> s) & 1u, nullptr))
                             atomicCAS(&g_grouped_error, 0, kErrDrainWait);
@@ -506,7 +523,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
             bool ok = true;
             int t_local = 0;
             for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-                const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
+                const WgradTile w = wgrad_tile(tile, num_m, num_n, offsets);
                 if (w.rows == 0) continue;
                 const int acc = t_local & 1;
                 if (!mbar_wait_cluster(smem_u32(&acce_bar[acc]), ((uint32_t)(t_local >> 1) & 1u) ^ 1u, &abort_flag)) {
@@ -516,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(acc * 256);
-                for (int done = 0; done < w.rows; done += kBK) {
+                for (int done = 0; done < w.rows; done += kStageRows) {
                     if (!mbar_wait_cluster(smem_u32(&full_bar[stage]), phase, &abort_flag)) {
                         atomicCAS(&g_grouped_error, 0, kErrMmaWait);
                         abort_flag = 1;
@@ -526,13 +543,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                     const uint64_t off = (uint64_t)((stage * kOperandStage) >> 4);
                     const int left = w.rows - done;
 #pragma unroll
-                    for (int ks = 0; ks < kBK / kInstrK; ++ks)
-                        if (ks * kInstrK < left)
-                            mma_pair_f16(d_tmem, a_desc0 + off + (uint64_t)(ks * kInstrK * 128 >> 4),
-                                         g_desc0 + off + (uint64_t)(ks * kInstrK * 128 >> 4), kIdesc,
-                                         (done != 0 || ks != 0) ? 1u : 0u);
+                    for (int ks = 0; ks < kStageRows / kInstrK; ++ks) {
+                        if (ks * kInstrK >= left) break;
+                        const uint64_t o = off + (uint64_t)(((ks >> 2) * kBlockBytes + (ks & 3) * kInstrK * 128) >> 4);
+                        mma_pair_f16(d_tmem, a_desc0 + o, g_desc0 + o, kIdesc, (done != 0 || ks != 0) ? 1u : 0u);
+                    }
                     tc_commit_pair_multicast(smem_u32(&empty_bar[stage]), 0x3);
-                    if (++stage == stages) {
+                    if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
                     }
@@ -549,11 +566,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         uint32_t stage = 0, part_phase = 0;  // part_phase: bit s = parity of part_bar[s]'s next use
         bool ok = true;
         for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-            const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
-            const int blocks = (w.rows + kBK - 1) / kBK;
-            const int left = w.rows - (blocks - 1) * kBK;  // rows of the last block
-            if (blocks > 0 && left % kInstrK != 0) {
-                const uint32_t s = (stage + (uint32_t)(blocks - 1)) % (uint32_t)stages;
+            const WgradTile w = wgrad_tile(tile, num_m, num_n, offsets);
+            const int stages = (w.rows + kStageRows - 1) / kStageRows;
+            const int left = w.rows - (stages - 1) * kStageRows;  // rows of the last stage
+            if (stages > 0 && left % kInstrK != 0) {
+                const uint32_t s = (stage + (uint32_t)(stages - 1)) % kStages;
                 ok = mbar_wait(smem_u32(&part_bar[s]), (part_phase >> s) & 1u, &abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
@@ -565,7 +582,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                 }
                 part_phase ^= 1u << s;
                 const int pieces = (((left + kInstrK - 1) & ~(kInstrK - 1)) - left) * 8;  // 16-byte pieces per box
-                const uint32_t first = sA + s * kOperandStage + (uint32_t)left * 128;
+                const uint32_t first = sA + s * kOperandStage + (uint32_t)(left / kBK * kBlockBytes + left % kBK * 128);
                 for (int i = lane; i < pieces; i += 32) {
                     const uint32_t at = first + (uint32_t)i * 16;
                     st_shared_v4(at, 0, 0, 0, 0);
@@ -577,7 +594,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(full_leader0 + s * 8);
             }
-            stage = (stage + (uint32_t)blocks) % (uint32_t)stages;
+            stage = (stage + (uint32_t)stages) % kStages;
         }
     } else {
         // ---------------- epilogue (both CTAs): warps 2..5 read the first accumulator, warps 6..9 the second, 32 rows
@@ -593,7 +610,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         const uint32_t st_row = buf + (uint32_t)((lane & 7) * 512);
         int t_local = 0, empty = 0;  // tiles with products, and without
         for (int tile = pair; tile < num_tiles; tile += num_pairs) {
-            const WgradTile w = wgrad_tile(tile, num_m, num_n, table);
+            const WgradTile w = wgrad_tile(tile, num_m, num_n, offsets);
             const bool products = w.rows > 0;
             const int count = products ? t_local++ : empty++;
             if ((count & 1) != group) continue;
@@ -668,10 +685,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
 
 // ------------------------------------------------------------------ host side
 template <typename Kernel, typename... Args>
-static int launch_kernel(Kernel kernel, int grid, int threads, size_t smem, size_t max_smem, int dev,
-                         bool (&attr_set)[64], cudaStream_t stream, Args... args) {
+static int launch_kernel(Kernel kernel, int grid, int threads, size_t smem, int dev, bool (&attr_set)[64],
+                         cudaStream_t stream, Args... args) {
     if (dev >= 64 || !attr_set[dev]) {
-        TRB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)max_smem));
+        TRB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
@@ -727,7 +744,7 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
     static bool attr_set[64] = {};
     CUtensorMap tmW, tmX128, tmX32;
     const uint64_t we[3] = {(uint64_t)(KB ? k : n), (uint64_t)(KB ? n : k), (uint64_t)groups};
-    const uint32_t wb[3] = {64, KB ? 128u : 64u, 1};
+    const uint32_t wb[3] = {64, 128, 1};  // KB: 64 k x 128 n, else 64 n x 128 k
     const uint64_t xe[2] = {(uint64_t)k, (uint64_t)rows};
     const uint32_t xb128[2] = {64, 128}, xb32[2] = {64, 32};
     int rc = gemm::encode_tiled(&tmW, b, 2, 3, we, wb, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -740,8 +757,8 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
         set_error("trb_grouped_gemm_launch: too many tiles (rows=%d n=%d groups=%d)", rows, n, groups);
         return TRB_SKIPPED;
     }
-    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, kProductSmem, kProductSmem, dev,
-                         attr_set, stream, tmW, tmX128, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
+    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, kProductSmem, dev, attr_set,
+                         stream, tmW, tmX128, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
 template <int DT>
@@ -761,10 +778,8 @@ static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const
         set_error("trb_grouped_wgrad_launch: too many tiles (groups=%d n=%d k=%d)", groups, n, k);
         return TRB_SKIPPED;
     }
-    const int stages = wgrad_smem(kStages, groups) <= kMaxDynamicSmem ? kStages : kStages - 1;
-    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, wgrad_smem(stages, groups),
-                         kMaxDynamicSmem, dev, attr_set, stream, tmA, tmG, offsets, static_cast<uint16_t*>(out), groups,
-                         rows, n, k, stages);
+    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, kWgradSmem, dev, attr_set,
+                         stream, tmA, tmG, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
 int read_error(bool clear) {

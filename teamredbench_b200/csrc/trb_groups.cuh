@@ -34,6 +34,16 @@ __device__ __forceinline__ int load_groups(const int* offsets, int groups, int t
     return 0;
 }
 
+// The check alone.
+__device__ __forceinline__ int check_groups(const int* offsets, int groups, int total_rows, int* error) {
+    bool bad = false;
+    for (int e = threadIdx.x; e < groups; e += blockDim.x)
+        bad = bad || offsets[e] < 0 || offsets[e + 1] < offsets[e] || offsets[e + 1] > total_rows;
+    if (!__syncthreads_or(bad)) return groups;
+    if (threadIdx.x == 0) atomicCAS(error, 0, kErrOffsets);
+    return 0;
+}
+
 // Exclusive scan of the groups' chunk counts, ceil(rows / chunk_rows) each (one warp).
 __device__ __forceinline__ void scan_chunks(int groups, int chunk_rows, const GroupTable& g, int lane) {
     int base = 0;
