@@ -34,6 +34,9 @@ def trb_dtype(tensor: Any) -> str:
     return name
 
 
+_RAW_STREAM: Any = None  # device index -> raw handle of its current stream, found on first use
+
+
 def _stream_handle(tensor: Any, stream: Any | None) -> int:
     """Raw cudaStream_t of ``stream``, or of the device's current stream.
 
@@ -41,14 +44,15 @@ def _stream_handle(tensor: Any, stream: Any | None) -> int:
     no Stream object built), which keeps the per-call host cost of a small
     GEMM close to the bare ctypes call; torch builds without it take the
     public ``torch.cuda.current_stream``."""
-    import torch
-
+    global _RAW_STREAM
     if stream is not None:
         return int(stream.cuda_stream)
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if raw is not None:
-        return int(raw(tensor.get_device()))
-    return int(torch.cuda.current_stream(tensor.device).cuda_stream)
+    if _RAW_STREAM is None:
+        import torch
+
+        _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return int(_RAW_STREAM(tensor.get_device()))
 
 
 def _require_cuda_contiguous(*tensors: Any) -> None:
@@ -114,16 +118,30 @@ def gemm(a: Any, b: Any, out: Any, *, dtype: str | None = None, scale_a: float =
     return out
 
 
-def _check_offsets(offsets: Any, groups: int) -> None:
-    if str(offsets.dtype) != "torch.int32" or offsets.dim() != 1 or offsets.shape[0] != groups + 1:
-        raise ValueError(f"offsets must be {groups + 1} int32 values, got {tuple(offsets.shape)} {offsets.dtype}")
+_INT32: Any = None  # torch.int32 and torch.uint8, looked up on first use
+_UINT8: Any = None
 
 
-def _check_one_device(*tensors: Any) -> None:
-    device = tensors[0].device
+def _check_operands(*tensors: Any) -> int:
+    """The one CUDA device (its index) that all tensors are on, contiguous.  A
+    call of a few microseconds is made of such checks: two queries a tensor,
+    and the wording of an error only once there is one."""
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors must share one device, got {t.device} beside {device}")
+        if t.get_device() != device or device < 0 or not t.is_contiguous():
+            _require_cuda_contiguous(*tensors)
+            raise ValueError(f"tensors must share one device, got {t.device} beside {tensors[0].device}")
+    return device
+
+
+def _check_offsets(offsets: Any, groups: int) -> None:
+    global _INT32
+    if _INT32 is None:
+        import torch
+
+        _INT32 = torch.int32
+    if offsets.dtype is not _INT32 or offsets.dim() != 1 or offsets.numel() != groups + 1:
+        raise ValueError(f"offsets must be {groups + 1} int32 values, got {tuple(offsets.shape)} {offsets.dtype}")
 
 
 def grouped_gemm(a: Any, b: Any, offsets: Any, out: Any, *, b_transposed: bool = False, stream: Any | None = None) -> Any:
@@ -137,8 +155,7 @@ def grouped_gemm(a: Any, b: Any, offsets: Any, out: Any, *, b_transposed: bool =
     they are.  n and k must be multiples of 8.  Offsets that decrease or leave
     [0, rows] compute nothing and set the device error word to 7
     (``_native.device_error``), which the host does not wait for here."""
-    _require_cuda_contiguous(a, b, offsets, out)
-    _check_one_device(a, b, offsets, out)
+    _check_operands(a, b, offsets, out)
     if a.dim() != 2 or b.dim() != 3:
         raise ValueError(f"grouped_gemm takes a 2-D a and a 3-D b, got {tuple(a.shape)} and {tuple(b.shape)}")
     rows, k = a.shape
@@ -149,7 +166,8 @@ def grouped_gemm(a: Any, b: Any, offsets: Any, out: Any, *, b_transposed: bool =
         raise ValueError(f"incompatible shapes {tuple(a.shape)} x {tuple(b.shape)} (b_transposed={b_transposed})")
     if out.shape != (rows, n):
         raise ValueError(f"out must be {(rows, n)}, got {tuple(out.shape)}")
-    if b.dtype != a.dtype or out.dtype != a.dtype:
+    dtype = a.dtype
+    if b.dtype is not dtype or out.dtype is not dtype:
         raise ValueError("a, b and out must share one dtype")
     _check_offsets(offsets, groups)
     _native.grouped_gemm_launch(trb_dtype(a), groups, rows, n, k, a.data_ptr(), b.data_ptr(),
@@ -164,19 +182,19 @@ def grouped_gemm_wgrad(a: Any, grad: Any, offsets: Any, out: Any, *, stream: Any
     (rows x n); zeros for a group without rows.  For weights kept
     (groups x n x k) pass grad first and a second.  offsets, types, sizes and
     errors as in grouped_gemm."""
-    _require_cuda_contiguous(a, grad, offsets, out)
-    _check_one_device(a, grad, offsets, out)
+    _check_operands(a, grad, offsets, out)
     if a.dim() != 2 or grad.dim() != 2 or out.dim() != 3:
         raise ValueError(f"grouped_gemm_wgrad takes 2-D a and grad and a 3-D out, got {tuple(a.shape)}, "
                          f"{tuple(grad.shape)} and {tuple(out.shape)}")
     rows, k = a.shape
-    n = grad.shape[1]
-    groups = out.shape[0]
-    if grad.shape[0] != rows:
-        raise ValueError(f"a and grad must have the same number of rows, got {rows} and {grad.shape[0]}")
-    if out.shape != (groups, k, n):
+    grad_rows, n = grad.shape
+    groups, out_k, out_n = out.shape
+    if grad_rows != rows:
+        raise ValueError(f"a and grad must have the same number of rows, got {rows} and {grad_rows}")
+    if out_k != k or out_n != n:
         raise ValueError(f"out must be {(groups, k, n)}, got {tuple(out.shape)}")
-    if grad.dtype != a.dtype or out.dtype != a.dtype:
+    dtype = a.dtype
+    if grad.dtype is not dtype or out.dtype is not dtype:
         raise ValueError("a, grad and out must share one dtype")
     _check_offsets(offsets, groups)
     _native.grouped_wgrad_launch(trb_dtype(a), groups, rows, n, k, a.data_ptr(), grad.data_ptr(), offsets.data_ptr(),
@@ -196,30 +214,36 @@ def gemv_w4(x: Any, q: Any, scales: Any, out: Any, *, zeros: Any | None = None, 
     be given without the leading dimension, and needs no offsets; otherwise
     offsets are those of grouped_gemm.  Meant for few rows a group: their weights
     are read once for each 8 or 16 rows.  k is at most 65536; n is free."""
-    _require_cuda_contiguous(x, q, scales, out, zeros, offsets)
-    _check_one_device(x, q, scales, out, zeros, offsets)
+    global _UINT8
+    _check_operands(*[t for t in (x, q, scales, out, zeros, offsets) if t is not None])
     if x.dim() != 2 or q.dim() not in (2, 3):
         raise ValueError(f"gemv_w4 takes a 2-D x and a 2-D or 3-D q, got {tuple(x.shape)} and {tuple(q.shape)}")
     rows, k = x.shape
-    groups = q.shape[0] if q.dim() == 3 else 1
-    n = q.shape[-2]
-    if 2 * q.shape[-1] != k:
-        raise ValueError(f"q holds {2 * q.shape[-1]} weights a row for k = {k}")
-    if scales.shape[:-1] != q.shape[:-1] or scales.shape[-1] == 0 or k % scales.shape[-1]:
-        raise ValueError(f"scales must be {tuple(q.shape[:-1])} x a divisor of {k}, got {tuple(scales.shape)}")
+    *lead, n, k_bytes = q.shape
+    groups = lead[0] if lead else 1
+    if 2 * k_bytes != k:
+        raise ValueError(f"q holds {2 * k_bytes} weights a row for k = {k}")
+    *outputs, k_groups = scales.shape
+    if outputs != [*lead, n] or k_groups == 0 or k % k_groups:
+        raise ValueError(f"scales must be {(*lead, n)} x a divisor of {k}, got {tuple(scales.shape)}")
     if zeros is not None and zeros.shape != scales.shape:
         raise ValueError(f"zeros must be {tuple(scales.shape)}, got {tuple(zeros.shape)}")
     if out.shape != (rows, n):
         raise ValueError(f"out must be {(rows, n)}, got {tuple(out.shape)}")
-    if scales.dtype != x.dtype or out.dtype != x.dtype:
+    dtype = x.dtype
+    if scales.dtype is not dtype or out.dtype is not dtype:
         raise ValueError("x, scales and out must share one dtype")
-    if str(q.dtype) != "torch.uint8" or (zeros is not None and zeros.dtype != q.dtype):
+    if _UINT8 is None:
+        import torch
+
+        _UINT8 = torch.uint8
+    if q.dtype is not _UINT8 or (zeros is not None and zeros.dtype is not _UINT8):
         raise ValueError("q and zeros must be uint8")
     if offsets is not None:
         _check_offsets(offsets, groups)
     elif groups != 1:
         raise ValueError(f"{groups} groups need offsets")
-    _native.gemv_w4_launch(trb_dtype(x), groups, rows, n, k, k // scales.shape[-1], x.data_ptr(), q.data_ptr(),
+    _native.gemv_w4_launch(trb_dtype(x), groups, rows, n, k, k // k_groups, x.data_ptr(), q.data_ptr(),
                            scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
                            None if offsets is None else offsets.data_ptr(), out.data_ptr(), _stream_handle(x, stream))
     return out
