@@ -357,6 +357,224 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
 }
 
+// ------------------------------------------------------------------ few tiles: K split over a cluster
+// The same transposed product with single CTAs (128 columns of out x up to 64
+// rows) when the tiles are too few to occupy the GPU: the CL CTAs of a cluster
+// take a tile's K in CL parts, each streaming its own share of the weights.
+// CTA r owns columns [128 r / CL, ...) of the tile: the others send it their
+// fp32 parts through distributed shared memory, and it adds them in the order
+// of K, so the result does not depend on timing.  One tile a cluster.
+constexpr int kSplitThreads = 192;  // producer warp, MMA warp, 4 epilogue warps
+constexpr int kSplitRows = 64;      // rows of a tile, at most
+constexpr int kSplitN = 128;
+constexpr int kSplitStages = 3;
+constexpr int kSplitX = 2 * kSplitRows * 128;  // two k-blocks of the rows of a
+constexpr int kSplitStage = kOperandStage + kSplitX;
+constexpr int kSplitReceive = kSplitRows * kSplitN * 4;
+constexpr size_t kSplitSmem = (size_t)kSplitStages * kSplitStage + kSplitReceive + 1024;
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+template <int DT>
+__device__ __forceinline__ uint16_t round16(float v) {
+    if constexpr (DT == TRB_FLOAT16) return __half_as_ushort(__float2half_rn(v));
+    else return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+template <int DT, bool KB>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+    grouped_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                         const int* __restrict__ offsets, uint16_t* __restrict__ out, int groups, int total_rows,
+                         int N, int K, int cl) {
+    constexpr uint32_t kIdesc = make_idesc<DT>(128, !KB, false);
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int group_words[3 * kMaxGroups + 1];
+    __shared__ __align__(8) uint64_t full_bar[kSplitStages];
+    __shared__ __align__(8) uint64_t empty_bar[kSplitStages];
+    __shared__ __align__(8) uint64_t done_bar;  // all products of the tile
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+
+    const uint32_t sW = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sX = sW + kSplitStages * kOperandStage;
+    const uint32_t receive = sX + kSplitStages * kSplitX;
+
+    const uint32_t rank = cluster_ctarank();
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int num_n = (N + kSplitN - 1) / kSplitN;
+    const int num_kb = (K + kBK - 1) / kBK;
+    const GroupTable table = {group_words, group_words + kMaxGroups, group_words + 2 * kMaxGroups};
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kSplitStages; ++s) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        mbar_init(smem_u32(&done_bar), 1);
+        abort_flag = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmX);
+    }
+    grid_launch_dependents();
+    grid_dependency_wait();
+    groups = load_groups(offsets, groups, total_rows, table, &g_grouped_error);
+    if (warp == 0) scan_chunks(groups, kSplitRows, table, lane);
+    __syncthreads();
+    const int tile = blockIdx.x / cl;
+    if (tile >= table.chunk0[groups] * num_n) return;  // the whole cluster: the grid covers the most tiles there can be
+
+    const int chunk = tile / num_n;
+    const int e = group_of_chunk(chunk, groups, table);
+    const int first = (chunk - table.chunk0[e]) * kSplitRows;
+    const int row0 = table.start[e] + first;
+    const int rows = min(kSplitRows, table.rows[e] - first);
+    const int padded = (rows + 15) & ~15;
+    const int n0 = (tile - chunk * num_n) * kSplitN;
+    const int kb0 = num_kb * (int)rank / cl, kb1 = num_kb * ((int)rank + 1) / cl;
+
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_slot), kSplitRows);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    cluster_arrive();  // peers may not write here before this CTA runs; the wait is before the first such write
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer
+            uint32_t stage = 0, phase = 0;
+            int issued = 0;
+            const int x_boxes = padded / 16;
+            for (int kb = kb0; kb < kb1; kb += 2) {
+                if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
+                    atomicCAS(&g_grouped_error, 0, kErrProducerWait);
+                    abort_flag = 1;
+                    break;
+                }
+                const int blocks = min(2, kb1 - kb);
+                const uint32_t bar = smem_u32(&full_bar[stage]);
+                const uint32_t w = sW + stage * kOperandStage, x = sX + stage * kSplitX;
+                mbar_arrive_expect_tx(bar, (KB ? blocks * kBlockBytes : kOperandStage) + blocks * x_boxes * 16 * 128);
+                if constexpr (!KB) {  // boxes of 128 k: a second k-block past this CTA's share is not multiplied
+                    tma_load_3d(w, &tmW, bar, n0, kb * kBK, e);
+                    tma_load_3d(w + kBlockBytes, &tmW, bar, n0 + 64, kb * kBK, e);
+                }
+                for (int i = 0; i < blocks; ++i) {
+                    if constexpr (KB) tma_load_3d(w + i * kBlockBytes, &tmW, bar, (kb + i) * kBK, n0, e);
+                    for (int j = 0; j < x_boxes; ++j)
+                        tma_load_2d(x + i * (kSplitX / 2) + j * 16 * 128, &tmX, bar, (kb + i) * kBK, row0 + j * 16);
+                }
+                ++issued;
+                if (++stage == kSplitStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            for (int i = min(issued, kSplitStages); i > 0; --i) {  // no copy in flight when this CTA ends
+                if (stage == 0) {
+                    stage = kSplitStages;
+                    phase ^= 1u;
+                }
+                --stage;
+                if (!mbar_wait(smem_u32(&full_bar[stage]), phase, nullptr)) atomicCAS(&g_grouped_error, 0, kErrDrainWait);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---------------- MMA issuer
+            const uint64_t w_desc0 = KB ? make_sdesc(sW, 16, 1024) : make_sdesc(sW, kBlockBytes, 1024);
+            const uint64_t x_desc0 = make_sdesc(sX, 16, 1024);
+            constexpr int kWStep = KB ? kInstrK * 2 : kInstrK * 128;
+            constexpr int kWBlock = KB ? kBlockBytes : kBlockBytes / 2;
+            const uint32_t idesc = idesc_n(kIdesc, padded);
+            uint32_t stage = 0, phase = 0;
+            for (int kb = kb0; kb < kb1; kb += 2) {
+                if (!mbar_wait(smem_u32(&full_bar[stage]), phase, &abort_flag)) {
+                    atomicCAS(&g_grouped_error, 0, kErrMmaWait);
+                    abort_flag = 1;
+                    break;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (kb + i >= kb1) break;
+#pragma unroll
+                    for (int ks = 0; ks < kBK / kInstrK; ++ks)
+                        mma_f16(tmem_base,
+                                w_desc0 + (uint64_t)((stage * kOperandStage + i * kWBlock + ks * kWStep) >> 4),
+                                x_desc0 + (uint64_t)((stage * kSplitX + i * (kSplitX / 2) + ks * kInstrK * 2) >> 4), idesc,
+                                (kb != kb0 || i != 0 || ks != 0) ? 1u : 0u);
+                }
+                tc_commit(smem_u32(&empty_bar[stage]));
+                if (++stage == kSplitStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            tc_commit(smem_u32(&done_bar));
+            if (!mbar_wait(smem_u32(&done_bar), 0, nullptr)) atomicCAS(&g_grouped_error, 0, kErrDrainWait);
+        }
+    }
+    __syncwarp();
+    cluster_wait();  // every CTA of the cluster runs
+    const int own = kSplitN / cl;  // columns this CTA owns
+    if (warp >= 2) {
+        // ---------------- epilogue: lane = column of out, TMEM column = row
+        const int q = warp & 3;
+        const int n = q * 32 + lane;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&done_bar), 0, &abort_flag));
+        if (!ok && lane == 0) {
+            atomicCAS(&g_grouped_error, 0, kErrEpilogueWait);
+            abort_flag = 1;
+        }
+        if (ok) {
+            tc_fence_after();
+            const uint32_t owner = mapa_shared(receive, (uint32_t)(n / own)) +
+                                   (uint32_t)(((int)rank * kSplitRows * own + n % own) * 4);
+            for (int c = 0; c < padded; c += 16) {
+                uint32_t v[16];
+                tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (c + i < rows) st_cluster_f32(owner + (uint32_t)((c + i) * own * 4), __uint_as_float(v[i]));
+            }
+            tc_fence_before();
+        }
+    }
+    // The parts have arrived, and no CTA leaves while a peer may still write into it.
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= 2 && ok) {
+        for (int i = threadIdx.x - 64; i < rows * own; i += 128) {
+            const int r = i / own, c = i - r * own;
+            float v = 0.0f;
+            for (int src = 0; src < cl; ++src) {
+                float p;
+                asm volatile("ld.shared.f32 %0, [%1];"
+                             : "=f"(p)
+                             : "r"(receive + (uint32_t)(((src * kSplitRows + r) * own + c) * 4)));
+                v += p;
+            }
+            const int n = n0 + (int)rank * own + c;
+            if (n < N) out[(size_t)(row0 + r) * N + n] = round16<DT>(v);
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kSplitRows);
+    }
+}
+
 // ------------------------------------------------------------------ out[e] = a^T * g over the rows of e
 // A CTA pair computes 256 x 256 of one group's K x N gradient; the products run
 // over the group's rows, 128 per stage, both operands MN-major (their rows are
@@ -685,22 +903,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
 
 // ------------------------------------------------------------------ host side
 template <typename Kernel, typename... Args>
-static int launch_kernel(Kernel kernel, int grid, int threads, size_t smem, int dev, bool (&attr_set)[64],
+static int launch_kernel(Kernel kernel, int grid, int threads, int cluster, size_t smem, int dev, bool (&attr_set)[64],
                          cudaStream_t stream, Args... args) {
     if (dev >= 64 || !attr_set[dev]) {
         TRB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev < 64) attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;  // 0: the kernel's own cluster size
     TRB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     return TRB_OK;
 }
@@ -746,8 +968,22 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
     const uint64_t we[3] = {(uint64_t)(KB ? k : n), (uint64_t)(KB ? n : k), (uint64_t)groups};
     const uint32_t wb[3] = {64, 128, 1};  // KB: 64 k x 128 n, else 64 n x 128 k
     const uint64_t xe[2] = {(uint64_t)k, (uint64_t)rows};
-    const uint32_t xb128[2] = {64, 128}, xb32[2] = {64, 32};
+    const uint32_t xb128[2] = {64, 128}, xb32[2] = {64, 32}, xb16[2] = {64, 16};
     int rc = gemm::encode_tiled(&tmW, b, 2, 3, we, wb, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != TRB_OK) return rc;
+    // K split over clusters where the tiles of 128 columns x 64 rows all run at once with CTAs to spare.
+    const int64_t split_tiles = (int64_t)((n + kSplitN - 1) / kSplitN) * (rows / kSplitRows + std::min(groups, rows));
+    const int num_kb = (k + kBK - 1) / kBK;
+    int cl = 1;
+    while (cl < 8 && split_tiles * cl * 2 <= device_sm_count(dev) && num_kb >= cl * 4) cl *= 2;
+    if (cl > 1) {
+        static bool split_attr_set[64] = {};
+        rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, xb16, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc != TRB_OK) return rc;
+        return launch_kernel(grouped_split_kernel<DT, KB>, (int)split_tiles * cl, kSplitThreads, cl, kSplitSmem, dev,
+                             split_attr_set, stream, tmW, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k,
+                             cl);
+    }
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX128, a, 2, 2, xe, xb128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, xb32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
@@ -757,7 +993,7 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
         set_error("trb_grouped_gemm_launch: too many tiles (rows=%d n=%d groups=%d)", rows, n, groups);
         return TRB_SKIPPED;
     }
-    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, kProductSmem, dev, attr_set,
+    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, 0, kProductSmem, dev, attr_set,
                          stream, tmW, tmX128, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
@@ -778,7 +1014,7 @@ static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const
         set_error("trb_grouped_wgrad_launch: too many tiles (groups=%d n=%d k=%d)", groups, n, k);
         return TRB_SKIPPED;
     }
-    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, kWgradSmem, dev, attr_set,
+    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, 0, kWgradSmem, dev, attr_set,
                          stream, tmA, tmG, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
