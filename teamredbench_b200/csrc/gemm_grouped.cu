@@ -365,13 +365,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // fp32 parts through distributed shared memory, and it adds them in the order
 // of K, so the result does not depend on timing.  One tile a cluster.
 constexpr int kSplitThreads = 192;  // producer warp, MMA warp, 4 epilogue warps
-constexpr int kSplitRows = 64;      // rows of a tile, at most
 constexpr int kSplitN = 128;
-constexpr int kSplitStages = 3;
-constexpr int kSplitX = 2 * kSplitRows * 128;  // two k-blocks of the rows of a
-constexpr int kSplitStage = kOperandStage + kSplitX;
-constexpr int kSplitReceive = kSplitRows * kSplitN * 4;
-constexpr size_t kSplitSmem = (size_t)kSplitStages * kSplitStage + kSplitReceive + 1024;
+// Tiles of up to R = 64 rows, or 16: then two CTAs fit an SM, each with its own ring, and one streams while the other
+// starts or ends.
+template <int R>
+struct SplitCfg {
+    static constexpr int kStages = R == 64 ? 3 : 2;
+    static constexpr int kX = 2 * R * 128;  // two k-blocks of the rows of a
+    static constexpr size_t kSmem = (size_t)kStages * (kOperandStage + kX) + R * kSplitN * 4 + 1024;
+    static constexpr int kPerSm = R == 64 ? 1 : 2;
+};
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
@@ -383,12 +386,16 @@ __device__ __forceinline__ uint16_t round16(float v) {
     else return __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
-template <int DT, bool KB>
-__global__ void __launch_bounds__(kSplitThreads, 1)
+template <int DT, bool KB, int R>
+__global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
     grouped_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                          const int* __restrict__ offsets, uint16_t* __restrict__ out, int groups, int total_rows,
                          int N, int K, int cl) {
     constexpr uint32_t kIdesc = make_idesc<DT>(128, !KB, false);
+    constexpr int kSplitStages = SplitCfg<R>::kStages;
+    constexpr int kSplitX = SplitCfg<R>::kX;
+    constexpr int kSplitRows = R;
+    constexpr int kTmemSplit = R < 32 ? 32 : R;
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ int group_words[3 * kMaxGroups + 1];
@@ -438,7 +445,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     const int kb0 = num_kb * (int)rank / cl, kb1 = num_kb * ((int)rank + 1) / cl;
 
     if (warp == 1) {
-        tmem_alloc(smem_u32(&tmem_slot), kSplitRows);
+        tmem_alloc(smem_u32(&tmem_slot), kTmemSplit);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -571,7 +578,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, kSplitRows);
+        tmem_dealloc(tmem_base, kTmemSplit);
     }
 }
 
@@ -971,18 +978,26 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
     const uint32_t xb128[2] = {64, 128}, xb32[2] = {64, 32}, xb16[2] = {64, 16};
     int rc = gemm::encode_tiled(&tmW, b, 2, 3, we, wb, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
-    // K split over clusters where the tiles of 128 columns x 64 rows all run at once with CTAs to spare.
-    const int64_t split_tiles = (int64_t)((n + kSplitN - 1) / kSplitN) * (rows / kSplitRows + std::min(groups, rows));
+    // Tiles of 128 columns, K split over clusters, where that gives every CTA a place at once: 2 rows, 2 of 8 groups,
+    // 2048 x 1024, 6.5 us against the pair's 13.0; 60 rows, 16 groups, 1024 x 1408, 14.1 against 15.6.  More tiles than
+    // places: the pair (96 rows, 32 groups, 2048 x 1408: 36 us against 40).  Up to 4 rows a group, tiles of 16 rows and
+    // two CTAs an SM (2 rows as above: 6.5 against 9.0 us); more rows make more tiles of 16 (40 rows, 8 groups, 4096 x
+    // 1024: 16.0 against 13.2 us).
+    const bool few = rows <= 4 * (int64_t)std::min(groups, rows);
+    const int split_rows = few ? 16 : 64;
+    const int64_t slots = (int64_t)device_sm_count(dev) * (few ? SplitCfg<16>::kPerSm : SplitCfg<64>::kPerSm);
+    const int64_t split_tiles = (int64_t)((n + kSplitN - 1) / kSplitN) * (rows / split_rows + std::min(groups, rows));
     const int num_kb = (k + kBK - 1) / kBK;
     int cl = 1;
-    while (cl < 8 && split_tiles * cl * 2 <= device_sm_count(dev) && num_kb >= cl * 4) cl *= 2;
-    if (cl > 1) {
-        static bool split_attr_set[64] = {};
+    while (cl < 8 && split_tiles * cl * 2 <= slots && num_kb >= cl * 4) cl *= 2;
+    if (cl > 1 || (few && split_tiles <= slots)) {
+        static bool split_attr_set[2][64] = {};
         rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, xb16, CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc != TRB_OK) return rc;
-        return launch_kernel(grouped_split_kernel<DT, KB>, (int)split_tiles * cl, kSplitThreads, cl, kSplitSmem, dev,
-                             split_attr_set, stream, tmW, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k,
-                             cl);
+        const auto kernel = few ? grouped_split_kernel<DT, KB, 16> : grouped_split_kernel<DT, KB, 64>;
+        return launch_kernel(kernel, (int)split_tiles * cl, kSplitThreads, cl,
+                             few ? SplitCfg<16>::kSmem : SplitCfg<64>::kSmem, dev, split_attr_set[few], stream, tmW, tmX32,
+                             offsets, static_cast<uint16_t*>(out), groups, rows, n, k, cl);
     }
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX128, a, 2, 2, xe, xb128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, xb32, CU_TENSOR_MAP_SWIZZLE_128B);
