@@ -84,17 +84,27 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 }
 // W words of q.  A step of W = 1 takes half a 32-byte sector of each output, the next step the other half, which
 // stays in L1 for it; wider steps use whole sectors once.
+// Predicated in place: as a branch around the load, every word was copied once more.
 template <int W>
-__device__ __forceinline__ void load_words(const uint8_t* p, bool in, uint32_t (&v)[W]) {
-    if (!in) return;
+__device__ __forceinline__ void load_words(const uint8_t* p, int in, uint32_t (&v)[W]) {
     if constexpr (W == 4)
-        asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                     : "l"(p));
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %5, 0;\n\t"
+            "@p ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+            : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3])
+            : "l"(p), "r"(in));
     else if constexpr (W == 2)
-        asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\t"
+            "@p ld.global.nc.L1::no_allocate.L2::256B.v2.u32 {%0, %1}, [%2];\n\t}"
+            : "+r"(v[0]), "+r"(v[1])
+            : "l"(p), "r"(in));
     else
-        asm volatile("ld.global.nc.L2::256B.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\t"
+            "@p ld.global.nc.L2::256B.u32 %0, [%1];\n\t}"
+            : "+r"(v[0])
+            : "l"(p), "r"(in));
 }
 
 // Pair p of a word of eight q: (q[p], q[p + 4]) as two 16-bit floats.  bf16: 128 + q each.  f16 has mantissa bits
