@@ -85,7 +85,15 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 // the R <= 256 rows of one group.  N goes in steps of 32, so a group of r rows
 // costs ceil(r / 32) * 32 rows of products instead of whole 128- or 256-row
 // tiles, and no row of another group ever meets this group's weights.  A group
-// of more than 256 rows is cut into equal chunks.  Rows past the group's end
+// of more than 256 rows is cut into equal chunks.  The price is an epilogue
+// that transposes, on the tensor-memory fragments in registers (stmatrix).
+// Measured: 32768 rows, 8 groups, 4096 x 4096, 810 to 860 us, 1280 to 1360
+// TFLOP/s under the power cap; 4109 rows, 16 groups, 2048 x 4096, 78 us; 96
+// rows, 32 groups, 2048 x 1408, 36 us, 4.8 TB/s of weights.  Between the two
+// bounds neither the weights' bytes nor the tensor pipe run alone: 37 groups of
+// 4096 x 1024 take 57 us with 16 rows each and 75 with 256, where both floors
+// are 48 us.  Asking the next stages' weights into L2 made it slower (96 rows
+// 43 us, 4109 rows 85).  Rows past the group's end
 // are loaded and multiplied but not stored; each output depends on its own row
 // only, so what stands there (the next group's rows, NaN) does not matter.
 // K past the end is zero in both operands (the tensor maps are per group).
@@ -593,6 +601,10 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
 // a stage lands on a barrier of its own CTA; a fixer warp clears the rows and
 // then signals the leader's full barrier.
 // A group without rows has a gradient of zeros, which the epilogue writes.
+// Measured: 32768 rows, 8 groups, 4096 x 4096, 800 to 880 us, 1250 to 1370
+// TFLOP/s under the power cap; 8111 rows, 64 groups, 2048 x 1544, 130 us, bound
+// by writing out tiles of two stages each (8192 rows, 64 groups, 2048 x 1536:
+// 111 us, the products without the epilogue 62, the stores alone 68).
 struct WgradTile {
     int e, row0, rows, m0, n0;
 };
@@ -826,7 +838,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         // of the tile each, so that one tile is read out of TMEM while another waits on its stores.  8 x 256 results at a
         // time go through shared memory (stmatrix) and leave as whole rows of the tile, 512 bytes a store: where N is not
         // a multiple of 16, rows begin in the middle of a sector and each end of a run writes a part of one (64 zero
-        // gradients of 2048 x 1544: 133 us in runs of 128 bytes, 100 in runs of 256, 67 us for 2048 x 1536).
+        // gradients of 2048 x 1544: 133 us in runs of 128 bytes, 100 in longer ones, 68 us for 2048 x 1536; 60 gradients
+        // of 127 rows on average 152, 132 and, with whole rows, 126 us).
         const int q = warp & 3, group = (warp - 2) >> 2;
         const uint32_t acce_leader = mapa_shared(smem_u32(&acce_bar[group]), 0);
         const uint32_t t_rows = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(group * 256);

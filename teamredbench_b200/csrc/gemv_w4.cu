@@ -13,8 +13,7 @@
 // become 16-bit floats by bit operations: a 4-bit q ORed into the mantissa of
 // 128 is 128 + q exactly, and subtracting 128 + z is exact too, so nothing is
 // rounded before the product, and the scale is applied in fp32 to each
-// group's sum.  Those operations (22 to 26 of some 35 instructions per 512
-// weights) are what the kernel spends its issue slots on.
+// group's sum.
 //
 // The order of k inside a product is free as long as q and x agree on it, so
 // each of the four threads that share an output takes W consecutive words (8
@@ -31,6 +30,18 @@
 // but its own loads.  What a warp has summed of a row goes to shared memory
 // when it leaves the row, and at the job's end the parts of each row are added
 // in the order of k.
+//
+// Measured (CUDA graph of calls on three sets of inputs): one row, 4096 x 4096,
+// 5.0 us, launch and latency; one row, 16384 x 8192, zero points, groups of 64,
+// 22 us, 3.3 TB/s; 40 rows of 22 experts, 2048 x 4096, 27 us, 3.6 TB/s; 15 rows,
+// 11009 x 4096, groups of 32, 18.5 us.  The two middle ones issue in 50% of the
+// cycles, 42 instructions per 512 weights, half of them the conversion; with
+// the conversion and the products taken out they ran 20 and 26 us, so what
+// bounds them is how the loads are kept in flight.  Tried and slower: the words
+// through TMA rings (a warp's own, 22 and 33 us, or a producer warp's, 26 and
+// 35), through cp.async (26 and 32), asked into L2 packs ahead (25 and 35), 24
+// warps a CTA (29 and 31), k shared by clusters of 4 CTAs (45 us for the 15
+// rows).
 //
 // No counterpart in the reference.
 #include <cuda_bf16.h>
@@ -415,6 +426,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------ host side
+constexpr size_t kMaxX = 128 * 1024;  // of x in shared memory
+static size_t x_row_bytes(int k) { return (size_t)(k + kPackK - 1) / kPackK * kPackK * 2; }
+
 struct Operands {
     const void *x, *q, *scales, *zeros;
     const int* offsets;
@@ -424,13 +438,13 @@ struct Operands {
 template <int DT, int NT, int W, bool Z, bool V>
 static int launch_kernel(const Operands& op, Shape sh, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
-    constexpr size_t kMaxSmem = 226 * 1024, kMaxX = 128 * 1024;
+    constexpr size_t kMaxSmem = 226 * 1024;
     if (dev >= 64 || !attr_set[dev]) {
         TRB_CUDA(cudaFuncSetAttribute(gemv_w4_kernel<DT, NT, W, Z, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)kMaxSmem));
         if (dev < 64) attr_set[dev] = true;
     }
-    const size_t row_bytes = (size_t)(sh.k + kPackK - 1) / kPackK * kPackK * 2;
+    const size_t row_bytes = x_row_bytes(sh.k);
     sh.tokens = std::min({sh.rows, NT * 8, (int)(kMaxX / row_bytes)});
     const size_t smem = row_bytes * sh.tokens + (size_t)(kWarps + kJobRows) * sh.tokens * kRows * 4 +
                         (size_t)(3 * sh.groups + 1) * 4;
@@ -475,8 +489,10 @@ static int launch_group(const Operands& op, const Shape& sh, int dev, cudaStream
 
 template <int DT>
 static int launch(const Operands& op, const Shape& sh, int dev, cudaStream_t stream) {
-    // More than 8 rows a group on average: 16 rows at once read the weights half as often.
-    if (sh.rows > 8 * (int64_t)sh.groups)
+    // More than 8 rows a group on average: 16 rows at once read the weights half as often (15 rows of one 11009 x 4096
+    // matrix in groups of 32: 18.5 against 22.5 us), if more than 8 rows of x fit (16 rows, 16384 x 8192: 8 rows twice
+    // 33.6 us, 16 by 16 with room for 8 of them 41.6).
+    if (sh.rows > 8 * (int64_t)sh.groups && kMaxX / x_row_bytes(sh.k) > 8)
         return op.zeros ? launch_group<DT, 2, true>(op, sh, dev, stream) : launch_group<DT, 2, false>(op, sh, dev, stream);
     return op.zeros ? launch_group<DT, 1, true>(op, sh, dev, stream) : launch_group<DT, 1, false>(op, sh, dev, stream);
 }
