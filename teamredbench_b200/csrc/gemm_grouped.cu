@@ -132,8 +132,8 @@ constexpr size_t kProductSmem = kRingBytes + 1024 + kEpiWarps * kEpiBytes;
 template <int DT, bool KB>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX128,
-                        const __grid_constant__ CUtensorMap tmX32, const int* __restrict__ offsets,
-                        uint16_t* __restrict__ out, int groups, int total_rows, int N, int K) {
+                        const __grid_constant__ CUtensorMap tmX32, const int* offsets,
+                        uint16_t* out, int groups, int total_rows, int N, int K) {
     constexpr uint32_t kIdesc = make_idesc<DT>(256, !KB, false);
 
     extern __shared__ uint8_t smem_raw[];
@@ -397,7 +397,7 @@ __device__ __forceinline__ uint16_t round16(float v) {
 template <int DT, bool KB, int R>
 __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
     grouped_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                         const int* __restrict__ offsets, uint16_t* __restrict__ out, int groups, int total_rows,
+                         const int* offsets, uint16_t* out, int groups, int total_rows,
                          int N, int K, int cl) {
     constexpr uint32_t kIdesc = make_idesc<DT>(128, !KB, false);
     constexpr int kSplitStages = SplitCfg<R>::kStages;
@@ -633,7 +633,7 @@ constexpr int kStageRows = 2 * kBK;
 template <int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmG,
-                         const int* __restrict__ offsets, uint16_t* __restrict__ out, int groups, int total_rows, int N,
+                         const int* offsets, uint16_t* out, int groups, int total_rows, int N,
                          int K) {
     constexpr uint32_t kIdesc = make_idesc<DT>(256, true, true) | ((uint32_t)(256 >> 3) << 17);
     constexpr uint32_t kBox = kBlockBytes / 2;  // 64 rows x 64 columns

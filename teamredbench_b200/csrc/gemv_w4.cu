@@ -182,9 +182,8 @@ struct Job {
 // read.
 template <int DT, int NT, int W, bool Z, bool V>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemv_w4_kernel(const uint8_t* __restrict__ weights, const uint16_t* __restrict__ x,
-                   const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros,
-                   const int* __restrict__ offsets, uint16_t* __restrict__ out, const Shape sh) {
+    gemv_w4_kernel(const uint8_t* weights, const uint16_t* x, const uint16_t* scales, const uint8_t* zeros,
+                   const int* offsets, uint16_t* out, const Shape sh) {
     constexpr int kSteps = 16 / W;      // of a pack
     constexpr int kStepK = 32 * W;
     constexpr int kHeld = kSteps / 4;   // steps of a pack whose scale a thread holds for the four of an output
@@ -204,6 +203,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* words = reinterpret_cast<int*>(red + (kWarps + kJobRows) * part);
     const GroupTable table = {words, words + sh.groups, words + 2 * sh.groups};
 
+    // No operand is read before the wait: the plain pointers (no __restrict__, no read-only loads but the volatile
+    // ones) keep the compiler from moving a load up over it.
     grid_launch_dependents();
     grid_dependency_wait();
     int groups = sh.groups;
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint4* dst = x_out + (step * W + w) * tokens * 4 + of;
 #pragma unroll 8
                 for (int c = 0; c < tokens; ++c) {
-                    const uint4 v = in ? __ldg(src + (size_t)c * (sh.k / 8)) : make_uint4(0, 0, 0, 0);
+                    const uint4 v = in ? src[(size_t)c * (sh.k / 8)] : make_uint4(0, 0, 0, 0);
                     dst[c * 4] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                                             __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
                 }
