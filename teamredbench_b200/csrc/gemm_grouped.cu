@@ -132,7 +132,8 @@ constexpr size_t kProductSmem = kRingBytes + 1024 + kEpiWarps * kEpiBytes;
 template <int DT, bool KB>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX128,
-                        const __grid_constant__ CUtensorMap tmX32, const int* offsets,
+                        const __grid_constant__ CUtensorMap tmX64, const __grid_constant__ CUtensorMap tmX32,
+                        const int* offsets,
                         uint16_t* out, int groups, int total_rows, int N, int K) {
     constexpr uint32_t kIdesc = make_idesc<DT>(256, !KB, false);
 
@@ -175,6 +176,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         fence_mbar_init();
         tma_prefetch_desc(&tmW);
         tma_prefetch_desc(&tmX128);
+        tma_prefetch_desc(&tmX64);
         tma_prefetch_desc(&tmX32);
     }
     if (warp == 0) {
@@ -202,8 +204,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const ProductTile p = product_tile(tile, groups, num_n, table);
                 const int half = ((p.rows + 31) & ~31) >> 1;  // rows this CTA loads
                 const int x_row = p.row0 + (int)rank * half;
-                const int x_boxes = (half + 31) / 32;
-                const uint32_t x_bytes = (uint32_t)x_boxes * 32 * 128;
+                // One box a k-block, of 128, 64 or 32 rows: a request costs more than the rows nobody uses (4109 rows:
+                // 76 us with up to three boxes of 32 a k-block, 74 with one).
+                const CUtensorMap* tmX = half > 64 ? &tmX128 : half > 32 ? &tmX64 : &tmX32;
+                const uint32_t x_bytes = (half > 64 ? 128 : half > 32 ? 64 : 32) * 128;
                 const int w_col = p.n0 + (int)rank * 128;
                 for (int kb = 0; kb < num_kb; kb += 2) {
                     const int blocks = min(2, num_kb - kb);
@@ -225,14 +229,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     for (int i = 0; i < blocks; ++i) {
                         if constexpr (KB) tma_load_3d_pair(w + i * kBlockBytes, &tmW, fb, (kb + i) * kBK, w_col, p.e);
-                        const uint32_t xi = x + i * kBlockBytes;
-                        if (x_boxes == 4) {
-                            tma_load_2d_pair(xi, &tmX128, fb, (kb + i) * kBK, x_row);
-                        } else {
-                            for (int j = 0; j < x_boxes; ++j)
-                                tma_load_2d_pair(xi + (uint32_t)j * 32 * 128, &tmX32, fb, (kb + i) * kBK,
-                                                 x_row + j * 32);
-                        }
+                        tma_load_2d_pair(x + i * kBlockBytes, tmX, fb, (kb + i) * kBK, x_row);
                     }
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
@@ -468,7 +465,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
             // ---------------- TMA producer
             uint32_t stage = 0, phase = 0;
             int issued = 0;
-            const int x_boxes = padded / 16;
             for (int kb = kb0; kb < kb1; kb += 2) {
                 if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
                     atomicCAS(&g_grouped_error, 0, kErrProducerWait);
@@ -478,15 +474,14 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
                 const int blocks = min(2, kb1 - kb);
                 const uint32_t bar = smem_u32(&full_bar[stage]);
                 const uint32_t w = sW + stage * kOperandStage, x = sX + stage * kSplitX;
-                mbar_arrive_expect_tx(bar, (KB ? blocks * kBlockBytes : kOperandStage) + blocks * x_boxes * 16 * 128);
+                mbar_arrive_expect_tx(bar, (KB ? blocks * kBlockBytes : kOperandStage) + blocks * (kSplitX / 2));
                 if constexpr (!KB) {  // boxes of 128 k: a second k-block past this CTA's share is not multiplied
                     tma_load_3d(w, &tmW, bar, n0, kb * kBK, e);
                     tma_load_3d(w + kBlockBytes, &tmW, bar, n0 + 64, kb * kBK, e);
                 }
                 for (int i = 0; i < blocks; ++i) {
                     if constexpr (KB) tma_load_3d(w + i * kBlockBytes, &tmW, bar, (kb + i) * kBK, n0, e);
-                    for (int j = 0; j < x_boxes; ++j)
-                        tma_load_2d(x + i * (kSplitX / 2) + j * 16 * 128, &tmX, bar, (kb + i) * kBK, row0 + j * 16);
+                    tma_load_2d(x + i * (kSplitX / 2), &tmX, bar, (kb + i) * kBK, row0);
                 }
                 ++issued;
                 if (++stage == kSplitStages) {
@@ -633,10 +628,11 @@ constexpr int kStageRows = 2 * kBK;
 template <int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmG,
+                         const __grid_constant__ CUtensorMap tmA64, const __grid_constant__ CUtensorMap tmG64,
                          const int* offsets, uint16_t* out, int groups, int total_rows, int N,
                          int K) {
     constexpr uint32_t kIdesc = make_idesc<DT>(256, true, true) | ((uint32_t)(256 >> 3) << 17);
-    constexpr uint32_t kBox = kBlockBytes / 2;  // 64 rows x 64 columns
+    constexpr uint32_t kBox = kBlockBytes;  // place of a box of 64 columns x up to 128 rows
 
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kStages];   // leader: the stage is ready in both CTAs
@@ -708,34 +704,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                         break;
                     }
                     const int left = w.rows - done;
-                    const int blocks = left > kBK ? 2 : 1;
+                    const CUtensorMap* mapA = left > kBK ? &tmA : &tmA64;  // boxes of 128 or 64 rows
+                    const CUtensorMap* mapG = left > kBK ? &tmG : &tmG64;
+                    const uint32_t bytes = left > kBK ? 4 * kBox : 2 * kBox;  // of this CTA
                     const bool fix = left < kStageRows && left % kInstrK != 0;
                     const uint32_t a = sA + stage * kOperandStage, g = sG + stage * kOperandStage;
                     const int row = w.row0 + done;
                     if (fix) {
                         const uint32_t bar = smem_u32(&part_bar[stage]);
-                        mbar_arrive_expect_tx(bar, blocks * 4 * kBox);
-                        for (int i = 0; i < blocks; ++i) {
-                            const uint32_t o = i * kBlockBytes;
-                            tma_load_2d(a + o, &tmA, bar, a_col, row + i * kBK);
-                            tma_load_2d(a + o + kBox, &tmA, bar, a_col + 64, row + i * kBK);
-                            tma_load_2d(g + o, &tmG, bar, g_col, row + i * kBK);
-                            tma_load_2d(g + o + kBox, &tmG, bar, g_col + 64, row + i * kBK);
-                        }
+                        mbar_arrive_expect_tx(bar, bytes);
+                        tma_load_2d(a, mapA, bar, a_col, row);
+                        tma_load_2d(a + kBox, mapA, bar, a_col + 64, row);
+                        tma_load_2d(g, mapG, bar, g_col, row);
+                        tma_load_2d(g + kBox, mapG, bar, g_col + 64, row);
                     } else {
                         const uint32_t fb_local = smem_u32(&full_bar[stage]);
                         if (leader) {
-                            mbar_arrive_expect_tx(fb_local, blocks * 8 * kBox);
+                            mbar_arrive_expect_tx(fb_local, 2 * bytes);
                             mbar_arrive(fb_local);
                         }
                         const uint32_t fb = fb_local & kPeerBitMask;
-                        for (int i = 0; i < blocks; ++i) {
-                            const uint32_t o = i * kBlockBytes;
-                            tma_load_2d_pair(a + o, &tmA, fb, a_col, row + i * kBK);
-                            tma_load_2d_pair(a + o + kBox, &tmA, fb, a_col + 64, row + i * kBK);
-                            tma_load_2d_pair(g + o, &tmG, fb, g_col, row + i * kBK);
-                            tma_load_2d_pair(g + o + kBox, &tmG, fb, g_col + 64, row + i * kBK);
-                        }
+                        tma_load_2d_pair(a, mapA, fb, a_col, row);
+                        tma_load_2d_pair(a + kBox, mapA, fb, a_col + 64, row);
+                        tma_load_2d_pair(g, mapG, fb, g_col, row);
+                        tma_load_2d_pair(g + kBox, mapG, fb, g_col + 64, row);
                     }
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
@@ -782,7 +774,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
 #pragma unroll
                     for (int ks = 0; ks < kStageRows / kInstrK; ++ks) {
                         if (ks * kInstrK >= left) break;
-                        const uint64_t o = off + (uint64_t)(((ks >> 2) * kBlockBytes + (ks & 3) * kInstrK * 128) >> 4);
+                        const uint64_t o = off + (uint64_t)(ks * kInstrK * 128 >> 4);
                         mma_pair_f16(d_tmem, a_desc0 + o, g_desc0 + o, kIdesc, (done != 0 || ks != 0) ? 1u : 0u);
                     }
                     tc_commit_pair_multicast(smem_u32(&empty_bar[stage]), 0x3);
@@ -819,7 +811,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                 }
                 part_phase ^= 1u << s;
                 const int pieces = (((left + kInstrK - 1) & ~(kInstrK - 1)) - left) * 8;  // 16-byte pieces per box
-                const uint32_t first = sA + s * kOperandStage + (uint32_t)(left / kBK * kBlockBytes + left % kBK * 128);
+                const uint32_t first = sA + s * kOperandStage + (uint32_t)left * 128;
                 for (int i = lane; i < pieces; i += 32) {
                     const uint32_t at = first + (uint32_t)i * 16;
                     st_shared_v4(at, 0, 0, 0, 0);
@@ -984,11 +976,11 @@ template <int DT, bool KB>
 static int launch_product(int groups, int rows, int n, int k, const void* a, const void* b, const int* offsets,
                           void* out, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
-    CUtensorMap tmW, tmX128, tmX32;
+    CUtensorMap tmW, tmX128, tmX64, tmX32;
     const uint64_t we[3] = {(uint64_t)(KB ? k : n), (uint64_t)(KB ? n : k), (uint64_t)groups};
     const uint32_t wb[3] = {64, 128, 1};  // KB: 64 k x 128 n, else 64 n x 128 k
     const uint64_t xe[2] = {(uint64_t)k, (uint64_t)rows};
-    const uint32_t xb128[2] = {64, 128}, xb32[2] = {64, 32}, xb16[2] = {64, 16};
+    const uint32_t xb128[2] = {64, 128}, xb64[2] = {64, 64}, xb32[2] = {64, 32}, xb16[2] = {64, 16};
     int rc = gemm::encode_tiled(&tmW, b, 2, 3, we, wb, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
     // Tiles of 128 columns, K split over clusters, where that gives every CTA a place at once: 2 rows, 2 of 8 groups,
@@ -1005,7 +997,7 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
     while (cl < 8 && split_tiles * cl * 2 <= slots && num_kb >= cl * 4) cl *= 2;
     if (cl > 1 || (few && split_tiles <= slots)) {
         static bool split_attr_set[2][64] = {};
-        rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, xb16, CU_TENSOR_MAP_SWIZZLE_128B);
+        rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, few ? xb16 : xb64, CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc != TRB_OK) return rc;
         const auto kernel = few ? grouped_split_kernel<DT, KB, 16> : grouped_split_kernel<DT, KB, 64>;
         return launch_kernel(kernel, (int)split_tiles * cl, kSplitThreads, cl,
@@ -1013,6 +1005,7 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
                              offsets, static_cast<uint16_t*>(out), groups, rows, n, k, cl);
     }
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX128, a, 2, 2, xe, xb128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX64, a, 2, 2, xe, xb64, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, xb32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
     const int64_t num_n = (n + kTileN - 1) / kTileN;
@@ -1022,20 +1015,23 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
         return TRB_SKIPPED;
     }
     return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, 0, kProductSmem, dev, attr_set,
-                         stream, tmW, tmX128, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
+                         stream, tmW, tmX128, tmX64, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
 template <int DT>
 static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const void* g, const int* offsets,
                         void* out, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
-    CUtensorMap tmA, tmG;
+    CUtensorMap tmA, tmG, tmA64, tmG64;
     // Without rows no operand is read; the maps then stand on the output, which is there.
     const uint64_t extent_rows = (uint64_t)std::max(rows, 1);
     const uint64_t ae[2] = {(uint64_t)k, extent_rows}, ge[2] = {(uint64_t)n, extent_rows};
-    const uint32_t box[2] = {64, 64};
-    int rc = gemm::encode_tiled(&tmA, rows > 0 ? a : out, 2, 2, ae, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmG, rows > 0 ? g : out, 2, 2, ge, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint32_t box[2] = {64, kStageRows}, box64[2] = {64, 64};
+    const void *pa = rows > 0 ? a : out, *pg = rows > 0 ? g : out;
+    int rc = gemm::encode_tiled(&tmA, pa, 2, 2, ae, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmG, pg, 2, 2, ge, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmA64, pa, 2, 2, ae, box64, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmG64, pg, 2, 2, ge, box64, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != TRB_OK) return rc;
     const int64_t tiles = (int64_t)groups * ((k + 255) / 256) * ((n + 255) / 256);
     if (tiles > INT32_MAX) {
@@ -1043,7 +1039,7 @@ static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const
         return TRB_SKIPPED;
     }
     return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, 0, kWgradSmem, dev, attr_set,
-                         stream, tmA, tmG, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
+                         stream, tmA, tmG, tmA64, tmG64, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
 int read_error(bool clear) {
