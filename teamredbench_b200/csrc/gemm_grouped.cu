@@ -611,12 +611,12 @@ __device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, con
     w.row0 = offsets[w.e];
     w.rows = offsets[w.e + 1] - w.row0;
     const int local = t - w.e * per;
-    const int run = 8 * num_n;
+    const int run = 8 * num_m;
     const int first = local / run * 8;
-    const int width = min(8, num_m - first);
-    const int in_run = local - first * num_n;
-    w.m0 = (first + in_run % width) * 256;
-    w.n0 = in_run / width * 256;
+    const int width = min(8, num_n - first);
+    const int in_run = local - first * num_m;
+    w.n0 = (first + in_run % width) * 256;
+    w.m0 = in_run / width * 256;
     return w;
 }
 
