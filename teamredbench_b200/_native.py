@@ -260,19 +260,26 @@ def gemm_host(dtype: str, m: int, n: int, k: int, a: int, b: int, c: int, scale_
 
 def grouped_gemm_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: int, b: int, b_layout: str,
                         offsets: int, out: int, stream: int = 0) -> None:
-    check(load().trb_grouped_gemm_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, b, B_LAYOUTS[b_layout], offsets,
-                                         out, stream or None))
+    status = (_lib or load()).trb_grouped_gemm_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, b,
+                                                      B_LAYOUTS[b_layout], offsets, out, stream or None)
+    if status:
+        check(status)
 
 
 def grouped_wgrad_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: int, g: int, offsets: int, out: int,
                          stream: int = 0) -> None:
-    check(load().trb_grouped_wgrad_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, g, offsets, out, stream or None))
+    status = (_lib or load()).trb_grouped_wgrad_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, g, offsets, out,
+                                                       stream or None)
+    if status:
+        check(status)
 
 
 def gemv_w4_launch(dtype: str, groups: int, rows: int, n: int, k: int, group_size: int, x: int, q: int, scales: int,
                    zeros: int | None, offsets: int | None, out: int, stream: int = 0) -> None:
-    check(load().trb_gemv_w4_launch(DTYPE_CODES[dtype], groups, rows, n, k, group_size, x, q, scales, zeros, offsets,
-                                    out, stream or None))
+    status = (_lib or load()).trb_gemv_w4_launch(DTYPE_CODES[dtype], groups, rows, n, k, group_size, x, q, scales,
+                                                 zeros, offsets, out, stream or None)
+    if status:
+        check(status)
 
 
 def round_tf32(data: int, count: int, stream: int = 0) -> None:

@@ -30,8 +30,9 @@ def expert_counts(torch_module: Any, rows: int, experts: int, skew: float, seed:
     torch = torch_module
     gen = torch.Generator().manual_seed(seed)
     share = torch.exp(skew * torch.randn(experts, generator=gen, dtype=torch.float64))
-    picks = torch.multinomial(share, rows, replacement=True, generator=gen) if rows else torch.empty(0, dtype=torch.int64)
-    return torch.bincount(picks, minlength=experts)
+    if rows == 0:
+        return torch.zeros(experts, dtype=torch.int64)
+    return torch.bincount(torch.multinomial(share, rows, replacement=True, generator=gen), minlength=experts)
 
 
 @register_benchmark("experts")

@@ -88,7 +88,7 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 // of more than 256 rows is cut into equal chunks.  The price is an epilogue
 // that transposes, on the tensor-memory fragments in registers (stmatrix).
 // Measured: 32768 rows, 8 groups, 4096 x 4096, 810 to 860 us, 1280 to 1360
-// TFLOP/s under the power cap; 4109 rows, 16 groups, 2048 x 4096, 78 us; 96
+// TFLOP/s under the power cap; 4109 rows, 16 groups, 2048 x 4096, 74 us; 96
 // rows, 32 groups, 2048 x 1408, 36 us, 4.8 TB/s of weights.  Between the two
 // bounds neither the weights' bytes nor the tensor pipe run alone: 37 groups of
 // 4096 x 1024 take 57 us with 16 rows each and 75 with 256, where both floors
@@ -296,8 +296,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     } else {
         // ---------------- epilogue (both CTAs): warps 2..9, a TMEM lane quarter (32 columns of out) and every other
-        // block of 32 rows each.  TMEM holds out^T, so 32 x 32 blocks go through shared memory transposed (stmatrix .trans) and leave
-        // as 64-byte runs of a row, 16 bytes a lane.
+        // block of 32 rows each.  TMEM holds out^T, so 32 x 32 blocks go through shared memory transposed (stmatrix
+        // .trans) and leave as 64-byte runs of a row, 16 bytes a lane.
         const int q = warp & 3, first_block = (warp - 2) >> 2;
         const uint32_t acce_leader0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
         const uint32_t acce_leader1 = mapa_shared(smem_u32(&acce_bar[1]), 0);
@@ -495,7 +495,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
                     phase ^= 1u;
                 }
                 --stage;
-                if (!mbar_wait(smem_u32(&full_bar[stage]), phase, nullptr)) atomicCAS(&g_grouped_error, 0, kErrDrainWait);
+                if (!mbar_wait(smem_u32(&full_bar[stage]), phase, nullptr))
+                    atomicCAS(&g_grouped_error, 0, kErrDrainWait);
             }
         }
     } else if (warp == 1) {
@@ -520,8 +521,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
                     for (int ks = 0; ks < kBK / kInstrK; ++ks)
                         mma_f16(tmem_base,
                                 w_desc0 + (uint64_t)((stage * kOperandStage + i * kWBlock + ks * kWStep) >> 4),
-                                x_desc0 + (uint64_t)((stage * kSplitX + i * (kSplitX / 2) + ks * kInstrK * 2) >> 4), idesc,
-                                (kb != kb0 || i != 0 || ks != 0) ? 1u : 0u);
+                                x_desc0 + (uint64_t)((stage * kSplitX + i * (kSplitX / 2) + ks * kInstrK * 2) >> 4),
+                                idesc, (kb != kb0 || i != 0 || ks != 0) ? 1u : 0u);
                 }
                 tc_commit(smem_u32(&empty_bar[stage]));
                 if (++stage == kSplitStages) {
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
 // then signals the leader's full barrier.
 // A group without rows has a gradient of zeros, which the epilogue writes.
 // Measured: 32768 rows, 8 groups, 4096 x 4096, 800 to 880 us, 1250 to 1370
-// TFLOP/s under the power cap; 8111 rows, 64 groups, 2048 x 1544, 130 us, bound
+// TFLOP/s under the power cap; 8111 rows, 64 groups, 2048 x 1544, 126 us, bound
 // by writing out tiles of two stages each (8192 rows, 64 groups, 2048 x 1536:
 // 111 us, the products without the epilogue 62, the stores alone 68).
 struct WgradTile {
@@ -615,7 +616,7 @@ __device__ __forceinline__ WgradTile wgrad_tile(int t, int num_m, int num_n, con
     const int first = local / run * 8;
     const int width = min(8, num_n - first);
     const int in_run = local - first * num_m;
-    w.n0 = (first + in_run % width) * 256;
+    w.n0 = (first + in_run % width) * 256;  // runs of 8 tiles along a row of the gradient
     w.m0 = in_run / width * 256;
     return w;
 }
@@ -826,12 +827,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
             stage = (stage + (uint32_t)stages) % kStages;
         }
     } else {
-        // ---------------- epilogue (both CTAs): warps 2..5 read the first accumulator, warps 6..9 the second, 32 rows
-        // of the tile each, so that one tile is read out of TMEM while another waits on its stores.  8 x 256 results at a
-        // time go through shared memory (stmatrix) and leave as whole rows of the tile, 512 bytes a store: where N is not
-        // a multiple of 16, rows begin in the middle of a sector and each end of a run writes a part of one (64 zero
-        // gradients of 2048 x 1544: 133 us in runs of 128 bytes, 100 in longer ones, 68 us for 2048 x 1536; 60 gradients
-        // of 127 rows on average 152, 132 and, with whole rows, 126 us).
+        // ---------------- epilogue (both CTAs): warps 2..5 read the first accumulator, warps 6..9 the second, 32
+        // rows of the tile each, so that one tile is read out of TMEM while another waits on its stores.  8 x 256
+        // results at a time go through shared memory (stmatrix) and leave as whole rows of the tile, 512 bytes a
+        // store: where N is not a multiple of 16, rows begin in the middle of a sector and each end of a run writes
+        // a part of one (64 zero gradients of 2048 x 1544: 133 us in runs of 128 bytes, 100 in longer ones, 83 with
+        // the tiles of a row of the gradient next to each other in time; 67 us for 2048 x 1536).  60 gradients of
+        // 127 rows on average: 152 us with one group of eight warps, 132 with a group for each accumulator, 129 with
+        // whole rows, 126 in that tile order; 133 with the stores moved to sector boundaries, 182 with sixteen warps
+        // and runs of 256 bytes.
         const int q = warp & 3, group = (warp - 2) >> 2;
         const uint32_t acce_leader = mapa_shared(smem_u32(&acce_bar[group]), 0);
         const uint32_t t_rows = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(group * 256);
@@ -1014,8 +1018,8 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
         set_error("trb_grouped_gemm_launch: too many tiles (rows=%d n=%d groups=%d)", rows, n, groups);
         return TRB_SKIPPED;
     }
-    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, 0, kProductSmem, dev, attr_set,
-                         stream, tmW, tmX128, tmX64, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
+    return launch_kernel(grouped_gemm_kernel<DT, KB>, 2 * pairs_for(tiles, dev), kThreads, 0, kProductSmem, dev,
+                         attr_set, stream, tmW, tmX128, tmX64, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
 template <int DT>
@@ -1038,8 +1042,8 @@ static int launch_wgrad(int groups, int rows, int n, int k, const void* a, const
         set_error("trb_grouped_wgrad_launch: too many tiles (groups=%d n=%d k=%d)", groups, n, k);
         return TRB_SKIPPED;
     }
-    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, 0, kWgradSmem, dev, attr_set,
-                         stream, tmA, tmG, tmA64, tmG64, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
+    return launch_kernel(grouped_wgrad_kernel<DT>, 2 * pairs_for(tiles, dev), kWgradThreads, 0, kWgradSmem, dev,
+                         attr_set, stream, tmA, tmG, tmA64, tmG64, offsets, static_cast<uint16_t*>(out), groups, rows, n, k);
 }
 
 int read_error(bool clear) {

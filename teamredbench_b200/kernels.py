@@ -128,6 +128,8 @@ def _check_operands(*tensors: Any) -> int:
     and the wording of an error only once there is one."""
     device = tensors[0].get_device()
     for t in tensors:
+        if t is None:
+            continue
         if t.get_device() != device or device < 0 or not t.is_contiguous():
             _require_cuda_contiguous(*tensors)
             raise ValueError(f"tensors must share one device, got {t.device} beside {tensors[0].device}")
@@ -215,18 +217,19 @@ def gemv_w4(x: Any, q: Any, scales: Any, out: Any, *, zeros: Any | None = None, 
     offsets are those of grouped_gemm.  Meant for few rows a group: their weights
     are read once for each 8 or 16 rows.  k is at most 65536; n is free."""
     global _UINT8
-    _check_operands(*[t for t in (x, q, scales, out, zeros, offsets) if t is not None])
+    _check_operands(x, q, scales, out, zeros, offsets)
     if x.dim() != 2 or q.dim() not in (2, 3):
         raise ValueError(f"gemv_w4 takes a 2-D x and a 2-D or 3-D q, got {tuple(x.shape)} and {tuple(q.shape)}")
     rows, k = x.shape
-    *lead, n, k_bytes = q.shape
-    groups = lead[0] if lead else 1
+    outputs, scale_shape = q.shape, scales.shape
+    groups = 1 if len(outputs) == 2 else outputs[0]
+    n, k_bytes = outputs[-2:]
     if 2 * k_bytes != k:
         raise ValueError(f"q holds {2 * k_bytes} weights a row for k = {k}")
-    *outputs, k_groups = scales.shape
-    if outputs != [*lead, n] or k_groups == 0 or k % k_groups:
-        raise ValueError(f"scales must be {(*lead, n)} x a divisor of {k}, got {tuple(scales.shape)}")
-    if zeros is not None and zeros.shape != scales.shape:
+    k_groups = scale_shape[-1] if len(scale_shape) else 0
+    if scale_shape[:-1] != outputs[:-1] or k_groups == 0 or k % k_groups:
+        raise ValueError(f"scales must be {tuple(outputs[:-1])} x a divisor of {k}, got {tuple(scale_shape)}")
+    if zeros is not None and zeros.shape != scale_shape:
         raise ValueError(f"zeros must be {tuple(scales.shape)}, got {tuple(zeros.shape)}")
     if out.shape != (rows, n):
         raise ValueError(f"out must be {(rows, n)}, got {tuple(out.shape)}")
