@@ -959,6 +959,10 @@ static int check(const char* what, int dtype, int groups, int rows, int n, int k
         set_error("%s: at most %d groups (got %d)", what, kMaxGroups, groups);
         return TRB_SKIPPED;
     }
+    if (std::max({rows, n, k}) > kMaxExtent) {
+        set_error("%s: rows, n and k at most %d (rows=%d n=%d k=%d)", what, kMaxExtent, rows, n, k);
+        return TRB_SKIPPED;
+    }
     if (n % 8 != 0 || k % 8 != 0) {
         set_error("%s: n and k must be multiples of 8 (n=%d k=%d)", what, n, k);
         return TRB_ERR_ALIGN;

@@ -535,6 +535,10 @@ extern "C" int trb_gemv_w4_launch(int dtype, int groups, int rows, int n, int k,
         set_error("trb_gemv_w4_launch: k at most 65536 and at most %d groups (k=%d groups=%d)", kMaxGroups, k, groups);
         return TRB_SKIPPED;
     }
+    if (std::max(rows, n) > kMaxExtent) {
+        set_error("trb_gemv_w4_launch: rows and n at most %d (rows=%d n=%d)", kMaxExtent, rows, n);
+        return TRB_SKIPPED;
+    }
     if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(q)) & 15u) != 0 ||
         ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(out)) & 1u) != 0 ||
         (reinterpret_cast<uintptr_t>(offsets) & 3u) != 0) {

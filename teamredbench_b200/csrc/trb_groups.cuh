@@ -6,6 +6,9 @@
 namespace trb {
 
 constexpr int kMaxGroups = 1024;
+// Largest rows, n and k.  The kernels round sizes up to whole tiles and stages (a chunk's rows: up to one part in 256
+// above them) and step past the end by a stage in 32-bit integers, so sizes near 2^31 would wrap.
+constexpr int kMaxExtent = 0x7F000000;
 
 #if defined(__CUDACC__)
 
