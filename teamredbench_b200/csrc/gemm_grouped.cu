@@ -183,15 +183,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
         tmem_relinquish_pair();
     }
-    grid_launch_dependents();
-    grid_dependency_wait();  // offsets, operands and out may belong to the previous grid until here
-    groups = load_groups(offsets, groups, total_rows, table, &g_grouped_error);
-    if (warp == 0) scan_chunks(groups, kTileRows, table, lane);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();  // barrier inits of both CTAs visible before any cross-CTA signal
     tc_fence_after();
     const uint32_t tmem_base = tmem_slot;
+    // Only now that this block has its TMEM: the next grid's blocks take theirs before they wait for this grid.
+    grid_launch_dependents();
+    grid_dependency_wait();  // offsets, operands and out may belong to the previous grid until here
+    groups = load_groups(offsets, groups, total_rows, table, &g_grouped_error);
+    if (warp == 0) scan_chunks(groups, kTileRows, table, lane);
+    __syncthreads();
     const int num_tiles = table.chunk0[groups] * num_n;
 
     if (warp == 0) {
@@ -432,13 +434,24 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
         tma_prefetch_desc(&tmW);
         tma_prefetch_desc(&tmX);
     }
-    grid_launch_dependents();
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_slot), kTmemSplit);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    grid_launch_dependents();  // after the allocation, as above
     grid_dependency_wait();
     groups = load_groups(offsets, groups, total_rows, table, &g_grouped_error);
     if (warp == 0) scan_chunks(groups, kSplitRows, table, lane);
     __syncthreads();
     const int tile = blockIdx.x / cl;
-    if (tile >= table.chunk0[groups] * num_n) return;  // the whole cluster: the grid covers the most tiles there can be
+    if (tile >= table.chunk0[groups] * num_n) {  // the whole cluster: the grid covers the most tiles there can be
+        if (warp == 1) tmem_dealloc(tmem_base, kTmemSplit);
+        return;
+    }
 
     const int chunk = tile / num_n;
     const int e = group_of_chunk(chunk, groups, table);
@@ -449,14 +462,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
     const int n0 = (tile - chunk * num_n) * kSplitN;
     const int kb0 = num_kb * (int)rank / cl, kb1 = num_kb * ((int)rank + 1) / cl;
 
-    if (warp == 1) {
-        tmem_alloc(smem_u32(&tmem_slot), kTmemSplit);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = tmem_slot;
     cluster_arrive();  // peers may not write here before this CTA runs; the wait is before the first such write
 
     bool ok = true;
@@ -678,14 +683,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
         tmem_relinquish_pair();
     }
-    grid_launch_dependents();
-    grid_dependency_wait();
-    groups = check_groups(offsets, groups, total_rows, &g_grouped_error);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = tmem_slot;
+    grid_launch_dependents();  // after the allocation, as above
+    grid_dependency_wait();
+    groups = check_groups(offsets, groups, total_rows, &g_grouped_error);
     const int num_tiles = groups * num_m * num_n;
 
     if (warp == 0) {
