@@ -271,8 +271,10 @@ int trb_gemm_host(int dtype, int m, int n, int k, const void* a_host, const void
  * rows outside every group are neither read nor written.  Offsets that
  * decrease or leave [0, rows] are found on the device: the call computes
  * nothing and sets the device error word to 7 (trb_device_error).  At most
- * 1024 groups; rows, n and k at most 2130706432.  Asynchronous on `stream`; no workspace, so calls on several
- * streams may overlap.  No reference counterpart: its GEMM takes one matrix
+ * 1024 groups; rows, n and k at most 2130706432.  Asynchronous on `stream`,
+ * on the calling thread's current device, which has to be the one that holds
+ * the operands and the stream; no workspace, so calls on several streams may
+ * overlap. No reference counterpart: its GEMM takes one matrix
  * per operand (src/teamredbench/benchmarks/mfu.py:229-234). */
 
 /* out[r] = a[r] * b[e] for the rows r of group e: a rows x k, out rows x n,

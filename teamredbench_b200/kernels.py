@@ -46,6 +46,9 @@ def _stream_handle(tensor: Any, stream: Any | None) -> int:
     public ``torch.cuda.current_stream``."""
     global _RAW_STREAM
     if stream is not None:
+        device = tensor.get_device()
+        if getattr(stream, "device_index", device) != device:
+            raise ValueError(f"stream is on cuda:{stream.device_index}, the tensors on cuda:{device}")
         return int(stream.cuda_stream)
     if _RAW_STREAM is None:
         import torch
@@ -53,6 +56,27 @@ def _stream_handle(tensor: Any, stream: Any | None) -> int:
         _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda device: torch.cuda.current_stream(device).cuda_stream)
     return int(_RAW_STREAM(tensor.get_device()))
+
+
+_CURRENT_DEVICE: Any = None  # () -> index of the calling thread's current device, found on first use
+
+
+def _launch_on(device: int, launch: Any, *args: Any) -> None:
+    """launch(*args) with `device`, the operands' own, as the current one.  The
+    library launches on the current device, and the default streams of all
+    devices have the same raw handle, so a stream alone does not name it."""
+    global _CURRENT_DEVICE
+    if _CURRENT_DEVICE is None:
+        import torch
+
+        _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    if _CURRENT_DEVICE() == device:
+        launch(*args)
+        return
+    import torch
+
+    with torch.cuda.device(device):
+        launch(*args)
 
 
 def _require_cuda_contiguous(*tensors: Any) -> None:
@@ -76,9 +100,9 @@ def stream_op(mode: str, dst: Any, src: Any, aux: Any | None = None, scale: floa
         raise ValueError("dst, src and aux must have the same number of elements")
     if mode == "triad" and aux is None:
         raise ValueError("triad needs aux")
-    _native.hbm_launch(trb_dtype(src), mode, dst.data_ptr(), src.data_ptr(),
-                       aux.data_ptr() if aux is not None else None, src.numel(), float(scale), variant,
-                       blocks_per_sm, _stream_handle(src, stream))
+    _launch_on(src.get_device(), _native.hbm_launch, trb_dtype(src), mode, dst.data_ptr(), src.data_ptr(),
+               aux.data_ptr() if aux is not None else None, src.numel(), float(scale), variant, blocks_per_sm,
+               _stream_handle(src, stream))
     return dst
 
 
@@ -112,9 +136,9 @@ def gemm(a: Any, b: Any, out: Any, *, dtype: str | None = None, scale_a: float =
     if out.shape != (m, n):
         raise ValueError(f"out must be {(m, n)}, got {tuple(out.shape)}")
     name = dtype or trb_dtype(a)
-    _native.gemm_launch_ex(name, m, n, k, a.data_ptr(), b.data_ptr(), out.data_ptr(), float(scale_a),
-                           float(scale_b), int(splits), int(cta_pair), "k_major" if b_transposed else "row_major",
-                           _stream_handle(a, stream), int(tile_n))
+    _launch_on(a.get_device(), _native.gemm_launch_ex, name, m, n, k, a.data_ptr(), b.data_ptr(), out.data_ptr(),
+               float(scale_a), float(scale_b), int(splits), int(cta_pair), "k_major" if b_transposed else "row_major",
+               _stream_handle(a, stream), int(tile_n))
     return out
 
 
@@ -157,7 +181,7 @@ def grouped_gemm(a: Any, b: Any, offsets: Any, out: Any, *, b_transposed: bool =
     they are.  n and k must be multiples of 8.  Offsets that decrease or leave
     [0, rows] compute nothing and set the device error word to 7
     (``_native.device_error``), which the host does not wait for here."""
-    _check_operands(a, b, offsets, out)
+    device = _check_operands(a, b, offsets, out)
     if a.dim() != 2 or b.dim() != 3:
         raise ValueError(f"grouped_gemm takes a 2-D a and a 3-D b, got {tuple(a.shape)} and {tuple(b.shape)}")
     rows, k = a.shape
@@ -172,9 +196,9 @@ def grouped_gemm(a: Any, b: Any, offsets: Any, out: Any, *, b_transposed: bool =
     if b.dtype is not dtype or out.dtype is not dtype:
         raise ValueError("a, b and out must share one dtype")
     _check_offsets(offsets, groups)
-    _native.grouped_gemm_launch(trb_dtype(a), groups, rows, n, k, a.data_ptr(), b.data_ptr(),
-                                "k_major" if b_transposed else "row_major", offsets.data_ptr(), out.data_ptr(),
-                                _stream_handle(a, stream))
+    _launch_on(device, _native.grouped_gemm_launch, trb_dtype(a), groups, rows, n, k, a.data_ptr(), b.data_ptr(),
+               "k_major" if b_transposed else "row_major", offsets.data_ptr(), out.data_ptr(),
+               _stream_handle(a, stream))
     return out
 
 
@@ -184,7 +208,7 @@ def grouped_gemm_wgrad(a: Any, grad: Any, offsets: Any, out: Any, *, stream: Any
     (rows x n); zeros for a group without rows.  For weights kept
     (groups x n x k) pass grad first and a second.  offsets, types, sizes and
     errors as in grouped_gemm."""
-    _check_operands(a, grad, offsets, out)
+    device = _check_operands(a, grad, offsets, out)
     if a.dim() != 2 or grad.dim() != 2 or out.dim() != 3:
         raise ValueError(f"grouped_gemm_wgrad takes 2-D a and grad and a 3-D out, got {tuple(a.shape)}, "
                          f"{tuple(grad.shape)} and {tuple(out.shape)}")
@@ -199,8 +223,8 @@ def grouped_gemm_wgrad(a: Any, grad: Any, offsets: Any, out: Any, *, stream: Any
     if grad.dtype is not dtype or out.dtype is not dtype:
         raise ValueError("a, grad and out must share one dtype")
     _check_offsets(offsets, groups)
-    _native.grouped_wgrad_launch(trb_dtype(a), groups, rows, n, k, a.data_ptr(), grad.data_ptr(), offsets.data_ptr(),
-                                 out.data_ptr(), _stream_handle(a, stream))
+    _launch_on(device, _native.grouped_wgrad_launch, trb_dtype(a), groups, rows, n, k, a.data_ptr(), grad.data_ptr(),
+               offsets.data_ptr(), out.data_ptr(), _stream_handle(a, stream))
     return out
 
 
@@ -217,7 +241,7 @@ def gemv_w4(x: Any, q: Any, scales: Any, out: Any, *, zeros: Any | None = None, 
     offsets are those of grouped_gemm.  Meant for few rows a group: their weights
     are read once for each 8 or 16 rows.  k is at most 65536; n is free."""
     global _UINT8
-    _check_operands(x, q, scales, out, zeros, offsets)
+    device = _check_operands(x, q, scales, out, zeros, offsets)
     if x.dim() != 2 or q.dim() not in (2, 3):
         raise ValueError(f"gemv_w4 takes a 2-D x and a 2-D or 3-D q, got {tuple(x.shape)} and {tuple(q.shape)}")
     rows, k = x.shape
@@ -246,7 +270,7 @@ def gemv_w4(x: Any, q: Any, scales: Any, out: Any, *, zeros: Any | None = None, 
         _check_offsets(offsets, groups)
     elif groups != 1:
         raise ValueError(f"{groups} groups need offsets")
-    _native.gemv_w4_launch(trb_dtype(x), groups, rows, n, k, k // k_groups, x.data_ptr(), q.data_ptr(),
-                           scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
-                           None if offsets is None else offsets.data_ptr(), out.data_ptr(), _stream_handle(x, stream))
+    _launch_on(device, _native.gemv_w4_launch, trb_dtype(x), groups, rows, n, k, k // k_groups, x.data_ptr(),
+               q.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
+               None if offsets is None else offsets.data_ptr(), out.data_ptr(), _stream_handle(x, stream))
     return out
