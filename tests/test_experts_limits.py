@@ -46,3 +46,17 @@ def test_grouped_entries_refuse(rows, n, k):
 def test_gemv_w4_entry_refuses(rows, n):
     assert _native.load().trb_gemv_w4_launch(BF16, 1, rows, n, 64, 32, P, P, P, None, None, P, None) == 1
     assert f"at most {LARGEST}" in _native.last_error()
+
+
+@pytest.mark.parametrize("launch", [
+    lambda r, n, k: _native.grouped_gemm_launch("bfloat16", 1, r, n, k, P, P, "row_major", P, P),
+    lambda r, n, k: _native.grouped_wgrad_launch("bfloat16", 1, r, n, k, P, P, P, P),
+    lambda r, n, k: _native.gemv_w4_launch("bfloat16", 1, r, n, k, 32, P, P, P, None, None, P),
+], ids=["grouped_gemm", "grouped_wgrad", "gemv_w4"])
+@pytest.mark.parametrize("which", "rnk")
+def test_sizes_past_32_bits_are_not_cut(launch, which):
+    """Cut to 32 bits, 2^32 rows would be a call of no rows, done at once, and n or k those of a smaller matrix."""
+    size = {"r": 0, "n": 64, "k": 64}
+    size[which] += 2 ** 32
+    with pytest.raises(ValueError, match="32 bits"):
+        launch(size["r"], size["n"], size["k"])
