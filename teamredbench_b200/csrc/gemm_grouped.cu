@@ -649,6 +649,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
     __shared__ __align__(8) uint64_t drain_bar;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
+    __shared__ volatile int issued;  // stages that this CTA's producer has asked for (may wrap: only changes count)
 
     const uint32_t sA = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t sG = sA + kStages * kOperandStage;
@@ -675,6 +676,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         }
         mbar_init(smem_u32(&drain_bar), 1);
         abort_flag = 0;
+        issued = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmG);
@@ -698,6 +700,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
             // ---------------- TMA producer
             uint32_t stage = 0, phase = 0;
             uint32_t issued_mask = 0, issued_phase = 0;
+            uint32_t stages_issued = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
                 const WgradTile w = wgrad_tile(tile, num_m, num_n, offsets);
@@ -735,6 +738,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
                         tma_load_2d_pair(g, mapG, fb, g_col, row);
                         tma_load_2d_pair(g + kBox, mapG, fb, g_col + 64, row);
                     }
+                    issued = (int)++stages_issued;
                     issued_mask |= 1u << stage;
                     issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
                     if (++stage == kStages) {
@@ -806,7 +810,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
             const int left = w.rows - (stages - 1) * kStageRows;  // rows of the last stage
             if (stages > 0 && left % kInstrK != 0) {
                 const uint32_t s = (stage + (uint32_t)(stages - 1)) % kStages;
-                ok = mbar_wait(smem_u32(&part_bar[s]), (part_phase >> s) & 1u, &abort_flag);
+                // from the start of the call on, if no tile before had rows to clear
+                ok = mbar_wait_progress(smem_u32(&part_bar[s]), (part_phase >> s) & 1u, &abort_flag, &issued);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
                     if (lane == 0) {
@@ -854,7 +859,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
             const int count = products ? t_local++ : empty++;
             if ((count & 1) != group) continue;
             if (products) {
-                bool ok = mbar_wait_cluster(smem_u32(&accf_bar[group]), (uint32_t)(count >> 1) & 1u, &abort_flag);
+                // for all stages of a tile, or of two
+                bool ok = mbar_wait_progress(smem_u32(&accf_bar[group]), (uint32_t)(count >> 1) & 1u, &abort_flag,
+                                             &issued);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) {
                     if (lane == 0) {

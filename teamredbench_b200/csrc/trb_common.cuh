@@ -343,6 +343,26 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
         if (globaltimer_ns() - t0 > kWaitTimeoutNs) return false;
     }
 }
+// The same for a wait that may last for many steps of a pipeline: *progress, a
+// count that another warp of the CTA raises at each step, starts the limit
+// anew, so that it bounds a step and not the call.
+__device__ __forceinline__ bool mbar_wait_progress(uint32_t bar, uint32_t parity, const volatile int* abort,
+                                                   const volatile int* progress) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    int seen = *progress;
+    uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        if (mbar_try_wait_cluster(bar, parity)) return true;
+        if (*abort) return false;
+        const int now = *progress;
+        if (now != seen) {
+            seen = now;
+            t0 = globaltimer_ns();
+        } else if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+            return false;
+        }
+    }
+}
 // Programmatic dependent launch.  wait: block until the grids this one
 // depends on have completed and their memory is visible (a no-op without a
 // programmatic dependency).  launch_dependents: allow the next grid in the
