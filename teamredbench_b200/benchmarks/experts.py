@@ -105,10 +105,13 @@ class ExpertsBenchmark(Benchmark):
                     try:
                         gen = torch.Generator(device=self.device).manual_seed(seed)
                         step, ops, moved = self._step(mode, getattr(torch, spec.torch_attr), counts, k, n, group, gen)
+                        _native.device_error(self.context.device_id, clear=True)  # of earlier calls
                         self.sync_ranks()
                         elapsed_s = timed_iterations(step, torch_module=torch, warmup=int(p.get("warmup", 10)),
                                                      iterations=int(p.get("iterations", 50)))
-                        metadata["device_error"] = _native.device_error(self.context.device_id, clear=True)
+                        code = metadata["device_error"] = _native.device_error(self.context.device_id, clear=True)
+                        if code:
+                            raise RuntimeError(f"the kernels set the device error word to {code}")
                     except Exception as exc:  # noqa: BLE001 - any failure becomes a skipped record
                         records.append(self.emit_record(self.skipped_record(case=case, dtype=spec.name, error=str(exc),
                                                                             metadata=metadata)))
