@@ -955,6 +955,32 @@ static int launch_kernel(Kernel kernel, int grid, int threads, int cluster, size
     return TRB_OK;
 }
 
+// Clusters of `cl` CTAs of the kernel that the device holds at once, asked once for each device.  Fewer than the SMs
+// divided by cl, since a cluster stays inside a GPC: 33 of 4 and 15 of 8 with one CTA an SM on 148 SMs.
+template <typename Kernel>
+static int clusters_at_once(Kernel kernel, int threads, size_t smem, int cl, int dev, int (&cache)[64]) {
+    if (dev < 64 && cache[dev] > 0) return cache[dev];
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cl;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)cl);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int count = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&count, kernel, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();  // not split, then
+        return 0;
+    }
+    if (dev < 64) cache[dev] = count;
+    return count;
+}
+
 // Checks shared by both products.
 static int check(const char* what, int dtype, int groups, int rows, int n, int k, const void* p0, const void* p1,
                  const void* p2, const int* offsets) {
@@ -1007,22 +1033,36 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
     // 2048 x 1024, 6.5 us against the pair's 13.0; 60 rows, 16 groups, 1024 x 1408, 14.1 against 15.6.  More tiles than
     // places: the pair (96 rows, 32 groups, 2048 x 1408: 36 us against 40).  Up to 4 rows a group, tiles of 16 rows and
     // two CTAs an SM (2 rows as above: 6.5 against 9.0 us); more rows make more tiles of 16 (40 rows, 8 groups, 4096 x
-    // 1024: 16.0 against 13.2 us).
+    // 1024: 16.0 against 13.2 us).  One cluster more than fit at once is a second round of the whole time: 50 rows, K =
+    // 4096, 16 tiles take 16.3 us in clusters of 8 and 11.5 of 4, 34 tiles 23.4 of 4 and 17.8 of 2; 3 rows, 72 tiles 22.9
+    // of 4 and 18.3 of 2.
     const bool few = rows <= 4 * (int64_t)std::min(groups, rows);
     const int split_rows = few ? 16 : 64;
-    const int64_t slots = (int64_t)device_sm_count(dev) * (few ? SplitCfg<16>::kPerSm : SplitCfg<64>::kPerSm);
+    const auto split_kernel = few ? grouped_split_kernel<DT, KB, 16> : grouped_split_kernel<DT, KB, 64>;
+    const size_t split_smem = few ? SplitCfg<16>::kSmem : SplitCfg<64>::kSmem;
+    static bool split_attr_set[2][64] = {};
     const int64_t split_tiles = (int64_t)((n + kSplitN - 1) / kSplitN) * (rows / split_rows + std::min(groups, rows));
     const int num_kb = (k + kBK - 1) / kBK;
-    int cl = 1;
-    while (cl < 8 && split_tiles * cl * 2 <= slots && num_kb >= cl * 4) cl *= 2;
-    if (cl > 1 || (few && split_tiles <= slots)) {
-        static bool split_attr_set[2][64] = {};
+    const auto sm_places = [&](int log2_cl) {  // of clusters with one CTA an SM
+        static int places[4][64] = {};
+        return clusters_at_once(grouped_split_kernel<DT, KB, 64>, kSplitThreads, SplitCfg<64>::kSmem, 1 << log2_cl, dev,
+                                places[log2_cl]);
+    };
+    // With two CTAs an SM the driver still answers for one.  Twice as many clusters fit for certain, and at most as many
+    // as clusters half the size with one; on 148 SMs 33 of 8 do (30 and 33), 71 of 4 (66 and 74) and 148 of 2 (148).
+    const auto fits = [&](int log2_cl) {
+        const int sure = (few ? 2 : 1) * sm_places(log2_cl);
+        return split_tiles <= (few && log2_cl > 0 ? (sure + sm_places(log2_cl - 1)) / 2 : sure);
+    };
+    int log2_cl = 0;
+    while (log2_cl < 3 && num_kb >= 4 << log2_cl && fits(log2_cl + 1)) ++log2_cl;
+    if (log2_cl > 0 || (few && fits(0))) {
         rc = gemm::encode_tiled(&tmX32, a, 2, 2, xe, few ? xb16 : xb64, CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc != TRB_OK) return rc;
-        const auto kernel = few ? grouped_split_kernel<DT, KB, 16> : grouped_split_kernel<DT, KB, 64>;
-        return launch_kernel(kernel, (int)split_tiles * cl, kSplitThreads, cl,
-                             few ? SplitCfg<16>::kSmem : SplitCfg<64>::kSmem, dev, split_attr_set[few], stream, tmW, tmX32,
-                             offsets, static_cast<uint16_t*>(out), groups, rows, n, k, cl);
+        const int cl = 1 << log2_cl;
+        return launch_kernel(split_kernel, (int)split_tiles * cl, kSplitThreads, cl, split_smem, dev,
+                             split_attr_set[few], stream, tmW, tmX32, offsets, static_cast<uint16_t*>(out), groups, rows, n,
+                             k, cl);
     }
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX128, a, 2, 2, xe, xb128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX64, a, 2, 2, xe, xb64, CU_TENSOR_MAP_SWIZZLE_128B);
