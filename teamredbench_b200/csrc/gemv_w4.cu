@@ -490,10 +490,16 @@ static int launch_group(const Operands& op, const Shape& sh, int dev, cudaStream
 
 template <int DT>
 static int launch(const Operands& op, const Shape& sh, int dev, cudaStream_t stream) {
-    // More than 8 rows a group on average: 16 rows at once read the weights half as often (15 rows of one 11009 x 4096
-    // matrix in groups of 32: 18.5 against 22.5 us), if more than 8 rows of x fit (16 rows, 16384 x 8192: 8 rows twice
-    // 33.6 us, 16 by 16 with room for 8 of them 41.6).
-    if (sh.rows > 8 * (int64_t)sh.groups && kMaxX / x_row_bytes(sh.k) > 8)
+    // 16 rows at once where that takes fewer passes over the weights than 8, on average rows a group: 15 rows of one
+    // 11009 x 4096 matrix in groups of 32, 18.5 against 22.5 us.  Less than 16 rows of a long k fit: 16 rows of 16384 x
+    // 6144 in groups of 128 take two passes either way, 33.6 us as 10 and 6 rows and 26.7 as 8 and 8, 9 rows 21.4 as one
+    // pass and 26.5 as two.
+    const int64_t rows = (sh.rows + (int64_t)sh.groups - 1) / sh.groups;
+    const auto passes = [&](int64_t at_once) {
+        const int64_t taken = std::min<int64_t>(at_once, kMaxX / x_row_bytes(sh.k));
+        return (rows + taken - 1) / taken;
+    };
+    if (passes(16) < passes(8))
         return op.zeros ? launch_group<DT, 2, true>(op, sh, dev, stream) : launch_group<DT, 2, false>(op, sh, dev, stream);
     return op.zeros ? launch_group<DT, 1, true>(op, sh, dev, stream) : launch_group<DT, 1, false>(op, sh, dev, stream);
 }

@@ -1,8 +1,6 @@
 """More columns of the same few rows never take much less time: K is split over no more clusters than the GPU holds."""
 from __future__ import annotations
 
-import statistics
-
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -12,34 +10,20 @@ if not torch.cuda.is_available():  # pragma: no cover - CPU container
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
 from teamredbench_b200.kernels import grouped_gemm  # noqa: E402
+from tests.timing_helpers import device_us  # noqa: E402
 
 
 def _us(rows, tiles, k=4096):
-    """Device time of a call on 128 * tiles columns: the median over graphs of calls on weights larger than L2."""
+    """Device time of a call on 128 * tiles columns."""
     n = 128 * tiles
     offsets = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
-    sets = []
-    for _ in range(-(-400_000_000 // (2 * k * n))):
-        sets.append((torch.zeros((rows, k), dtype=torch.bfloat16, device="cuda"),
-                     torch.zeros((1, k, n), dtype=torch.bfloat16, device="cuda"), offsets,
-                     torch.empty((rows, n), dtype=torch.bfloat16, device="cuda")))
-    for s in sets:
-        grouped_gemm(*s)
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        for s in sets * 2:
-            grouped_gemm(*s)
-    graph.replay()
-    times = []
-    for _ in range(15):
-        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        begin.record()
-        graph.replay()
-        end.record()
-        torch.cuda.synchronize()
-        times.append(begin.elapsed_time(end) * 1e3 / (2 * len(sets)))
-    return statistics.median(times)
+
+    def operands():
+        return (torch.zeros((rows, k), dtype=torch.bfloat16, device="cuda"),
+                torch.zeros((1, k, n), dtype=torch.bfloat16, device="cuda"), offsets,
+                torch.empty((rows, n), dtype=torch.bfloat16, device="cuda"))
+
+    return device_us(grouped_gemm, operands, 2 * k * n)
 
 
 # The later count takes the next smaller cluster in any case; a second round of clusters costs 1.3 to 1.4 times its time.
