@@ -258,15 +258,14 @@ def gemm_host(dtype: str, m: int, n: int, k: int, a: int, b: int, c: int, scale_
     return result
 
 
-def _fit_32_bits(*sizes: int) -> None:
-    """ctypes cuts larger sizes off without a word."""
-    if max(sizes) > 0x7FFFFFFF:
-        raise ValueError(f"a size of {max(sizes)} does not fit 32 bits")
+def _refuse_past_32_bits(*sizes: int) -> None:
+    raise ValueError(f"a size of {max(sizes)} does not fit 32 bits")
 
 
 def grouped_gemm_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: int, b: int, b_layout: str,
                         offsets: int, out: int, stream: int = 0) -> None:
-    _fit_32_bits(groups, rows, n, k)
+    if (groups | rows | n | k) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(groups, rows, n, k)
     status = (_lib or load()).trb_grouped_gemm_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, b,
                                                       B_LAYOUTS[b_layout], offsets, out, stream or None)
     if status:
@@ -275,7 +274,8 @@ def grouped_gemm_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: i
 
 def grouped_wgrad_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: int, g: int, offsets: int, out: int,
                          stream: int = 0) -> None:
-    _fit_32_bits(groups, rows, n, k)
+    if (groups | rows | n | k) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(groups, rows, n, k)
     status = (_lib or load()).trb_grouped_wgrad_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, g, offsets, out,
                                                        stream or None)
     if status:
@@ -284,7 +284,8 @@ def grouped_wgrad_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: 
 
 def gemv_w4_launch(dtype: str, groups: int, rows: int, n: int, k: int, group_size: int, x: int, q: int, scales: int,
                    zeros: int | None, offsets: int | None, out: int, stream: int = 0) -> None:
-    _fit_32_bits(groups, rows, n, k)
+    if (groups | rows | n | k) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(groups, rows, n, k)
     status = (_lib or load()).trb_gemv_w4_launch(DTYPE_CODES[dtype], groups, rows, n, k, group_size, x, q, scales,
                                                  zeros, offsets, out, stream or None)
     if status:
