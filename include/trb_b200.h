@@ -270,7 +270,8 @@ int trb_gemm_host(int dtype, int m, int n, int k, const void* a_host, const void
  * group e owns rows [offsets[e], offsets[e + 1]); groups may be empty, and
  * rows outside every group are neither read nor written.  Offsets that
  * decrease or leave [0, rows] are found on the device: the call computes
- * nothing and sets the device error word to 7 (trb_device_error).  At most
+ * nothing and sets the device error word to 7 (trb_device_error).  With 0 rows
+ * only the weight gradient launches (its zeros) and looks at offsets.  At most
  * 1024 groups; rows, n and k at most 2130706432.  Asynchronous on `stream`,
  * on the calling thread's current device, which has to be the one that holds
  * the operands and the stream; no workspace, so calls on several streams may
@@ -295,8 +296,9 @@ int trb_grouped_wgrad_launch(int dtype, int groups, int rows, int n, int k, cons
 
 /* Products with 4-bit weights: out[r, n] = the sum over k of
  * x[r, k] * (q[e, n, k] - z[e, n, k / group_size]) * s[e, n, k / group_size]
- * for the rows r of group e; meant for few rows a group (each 8 or 16 rows of
- * a group read its weights once).  x rows x k, out rows x n, s groups x n x
+ * for the rows r of group e; meant for few rows a group: the rows of a group
+ * that are taken at once, 8 or 16 up to k = 4096 and no more than 65536 / k,
+ * read its weights once.  x rows x k, out rows x n, s groups x n x
  * (k / group_size), bfloat16 or float16 alike; q groups x n x (k / 2) bytes,
  * the even k in the low four bits; zeros bytes shaped as s (the low four bits
  * count), or NULL for 8 throughout.  offsets as above, or NULL for one group of

@@ -87,16 +87,17 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 // tiles, and no row of another group ever meets this group's weights.  A group
 // of more than 256 rows is cut into equal chunks.  The price is an epilogue
 // that transposes, on the tensor-memory fragments in registers (stmatrix).
-// Measured: 32768 rows, 8 groups, 4096 x 4096, 810 to 860 us, 1280 to 1360
-// TFLOP/s under the power cap; 4109 rows, 16 groups, 2048 x 4096, 74 us; 96
-// rows, 32 groups, 2048 x 1408, 36 us, 4.8 TB/s of weights.  Between the two
-// bounds neither the weights' bytes nor the tensor pipe run alone: 37 groups of
-// 4096 x 1024 take 57 us with 16 rows each and 75 with 256, where both floors
-// are 48 us.  Asking the next stages' weights into L2 made it slower (96 rows
-// 43 us, 4109 rows 85).  Rows past the group's end
-// are loaded and multiplied but not stored; each output depends on its own row
-// only, so what stands there (the next group's rows, NaN) does not matter.
-// K past the end is zero in both operands (the tensor maps are per group).
+// Measured: 32768 rows, 8 groups, 4096 x 4096, 850 to 880 us, 1250 to 1290
+// TFLOP/s under the power cap; 4109 rows, 16 groups, 2048 x 4096, 70 us in a
+// burst at 1965 MHz and 84 sustained at the cap's 1180; 96 rows, 32 groups,
+// 2048 x 1408, 36 us, 4.8 TB/s of weights.  Between the two bounds neither the
+// weights' bytes nor the tensor pipe run alone: 37 groups of 4096 x 1024 take
+// 57 us with 16 rows each and 75 with 256, where both floors are 48 us.
+// Asking the next stages' weights into L2 made it slower (in bursts, 96 rows
+// 43 us, 4109 rows 85).  Rows past the group's end are loaded and multiplied
+// but not stored; each output depends on its own row only, so what stands
+// there (the next group's rows, NaN) does not matter. K past the end is zero
+// in both operands (the tensor maps are per group).
 struct ProductTile {
     int e, row0, rows, n0;
 };
@@ -602,10 +603,11 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
 // a stage lands on a barrier of its own CTA; a fixer warp clears the rows and
 // then signals the leader's full barrier.
 // A group without rows has a gradient of zeros, which the epilogue writes.
-// Measured: 32768 rows, 8 groups, 4096 x 4096, 800 to 880 us, 1250 to 1370
-// TFLOP/s under the power cap; 8111 rows, 64 groups, 2048 x 1544, 126 us, bound
-// by writing out tiles of two stages each (8192 rows, 64 groups, 2048 x 1536:
-// 111 us, the products without the epilogue 62, the stores alone 68).
+// Measured: 32768 rows, 8 groups, 4096 x 4096, 870 to 910 us, 1210 to 1260
+// TFLOP/s under the power cap; 8111 rows, 64 groups, 2048 x 1544, 125 us in a
+// burst at 1965 MHz and 140 sustained, bound by reading out tiles of two stages
+// each, a seventh column of them for 8 columns (1536 columns: 109 us, 1552: 123;
+// zeros alone 64 and 71 us for 1536 and 1544).  4 bytes spill at 168 registers.
 struct WgradTile {
     int e, row0, rows, m0, n0;
 };
@@ -841,11 +843,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgradThreads, 1)
         // rows of the tile each, so that one tile is read out of TMEM while another waits on its stores.  8 x 256
         // results at a time go through shared memory (stmatrix) and leave as whole rows of the tile, 512 bytes a
         // store: where N is not a multiple of 16, rows begin in the middle of a sector and each end of a run writes
-        // a part of one (64 zero gradients of 2048 x 1544: 133 us in runs of 128 bytes, 100 in longer ones, 83 with
-        // the tiles of a row of the gradient next to each other in time; 67 us for 2048 x 1536).  60 gradients of
-        // 127 rows on average: 152 us with one group of eight warps, 132 with a group for each accumulator, 129 with
-        // whole rows, 126 in that tile order; 133 with the stores moved to sector boundaries, 182 with sixteen warps
-        // and runs of 256 bytes.
+        // a part of one (64 zero gradients of 2048 x 1544: 133 us in runs of 128 bytes, 100 in longer ones, 71 with
+        // the tiles of a row of the gradient next to each other in time; 64 us for 2048 x 1536).  60 gradients of
+        // 127 rows on average, in bursts: 152 us with one group of eight warps, 132 with a group for each
+        // accumulator, 129 with whole rows, 126 in that tile order; 133 with the stores moved to sector boundaries,
+        // 182 with sixteen warps and runs of 256 bytes.
         const int q = warp & 3, group = (warp - 2) >> 2;
         const uint32_t acce_leader = mapa_shared(smem_u32(&acce_bar[group]), 0);
         const uint32_t t_rows = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(group * 256);

@@ -5,15 +5,15 @@
 // for the rows r of expert e (one expert: a plain matrix).  q is stored two to
 // a byte along k, the low four bits first.
 //
-// The bytes of q bound it: 1/2 byte per weight, read once for up to 8 (16)
-// rows of x.  The products run on mma.sync m16n8k16, 16 outputs x 8 rows of x
-// per instruction -- at one row the tensor pipe still does with one
-// instruction per 256 weights what would take 256 FMA lanes, and the exact
-// products of small whole numbers with 16-bit x accumulate in fp32.  Weights
-// become 16-bit floats by bit operations: a 4-bit q ORed into the mantissa of
-// 128 is 128 + q exactly, and subtracting 128 + z is exact too, so nothing is
-// rounded before the product, and the scale is applied in fp32 to each
-// group's sum.
+// The bytes of q are its floor: 1/2 byte per weight, read once for the rows of
+// x taken at once (up to 8 or 16, as far as they fit).  The products run on
+// mma.sync m16n8k16, 16 outputs x 8 rows of x per instruction -- at one row
+// the tensor pipe still does with one instruction per 256 weights what would
+// take 256 FMA lanes, and the exact products of small whole numbers with
+// 16-bit x accumulate in fp32.  Weights become 16-bit floats by bit
+// operations: a 4-bit q ORed into the mantissa of 128 is 128 + q exactly, and
+// subtracting 128 + z is exact too, so nothing is rounded before the product,
+// and the scale is applied in fp32 to each group's sum.
 //
 // The order of k inside a product is free as long as q and x agree on it, so
 // each of the four threads that share an output takes W consecutive words (8
@@ -32,16 +32,20 @@
 // in the order of k.
 //
 // Measured (CUDA graph of calls on three sets of inputs): one row, 4096 x 4096,
-// 5.0 us, launch and latency; one row, 16384 x 8192, zero points, groups of 64,
-// 22 us, 3.3 TB/s; 40 rows of 22 experts, 2048 x 4096, 27 us, 3.6 TB/s; 15 rows,
-// 11009 x 4096, groups of 32, 18.5 us.  The two middle ones issue in 50% of the
-// cycles, 42 instructions per 512 weights, half of them the conversion; with
-// the conversion and the products taken out they ran 20 and 26 us, so what
-// bounds them is how the loads are kept in flight.  Tried and slower: the words
-// through TMA rings (a warp's own, 22 and 33 us, or a producer warp's, 26 and
-// 35), through cp.async (26 and 32), asked into L2 packs ahead (25 and 35), 24
-// warps a CTA (29 and 31), k shared by clusters of 4 CTAs (45 us for the 15
-// rows).
+// 4.9 us, launch and latency; one row, 16384 x 8192, zero points, groups of 64,
+// 22.3 us, 3.3 TB/s; 40 rows of 22 experts, 2048 x 4096, 27.4 us, 3.6 TB/s; 15
+// rows, 11009 x 4096, groups of 32, 17.9 us.  A copy that moves as many bytes
+// takes 3.2, 13.3, 16.6 and 6.0 us.  What bounds the middle two is not known:
+// they issue in 50% of the cycles, 42 instructions per 512 weights, half of
+// them the conversion; with the conversion and the products taken out they ran
+// 20 and 26 us; 12, 16 and 20 warps take the same; and it matters little
+// whether the words come from L2 or from memory (8 rows of 5 experts, 4096 x
+// 4096: 16.2 and 17.4 us).  Tried and slower: the words through TMA rings (a
+// warp's own, 22 and 33 us, or a producer warp's, 26 and 35), through cp.async
+// (26 and 32), asked into L2 packs ahead (25 and 35), 24 warps a CTA (29 and
+// 31), k shared by clusters of 4 CTAs (45 us for the 15 rows), packs dealt to
+// the warps in turn, so that an SM reads runs of whole rows.  14 of the 40
+// variants spill 4 to 20 bytes at 128 registers.
 //
 // No counterpart in the reference.
 #include <cuda_bf16.h>

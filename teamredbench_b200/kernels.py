@@ -239,7 +239,8 @@ def gemv_w4(x: Any, q: Any, scales: Any, out: Any, *, zeros: Any | None = None, 
     uint8 of the same shape (values 0 to 15), or None for 8.  A single matrix may
     be given without the leading dimension, and needs no offsets; otherwise
     offsets are those of grouped_gemm.  Meant for few rows a group: their weights
-    are read once for each 8 or 16 rows.  k is at most 65536; n is free."""
+    are read once for the rows taken at once, 8 or 16 of them and no more than
+    65536 / k.  k is at most 65536; n is free."""
     global _UINT8
     device = _check_operands(x, q, scales, out, zeros, offsets)
     if x.dim() != 2 or q.dim() not in (2, 3):
