@@ -309,6 +309,84 @@ int trb_grouped_wgrad_launch(int dtype, int groups, int rows, int n, int k, cons
 int trb_gemv_w4_launch(int dtype, int groups, int rows, int n, int k, int group_size, const void* x, const void* q,
                        const void* scales, const void* zeros, const int32_t* offsets, void* out, void* stream);
 
+/* ---- rows to the experts and back --------------------------------------- */
+
+/* A router gives each of `tokens` tokens `choices` experts: ids, tokens x
+ * choices, int32 or int64 (id_bytes 4 or 8).  Writes, in one launch and without
+ * a workspace, what the grouped products take: offsets (experts + 1), where the
+ * rows of each expert begin once all choices are sorted by expert, and
+ * slots[t, j] (tokens x choices), the place of choice j of token t among them,
+ * in the order of the choices inside an expert; -1 for an id outside [0,
+ * experts), which no expert here takes (another rank's, a token left out).
+ * At most 1024 experts; tokens * choices at most 2130706432; tokens may be 0.
+ * Asynchronous on `stream`, on the calling thread's current device, as all
+ * entries of this section.  No reference counterpart. */
+int trb_expert_sort_launch(int id_bytes, int tokens, int choices, int experts, const void* ids, int32_t* offsets,
+                           int32_t* slots, void* stream);
+
+/* out[slots[t, j]] = x[t], or weights[t, j] * x[t] with weights: x tokens x
+ * width, out rows x width, bfloat16, float16 or float32; weights tokens x
+ * choices in float32 or that type (weight_dtype), or NULL.  A negative slot is
+ * a choice without a row; a slot of `rows` or more is skipped and sets the
+ * device error word to 8.  Rows of out that no slot names are left as they are;
+ * one that two slots name gets either.  Products are made in fp32 and rounded
+ * once.  Any width; rows move 16 bytes at a time where width and pointers are
+ * multiples of 16 bytes.  rows, width and tokens * choices at most 2130706432. */
+int trb_expert_dispatch_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width, const void* x,
+                               const int32_t* slots, const void* weights, void* out, void* stream);
+
+/* out[t] = the sum over j of weights[t, j] * y[slots[t, j]] (weights NULL: of
+ * the rows): y rows x width, out tokens x width, zeros for a token whose slots
+ * are all negative.  fp32 sums in the order of j, one rounding.  Types, slots
+ * and limits as trb_expert_dispatch_launch, whose gradient for x this is. */
+int trb_expert_combine_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width, const void* y,
+                              const int32_t* slots, const void* weights, void* out, void* stream);
+
+/* Gradient of trb_expert_combine_launch from that of its result, grad (tokens x
+ * width): grad_y[slots[t, j]] = weights[t, j] * grad[t] (rows x width; other
+ * rows are left as they are) and grad_weights[t, j] = the sum over the width of
+ * grad[t] * y[slots[t, j]] (tokens x choices, the weights' type; 0 for a
+ * negative slot), in fp32 and in the same order at every call.  Types, slots and
+ * limits as above. */
+int trb_expert_combine_grad_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width,
+                                   const void* grad, const void* y, const int32_t* slots, const void* weights,
+                                   void* grad_y, void* grad_weights, void* stream);
+
+/* ---- microscaled 4-bit floating point ----------------------------------- */
+
+/* Storage: a row of k values is k / 2 bytes of e2m1 codes, the even k in the
+ * low four bits, and a byte b of e8m0, 2^(b - 127), for every 32 values, 255
+ * for NaN; the scales of a row begin at a multiple of 16 bytes, pitch = k / 32
+ * rounded up to it.  k is a multiple of 32 and all pointers are 16-byte
+ * aligned. */
+
+/* x (rows x k, bfloat16, float16 or float32) to q (rows x k / 2) and scales
+ * (rows x pitch, zeros behind the last block).  The scale of a block is
+ * 2^(floor(log2 max|x|) - 2), at least 2^-127; values are rounded to the nearest
+ * code, ties to the even one, at most 6.  A block with a NaN or an infinity
+ * gets the scale NaN and codes 0.  With slots (rows x choices, as from
+ * trb_expert_sort_launch) row t goes to the rows slots[t, j] of q and scales,
+ * which have out_rows; otherwise choices and out_rows are not looked at.
+ * Negative slots, slots of out_rows or more and rows that no slot names: as for
+ * trb_expert_dispatch_launch.  rows, k, out_rows and rows * choices at most
+ * 2130706432. */
+int trb_quantize_fp4_launch(int dtype, int rows, int k, const void* x, int choices, const int32_t* slots, int out_rows,
+                            void* q, void* scales, void* stream);
+
+/* out (rows x k, bfloat16, float16 or float32) = the values of q and scales;
+ * exact in bfloat16 and float32, rounded in float16 where they are too small
+ * for it (or infinite, where too large). */
+int trb_dequantize_fp4_launch(int dtype, int rows, int k, const void* q, const void* scales, void* out, void* stream);
+
+/* out[r, n] = the sum over k of a[r, k] * b[e, n, k], both 4-bit floating point
+ * as above: a rows x k, b groups x n x k, out rows x n in bfloat16 or float16
+ * (dtype).  offsets as for trb_grouped_gemm_launch, or NULL for one group of all
+ * rows.  fp32 sums, one rounding; a NaN scale makes a NaN of the row's results
+ * (of a) or of the column's (of b).  Any n; k at most 2^26.  Error word, streams
+ * and limits as for the other grouped entry points. */
+int trb_gemm_fp4_launch(int dtype, int groups, int rows, int n, int k, const void* a, const void* a_scales, const void* b,
+                        const void* b_scales, const int32_t* offsets, void* out, void* stream);
+
 /* Round f32 values in place on the device to tf32 (round to nearest, ties
  * away from zero; cvt.rna.tf32.f32).  Used to prepare tf32 GEMM inputs. */
 int trb_round_tf32(void* data, uint64_t count, void* stream);

@@ -48,6 +48,13 @@ EXPORTED_SYMBOLS = (
     "trb_grouped_gemm_launch",
     "trb_grouped_wgrad_launch",
     "trb_gemv_w4_launch",
+    "trb_expert_sort_launch",
+    "trb_expert_dispatch_launch",
+    "trb_expert_combine_launch",
+    "trb_expert_combine_grad_launch",
+    "trb_quantize_fp4_launch",
+    "trb_dequantize_fp4_launch",
+    "trb_gemm_fp4_launch",
     "trb_round_tf32",
     "trb_selftest_bounded_wait",
 )
@@ -177,6 +184,20 @@ def load() -> ctypes.CDLL:
     lib.trb_grouped_wgrad_launch.restype = i32
     lib.trb_gemv_w4_launch.argtypes = [i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]
     lib.trb_gemv_w4_launch.restype = i32
+    lib.trb_expert_sort_launch.argtypes = [i32, i32, i32, i32, vp, vp, vp, vp]
+    lib.trb_expert_sort_launch.restype = i32
+    lib.trb_expert_dispatch_launch.argtypes = [i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]
+    lib.trb_expert_dispatch_launch.restype = i32
+    lib.trb_expert_combine_launch.argtypes = [i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp]
+    lib.trb_expert_combine_launch.restype = i32
+    lib.trb_expert_combine_grad_launch.argtypes = [i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]
+    lib.trb_expert_combine_grad_launch.restype = i32
+    lib.trb_quantize_fp4_launch.argtypes = [i32, i32, i32, vp, i32, vp, i32, vp, vp, vp]
+    lib.trb_quantize_fp4_launch.restype = i32
+    lib.trb_dequantize_fp4_launch.argtypes = [i32, i32, i32, vp, vp, vp, vp]
+    lib.trb_dequantize_fp4_launch.restype = i32
+    lib.trb_gemm_fp4_launch.argtypes = [i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]
+    lib.trb_gemm_fp4_launch.restype = i32
     lib.trb_round_tf32.argtypes = [vp, u64, vp]
     lib.trb_round_tf32.restype = i32
     lib.trb_selftest_bounded_wait.argtypes = [ctypes.c_uint32, i32, res_p]
@@ -288,6 +309,76 @@ def gemv_w4_launch(dtype: str, groups: int, rows: int, n: int, k: int, group_siz
         _refuse_past_32_bits(groups, rows, n, k)
     status = (_lib or load()).trb_gemv_w4_launch(DTYPE_CODES[dtype], groups, rows, n, k, group_size, x, q, scales,
                                                  zeros, offsets, out, stream or None)
+    if status:
+        check(status)
+
+
+def expert_sort_launch(id_bytes: int, tokens: int, choices: int, experts: int, ids: int, offsets: int, slots: int,
+                       stream: int = 0) -> None:
+    if (tokens | choices | experts) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(tokens, choices, experts)
+    status = (_lib or load()).trb_expert_sort_launch(id_bytes, tokens, choices, experts, ids, offsets, slots,
+                                                     stream or None)
+    if status:
+        check(status)
+
+
+def expert_dispatch_launch(dtype: str, weight_dtype: str, tokens: int, choices: int, rows: int, width: int, x: int,
+                           slots: int, weights: int | None, out: int, stream: int = 0) -> None:
+    if (tokens | choices | rows | width) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(tokens, choices, rows, width)
+    status = (_lib or load()).trb_expert_dispatch_launch(DTYPE_CODES[dtype], DTYPE_CODES[weight_dtype], tokens, choices,
+                                                         rows, width, x, slots, weights, out, stream or None)
+    if status:
+        check(status)
+
+
+def expert_combine_launch(dtype: str, weight_dtype: str, tokens: int, choices: int, rows: int, width: int, y: int,
+                          slots: int, weights: int | None, out: int, stream: int = 0) -> None:
+    if (tokens | choices | rows | width) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(tokens, choices, rows, width)
+    status = (_lib or load()).trb_expert_combine_launch(DTYPE_CODES[dtype], DTYPE_CODES[weight_dtype], tokens, choices,
+                                                        rows, width, y, slots, weights, out, stream or None)
+    if status:
+        check(status)
+
+
+def expert_combine_grad_launch(dtype: str, weight_dtype: str, tokens: int, choices: int, rows: int, width: int,
+                               grad: int, y: int, slots: int, weights: int, grad_y: int, grad_weights: int,
+                               stream: int = 0) -> None:
+    if (tokens | choices | rows | width) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(tokens, choices, rows, width)
+    status = (_lib or load()).trb_expert_combine_grad_launch(DTYPE_CODES[dtype], DTYPE_CODES[weight_dtype], tokens,
+                                                             choices, rows, width, grad, y, slots, weights, grad_y,
+                                                             grad_weights, stream or None)
+    if status:
+        check(status)
+
+
+def quantize_fp4_launch(dtype: str, rows: int, k: int, x: int, choices: int, slots: int | None, out_rows: int, q: int,
+                        scales: int, stream: int = 0) -> None:
+    if (rows | k | choices | out_rows) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(rows, k, choices, out_rows)
+    status = (_lib or load()).trb_quantize_fp4_launch(DTYPE_CODES[dtype], rows, k, x, choices, slots, out_rows, q, scales,
+                                                      stream or None)
+    if status:
+        check(status)
+
+
+def dequantize_fp4_launch(dtype: str, rows: int, k: int, q: int, scales: int, out: int, stream: int = 0) -> None:
+    if (rows | k) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(rows, k)
+    status = (_lib or load()).trb_dequantize_fp4_launch(DTYPE_CODES[dtype], rows, k, q, scales, out, stream or None)
+    if status:
+        check(status)
+
+
+def gemm_fp4_launch(dtype: str, groups: int, rows: int, n: int, k: int, a: int, a_scales: int, b: int, b_scales: int,
+                    offsets: int | None, out: int, stream: int = 0) -> None:
+    if (groups | rows | n | k) > 0x7FFFFFFF:  # ctypes would cut it off without a word
+        _refuse_past_32_bits(groups, rows, n, k)
+    status = (_lib or load()).trb_gemm_fp4_launch(DTYPE_CODES[dtype], groups, rows, n, k, a, a_scales, b, b_scales,
+                                                  offsets, out, stream or None)
     if status:
         check(status)
 

@@ -1,0 +1,553 @@
+// expert_rows.cu -- rows of tokens to their experts and back, with weights, and the gradients.
+//
+// A router gives each token J choices of experts.  For the choice j of token t
+//   sort      slots[t, j] = the place of (t, j) among all choices sorted by expert, in the order of (t, j) inside an
+//             expert; -1 where the choice is no expert of this layer.  offsets[e] = where expert e's places begin
+//   dispatch  out[slots[t, j]] = x[t], or w[t, j] * x[t]
+//   combine   out[t] = sum over j of w[t, j] * y[slots[t, j]]
+//   gradient  of combine: gy[slots[t, j]] = w[t, j] * g[t],  gw[t, j] = <g[t], y[slots[t, j]]>
+// and the gradient of dispatch is combine.  offsets and the sorted rows are what the products of trb_groups.cuh take.
+//
+// No counterpart in the reference.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "trb_common.cuh"
+#include "trb_groups.cuh"
+
+namespace trb {
+namespace rows {
+
+__device__ int g_rows_error;
+
+// ------------------------------------------------------------------ sort
+// Counting sort in one launch, by one cluster: no workspace, no atomics, and the order inside an expert is that of the
+// choices.  A CTA takes a contiguous part of the choices, a warp a contiguous part of the CTA's, 32 at a time:
+// match.any tells each lane which others chose its expert, so the first of them adds their number to the warp's own
+// count.  The counts are then summed over the warps before, the CTAs before (distributed shared memory) and the experts
+// before, and a second pass over the choices gives each its place.
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+
+template <typename Id>
+__device__ __forceinline__ int expert_of(const Id* ids, int i, int end, int experts) {
+    if (i >= end) return -1;
+    const Id id = ids[i];
+    return id >= 0 && id < (Id)experts ? (int)id : -1;
+}
+
+template <typename Id>
+__global__ void __launch_bounds__(kSortThreads)
+    expert_sort_kernel(const Id* ids, int entries, int experts, int* offsets, int* slots) {
+    extern __shared__ int counts[];  // [warps][experts], then the CTA's totals and where each expert's places begin
+    int* const totals = counts + (blockDim.x >> 5) * experts;
+    int* const begin = totals + experts;
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ctas = gridDim.x, rank = blockIdx.x;  // the grid is one cluster
+    int* const mine = counts + warp * experts;
+
+    for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) counts[i] = 0;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    __syncthreads();
+
+    // Whole groups of 32 to every warp of the cluster, as evenly as they go.
+    const int64_t groups = ((int64_t)entries + 31) / 32;
+    const int64_t part = (int64_t)rank * warps + warp, parts = (int64_t)ctas * warps;
+    const int first = (int)(groups * part / parts * 32);
+    const int end = (int)min((int64_t)entries, groups * (part + 1) / parts * 32);
+
+    int next = expert_of(ids, first + lane, end, experts);
+    for (int i = first; i < end; i += 32) {
+        const int e = next;
+        next = expert_of(ids, i + 32 + lane, end, experts);
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+        int sum = 0;
+        for (int w = 0; w < warps; ++w) {
+            const int c = counts[w * experts + e];
+            counts[w * experts + e] = sum;
+            sum += c;
+        }
+        totals[e] = sum;
+    }
+    cluster_sync_all();
+    // begin[e] = this CTA's first place among the expert's; then the experts before are added.
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+        int before = 0, all = 0;
+        for (int r = 0; r < ctas; ++r) {
+            int c;
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c) : "r"(mapa_shared(smem_u32(totals + e), r)));
+            if (r < rank) before += c;
+            all += c;
+        }
+        begin[e] = before;
+        begin[experts + e] = all;
+    }
+    __syncthreads();
+    cluster_arrive();  // the other CTAs' totals have been read
+    if (warp == 0) {
+        int base = 0;
+        for (int e0 = 0; e0 < experts; e0 += 32) {
+            const int e = e0 + lane;
+            const int all = e < experts ? begin[experts + e] : 0;
+            int sum = all;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += up;
+            }
+            if (e < experts) {
+                begin[e] += base + sum - all;
+                if (rank == 0) offsets[e] = base + sum - all;
+            }
+            base += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0 && rank == 0) offsets[experts] = base;
+    }
+    __syncthreads();
+    next = expert_of(ids, first + lane, end, experts);
+    for (int i = first; i < end; i += 32) {
+        const int e = next;
+        next = expert_of(ids, i + 32 + lane, end, experts);
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        const int before = __popc(same & ((1u << lane) - 1u));
+        int place = -1;
+        if (e >= 0) place = begin[e] + mine[e] + before;
+        __syncwarp();
+        if (e >= 0 && before == 0) mine[e] += __popc(same);
+        if (i + lane < end) slots[i + lane] = place;
+        __syncwarp();
+    }
+    cluster_wait();
+}
+
+// ------------------------------------------------------------------ rows there and back
+// V values of a row that move together: 16 bytes, or one value where the rows are not 16-byte aligned.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+    T v[V];
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T round_to(float v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+    else return __float2bfloat16_rn(v);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load(const T* p) {
+    return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const Pack<T, V>& v) {
+    *reinterpret_cast<Pack<T, V>*>(p) = v;
+}
+
+// The row of a slot, or -1 where there is none.  A slot behind the last row is an error of the caller's.
+__device__ __forceinline__ int row_of(const int* slots, int64_t i, int rows) {
+    const int s = slots[i];
+    if (s >= rows) {
+        atomicCAS(&g_rows_error, 0, kErrSlots);
+        return -1;
+    }
+    return s;
+}
+
+constexpr int kRowThreads = 256;
+
+// Threads of a CTA: 1 << log2_lanes of them for one token's row, several tokens side by side; blockIdx.y shares a row
+// among CTAs where there are few tokens.
+struct RowWalk {
+    int64_t token, token_step;
+    int pack, pack_step;
+};
+__device__ __forceinline__ RowWalk row_walk(int log2_lanes) {
+    RowWalk w;
+    const int side = kRowThreads >> log2_lanes;
+    w.token = (int64_t)blockIdx.x * side + (threadIdx.x >> log2_lanes);
+    w.token_step = (int64_t)gridDim.x * side;
+    w.pack = (int)(blockIdx.y << log2_lanes) + (threadIdx.x & ((1 << log2_lanes) - 1));
+    w.pack_step = (int)(gridDim.y << log2_lanes);
+    return w;
+}
+
+// Each row of x is read once, whatever the number of its choices.
+template <typename T, typename W, int V>
+__global__ void __launch_bounds__(kRowThreads)
+    expert_dispatch_kernel(const T* x, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
+                           int width, int log2_lanes) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const RowWalk w = row_walk(log2_lanes);
+    const int packs = width / V;
+    for (int64_t t = w.token; t < tokens; t += w.token_step) {
+        for (int p = w.pack; p < packs; p += w.pack_step) {
+            const Pack<T, V> v = load<T, V>(x + t * width + (int64_t)p * V);
+            for (int j = 0; j < choices; ++j) {
+                const int row = row_of(slots, t * choices + j, rows);
+                if (row < 0) continue;
+                Pack<T, V> o = v;
+                if (weights != nullptr) {
+                    const float f = to_f32(weights[t * choices + j]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(f * to_f32(v.v[i]));
+                }
+                store<T, V>(out + (int64_t)row * width + (int64_t)p * V, o);
+            }
+        }
+    }
+}
+
+// Choices whose rows are on their way at the same time.
+constexpr int kAtOnce = 4;
+
+// Sums in fp32, in the order of the choices, rounded once.
+template <typename T, typename W, int V>
+__global__ void __launch_bounds__(kRowThreads)
+    expert_combine_kernel(const T* y, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
+                          int width, int log2_lanes) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const RowWalk w = row_walk(log2_lanes);
+    const int packs = width / V;
+    for (int64_t t = w.token; t < tokens; t += w.token_step) {
+        for (int p = w.pack; p < packs; p += w.pack_step) {
+            float sum[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+            for (int j0 = 0; j0 < choices; j0 += kAtOnce) {
+                int row[kAtOnce];
+                Pack<T, V> v[kAtOnce];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    row[j] = j0 + j < choices ? row_of(slots, t * choices + j0 + j, rows) : -1;
+                    if (row[j] >= 0) v[j] = load<T, V>(y + (int64_t)row[j] * width + (int64_t)p * V);
+                }
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    if (row[j] < 0) continue;
+                    const float f = weights != nullptr ? to_f32(weights[t * choices + j0 + j]) : 1.0f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum[i] = fmaf(f, to_f32(v[j].v[i]), sum[i]);
+                }
+            }
+            Pack<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(sum[i]);
+            store<T, V>(out + t * width + (int64_t)p * V, o);
+        }
+    }
+}
+
+// One pass over a token's rows for both gradients.  The products of a weight's gradient are added in fp32: in a
+// thread, in its warp, then over the row's warps, always in the same order.
+template <typename T, typename W, int V>
+__global__ void __launch_bounds__(kRowThreads)
+    expert_combine_grad_kernel(const T* grad, const T* y, const int* slots, const W* weights, T* grad_y, W* grad_weights,
+                               int64_t tokens, int choices, int rows, int width, int log2_lanes) {
+    __shared__ float part[kRowThreads / 32][kAtOnce];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int lanes = 1 << log2_lanes;  // 32 or more
+    const int side = kRowThreads >> log2_lanes, own = threadIdx.x >> log2_lanes, l = threadIdx.x & (lanes - 1);
+    const int packs = width / V;
+    for (int64_t t0 = (int64_t)blockIdx.x * side; t0 < tokens; t0 += (int64_t)gridDim.x * side) {
+        const int64_t t = t0 + own;
+        for (int j0 = 0; j0 < choices; j0 += kAtOnce) {
+            int row[kAtOnce];
+            float f[kAtOnce], dot[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                dot[j] = 0.0f;
+                f[j] = 0.0f;
+                row[j] = t < tokens && j0 + j < choices ? row_of(slots, t * choices + j0 + j, rows) : -1;
+                if (row[j] >= 0) f[j] = to_f32(weights[t * choices + j0 + j]);
+            }
+            if (t < tokens) {
+                for (int p = l; p < packs; p += lanes) {
+                    const int64_t at = (int64_t)p * V;
+                    const Pack<T, V> g = load<T, V>(grad + t * width + at);
+                    Pack<T, V> v[kAtOnce];
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j)
+                        if (row[j] >= 0) v[j] = load<T, V>(y + (int64_t)row[j] * width + at);
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j) {
+                        if (row[j] < 0) continue;
+                        Pack<T, V> o;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            const float gi = to_f32(g.v[i]);
+                            dot[j] = fmaf(gi, to_f32(v[j].v[i]), dot[j]);
+                            o.v[i] = round_to<T>(f[j] * gi);
+                        }
+                        store<T, V>(grad_y + (int64_t)row[j] * width + at, o);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
+                if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot[j];
+            }
+            __syncthreads();
+            if (l < kAtOnce && j0 + l < choices && t < tokens) {
+                float sum = 0.0f;
+                for (int w = 0; w < lanes / 32; ++w) sum += part[own * (lanes / 32) + w][l];
+                grad_weights[t * choices + j0 + l] = round_to<W>(sum);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+template <typename Kernel, typename... Args>
+static int launch(Kernel kernel, dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
+    TRB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return TRB_OK;
+}
+
+template <typename Id>
+static int launch_sort(const void* ids, int entries, int experts, int* offsets, int* slots, int dev,
+                       cudaStream_t stream) {
+    static bool attr_set[64] = {};
+    if (dev >= 64 || !attr_set[dev]) {
+        const int most = (int)sizeof(int) * (kSortWarps + 3) * kMaxGroups;
+        TRB_CUDA(cudaFuncSetAttribute(expert_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        if (dev < 64) attr_set[dev] = true;
+    }
+    const int64_t groups = ((int64_t)entries + 31) / 32;
+    const int ctas = groups <= 2 * kSortWarps ? 1 : groups <= 8 * kSortWarps ? 4 : 8;
+    const int warps = (int)std::min<int64_t>(kSortWarps, std::max<int64_t>(groups, 8));
+    const size_t smem = sizeof(int) * (size_t)(warps + 3) * experts;
+    return launch(expert_sort_kernel<Id>, dim3((unsigned)ctas), 32 * warps, ctas, smem, stream,
+                  static_cast<const Id*>(ids), entries, experts, offsets, slots);
+}
+
+struct RowShape {
+    dim3 grid;
+    int log2_lanes;
+};
+// As many lanes a token as its row has packs, between a warp and a CTA; a row is shared among CTAs while the GPU is not full.
+static RowShape row_shape(int64_t tokens, int packs, bool whole_rows, int dev) {
+    RowShape s;
+    s.log2_lanes = 5;
+    while (s.log2_lanes < 8 && (1 << s.log2_lanes) < packs) ++s.log2_lanes;
+    const int64_t side = kRowThreads >> s.log2_lanes, blocks = (tokens + side - 1) / side;
+    const int64_t full = 8 * (int64_t)device_sm_count(dev);  // CTAs of 256 threads that the GPU holds
+    const int64_t share = whole_rows ? 1 : std::max<int64_t>(1, std::min<int64_t>((packs + kRowThreads - 1) / kRowThreads,
+                                                                                  full / std::max<int64_t>(blocks, 1)));
+    s.grid = dim3((unsigned)std::min<int64_t>(blocks, 1 << 30), (unsigned)std::min<int64_t>(share, 1024));
+    return s;
+}
+
+static int check(const char* what, int dtype, int weight_dtype, int tokens, int choices, int rows, int width,
+                 const void* slots, const void* weights) {
+    if (tokens < 0 || choices <= 0 || rows < 0 || width <= 0 || (tokens > 0 && slots == nullptr)) {
+        set_error("%s: sizes must be positive (tokens and rows may be 0) and pointers non-null", what);
+        return TRB_ERR_ARGS;
+    }
+    if (dtype != TRB_BFLOAT16 && dtype != TRB_FLOAT16 && dtype != TRB_FLOAT32) {
+        set_error("%s: unsupported dtype %s (bfloat16, float16 and float32)", what, dtype_name(dtype));
+        return TRB_SKIPPED;
+    }
+    if (weights != nullptr && weight_dtype != TRB_FLOAT32 && weight_dtype != dtype) {
+        set_error("%s: weights must be float32 or %s, not %s", what, dtype_name(dtype), dtype_name(weight_dtype));
+        return TRB_SKIPPED;
+    }
+    if (std::max({rows, width}) > kMaxExtent || (int64_t)tokens * choices > kMaxExtent) {
+        set_error("%s: rows, width and tokens * choices at most %d (rows=%d width=%d tokens=%d choices=%d)", what,
+                  kMaxExtent, rows, width, tokens, choices);
+        return TRB_SKIPPED;
+    }
+    return TRB_OK;
+}
+
+static uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// Pointers of values are aligned to a value, and those of rows that move 16 bytes at a time to 16 bytes.
+static int check_align(const char* what, int dtype, int weight_dtype, uintptr_t values, const void* weights,
+                       const void* grad_weights, const void* slots) {
+    const size_t size = dtype_size(dtype), weight_size = dtype_size(weight_dtype);
+    if (values % size != 0 || bits(slots) % 4 != 0 ||
+        (weights != nullptr && (bits(weights) | bits(grad_weights)) % weight_size != 0)) {
+        set_error("%s: pointers must be aligned to their elements", what);
+        return TRB_ERR_ALIGN;
+    }
+    return TRB_OK;
+}
+
+template <typename T, typename W, int V>
+static int launch_move(bool back, const void* src, const int* slots, const void* weights, void* dst, int tokens,
+                       int choices, int rows, int width, int dev, cudaStream_t stream) {
+    const RowShape s = row_shape(tokens, width / V, false, dev);
+    return launch(back ? expert_combine_kernel<T, W, V> : expert_dispatch_kernel<T, W, V>, s.grid, kRowThreads, 0, 0,
+                  stream, static_cast<const T*>(src), slots, static_cast<const W*>(weights), static_cast<T*>(dst),
+                  (int64_t)tokens, choices, rows, width, s.log2_lanes);
+}
+
+template <typename T>
+static int move_rows(bool back, bool weights_f32, const void* src, const int* slots, const void* weights, void* dst,
+                     int tokens, int choices, int rows, int width, int dev, cudaStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = width % V == 0 && (bits(src) | bits(dst)) % 16 == 0;
+    if (weights_f32)
+        return wide ? launch_move<T, float, V>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
+                    : launch_move<T, float, 1>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+    return wide ? launch_move<T, T, V>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
+                : launch_move<T, T, 1>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+}
+
+static int move(const char* what, bool back, int dtype, int weight_dtype, int tokens, int choices, int rows, int width,
+                const void* src, const int32_t* slots, const void* weights, void* dst, void* stream) {
+    clear_error();
+    int rc = check(what, dtype, weight_dtype, tokens, choices, rows, width, slots, weights);
+    if (rc != TRB_OK) return rc;
+    if (tokens == 0) return TRB_OK;
+    const void* const tokens_side = back ? dst : src;
+    const void* const rows_side = back ? src : dst;
+    if (tokens_side == nullptr || (rows > 0 && rows_side == nullptr)) {
+        set_error("%s: rows must be non-null", what);
+        return TRB_ERR_ARGS;
+    }
+    rc = check_align(what, dtype, weight_dtype, bits(src) | bits(dst), weights, nullptr, slots);
+    if (rc != TRB_OK) return rc;
+    int dev = 0;
+    TRB_CUDA(cudaGetDevice(&dev));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool f32 = weight_dtype == TRB_FLOAT32;
+    if (dtype == TRB_BFLOAT16)
+        return move_rows<__nv_bfloat16>(back, f32, src, slots, weights, dst, tokens, choices, rows, width, dev, s);
+    if (dtype == TRB_FLOAT16)
+        return move_rows<__half>(back, f32, src, slots, weights, dst, tokens, choices, rows, width, dev, s);
+    return move_rows<float>(back, true, src, slots, weights, dst, tokens, choices, rows, width, dev, s);
+}
+
+template <typename T, typename W>
+static int launch_grad(const void* grad, const void* y, const int* slots, const void* weights, void* grad_y,
+                       void* grad_weights, int tokens, int choices, int rows, int width, int dev, cudaStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = width % V == 0 && (bits(grad) | bits(y) | bits(grad_y)) % 16 == 0;
+    const RowShape s = row_shape(tokens, wide ? width / V : width, true, dev);
+    return launch(wide ? expert_combine_grad_kernel<T, W, V> : expert_combine_grad_kernel<T, W, 1>, s.grid, kRowThreads,
+                  0, 0, stream, static_cast<const T*>(grad), static_cast<const T*>(y), slots,
+                  static_cast<const W*>(weights), static_cast<T*>(grad_y), static_cast<W*>(grad_weights), (int64_t)tokens,
+                  choices, rows, width, s.log2_lanes);
+}
+
+int read_error(bool clear) {
+    int v = 0;
+    TRB_CUDA(cudaMemcpyFromSymbol(&v, g_rows_error, sizeof(int)));
+    if (clear) {
+        const int zero = 0;
+        TRB_CUDA(cudaMemcpyToSymbol(g_rows_error, &zero, sizeof(int)));
+    }
+    return v;
+}
+
+}  // namespace rows
+}  // namespace trb
+
+extern "C" int trb_expert_sort_launch(int id_bytes, int tokens, int choices, int experts, const void* ids,
+                                      int32_t* offsets, int32_t* slots, void* stream) {
+    using namespace trb;
+    clear_error();
+    if (tokens < 0 || choices <= 0 || experts <= 0 || offsets == nullptr ||
+        (tokens > 0 && (ids == nullptr || slots == nullptr))) {
+        set_error("trb_expert_sort_launch: sizes must be positive (tokens may be 0) and pointers non-null");
+        return TRB_ERR_ARGS;
+    }
+    if (id_bytes != 4 && id_bytes != 8) {
+        set_error("trb_expert_sort_launch: choices must be int32 or int64 (got %d bytes)", id_bytes);
+        return TRB_SKIPPED;
+    }
+    if (experts > kMaxGroups) {
+        set_error("trb_expert_sort_launch: at most %d experts (got %d)", kMaxGroups, experts);
+        return TRB_SKIPPED;
+    }
+    if ((int64_t)tokens * choices > kMaxExtent) {
+        set_error("trb_expert_sort_launch: tokens * choices at most %d (tokens=%d choices=%d)", kMaxExtent, tokens,
+                  choices);
+        return TRB_SKIPPED;
+    }
+    if (rows::bits(ids) % id_bytes != 0 || (rows::bits(offsets) | rows::bits(slots)) % 4 != 0) {
+        set_error("trb_expert_sort_launch: pointers must be aligned to their elements");
+        return TRB_ERR_ALIGN;
+    }
+    int dev = 0;
+    TRB_CUDA(cudaGetDevice(&dev));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return id_bytes == 4 ? rows::launch_sort<int>(ids, tokens * choices, experts, offsets, slots, dev, s)
+                         : rows::launch_sort<long long>(ids, tokens * choices, experts, offsets, slots, dev, s);
+}
+
+extern "C" int trb_expert_dispatch_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width,
+                                          const void* x, const int32_t* slots, const void* weights, void* out,
+                                          void* stream) {
+    return trb::rows::move("trb_expert_dispatch_launch", false, dtype, weight_dtype, tokens, choices, rows, width, x, slots,
+                           weights, out, stream);
+}
+
+extern "C" int trb_expert_combine_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width,
+                                         const void* y, const int32_t* slots, const void* weights, void* out,
+                                         void* stream) {
+    return trb::rows::move("trb_expert_combine_launch", true, dtype, weight_dtype, tokens, choices, rows, width, y, slots,
+                           weights, out, stream);
+}
+
+extern "C" int trb_expert_combine_grad_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width,
+                                              const void* grad, const void* y, const int32_t* slots, const void* weights,
+                                              void* grad_y, void* grad_weights, void* stream) {
+    using namespace trb;
+    const char* const what = "trb_expert_combine_grad_launch";
+    clear_error();
+    int rc = rows::check(what, dtype, weight_dtype, tokens, choices, rows, width, slots, weights);
+    if (rc != TRB_OK) return rc;
+    if (tokens == 0) return TRB_OK;
+    if (grad == nullptr || weights == nullptr || grad_weights == nullptr ||
+        (rows > 0 && (y == nullptr || grad_y == nullptr))) {
+        set_error("%s: pointers must be non-null", what);
+        return TRB_ERR_ARGS;
+    }
+    rc = rows::check_align(what, dtype, weight_dtype, rows::bits(grad) | rows::bits(y) | rows::bits(grad_y), weights,
+                           grad_weights, slots);
+    if (rc != TRB_OK) return rc;
+    int dev = 0;
+    TRB_CUDA(cudaGetDevice(&dev));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool f32 = weight_dtype == TRB_FLOAT32;
+    const auto call = [&](auto f) {
+        return f(grad, y, slots, weights, grad_y, grad_weights, tokens, choices, rows, width, dev, s);
+    };
+    if (dtype == TRB_BFLOAT16)
+        return f32 ? call(rows::launch_grad<__nv_bfloat16, float>) : call(rows::launch_grad<__nv_bfloat16, __nv_bfloat16>);
+    if (dtype == TRB_FLOAT16) return f32 ? call(rows::launch_grad<__half, float>) : call(rows::launch_grad<__half, __half>);
+    return call(rows::launch_grad<float, float>);
+}

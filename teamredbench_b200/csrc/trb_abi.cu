@@ -222,11 +222,17 @@ extern "C" int trb_device_error(int device_id, int clear) {
     const int e2 = gemm::read_error(clear != 0);
     const int e3 = grouped::read_error(clear != 0);
     const int e4 = w4::read_error(clear != 0);
+    const int e5 = rows::read_error(clear != 0);
+    const int e6 = fp4::read_error(clear != 0);
+    const int e7 = fp4::read_product_error(clear != 0);
     if (e1 < 0) return e1;
     if (e2 < 0) return e2;
     if (e3 < 0) return e3;
     if (e4 < 0) return e4;
-    return e1 ? e1 : e2 ? e2 : e3 ? e3 : e4;
+    if (e5 < 0) return e5;
+    if (e6 < 0) return e6;
+    if (e7 < 0) return e7;
+    return e1 ? e1 : e2 ? e2 : e3 ? e3 : e4 ? e4 : e5 ? e5 : e6 ? e6 : e7;
 }
 
 extern "C" int trb_hbm_run(const trb_hbm_args* args, trb_result* out) {

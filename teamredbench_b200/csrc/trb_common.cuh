@@ -80,6 +80,15 @@ namespace w4 {
 int read_error(bool clear);
 }  // namespace w4
 
+namespace rows {
+int read_error(bool clear);
+}  // namespace rows
+
+namespace fp4 {
+int read_error(bool clear);          // of the quantisation
+int read_product_error(bool clear);  // of the product
+}  // namespace fp4
+
 namespace dgemm {
 // float64 C = A * B on the DMMA tensor path (no tcgen05 kind takes fp64); any m, n, k.
 int launch(int m, int n, int k, const void* a, const void* b, void* c, int b_kmajor, cudaStream_t stream,
@@ -100,6 +109,7 @@ enum : int {
     kErrBulkWait = 5,
     kErrSelfTestWait = 6,  // the bounded-wait self-test's deliberate give-up
     kErrOffsets = 7,       // a grouped product's offsets decrease or leave [0, rows]
+    kErrSlots = 8,         // a slot of a token's row is behind the last row
 };
 
 #if defined(__CUDACC__)

@@ -275,3 +275,225 @@ def gemv_w4(x: Any, q: Any, scales: Any, out: Any, *, zeros: Any | None = None, 
                q.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
                None if offsets is None else offsets.data_ptr(), out.data_ptr(), _stream_handle(x, stream))
     return out
+
+
+_ID_BYTES: Any = None  # {torch.int32: 4, torch.int64: 8}, found on first use
+
+
+def expert_sort(experts: Any, offsets: Any, slots: Any, *, stream: Any | None = None) -> tuple[Any, Any]:
+    """Sorts a router's choices by expert; returns (offsets, slots).
+
+    experts (tokens x choices, int32 or int64, as topk's indices) holds the
+    expert of each choice.  offsets (int32, one more than there are experts)
+    gets what the grouped products take, slots (tokens x choices, int32) the row
+    of each choice among the rows sorted by expert, in the order of the tokens
+    inside an expert.  A choice outside [0, experts) -- another rank's expert,
+    or -1 for a token left out -- gets the slot -1 and no row.  One launch,
+    nothing allocated, the same result at every call."""
+    global _ID_BYTES
+    device = _check_operands(experts, offsets, slots)
+    if _ID_BYTES is None:
+        import torch
+
+        _ID_BYTES = {torch.int32: 4, torch.int64: 8}
+    id_bytes = _ID_BYTES.get(experts.dtype)
+    if experts.dim() != 2 or id_bytes is None:
+        raise ValueError(f"experts must be tokens x choices in int32 or int64, got {tuple(experts.shape)} {experts.dtype}")
+    tokens, choices = experts.shape
+    _check_slots(slots, tokens, choices)
+    groups = offsets.numel() - 1
+    if groups < 1:
+        raise ValueError("offsets must hold one more value than there are experts")
+    _check_offsets(offsets, groups)
+    _launch_on(device, _native.expert_sort_launch, id_bytes, tokens, choices, groups, experts.data_ptr(),
+               offsets.data_ptr(), slots.data_ptr(), _stream_handle(slots, stream))
+    return offsets, slots
+
+
+def _check_slots(slots: Any, tokens: int, choices: int | None = None) -> int:
+    """The number of choices of (tokens x choices) int32 slots."""
+    global _INT32
+    if _INT32 is None:
+        import torch
+
+        _INT32 = torch.int32
+    if slots.dtype is not _INT32 or slots.dim() != 2:
+        raise ValueError(f"slots must be tokens x choices in int32, got {tuple(slots.shape)} {slots.dtype}")
+    if slots.shape[0] != tokens or (choices is not None and slots.shape[1] != choices):
+        want = f"{tokens} x {'choices' if choices is None else choices}"
+        raise ValueError(f"slots must be {want}, got {tuple(slots.shape)}")
+    return slots.shape[1]
+
+
+def _check_rows(tokens_side: Any, rows_side: Any, slots: Any, weights: Any, name: str) -> tuple[int, int, int, int]:
+    """(tokens, choices, rows, width) of the rows of tokens and of their experts."""
+    if tokens_side.dim() != 2 or rows_side.dim() != 2 or tokens_side.shape[1] != rows_side.shape[1]:
+        raise ValueError(f"{name} must be 2-D and equally wide, got {tuple(tokens_side.shape)} and "
+                         f"{tuple(rows_side.shape)}")
+    if tokens_side.dtype is not rows_side.dtype:
+        raise ValueError(f"{name} must share one dtype")
+    tokens, width = tokens_side.shape
+    choices = _check_slots(slots, tokens)
+    if weights is not None and weights.shape != slots.shape:
+        raise ValueError(f"weights must be {tuple(slots.shape)}, got {tuple(weights.shape)}")
+    return tokens, choices, rows_side.shape[0], width
+
+
+def expert_dispatch(x: Any, slots: Any, out: Any, *, weights: Any | None = None, stream: Any | None = None) -> Any:
+    """out[slots[t, j]] = x[t], times weights[t, j] if they are given: the rows of
+    tokens to the rows of their experts.
+
+    x is (tokens x width) and out (rows x width), bf16, f16 or float32; slots are
+    expert_sort's; weights (tokens x choices) are float32 or of x's dtype.  Rows
+    of out that no slot names stay as they are, a negative slot is skipped, and
+    one behind the last row is skipped and sets the device error word to 8
+    (``_native.device_error``), which the host does not wait for here.  The
+    gradient of x is expert_combine on the gradient of out, with the same
+    weights."""
+    device = _check_operands(x, slots, out, weights)
+    tokens, choices, rows, width = _check_rows(x, out, slots, weights, "x and out")
+    dtype = trb_dtype(x)
+    _launch_on(device, _native.expert_dispatch_launch, dtype, dtype if weights is None else trb_dtype(weights), tokens,
+               choices, rows, width, x.data_ptr(), slots.data_ptr(), None if weights is None else weights.data_ptr(),
+               out.data_ptr(), _stream_handle(x, stream))
+    return out
+
+
+def expert_combine(y: Any, slots: Any, out: Any, *, weights: Any | None = None, stream: Any | None = None) -> Any:
+    """out[t] = the sum over j of weights[t, j] * y[slots[t, j]] (of the rows
+    themselves without weights): the rows of experts back to their tokens.
+
+    y is (rows x width) and out (tokens x width); a token without a row gets
+    zeros.  fp32 sums in the order of the choices, rounded once.  Types, slots and
+    errors as in expert_dispatch, whose gradient for x this is; its own
+    gradient is expert_combine_grad."""
+    device = _check_operands(y, slots, out, weights)
+    tokens, choices, rows, width = _check_rows(out, y, slots, weights, "out and y")
+    dtype = trb_dtype(y)
+    _launch_on(device, _native.expert_combine_launch, dtype, dtype if weights is None else trb_dtype(weights), tokens,
+               choices, rows, width, y.data_ptr(), slots.data_ptr(), None if weights is None else weights.data_ptr(),
+               out.data_ptr(), _stream_handle(y, stream))
+    return out
+
+
+def expert_combine_grad(grad: Any, y: Any, slots: Any, weights: Any, grad_y: Any, grad_weights: Any, *,
+                        stream: Any | None = None) -> tuple[Any, Any]:
+    """The gradients of expert_combine's y and weights from grad, that of its
+    result, in one pass; returns (grad_y, grad_weights).
+
+    grad_y[slots[t, j]] = weights[t, j] * grad[t] (rows x width; rows that no
+    slot names stay as they are), grad_weights[t, j] = the sum of grad[t] *
+    y[slots[t, j]] over the width (tokens x choices, 0 for a negative slot), of
+    the weights' dtype, summed in fp32.  Types, slots and errors as in
+    expert_dispatch."""
+    device = _check_operands(grad, y, slots, weights, grad_y, grad_weights)
+    tokens, choices, rows, width = _check_rows(grad, y, slots, weights, "grad and y")
+    if grad_y.shape != y.shape or grad_y.dtype is not y.dtype:
+        raise ValueError(f"grad_y must be {tuple(y.shape)} {y.dtype}, got {tuple(grad_y.shape)} {grad_y.dtype}")
+    if grad_weights.shape != weights.shape or grad_weights.dtype is not weights.dtype:
+        raise ValueError(f"grad_weights must be {tuple(weights.shape)} {weights.dtype}, got "
+                         f"{tuple(grad_weights.shape)} {grad_weights.dtype}")
+    _launch_on(device, _native.expert_combine_grad_launch, trb_dtype(grad), trb_dtype(weights), tokens, choices, rows,
+               width, grad.data_ptr(), y.data_ptr(), slots.data_ptr(), weights.data_ptr(), grad_y.data_ptr(),
+               grad_weights.data_ptr(), _stream_handle(grad, stream))
+    return grad_y, grad_weights
+
+
+def fp4_scale_pitch(k: int) -> int:
+    """Bytes of scales a row of k values of 4-bit floating point has: one for 32
+    values, up to a multiple of 16."""
+    return (k // 32 + 15) // 16 * 16
+
+
+def _check_fp4(q: Any, scales: Any, name: str) -> None:
+    """q (... x k/2) and scales (... x pitch) belong together."""
+    global _UINT8
+    if _UINT8 is None:
+        import torch
+
+        _UINT8 = torch.uint8
+    if q.dtype is not _UINT8 or scales.dtype is not _UINT8:
+        raise ValueError(f"{name} and its scales must be uint8")
+    shape = q.shape
+    if scales.shape[:-1] != shape[:-1] or scales.shape[-1] != (shape[-1] // 16 + 15) // 16 * 16:
+        raise ValueError(f"the scales of {name} must be {(*shape[:-1], fp4_scale_pitch(2 * shape[-1]))}, got "
+                         f"{tuple(scales.shape)}")
+
+
+def quantize_fp4(x: Any, q: Any, scales: Any, *, slots: Any | None = None, stream: Any | None = None) -> tuple[Any, Any]:
+    """Rows of x (rows x k, bf16, f16 or float32) to microscaled 4-bit floating
+    point; returns (q, scales).
+
+    q (rows x k/2, uint8) holds two e2m1 values a byte, the even k in the low
+    four bits; scales (rows x fp4_scale_pitch(k), uint8) one power of two (e8m0)
+    for 32 values, 2^(floor(log2 max|x|) - 2), and zeros behind the last block.
+    Values are rounded to the nearest code, ties to the even one, and stop at 6
+    times the scale; a block with a NaN or an infinity becomes NaN.  k is a
+    multiple of 32.  With slots (expert_sort's) row t of x goes to the rows
+    slots[t, j] of q and scales, quantised once: expert_dispatch in 4 bits, with
+    its rules for slots and other rows.  A matrix of weights (n x k) is
+    quantised the same way, and a stack of them as its rows."""
+    device = _check_operands(x, q, scales, slots)
+    if x.dim() != 2 or q.dim() != 2 or scales.dim() != 2:
+        raise ValueError(f"quantize_fp4 takes a 2-D x, q and scales, got {tuple(x.shape)}, {tuple(q.shape)} and "
+                         f"{tuple(scales.shape)}")
+    rows, k = x.shape
+    _check_fp4(q, scales, "q")
+    if 2 * q.shape[1] != k or (slots is None and q.shape[0] != rows):
+        raise ValueError(f"q must be {(rows if slots is None else 'rows', k // 2)} for k = {k}, got {tuple(q.shape)}")
+    choices = 1 if slots is None else _check_slots(slots, rows)
+    _launch_on(device, _native.quantize_fp4_launch, trb_dtype(x), rows, k, x.data_ptr(), choices,
+               None if slots is None else slots.data_ptr(), q.shape[0], q.data_ptr(), scales.data_ptr(),
+               _stream_handle(x, stream))
+    return q, scales
+
+
+def dequantize_fp4(q: Any, scales: Any, out: Any, *, stream: Any | None = None) -> Any:
+    """out (rows x k, bf16, f16 or float32) = the values of quantize_fp4's q and
+    scales: exact in bf16 and float32."""
+    device = _check_operands(q, scales, out)
+    if q.dim() != 2 or scales.dim() != 2 or out.dim() != 2:
+        raise ValueError(f"dequantize_fp4 takes a 2-D q, scales and out, got {tuple(q.shape)}, {tuple(scales.shape)} and "
+                         f"{tuple(out.shape)}")
+    _check_fp4(q, scales, "q")
+    rows, k = out.shape
+    if q.shape[0] != rows or 2 * q.shape[1] != k:
+        raise ValueError(f"out must be {(q.shape[0], 2 * q.shape[1])}, got {tuple(out.shape)}")
+    _launch_on(device, _native.dequantize_fp4_launch, trb_dtype(out), rows, k, q.data_ptr(), scales.data_ptr(),
+               out.data_ptr(), _stream_handle(out, stream))
+    return out
+
+
+def gemm_fp4(a: Any, a_scales: Any, b: Any, b_scales: Any, out: Any, *, offsets: Any | None = None,
+             stream: Any | None = None) -> Any:
+    """out[r] = b[e] @ a[r] for the rows r of group (expert) e, both operands in
+    microscaled 4-bit floating point as quantize_fp4 makes it.
+
+    a and a_scales hold (rows x k), b and b_scales (groups x n x k); a single
+    matrix may be given without the leading dimension, and needs no offsets;
+    otherwise offsets are those of grouped_gemm.  out is (rows x n), bf16 or f16:
+    fp32 sums, rounded once.  k is a multiple of 32, n is free.  What stands
+    behind the last scale of a row does not matter.  Rows outside every group
+    and wrong offsets as in grouped_gemm."""
+    device = _check_operands(a, a_scales, b, b_scales, out, offsets)
+    if a.dim() != 2 or b.dim() not in (2, 3) or out.dim() != 2:
+        raise ValueError(f"gemm_fp4 takes a 2-D a, a 2-D or 3-D b and a 2-D out, got {tuple(a.shape)}, {tuple(b.shape)} "
+                         f"and {tuple(out.shape)}")
+    _check_fp4(a, a_scales, "a")
+    _check_fp4(b, b_scales, "b")
+    rows, k_bytes = a.shape
+    outputs = b.shape
+    groups = 1 if len(outputs) == 2 else outputs[0]
+    n = outputs[-2]
+    if outputs[-1] != k_bytes:
+        raise ValueError(f"incompatible shapes {tuple(a.shape)} and {tuple(b.shape)}")
+    if out.shape != (rows, n):
+        raise ValueError(f"out must be {(rows, n)}, got {tuple(out.shape)}")
+    if offsets is not None:
+        _check_offsets(offsets, groups)
+    elif groups != 1:
+        raise ValueError(f"{groups} groups need offsets")
+    _launch_on(device, _native.gemm_fp4_launch, trb_dtype(out), groups, rows, n, 2 * k_bytes, a.data_ptr(),
+               a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(), None if offsets is None else offsets.data_ptr(),
+               out.data_ptr(), _stream_handle(a, stream))
+    return out
