@@ -39,12 +39,11 @@ __device__ __forceinline__ void mma_pair_mxf4(uint32_t d_tmem, uint64_t a_desc, 
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(a_scales), "r"(b_scales)
         : "memory");
 }
-// 32 rows of 16 bytes from each CTA's shared memory to four columns of its TMEM, the same in every quarter of the lanes.
-__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// Arrival on a barrier of either CTA after reads or writes of TMEM, which tcgen05.wait and the fence before it have
+// ordered: nothing in memory is handed over, and a release at cluster scope would take a thousand cycles.
+__device__ __forceinline__ void mbar_arrive_tmem(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// The descriptor of such a block: rows of 16 bytes without swizzle, 8 rows 128 bytes apart.
-__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) { return make_sdesc(saddr, 16, 128, 0); }
 
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
@@ -72,37 +71,45 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 
 // ------------------------------------------------------------------ the product
 // A CTA pair computes the transposed tile out^T[256 columns n, R rows r] = b[n, k] * a[r, k]^T, as the 16-bit product
-// grouped by expert does: the pair's 256 TMEM lanes run along n, the instruction's N side along up to kTileRows rows of
-// one group in steps of 32, so that few rows cost few.
+// grouped by expert does: the pair's 256 TMEM lanes run along n, the instruction's N side along up to 256 rows of one
+// group in steps of 32, so that few rows cost few.
 //
-// A stage holds 512 k: two k-blocks of 128 bytes (256 values) of each operand, by TMA, and the 16 scale bytes of each
-// row.  The scales are in memory as rows and go to TMEM as columns: lane l of columns 4j .. 4j + 3 holds the four
-// bytes, 128 k, of rows l, 32 + l, 64 + l and 96 + l.  Three scale warps load them, 128 rows a warp (the CTA's columns n,
-// two of the tile's rows), 16 bytes a row, and write them to shared memory turned; the MMA thread copies them from there
-// (tcgen05.cp) before the stage's products.  Scales in TMEM have two sets of columns for three stages: a set is
-// written anew only after the products that read it.
-constexpr int kEpiWarps = 8;                    // two for each quarter of the TMEM lanes
-constexpr int kScaleWarps = 3;
-constexpr int kProductThreads = 64 + 32 * (kEpiWarps + kScaleWarps);
+// A stage holds 512 k, two k-blocks of 128 bytes of each operand, by TMA; the MMA thread waits once a stage (a wait costs
+// it as much as four products of few rows) and gives its k-blocks back one by one.
+//
+// The scales are in memory as rows and belong into TMEM as columns: lane l of columns 4i .. 4i + 3 holds the four bytes,
+// 128 k, of rows l, 32 + l, 64 + l and 96 + l, and every quarter of the lanes holds a copy.  TMA brings 16 bytes a row
+// (512 k) to shared memory, and four scale warps, one for each quarter, store them to TMEM (tcgen05.st), where four
+// k-blocks have columns.  The tensor cores' own copy (tcgen05.cp) takes 33 ns of their time for every 128 rows x 128 k:
+// with 12 a stage 8192^3 took 399 us where the products alone take 183.  Loads of the scale warps' own held up their
+// signal to the MMA thread, which waits for them: 403 us.
+//
+// What is left of TMEM holds two accumulators of 256 columns that share 96: the epilogue takes the shared columns into
+// registers first, and then the next tile's products may start.
+constexpr int kEpiWarps = 4;                    // one for each quarter of the TMEM lanes
+constexpr int kScaleWarps = 4;
+constexpr int kProductThreads = 96 + 32 * (kEpiWarps + kScaleWarps);
 constexpr int kTileN = 256;                     // columns of a tile (pair)
-constexpr int kTileRows = 192;                  // most rows of a tile: two accumulators and the scales fit TMEM
+constexpr int kTileRows = 256;                  // most rows of a tile
 constexpr int kBK = 256;                        // k of a k-block: 128 bytes
 constexpr int kStageK = 2 * kBK;
 constexpr int kStages = 3;
+constexpr int kSlots = 2 * kStages;             // k-blocks
 constexpr int kWBlock = 128 * 128;              // bytes of one CTA's share of a k-block
 constexpr int kXBlock = kTileRows / 2 * 128;
-constexpr int kWStage = 2 * kWBlock, kXStage = 2 * kXBlock;
-constexpr int kScaleBlock = 512;                // 128 rows x 4 bytes
-constexpr int kScaleSets = 4;                   // of 128 k in a stage
-constexpr int kScaleStage = kScaleWarps * kScaleSets * kScaleBlock;
-constexpr int kScaleCols = kScaleWarps * kScaleSets * 4;
+constexpr int kScaleRows = 128 + kTileRows;     // of b and of a that a CTA's products need
+constexpr int kScaleStage = kScaleRows * 16;    // a stage's scales as rows
+constexpr int kScaleCols = kScaleRows / 32 * 2; // of a k-block in TMEM
+constexpr int kScaleSlots = 4;                  // k-blocks whose scales TMEM holds
 constexpr int kEpiBytes = 32 * 64;              // a 32 x 32 block of 16-bit results
 constexpr int kMaxK = 1 << 26;                  // a tile takes less than the limit of a wait
 constexpr int kTmemCols = 512;
-constexpr int kTmemScales = 2 * kTileRows;
-static_assert(kTmemScales + 2 * kScaleCols <= kTmemCols, "accumulators and scales exceed TMEM");
-static_assert(kXBlock % 1024 == 0, "k-blocks begin at the swizzle's period");
-constexpr size_t kProductSmem = (size_t)kStages * (kWStage + kXStage + kScaleStage) + kEpiWarps * kEpiBytes + 1024;
+constexpr int kTmemScales = kTmemCols - kScaleSlots * kScaleCols;
+constexpr int kSecondAcc = kTmemScales - kTileRows;    // columns kSecondAcc .. kTileRows - 1 are both accumulators'
+constexpr int kSharedBlocks = (kTileRows - kSecondAcc) / 32;
+static_assert(kSecondAcc % 32 == 0 && kSecondAcc >= kTileRows - kSecondAcc, "whole blocks of 32 columns are shared");
+constexpr size_t kProductSmem =
+    (size_t)kSlots * (kWBlock + kXBlock) + 2 * kScaleStage + kEpiWarps * kEpiBytes + 1024;
 
 struct ProductTile {
     int e, row0, rows, n0;
@@ -140,27 +147,30 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int valid) {
     }
     return v;
 }
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 template <int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
-    gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX96,
+    gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX128,
                     const __grid_constant__ CUtensorMap tmX64, const __grid_constant__ CUtensorMap tmX32,
-                    const uint8_t* x_scales, const uint8_t* w_scales, const int* offsets, uint16_t* out, int groups,
+                    const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmXS, const int* offsets, uint16_t* out, int groups,
                     int total_rows, int N, int K) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ int group_words[3 * kMaxGroups + 1];
     __shared__ __align__(8) uint64_t full_bar[kStages];   // leader: both CTAs' TMA bytes land here, and their scale warps
-    __shared__ __align__(8) uint64_t empty_bar[kStages];  // both: MMA finished reading the stage
-    __shared__ __align__(8) uint64_t accf_bar[2];         // both: accumulator ready for the epilogue
-    __shared__ __align__(8) uint64_t acce_bar[2];         // leader: both CTAs' epilogues drained it
+    __shared__ __align__(8) uint64_t empty_bar[kSlots];   // both: the products that read the k-block are done
+    __shared__ __align__(8) uint64_t scalef_bar[2];       // each CTA: a stage's scales have landed as rows
+    __shared__ __align__(8) uint64_t scalee_bar[2];       // each CTA: its scale warps have read them
+    __shared__ __align__(8) uint64_t accf_bar;            // both: accumulator ready for the epilogue
+    __shared__ __align__(8) uint64_t acce_bar;            // leader: both CTAs' epilogues have taken the shared columns
     __shared__ __align__(8) uint64_t drain_bar;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
 
     const uint32_t sW = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sX = sW + kStages * kWStage;
-    const uint32_t sScale = sX + kStages * kXStage;
-    const uint32_t sEpi = sScale + kStages * kScaleStage;
+    const uint32_t sX = sW + kSlots * kWBlock;
+    const uint32_t sScale = sX + kSlots * kXBlock;
+    const uint32_t sEpi = sScale + 2 * kScaleStage;
 
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
@@ -173,21 +183,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
     const GroupTable table = {group_words, group_words + kMaxGroups, group_words + 2 * kMaxGroups};
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(smem_u32(&full_bar[s]), 1 + 2 * kScaleWarps);
-            mbar_init(smem_u32(&empty_bar[s]), 1);
+        for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1 + 2 * kScaleWarps);
+        for (int s = 0; s < kSlots; ++s) mbar_init(smem_u32(&empty_bar[s]), 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(smem_u32(&scalef_bar[s]), 1);
+            mbar_init(smem_u32(&scalee_bar[s]), kScaleWarps);
         }
-        for (int a = 0; a < 2; ++a) {
-            mbar_init(smem_u32(&accf_bar[a]), 1);
-            mbar_init(smem_u32(&acce_bar[a]), 2 * kEpiWarps);  // of both CTAs
-        }
+        mbar_init(smem_u32(&accf_bar), 1);
+        mbar_init(smem_u32(&acce_bar), 2 * kEpiWarps);  // of both CTAs
         mbar_init(smem_u32(&drain_bar), 1);
         abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tmW);
-        tma_prefetch_desc(&tmX96);
+        tma_prefetch_desc(&tmX128);
         tma_prefetch_desc(&tmX64);
         tma_prefetch_desc(&tmX32);
+        tma_prefetch_desc(&tmWS);
+        tma_prefetch_desc(&tmXS);
     }
     if (warp == 0) {
         tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
@@ -216,28 +228,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                 const ProductTile p = product_tile(tile, groups, num_n, table);
                 const int half = ((p.rows + 31) & ~31) >> 1;  // rows this CTA loads
                 const int x_row = p.row0 + (int)rank * half;
-                // One box a k-block, of 96, 64 or 32 rows: a request costs more than the rows nobody uses.
-                const CUtensorMap* tmX = half > 64 ? &tmX96 : half > 32 ? &tmX64 : &tmX32;
-                const uint32_t x_bytes = (half > 64 ? 96 : half > 32 ? 64 : 32) * 128;
+                // One box a k-block, of 128, 64 or 32 rows: a request costs more than the rows nobody uses.
+                const CUtensorMap* tmX = half > 64 ? &tmX128 : half > 32 ? &tmX64 : &tmX32;
+                const uint32_t x_bytes = (half > 64 ? 128 : half > 32 ? 64 : 32) * 128;
                 const int w_col = p.n0 + (int)rank * 128;
-                for (int s = 0; s < num_stages; ++s) {
+                for (int s = 0; ok && s < num_stages; ++s) {
                     const int blocks = s * kStageK + kBK < K ? 2 : 1;
-                    if (!mbar_wait_cluster(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
-                        atomicCAS(&g_fp4_gemm_error, 0, kErrProducerWait);
-                        abort_flag = 1;
-                        ok = false;
-                        break;
-                    }
                     const uint32_t fb_local = smem_u32(&full_bar[stage]);
-                    if (leader) mbar_arrive_expect_tx(fb_local, 2 * blocks * (kWBlock + x_bytes));
                     const uint32_t fb = fb_local & kPeerBitMask;
-                    for (int i = 0; i < blocks; ++i) {
-                        const int byte = (s * 2 + i) * 128;
-                        tma_load_3d_pair(sW + stage * kWStage + i * kWBlock, &tmW, fb, byte, w_col, p.e);
-                        tma_load_2d_pair(sX + stage * kXStage + i * kXBlock, tmX, fb, byte, x_row);
+                    for (int i = 0; i < 2; ++i) {  // a k-block past K is not loaded, but its turn is taken
+                        const uint32_t slot = 2 * stage + i;
+                        if (!mbar_wait(smem_u32(&empty_bar[slot]), phase ^ 1u, &abort_flag)) {
+                            atomicCAS(&g_fp4_gemm_error, 0, kErrProducerWait);
+                            abort_flag = 1;
+                            ok = false;
+                            break;
+                        }
+                        if (i == 0) {
+                            if (leader) mbar_arrive_expect_tx(fb_local, 2 * blocks * (kWBlock + x_bytes));
+                            issued_mask |= 1u << stage;
+                            issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+                        }
+                        if (i < blocks) {
+                            const int byte = (s * 2 + i) * 128;
+                            tma_load_3d_pair(sW + slot * kWBlock, &tmW, fb, byte, w_col, p.e);
+                            tma_load_2d_pair(sX + slot * kXBlock, tmX, fb, byte, x_row);
+                        }
                     }
-                    issued_mask |= 1u << stage;
-                    issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
                     if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
@@ -247,81 +264,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
             if (leader)  // every armed phase completes only once both CTAs' bytes have landed
                 for (int s = 0; s < kStages; ++s)
                     if (issued_mask & (1u << s))
-                        if (!mbar_wait_cluster(smem_u32(&full_bar[s]), (issued_phase >> s) & 1u, nullptr))
+                        if (!mbar_wait(smem_u32(&full_bar[s]), (issued_phase >> s) & 1u, nullptr))
                             atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
             // ---------------- MMA issuer: the leader CTA only
             const uint64_t w_desc0 = make_sdesc(sW, 16, 1024), x_desc0 = make_sdesc(sX, 16, 1024);
-            uint32_t stage = 0, phase = 0;
-            int used = 0;  // stages so far
+            uint32_t stage = 0, phase = 0, scale_slot = 0;
             bool ok = true;
             int t_local = 0;
             for (int tile = pair; ok && tile < num_tiles; tile += num_pairs, ++t_local) {
                 const ProductTile p = product_tile(tile, groups, num_n, table);
-                const int padded = (p.rows + 31) & ~31;
-                const uint32_t idesc = idesc_n(make_idesc(256), padded);
-                const int acc = t_local & 1;
-                if (!mbar_wait_cluster(smem_u32(&acce_bar[acc]), ((uint32_t)(t_local >> 1) & 1u) ^ 1u, &abort_flag)) {
+                const uint32_t idesc = idesc_n(make_idesc(256), (p.rows + 31) & ~31);
+                // The epilogue takes the tiles in order: with the last tile's shared columns, all of the one before.
+                if (t_local > 0 && !mbar_wait(smem_u32(&acce_bar), (uint32_t)(t_local - 1) & 1u, &abort_flag)) {
                     atomicCAS(&g_fp4_gemm_error, 0, kErrMmaWait);
                     abort_flag = 1;
                     break;
                 }
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + (uint32_t)(acc * kTileRows);
-                for (int s = 0; s < num_stages; ++s, ++used) {
-                    // The set of scale columns was read by the products of two stages ago: their commit is the phase of
-                    // that stage's empty barrier that belongs to its use.
-                    const int before = used - 2;
-                    bool here = before < 0 || mbar_wait_cluster(smem_u32(&empty_bar[before % kStages]),
-                                                                (uint32_t)(before / kStages) & 1u, &abort_flag);
-                    here = here && mbar_wait_cluster(smem_u32(&full_bar[stage]), phase, &abort_flag);
-                    if (!here) {
+                const uint32_t d_tmem = tmem_base + (t_local & 1 ? kSecondAcc : 0);
+                for (int s = 0; s < num_stages; ++s) {
+                    if (!mbar_wait(smem_u32(&full_bar[stage]), phase, &abort_flag)) {
                         atomicCAS(&g_fp4_gemm_error, 0, kErrMmaWait);
                         abort_flag = 1;
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t scales = sScale + stage * kScaleStage;
-                    const uint32_t t_scales = tmem_base + (uint32_t)(kTmemScales + (used & 1) * kScaleCols);
-                    // Columns of a set of 128 k: 4 of b's rows, then 4 or 8 of a's.
-                    const int sets = min(kScaleSets, (K - s * kStageK + 127) / 128);
-                    for (int j = 0; j < sets; ++j) {
-                        const uint32_t from = scales + (uint32_t)(j * kScaleBlock), to = t_scales + (uint32_t)(j * 12);
-                        copy_scales_pair(to, scale_desc(from));
-                        copy_scales_pair(to + 4, scale_desc(from + kScaleSets * kScaleBlock));
-                        if (padded > 128) copy_scales_pair(to + 8, scale_desc(from + 2 * kScaleSets * kScaleBlock));
-                    }
-                    const uint64_t w = w_desc0 + (uint64_t)((stage * kWStage) >> 4);
-                    const uint64_t x = x_desc0 + (uint64_t)((stage * kXStage) >> 4);
 #pragma unroll
-                    for (int i = 0; i < kStageK / 64; ++i) {  // 64 k: 32 bytes of a k-block's 128
-                        if (s * kStageK + i * 64 >= K) break;
-                        const uint32_t t = t_scales + (uint32_t)((i >> 1) * 12);
-                        mma_pair_mxf4(d_tmem, w + (uint64_t)(((i >> 2) * kWBlock + (i & 3) * 32) >> 4),
-                                      x + (uint64_t)(((i >> 2) * kXBlock + (i & 3) * 32) >> 4),
-                                      (i & 1) ? idesc | kSecondHalf : idesc, t, t + 4, (s != 0 || i != 0) ? 1u : 0u);
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t slot = 2 * stage + b;
+                        const uint64_t w = w_desc0 + (uint64_t)((slot * kWBlock) >> 4);
+                        const uint64_t x = x_desc0 + (uint64_t)((slot * kXBlock) >> 4);
+                        const uint32_t scales = tmem_base + (uint32_t)(kTmemScales + (scale_slot + b) * kScaleCols);
+#pragma unroll
+                        for (int i = 0; i < kBK / 64; ++i) {  // 64 k: 32 bytes of a k-block's 128, half of a scale word
+                            if (s * kStageK + b * kBK + i * 64 >= K) break;
+                            const uint32_t t = scales + (uint32_t)((i >> 1) * (kScaleCols / 2));
+                            mma_pair_mxf4(d_tmem, w + (uint64_t)((i * 32) >> 4), x + (uint64_t)((i * 32) >> 4),
+                                          (i & 1) ? idesc | kSecondHalf : idesc, t, t + 4,
+                                          (s != 0 || b != 0 || i != 0) ? 1u : 0u);
+                        }
+                        tc_commit_pair_multicast(smem_u32(&empty_bar[slot]), 0x3);
                     }
-                    tc_commit_pair_multicast(smem_u32(&empty_bar[stage]), 0x3);
+                    scale_slot ^= 2;
                     if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
-                if (ok) tc_commit_pair_multicast(smem_u32(&accf_bar[acc]), 0x3);
+                if (ok) tc_commit_pair_multicast(smem_u32(&accf_bar), 0x3);
             }
             tc_commit_pair_multicast(smem_u32(&drain_bar), 0x1);
-            if (!mbar_wait_cluster(smem_u32(&drain_bar), 0, nullptr)) atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
+            if (!mbar_wait(smem_u32(&drain_bar), 0, nullptr)) atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
         }
     } else if (warp < 2 + kEpiWarps) {
-        // ---------------- epilogue (both CTAs): warps 2..9, a TMEM lane quarter (32 columns of out) and every other
-        // block of 32 rows each.  TMEM holds out^T, so 32 x 32 blocks go through shared memory transposed (stmatrix
-        // .trans) and leave as 64-byte runs of a row, 16 bytes a lane.
-        const int q = warp & 3, first_block = (warp - 2) >> 2;
-        const uint32_t acce_leader0 = mapa_shared(smem_u32(&acce_bar[0]), 0);
-        const uint32_t acce_leader1 = mapa_shared(smem_u32(&acce_bar[1]), 0);
+        // ---------------- epilogue (both CTAs): a TMEM lane quarter (32 columns of out) each, in blocks of 32 rows.  TMEM
+        // holds out^T, so the blocks go through shared memory transposed (stmatrix.trans) and leave as 64-byte runs of a
+        // row, 16 bytes a lane.
+        const int q = warp & 3;
+        const uint32_t acce_leader = mapa_shared(smem_u32(&acce_bar), 0);
         const uint32_t buf = sEpi + (uint32_t)((warp - 2) * kEpiBytes);
         // block row j is 64 bytes; its 16-byte piece i stands at i ^ ((j >> 1) & 3), free of bank conflicts both ways
         const uint32_t st_row = buf + (uint32_t)((lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) * 16));
@@ -330,8 +333,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         int t_local = 0;
         for (int tile = pair; tile < num_tiles; tile += num_pairs, ++t_local) {
             const ProductTile p = product_tile(tile, groups, num_n, table);
-            const int acc = t_local & 1;
-            bool ok = mbar_wait_cluster(smem_u32(&accf_bar[acc]), (uint32_t)(t_local >> 1) & 1u, &abort_flag);
+            const bool odd = t_local & 1;
+            bool ok = mbar_wait(smem_u32(&accf_bar), (uint32_t)t_local & 1u, &abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) {
                 if (lane == 0) {
@@ -341,23 +344,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                 break;
             }
             tc_fence_after();
-            const uint32_t t_tile = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kTileRows);
+            const uint32_t t_tile = tmem_base + ((uint32_t)(q * 32) << 16) + (odd ? kSecondAcc : 0);
             const int col = p.n0 + (int)rank * 128 + q * 32 + (lane & 3) * 8;
-            uint16_t* out_lane = out + (size_t)(p.row0 + (lane >> 2)) * N + col;
-#pragma unroll 1
-            for (int c = first_block; c * 32 < p.rows; c += 2) {
-                uint32_t lo[16], hi[16];  // TMEM lanes 0..15 and 16..31 of the quarter, 32 rows of out
+            uint16_t* const out_lane = out + (size_t)(p.row0 + (lane >> 2)) * N + col;
+            const auto take = [&](int c, uint32_t (&r)[16]) {  // 32 rows, rounded
+                uint32_t lo[16], hi[16];  // TMEM lanes 0..15 and 16..31 of the quarter
                 tmem_ld_16x256b_x4(t_tile + (uint32_t)(c * 32), lo);
                 tmem_ld_16x256b_x4(t_tile + (16u << 16) + (uint32_t)(c * 32), hi);
                 tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    r[4 * j] = pack2<DT>(lo[4 * j], lo[4 * j + 1]);
+                    r[4 * j + 1] = pack2<DT>(lo[4 * j + 2], lo[4 * j + 3]);
+                    r[4 * j + 2] = pack2<DT>(hi[4 * j], hi[4 * j + 1]);
+                    r[4 * j + 3] = pack2<DT>(hi[4 * j + 2], hi[4 * j + 3]);
+                }
+            };
+            const auto put = [&](int c, const uint32_t (&r)[16]) {
                 __syncwarp();  // the previous block has been read out of buf
 #pragma unroll
                 for (int j = 0; j < 4; ++j)  // rows 8j .. 8j + 7; columns in octets 0..3
-                    stmatrix_x4_trans(st_row + (uint32_t)(j * 8 * 64), pack2<DT>(lo[4 * j], lo[4 * j + 1]),
-                                      pack2<DT>(lo[4 * j + 2], lo[4 * j + 3]), pack2<DT>(hi[4 * j], hi[4 * j + 1]),
-                                      pack2<DT>(hi[4 * j + 2], hi[4 * j + 3]));
+                    stmatrix_x4_trans(st_row + (uint32_t)(j * 8 * 64), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
                 __syncwarp();
-                if (col >= N) continue;
+                if (col >= N) return;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = c * 32 + i * 8;
@@ -367,69 +376,136 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                     if (whole) {
                         *reinterpret_cast<uint4*>(to) = v;
                     } else {
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                         for (int h = 0; h < 8; ++h)
-                            if (col + h < N) to[h] = (uint16_t)(w[h >> 1] >> (16 * (h & 1)));
+                            if (col + h < N) to[h] = (uint16_t)(word(v, h >> 1) >> (16 * (h & 1)));
                     }
                 }
-            }
+            };
+            // The shared columns: the last ones of the first accumulator, the first ones of the second.
+            const int shared0 = odd ? 0 : kSecondAcc / 32;
+            uint32_t r[kSharedBlocks][16];
+#pragma unroll
+            for (int c = 0; c < kSharedBlocks; ++c)
+                if ((shared0 + c) * 32 < p.rows) take(shared0 + c, r[c]);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc ? acce_leader1 : acce_leader0);
+            if (lane == 0) mbar_arrive_tmem(acce_leader);
+#pragma unroll
+            for (int c = 0; c < kSharedBlocks; ++c)
+                if ((shared0 + c) * 32 < p.rows) put(shared0 + c, r[c]);
+            const int first = odd ? kSharedBlocks : 0, last = odd ? kTileRows / 32 : kSecondAcc / 32;
+#pragma unroll 1
+            for (int c = first; c < last && c * 32 < p.rows; ++c) {
+                take(c, r[0]);
+                put(c, r[0]);
+            }
         }
-    } else {
-        // ---------------- scales (both CTAs): warp 0 of the three those of the CTA's 128 columns n, the others those of
-        // 128 rows of the tile each (both CTAs need all of them).
-        const int part = warp - 2 - kEpiWarps;
-        const int valid_all = K / kBlock, pitch = scale_pitch(K);
+    } else if (warp < 2 + kEpiWarps + kScaleWarps) {
+        // ---------------- scales (both CTAs, each for its 128 columns n and all rows of the tile), to this warp's quarter
+        // of the TMEM lanes
+        const int q = warp & 3;
         const uint32_t full_leader = mapa_shared(smem_u32(&full_bar[0]), 0);
-        uint32_t stage = 0, phase = 0;
+        const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16) + kTmemScales;
+        uint32_t stage = 0, scale_slot = 0, buffer = 0, phase = 0;
+        int before = -kScaleSlots;  // the k-block whose columns are next
+        uint32_t parity = 0;        // of the empty barrier's phase that ends with that k-block
         bool ok = true;
         for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-            const ProductTile p = product_tile(tile, groups, num_n, table);
-            const bool some = part < 2 || p.rows > 128;
-            const uint8_t* row[4];  // of the rows l, 32 + l, 64 + l, 96 + l; past the end the last row's, which nobody reads
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                row[i] = part == 0 ? w_scales + ((int64_t)p.e * N + min(p.n0 + (int)rank * 128 + 32 * i + lane, N - 1)) * pitch
-                                   : x_scales + (int64_t)min(p.row0 + (part - 1) * 128 + 32 * i + lane, total_rows - 1) * pitch;
-            uint4 next[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (some) next[i] = *reinterpret_cast<const uint4*>(row[i]);
+            const bool second = product_tile(tile, groups, num_n, table).rows > 128;
             for (int s = 0; s < num_stages; ++s) {
-                uint4 v[4];
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&scalef_bar[buffer]), phase, &abort_flag));
+                const uint32_t rows = sScale + buffer * kScaleStage + lane * 16;
+                uint4 v[3][4];  // of b, of the tile's first 128 rows of a, of the others
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[i] = first_bytes(next[i], valid_all - 16 * s);
-                    if (some && s + 1 < num_stages) next[i] = reinterpret_cast<const uint4*>(row[i])[s + 1];
+                for (int part = 0; part < 3; ++part)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (part < 2 || second) v[part][j] = ld_shared_v4(rows + (uint32_t)((part * 128 + 32 * j) * 16));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&scalee_bar[buffer]));
+                if (++buffer == 2) {
+                    buffer = 0;
+                    phase ^= 1u;
                 }
-                bool free = mbar_wait_cluster(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag);
-                free = __all_sync(0xffffffffu, free);
-                if (!free) {
+                if ((s + 1) * kStageK > K)  // the last stage
+#pragma unroll
+                    for (int part = 0; part < 3; ++part)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[part][j] = first_bytes(v[part][j], K / kBlock - s * (kStageK / kBlock));
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    if (before >= 0) {
+                        const bool free = mbar_wait(smem_u32(&empty_bar[before]), parity, &abort_flag);
+                        ok = __all_sync(0xffffffffu, free) && ok;
+                    }
+                    if (++before == kSlots) {
+                        before = 0;
+                        parity ^= 1u;
+                    }
+                    tc_fence_after();
+                    // 128 k: 4 columns of b, 8 of a; then the other 128 k
+                    const auto column = [&](int c) { return word(v[c % 12 / 4][c % 4], 2 * b + c / 12); };
+                    uint32_t cols0[16], cols1[8];
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) cols0[c] = column(c);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) cols1[c] = column(16 + c);
+                    if (ok) {
+                        tmem_st_32x32b_x16(t_quarter + (scale_slot + b) * kScaleCols, cols0);
+                        tmem_st_32x32b_x8(t_quarter + (scale_slot + b) * kScaleCols + 16, cols1);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (!ok) {
                     if (lane == 0) {
                         atomicCAS(&g_fp4_gemm_error, 0, kErrProducerWait);
                         abort_flag = 1;
                     }
+                    break;
+                }
+                if (lane == 0) mbar_arrive_tmem(full_leader + (uint32_t)(stage * sizeof(uint64_t)));
+                scale_slot ^= 2;
+                if (++stage == kStages) stage = 0;
+            }
+        }
+    } else if (lane == 0) {
+        // ---------------- TMA producer of the scales (both CTAs, each for itself)
+        uint32_t buffer = 0, phase = 0;
+        int issued = 0;
+        bool ok = true;
+        for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
+            const ProductTile p = product_tile(tile, groups, num_n, table);
+            const uint32_t bytes = (p.rows > 128 ? 3 : 2) * 128 * 16;
+            for (int s = 0; s < num_stages; ++s) {
+                if (!mbar_wait(smem_u32(&scalee_bar[buffer]), phase ^ 1u, &abort_flag)) {
+                    atomicCAS(&g_fp4_gemm_error, 0, kErrProducerWait);
+                    abort_flag = 1;
                     ok = false;
                     break;
                 }
-                const uint32_t to = sScale + stage * kScaleStage + (uint32_t)(part * kScaleSets * kScaleBlock + lane * 16);
-                if (some) {
-                    st_shared_v4(to, v[0].x, v[1].x, v[2].x, v[3].x);
-                    st_shared_v4(to + kScaleBlock, v[0].y, v[1].y, v[2].y, v[3].y);
-                    st_shared_v4(to + 2 * kScaleBlock, v[0].z, v[1].z, v[2].z, v[3].z);
-                    st_shared_v4(to + 3 * kScaleBlock, v[0].w, v[1].w, v[2].w, v[3].w);
-                    fence_proxy_async_smem();
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(full_leader + (uint32_t)(stage * sizeof(uint64_t)));
-                if (++stage == kStages) {
-                    stage = 0;
+                const uint32_t bar = smem_u32(&scalef_bar[buffer]), to = sScale + buffer * kScaleStage;
+                mbar_arrive_expect_tx(bar, bytes);
+                tma_load_3d(to, &tmWS, bar, s * 16, p.n0 + (int)rank * 128, p.e);
+                tma_load_2d(to + 128 * 16, &tmXS, bar, s * 16, p.row0);
+                if (p.rows > 128) tma_load_2d(to + 256 * 16, &tmXS, bar, s * 16, p.row0 + 128);
+                ++issued;
+                if (++buffer == 2) {
+                    buffer = 0;
                     phase ^= 1u;
                 }
             }
+        }
+        for (int i = min(issued, 2); i > 0; --i) {  // no copy in flight when this CTA ends
+            if (buffer == 0) {
+                buffer = 2;
+                phase ^= 1u;
+            }
+            --buffer;
+            if (!mbar_wait(smem_u32(&scalef_bar[buffer]), phase, nullptr))
+                atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
         }
     }
 
@@ -453,13 +529,18 @@ template <int DT>
 static int launch_product(int groups, int rows, int n, int k, const void* a, const void* a_scales, const void* b,
                           const void* b_scales, const int* offsets, void* out, int dev, cudaStream_t stream) {
     static bool attr_set[64] = {};
-    CUtensorMap tmW, tmX96, tmX64, tmX32;
+    CUtensorMap tmW, tmX128, tmX64, tmX32, tmWS, tmXS;
     const uint64_t we[3] = {(uint64_t)k / 2, (uint64_t)n, (uint64_t)groups}, xe[2] = {(uint64_t)k / 2, (uint64_t)rows};
-    const uint32_t wb[3] = {128, 128, 1}, xb96[2] = {128, 96}, xb64[2] = {128, 64}, xb32[2] = {128, 32};
+    const uint32_t wb[3] = {128, 128, 1}, xb128[2] = {128, 128}, xb64[2] = {128, 64}, xb32[2] = {128, 32};
     int rc = gemm::encode_tiled(&tmW, b, 1, 3, we, wb, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX96, a, 1, 2, xe, xb96, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX128, a, 1, 2, xe, xb128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX64, a, 1, 2, xe, xb64, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX32, a, 1, 2, xe, xb32, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint64_t wse[3] = {(uint64_t)scale_pitch(k), (uint64_t)n, (uint64_t)groups};
+    const uint64_t xse[2] = {(uint64_t)scale_pitch(k), (uint64_t)rows};
+    const uint32_t scale_box[3] = {16, 128, 1};
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmWS, b_scales, 1, 3, wse, scale_box, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmXS, a_scales, 1, 2, xse, scale_box, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (rc != TRB_OK) return rc;
     const int64_t num_n = (n + kTileN - 1) / kTileN;
     const int64_t tiles = num_n * ((int64_t)rows / kTileRows + std::min(groups, rows));
@@ -481,8 +562,7 @@ static int launch_product(int groups, int rows, int n, int k, const void* a, con
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp4_kernel<DT>, tmW, tmX96, tmX64, tmX32,
-                                static_cast<const uint8_t*>(a_scales), static_cast<const uint8_t*>(b_scales), offsets,
+    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp4_kernel<DT>, tmW, tmX128, tmX64, tmX32, tmWS, tmXS, offsets,
                                 static_cast<uint16_t*>(out), groups, rows, n, k));
     return TRB_OK;
 }
