@@ -45,6 +45,13 @@ __device__ __forceinline__ void mbar_arrive_tmem(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// One lane of a warp that runs together.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
     if constexpr (DT == TRB_FLOAT16) {
@@ -86,7 +93,7 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 //
 // What is left of TMEM holds two accumulators of 256 columns that share 96: the epilogue takes the shared columns into
 // registers first, and then the next tile's products may start.
-constexpr int kEpiWarps = 4;                    // one for each quarter of the TMEM lanes
+constexpr int kEpiWarps = 8;                    // two for each quarter of the TMEM lanes
 constexpr int kScaleWarps = 4;
 constexpr int kProductThreads = 96 + 32 * (kEpiWarps + kScaleWarps);
 constexpr int kTileN = 256;                     // columns of a tile (pair)
@@ -101,7 +108,7 @@ constexpr int kScaleRows = 128 + kTileRows;     // of b and of a that a CTA's pr
 constexpr int kScaleStage = kScaleRows * 16;    // a stage's scales as rows
 constexpr int kScaleCols = kScaleRows / 32 * 2; // of a k-block in TMEM
 constexpr int kScaleSlots = 4;                  // k-blocks whose scales TMEM holds
-constexpr int kEpiBytes = 32 * 64;              // a 32 x 32 block of 16-bit results
+constexpr int kEpiBytes = 16 * 64;              // 16 rows x 32 columns of 16-bit results
 constexpr int kMaxK = 1 << 26;                  // a tile takes less than the limit of a wait
 constexpr int kTmemCols = 512;
 constexpr int kTmemScales = kTmemCols - kScaleSlots * kScaleCols;
@@ -268,8 +275,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                             atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
-            // ---------------- MMA issuer: the leader CTA only
+        if (leader) {
+            // ---------------- MMA issuer: the leader CTA only; the whole warp goes along, so that what the instructions
+            // take is in uniform registers
+            const bool elected = elect_one();
             const uint64_t w_desc0 = make_sdesc(sW, 16, 1024), x_desc0 = make_sdesc(sX, 16, 1024);
             uint32_t stage = 0, phase = 0, scale_slot = 0;
             bool ok = true;
@@ -279,14 +288,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                 const uint32_t idesc = idesc_n(make_idesc(256), (p.rows + 31) & ~31);
                 // The epilogue takes the tiles in order: with the last tile's shared columns, all of the one before.
                 if (t_local > 0 && !mbar_wait(smem_u32(&acce_bar), (uint32_t)(t_local - 1) & 1u, &abort_flag)) {
-                    atomicCAS(&g_fp4_gemm_error, 0, kErrMmaWait);
+                    if (elected) atomicCAS(&g_fp4_gemm_error, 0, kErrMmaWait);
                     abort_flag = 1;
                     break;
                 }
                 const uint32_t d_tmem = tmem_base + (t_local & 1 ? kSecondAcc : 0);
                 for (int s = 0; s < num_stages; ++s) {
                     if (!mbar_wait(smem_u32(&full_bar[stage]), phase, &abort_flag)) {
-                        atomicCAS(&g_fp4_gemm_error, 0, kErrMmaWait);
+                        if (elected) atomicCAS(&g_fp4_gemm_error, 0, kErrMmaWait);
                         abort_flag = 1;
                         ok = false;
                         break;
@@ -302,11 +311,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                         for (int i = 0; i < kBK / 64; ++i) {  // 64 k: 32 bytes of a k-block's 128, half of a scale word
                             if (s * kStageK + b * kBK + i * 64 >= K) break;
                             const uint32_t t = scales + (uint32_t)((i >> 1) * (kScaleCols / 2));
-                            mma_pair_mxf4(d_tmem, w + (uint64_t)((i * 32) >> 4), x + (uint64_t)((i * 32) >> 4),
+                            if (elected) mma_pair_mxf4(d_tmem, w + (uint64_t)((i * 32) >> 4), x + (uint64_t)((i * 32) >> 4),
                                           (i & 1) ? idesc | kSecondHalf : idesc, t, t + 4,
                                           (s != 0 || b != 0 || i != 0) ? 1u : 0u);
                         }
-                        tc_commit_pair_multicast(smem_u32(&empty_bar[slot]), 0x3);
+                        if (elected) tc_commit_pair_multicast(smem_u32(&empty_bar[slot]), 0x3);
                     }
                     scale_slot ^= 2;
                     if (++stage == kStages) {
@@ -314,16 +323,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                         phase ^= 1u;
                     }
                 }
-                if (ok) tc_commit_pair_multicast(smem_u32(&accf_bar), 0x3);
+                if (ok && elected) tc_commit_pair_multicast(smem_u32(&accf_bar), 0x3);
             }
-            tc_commit_pair_multicast(smem_u32(&drain_bar), 0x1);
+            if (elected) tc_commit_pair_multicast(smem_u32(&drain_bar), 0x1);
             if (!mbar_wait(smem_u32(&drain_bar), 0, nullptr)) atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
         }
     } else if (warp < 2 + kEpiWarps) {
-        // ---------------- epilogue (both CTAs): a TMEM lane quarter (32 columns of out) each, in blocks of 32 rows.  TMEM
-        // holds out^T, so the blocks go through shared memory transposed (stmatrix.trans) and leave as 64-byte runs of a
-        // row, 16 bytes a lane.
-        const int q = warp & 3;
+        // ---------------- epilogue (both CTAs): a TMEM lane quarter (32 columns of out) and every other block of 32 rows
+        // each.  TMEM holds out^T, so the blocks go through shared memory transposed (stmatrix.trans), 16 rows at a time,
+        // and leave as 64-byte runs of a row, 16 bytes a lane.
+        const int q = warp & 3, own = (warp - 2) >> 2;
         const uint32_t acce_leader = mapa_shared(smem_u32(&acce_bar), 0);
         const uint32_t buf = sEpi + (uint32_t)((warp - 2) * kEpiBytes);
         // block row j is 64 bytes; its 16-byte piece i stands at i ^ ((j >> 1) & 3), free of bank conflicts both ways
@@ -361,42 +370,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                 }
             };
             const auto put = [&](int c, const uint32_t (&r)[16]) {
-                __syncwarp();  // the previous block has been read out of buf
 #pragma unroll
-                for (int j = 0; j < 4; ++j)  // rows 8j .. 8j + 7; columns in octets 0..3
-                    stmatrix_x4_trans(st_row + (uint32_t)(j * 8 * 64), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-                __syncwarp();
-                if (col >= N) return;
+                for (int half = 0; half < 2; ++half) {
+                    __syncwarp();  // what was in buf has been read
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = c * 32 + i * 8;
-                    if (row + (lane >> 2) >= p.rows) continue;
-                    const uint4 v = ld_shared_v4(ld_row + (uint32_t)(i * 8 * 64));
-                    uint16_t* const to = out_lane + (size_t)row * N;
-                    if (whole) {
-                        *reinterpret_cast<uint4*>(to) = v;
-                    } else {
+                    for (int j = 0; j < 2; ++j) {  // rows 8j .. 8j + 7; columns in octets 0..3
+                        const uint32_t* const v = r + 8 * half + 4 * j;
+                        stmatrix_x4_trans(st_row + (uint32_t)(j * 8 * 64), v[0], v[1], v[2], v[3]);
+                    }
+                    __syncwarp();
+                    if (col >= N) continue;
 #pragma unroll
-                        for (int h = 0; h < 8; ++h)
-                            if (col + h < N) to[h] = (uint16_t)(word(v, h >> 1) >> (16 * (h & 1)));
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = c * 32 + half * 16 + i * 8;
+                        if (row + (lane >> 2) >= p.rows) continue;
+                        const uint4 v = ld_shared_v4(ld_row + (uint32_t)(i * 8 * 64));
+                        uint16_t* const to = out_lane + (size_t)row * N;
+                        if (whole) {
+                            *reinterpret_cast<uint4*>(to) = v;
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < 8; ++h)
+                                if (col + h < N) to[h] = (uint16_t)(word(v, h >> 1) >> (16 * (h & 1)));
+                        }
                     }
                 }
             };
             // The shared columns: the last ones of the first accumulator, the first ones of the second.
             const int shared0 = odd ? 0 : kSecondAcc / 32;
-            uint32_t r[kSharedBlocks][16];
+            uint32_t r[(kSharedBlocks + 1) / 2][16];
 #pragma unroll
-            for (int c = 0; c < kSharedBlocks; ++c)
-                if ((shared0 + c) * 32 < p.rows) take(shared0 + c, r[c]);
+            for (int c = 0; c < kSharedBlocks; c += 2)
+                if (c + own < kSharedBlocks && (shared0 + c + own) * 32 < p.rows) take(shared0 + c + own, r[c / 2]);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_tmem(acce_leader);
 #pragma unroll
-            for (int c = 0; c < kSharedBlocks; ++c)
-                if ((shared0 + c) * 32 < p.rows) put(shared0 + c, r[c]);
+            for (int c = 0; c < kSharedBlocks; c += 2)
+                if (c + own < kSharedBlocks && (shared0 + c + own) * 32 < p.rows) put(shared0 + c + own, r[c / 2]);
+            // The others; the warp that had one block less above begins.
             const int first = odd ? kSharedBlocks : 0, last = odd ? kTileRows / 32 : kSecondAcc / 32;
 #pragma unroll 1
-            for (int c = first; c < last && c * 32 < p.rows; ++c) {
+            for (int c = first + (own ^ 1); c < last && c * 32 < p.rows; c += 2) {
                 take(c, r[0]);
                 put(c, r[0]);
             }
