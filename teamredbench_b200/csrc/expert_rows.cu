@@ -25,11 +25,12 @@ __device__ int g_rows_error;
 // ------------------------------------------------------------------ sort
 // Counting sort in one launch, by one cluster: no workspace, no atomics, and the order inside an expert is that of the
 // choices.  A CTA takes a contiguous part of the choices, a warp a contiguous part of the CTA's, 32 at a time:
-// match.any tells each lane which others chose its expert, so the first of them adds their number to the warp's own
-// count.  The counts are then summed over the warps before, the CTAs before (distributed shared memory) and the experts
-// before, and a second pass over the choices gives each its place.
+// match.any tells each lane which others chose its expert, so each choice's place inside the warp's part is the warp's
+// count of its expert so far and the lanes before, and the first of them adds their number to the count.  The counts are
+// then summed over the warps before, the CTAs before (distributed shared memory) and the experts before, and added.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kBatch = 8;  // groups of 32 choices that a warp loads at once
 
 template <typename Id>
 __device__ __forceinline__ int expert_of(const Id* ids, int i, int end, int experts) {
@@ -41,10 +42,11 @@ __device__ __forceinline__ int expert_of(const Id* ids, int i, int end, int expe
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
     expert_sort_kernel(const Id* ids, int entries, int experts, int* offsets, int* slots) {
-    extern __shared__ int counts[];  // [warps][experts], then the CTA's totals and where each expert's places begin
-    int* const totals = counts + (blockDim.x >> 5) * experts;
-    int* const begin = totals + experts;
+    extern __shared__ int counts[];  // [warps][experts], then the CTA's totals, where its places begin, the cluster's totals
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int* const totals = counts + warps * experts;
+    int* const begin = totals + experts;
+    int* const alls = begin + experts;
     const int ctas = gridDim.x, rank = blockIdx.x;  // the grid is one cluster
     int* const mine = counts + warp * experts;
 
@@ -58,74 +60,94 @@ __global__ void __launch_bounds__(kSortThreads)
     const int64_t part = (int64_t)rank * warps + warp, parts = (int64_t)ctas * warps;
     const int first = (int)(groups * part / parts * 32);
     const int end = (int)min((int64_t)entries, groups * (part + 1) / parts * 32);
+    const bool once = end - first <= 32 * kBatch;  // all of them stay in registers
 
-    int next = expert_of(ids, first + lane, end, experts);
-    for (int i = first; i < end; i += 32) {
-        const int e = next;
-        next = expert_of(ids, i + 32 + lane, end, experts);
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-        __syncwarp();
+    int e[kBatch], place[kBatch];
+    for (int i = first; i < end; i += 32 * kBatch) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) e[b] = expert_of(ids, i + 32 * b + lane, end, experts);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (i + 32 * b >= end) break;
+            const uint32_t same = __match_any_sync(0xffffffffu, e[b]);
+            const int before = __popc(same & ((1u << lane) - 1u));
+            place[b] = e[b] >= 0 ? mine[e[b]] + before : -1;
+            __syncwarp();
+            if (e[b] >= 0 && before == 0) mine[e[b]] = place[b] + __popc(same);
+            __syncwarp();
+        }
+        if (!once)
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (i + 32 * b + lane < end) slots[i + 32 * b + lane] = place[b];
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+    for (int x = threadIdx.x; x < experts; x += blockDim.x) {
         int sum = 0;
+#pragma unroll 8
         for (int w = 0; w < warps; ++w) {
-            const int c = counts[w * experts + e];
-            counts[w * experts + e] = sum;
+            const int c = counts[w * experts + x];
+            counts[w * experts + x] = sum;
             sum += c;
         }
-        totals[e] = sum;
+        totals[x] = sum;
     }
-    cluster_sync_all();
-    // begin[e] = this CTA's first place among the expert's; then the experts before are added.
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+    if (ctas > 1) cluster_sync_all();
+    else __syncthreads();
+    for (int x = threadIdx.x; x < experts; x += blockDim.x) {
         int before = 0, all = 0;
-        for (int r = 0; r < ctas; ++r) {
-            int c;
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c) : "r"(mapa_shared(smem_u32(totals + e), r)));
-            if (r < rank) before += c;
-            all += c;
+        if (ctas == 1) {
+            all = totals[x];
+        } else {
+#pragma unroll 4
+            for (int r = 0; r < ctas; ++r) {
+                int c;
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c) : "r"(mapa_shared(smem_u32(totals + x), r)));
+                before += r < rank ? c : 0;
+                all += c;
+            }
         }
-        begin[e] = before;
-        begin[experts + e] = all;
+        begin[x] = before;
+        alls[x] = all;
     }
     __syncthreads();
-    cluster_arrive();  // the other CTAs' totals have been read
+    if (ctas > 1) cluster_arrive();  // the other CTAs' totals have been read
     if (warp == 0) {
         int base = 0;
-        for (int e0 = 0; e0 < experts; e0 += 32) {
-            const int e = e0 + lane;
-            const int all = e < experts ? begin[experts + e] : 0;
+        for (int x0 = 0; x0 < experts; x0 += 32) {
+            const int x = x0 + lane;
+            const int all = x < experts ? alls[x] : 0;
             int sum = all;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, sum, d);
                 if (lane >= d) sum += up;
             }
-            if (e < experts) {
-                begin[e] += base + sum - all;
-                if (rank == 0) offsets[e] = base + sum - all;
+            if (x < experts) {
+                begin[x] += base + sum - all;
+                if (rank == 0) offsets[x] = base + sum - all;
             }
             base += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (lane == 0 && rank == 0) offsets[experts] = base;
     }
     __syncthreads();
-    next = expert_of(ids, first + lane, end, experts);
-    for (int i = first; i < end; i += 32) {
-        const int e = next;
-        next = expert_of(ids, i + 32 + lane, end, experts);
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        const int before = __popc(same & ((1u << lane) - 1u));
-        int place = -1;
-        if (e >= 0) place = begin[e] + mine[e] + before;
-        __syncwarp();
-        if (e >= 0 && before == 0) mine[e] += __popc(same);
-        if (i + lane < end) slots[i + lane] = place;
-        __syncwarp();
+    for (int i = first; i < end; i += 32 * kBatch) {
+        if (!once) {
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int at = i + 32 * b + lane;
+                e[b] = expert_of(ids, at, end, experts);
+                place[b] = at < end ? slots[at] : -1;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int at = i + 32 * b + lane;
+            if (at < end) slots[at] = e[b] >= 0 ? begin[e[b]] + mine[e[b]] + place[b] : -1;
+        }
     }
-    cluster_wait();
+    if (ctas > 1) cluster_wait();
 }
 
 // ------------------------------------------------------------------ rows there and back
@@ -182,8 +204,8 @@ __device__ __forceinline__ RowWalk row_walk(int log2_lanes) {
     return w;
 }
 
-// Each row of x is read once, whatever the number of its choices.
-template <typename T, typename W, int V>
+// Each row of x is read once, whatever the number of its choices.  U packs of it move at the same time.
+template <typename T, typename W, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
     expert_dispatch_kernel(const T* x, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
                            int width, int log2_lanes) {
@@ -192,28 +214,36 @@ __global__ void __launch_bounds__(kRowThreads)
     const RowWalk w = row_walk(log2_lanes);
     const int packs = width / V;
     for (int64_t t = w.token; t < tokens; t += w.token_step) {
-        for (int p = w.pack; p < packs; p += w.pack_step) {
-            const Pack<T, V> v = load<T, V>(x + t * width + (int64_t)p * V);
+        for (int p0 = w.pack; p0 < packs; p0 += U * w.pack_step) {
+            Pack<T, V> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (p0 + u * w.pack_step < packs) v[u] = load<T, V>(x + t * width + (int64_t)(p0 + u * w.pack_step) * V);
             for (int j = 0; j < choices; ++j) {
                 const int row = row_of(slots, t * choices + j, rows);
                 if (row < 0) continue;
-                Pack<T, V> o = v;
-                if (weights != nullptr) {
-                    const float f = to_f32(weights[t * choices + j]);
+                const float f = weights != nullptr ? to_f32(weights[t * choices + j]) : 1.0f;
+                T* const to = out + (int64_t)row * width;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(f * to_f32(v.v[i]));
+                for (int u = 0; u < U; ++u) {
+                    const int p = p0 + u * w.pack_step;
+                    if (p >= packs) break;
+                    Pack<T, V> o = v[u];
+                    if (weights != nullptr)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(f * to_f32(v[u].v[i]));
+                    store<T, V>(to + (int64_t)p * V, o);
                 }
-                store<T, V>(out + (int64_t)row * width + (int64_t)p * V, o);
             }
         }
     }
 }
 
-// Choices whose rows are on their way at the same time.
+// Choices whose rows are on their way at the same time, in the gradient.
 constexpr int kAtOnce = 4;
 
-// Sums in fp32, in the order of the choices, rounded once.
-template <typename T, typename W, int V>
+// Sums in fp32, in the order of the choices, rounded once.  For rows that are not 16-byte aligned: single values.
+template <typename T, typename W, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
     expert_combine_kernel(const T* y, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
                           int width, int log2_lanes) {
@@ -222,32 +252,162 @@ __global__ void __launch_bounds__(kRowThreads)
     const RowWalk w = row_walk(log2_lanes);
     const int packs = width / V;
     for (int64_t t = w.token; t < tokens; t += w.token_step) {
-        for (int p = w.pack; p < packs; p += w.pack_step) {
-            float sum[V];
+        for (int p0 = w.pack; p0 < packs; p0 += U * w.pack_step) {
+            float sum[U][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[u][i] = 0.0f;
             for (int j0 = 0; j0 < choices; j0 += kAtOnce) {
                 int row[kAtOnce];
-                Pack<T, V> v[kAtOnce];
+                float f[kAtOnce];
+                Pack<T, V> v[kAtOnce][U];
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) {
                     row[j] = j0 + j < choices ? row_of(slots, t * choices + j0 + j, rows) : -1;
-                    if (row[j] >= 0) v[j] = load<T, V>(y + (int64_t)row[j] * width + (int64_t)p * V);
+                    f[j] = weights != nullptr && row[j] >= 0 ? to_f32(weights[t * choices + j0 + j]) : 1.0f;
                 }
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) {
                     if (row[j] < 0) continue;
-                    const float f = weights != nullptr ? to_f32(weights[t * choices + j0 + j]) : 1.0f;
+                    const T* const from = y + (int64_t)row[j] * width;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) sum[i] = fmaf(f, to_f32(v[j].v[i]), sum[i]);
+                    for (int u = 0; u < U; ++u)
+                        if (p0 + u * w.pack_step < packs) v[j][u] = load<T, V>(from + (int64_t)(p0 + u * w.pack_step) * V);
+                }
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    if (row[j] < 0) continue;
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) sum[u][i] = fmaf(f[j], to_f32(v[j][u].v[i]), sum[u][i]);
                 }
             }
-            Pack<T, V> o;
 #pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(sum[i]);
-            store<T, V>(out + t * width + (int64_t)p * V, o);
+            for (int u = 0; u < U; ++u) {
+                if (p0 + u * w.pack_step >= packs) break;
+                Pack<T, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(sum[u][i]);
+                store<T, V>(out + t * width + (int64_t)(p0 + u * w.pack_step) * V, o);
+            }
         }
     }
+}
+
+// The same where rows move 16 bytes at a time.  The kernel above keeps too few bytes in flight there, for a slot has to be
+// read before its row can be and registers are few (16384 tokens of 2 rows of 4096 bf16: 119 us).  Here a thread copies
+// its 16 bytes of J rows to shared memory (cp.async) kDeep - 1 steps before it adds them up; nobody else reads them, so
+// there is no barrier.  A lane reads the slot and weight of one of a step's choices a step before the rows are asked for,
+// and shuffles pass them round.  Four CTAs an SM and 96 bytes a thread on their way: 70 us; three CTAs and 112 bytes 78,
+// five and 64 83.  Rows through a ring of bulk copies of 4 KB with a producer warp took 73 us and two waits a row.
+constexpr int kRingCtas = 4;  // of an SM
+template <int J>
+struct Ring {
+    static constexpr int kDeep = J == 2 ? 6 : 3;
+    static constexpr size_t kSmem = (size_t)kDeep * J * kRowThreads * 16;
+};
+
+// A warp's way through its tokens, 32 packs of their rows and J choices at a time.
+struct Step {
+    int64_t token;
+    int pack0, chunk;
+};
+
+template <typename T, typename W, int J>
+__global__ void __launch_bounds__(kRowThreads, kRingCtas)
+    expert_combine_ring_kernel(const T* y, const int* slots, const W* weights, T* out, int64_t tokens, int choices,
+                               int rows, int width, int log2_lanes) {
+    constexpr int V = 16 / sizeof(T), kDeep = Ring<J>::kDeep;
+    extern __shared__ __align__(16) uint8_t ring[];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const RowWalk w = row_walk(log2_lanes);
+    const int packs = width / V, lane = threadIdx.x & 31, chunks = (choices + J - 1) / J;
+    const uint32_t own = smem_u32(ring) + threadIdx.x * 16;
+    const auto at = [&](int deep, int j) { return own + (uint32_t)((deep * J + j) * kRowThreads * 16); };
+    const auto next = [&](Step& s) {
+        if (++s.chunk < chunks) return;
+        s.chunk = 0;
+        s.pack0 += w.pack_step;
+        if (s.pack0 < packs) return;
+        s.pack0 = w.pack - lane;
+        s.token += w.token_step;
+    };
+    struct Choice {
+        int row;
+        float weight;
+    };
+    const auto choice = [&](Step& s) {
+        Choice c = {-1, 1.0f};
+        const int j = s.chunk * J + lane;
+        if (lane < J && j < choices && s.token < tokens) {
+            c.row = row_of(slots, s.token * choices + j, rows);
+            if (weights != nullptr) c.weight = to_f32(weights[s.token * choices + j]);
+        }
+        next(s);
+        return c;
+    };
+    uint32_t present[kDeep];  // which of a step's choices have a row, and (lane j) the weight of choice j
+    float weight[kDeep];
+    const auto ask = [&](int deep, Step& s, const Choice& c) {
+        present[deep] = __ballot_sync(0xffffffffu, c.row >= 0);
+        weight[deep] = c.weight;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int row = __shfl_sync(0xffffffffu, c.row, j);
+            if (row >= 0 && s.pack0 + lane < packs)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(deep, j)),
+                             "l"(y + (int64_t)row * width + (int64_t)(s.pack0 + lane) * V)
+                             : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next(s);
+    };
+    Step now = {w.token, w.pack - lane, 0};
+    if (now.pack0 >= packs) return;  // more lanes than packs
+    Step asked = now, read = now;
+    Choice known = choice(read);
+#pragma unroll
+    for (int i = 0; i < kDeep - 1; ++i) {
+        ask(i, asked, known);
+        known = choice(read);
+    }
+    float sum[V];
+    while (now.token < tokens) {
+#pragma unroll
+        for (int i = 0; i < kDeep; ++i) {
+            if (now.token >= tokens) break;
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDeep - 2) : "memory");
+            if (now.chunk == 0)
+#pragma unroll
+                for (int x = 0; x < V; ++x) sum[x] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float f = __shfl_sync(0xffffffffu, weight[i], j);
+                if (!(present[i] >> j & 1)) continue;
+                Pack<T, V> v;
+                uint4* const raw = reinterpret_cast<uint4*>(&v);
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(raw->x), "=r"(raw->y), "=r"(raw->z), "=r"(raw->w)
+                             : "r"(at(i, j))
+                             : "memory");
+#pragma unroll
+                for (int x = 0; x < V; ++x) sum[x] = fmaf(f, to_f32(v.v[x]), sum[x]);
+            }
+            if (now.chunk == chunks - 1 && now.pack0 + lane < packs) {
+                Pack<T, V> o;
+#pragma unroll
+                for (int x = 0; x < V; ++x) o.v[x] = round_to<T>(sum[x]);
+                store<T, V>(out + now.token * width + (int64_t)(now.pack0 + lane) * V, o);
+            }
+            next(now);
+            ask((i + kDeep - 1) % kDeep, asked, known);
+            known = choice(read);
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // One pass over a token's rows for both gradients.  The products of a weight's gradient are added in fp32: in a
@@ -341,10 +501,11 @@ static int launch_sort(const void* ids, int entries, int experts, int* offsets, 
     if (dev >= 64 || !attr_set[dev]) {
         const int most = (int)sizeof(int) * (kSortWarps + 3) * kMaxGroups;
         TRB_CUDA(cudaFuncSetAttribute(expert_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        TRB_CUDA(cudaFuncSetAttribute(expert_sort_kernel<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         if (dev < 64) attr_set[dev] = true;
     }
     const int64_t groups = ((int64_t)entries + 31) / 32;
-    const int ctas = groups <= 2 * kSortWarps ? 1 : groups <= 8 * kSortWarps ? 4 : 8;
+    const int ctas = groups <= 2 * kSortWarps ? 1 : groups <= 8 * kSortWarps ? 4 : groups <= 16 * kSortWarps ? 8 : 16;
     const int warps = (int)std::min<int64_t>(kSortWarps, std::max<int64_t>(groups, 8));
     const size_t smem = sizeof(int) * (size_t)(warps + 3) * experts;
     return launch(expert_sort_kernel<Id>, dim3((unsigned)ctas), 32 * warps, ctas, smem, stream,
@@ -355,11 +516,14 @@ struct RowShape {
     dim3 grid;
     int log2_lanes;
 };
-// As many lanes a token as its row has packs, between a warp and a CTA; a row is shared among CTAs while the GPU is not full.
-static RowShape row_shape(int64_t tokens, int packs, bool whole_rows, int dev) {
+// As many lanes a token as its row has packs for each to take `at_once` of, between a warp and a CTA, and more while the
+// GPU is not full; then a row is shared among CTAs.
+static RowShape row_shape(int64_t tokens, int packs, int at_once, bool whole_rows, int dev) {
     RowShape s;
     s.log2_lanes = 5;
-    while (s.log2_lanes < 8 && (1 << s.log2_lanes) < packs) ++s.log2_lanes;
+    while (s.log2_lanes < 8 && (1 << s.log2_lanes) < packs &&
+           ((at_once << s.log2_lanes) < packs || tokens << s.log2_lanes < (int64_t)kRowThreads * 4 * device_sm_count(dev)))
+        ++s.log2_lanes;
     const int64_t side = kRowThreads >> s.log2_lanes, blocks = (tokens + side - 1) / side;
     const int64_t full = 8 * (int64_t)device_sm_count(dev);  // CTAs of 256 threads that the GPU holds
     const int64_t share = whole_rows ? 1 : std::max<int64_t>(1, std::min<int64_t>((packs + kRowThreads - 1) / kRowThreads,
@@ -404,13 +568,41 @@ static int check_align(const char* what, int dtype, int weight_dtype, uintptr_t 
     return TRB_OK;
 }
 
+template <typename T, typename W, int J>
+static int launch_ring(const void* y, const int* slots, const void* weights, void* out, int tokens, int choices, int rows,
+                       int width, int dev, cudaStream_t stream) {
+    static bool attr_set[64] = {};
+    if (dev >= 64 || !attr_set[dev]) {
+        TRB_CUDA(cudaFuncSetAttribute(expert_combine_ring_kernel<T, W, J>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)Ring<J>::kSmem));
+        if (dev < 64) attr_set[dev] = true;
+    }
+    RowShape s = row_shape(tokens, width * (int)sizeof(T) / 16, 1, false, dev);
+    // No more CTAs than the GPU holds, each for several tokens.
+    const unsigned places = (unsigned)(device_sm_count(dev) * kRingCtas);
+    s.grid.x = std::max(1u, std::min(s.grid.x, places / s.grid.y));
+    return launch(expert_combine_ring_kernel<T, W, J>, s.grid, kRowThreads, 0, Ring<J>::kSmem, stream,
+                  static_cast<const T*>(y), slots, static_cast<const W*>(weights), static_cast<T*>(out), (int64_t)tokens,
+                  choices, rows, width, s.log2_lanes);
+}
+
 template <typename T, typename W, int V>
 static int launch_move(bool back, const void* src, const int* slots, const void* weights, void* dst, int tokens,
                        int choices, int rows, int width, int dev, cudaStream_t stream) {
-    const RowShape s = row_shape(tokens, width / V, false, dev);
-    return launch(back ? expert_combine_kernel<T, W, V> : expert_dispatch_kernel<T, W, V>, s.grid, kRowThreads, 0, 0,
-                  stream, static_cast<const T*>(src), slots, static_cast<const W*>(weights), static_cast<T*>(dst),
-                  (int64_t)tokens, choices, rows, width, s.log2_lanes);
+    constexpr int kWide = V > 1 ? 1 : 4;  // single values: four times as many packs, each a fraction of 16 bytes
+    const auto run = [&](auto kernel, int at_once) {
+        const RowShape s = row_shape(tokens, width / V, at_once, false, dev);
+        return launch(kernel, s.grid, kRowThreads, 0, 0, stream, static_cast<const T*>(src), slots,
+                      static_cast<const W*>(weights), static_cast<T*>(dst), (int64_t)tokens, choices, rows, width,
+                      s.log2_lanes);
+    };
+    if (!back) return run(expert_dispatch_kernel<T, W, V, kWide>, kWide);
+    if constexpr (V > 1) {
+        return choices <= 2
+                   ? launch_ring<T, W, 2>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
+                   : launch_ring<T, W, 4>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+    }
+    else return run(expert_combine_kernel<T, W, V, kWide>, kWide);
 }
 
 template <typename T>
@@ -455,7 +647,7 @@ static int launch_grad(const void* grad, const void* y, const int* slots, const 
                        void* grad_weights, int tokens, int choices, int rows, int width, int dev, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     const bool wide = width % V == 0 && (bits(grad) | bits(y) | bits(grad_y)) % 16 == 0;
-    const RowShape s = row_shape(tokens, wide ? width / V : width, true, dev);
+    const RowShape s = row_shape(tokens, wide ? width / V : width, 1, true, dev);
     return launch(wide ? expert_combine_grad_kernel<T, W, V> : expert_combine_grad_kernel<T, W, 1>, s.grid, kRowThreads,
                   0, 0, stream, static_cast<const T*>(grad), static_cast<const T*>(y), slots,
                   static_cast<const W*>(weights), static_cast<T*>(grad_y), static_cast<W*>(grad_weights), (int64_t)tokens,
