@@ -27,7 +27,8 @@ INCLUDE = ROOT / "include"
 
 CUDA_SOURCES = ["trb_abi.cu", "hbm_stream.cu", "gemm_tcgen05.cu", "gemm_fp64.cu", "gemm_grouped.cu", "gemv_w4.cu",
                 "expert_rows.cu", "fp4_blocks.cu", "gemm_fp4.cu"]
-HEADERS = [CSRC / "trb_common.cuh", CSRC / "trb_groups.cuh", CSRC / "trb_fp4.cuh", INCLUDE / "trb_b200.h"]
+HEADERS = [CSRC / "trb_common.cuh", CSRC / "trb_groups.cuh", CSRC / "trb_fp4.cuh",
+           CSRC / "trb_launch.cuh", INCLUDE / "trb_b200.h"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
               f"-I{INCLUDE}", "-Xptxas", "-warn-spills"]

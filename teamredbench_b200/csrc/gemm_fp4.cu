@@ -15,6 +15,7 @@
 #include "trb_common.cuh"
 #include "trb_fp4.cuh"
 #include "trb_groups.cuh"
+#include "trb_launch.cuh"
 
 namespace trb {
 namespace fp4 {
@@ -43,6 +44,16 @@ __device__ __forceinline__ void mma_pair_mxf4(uint32_t d_tmem, uint64_t a_desc, 
 // ordered: nothing in memory is handed over, and a release at cluster scope would take a thousand cycles.
 __device__ __forceinline__ void mbar_arrive_tmem(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(a_scales), "r"(b_scales)
+        : "memory");
 }
 
 // One lane of a warp that runs together.
@@ -123,11 +134,11 @@ struct ProductTile {
 };
 
 // Tile t: groups in order; inside a group, runs of 8 chunks walk the columns together (a panel of b is read by the
-// chunks next to each other in time).
-__device__ __forceinline__ ProductTile product_tile(int t, int groups, int num_n, const GroupTable& g) {
-    const int e = group_of_chunk(t / num_n, groups, g);
-    const int local = t - g.chunk0[e] * num_n;
-    const int rows = g.rows[e];
+// chunks next to each other in time).  Without groups (0) there is one of all rows.
+__device__ __forceinline__ ProductTile product_tile(int t, int groups, int total_rows, int num_n, const GroupTable& g) {
+    const int e = groups > 0 ? group_of_chunk(t / num_n, groups, g) : 0;
+    const int local = groups > 0 ? t - g.chunk0[e] * num_n : t;
+    const int rows = groups > 0 ? g.rows[e] : total_rows;
     const int chunks = (rows + kTileRows - 1) / kTileRows;
     const int run = 8 * num_n;
     const int first = local / run * 8;
@@ -137,7 +148,7 @@ __device__ __forceinline__ ProductTile product_tile(int t, int groups, int num_n
     const int per = ((rows + chunks - 1) / chunks + 31) & ~31;
     ProductTile p;
     p.e = e;
-    p.row0 = g.start[e] + chunk * per;
+    p.row0 = (groups > 0 ? g.start[e] : 0) + chunk * per;
     p.rows = min(per, rows - chunk * per);
     p.n0 = in_run / width * kTileN;
     return p;
@@ -220,10 +231,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
     // Only now that this block has its TMEM: the next grid's blocks take theirs before they wait for this grid.
     grid_launch_dependents();
     grid_dependency_wait();  // offsets, operands and out may belong to the previous grid until here
-    groups = load_groups_or_all(offsets, groups, total_rows, table, &g_fp4_gemm_error);
-    if (warp == 0) scan_chunks(groups, kTileRows, table, lane);
-    __syncthreads();
-    const int num_tiles = table.chunk0[groups] * num_n;
+    int num_tiles = (total_rows + kTileRows - 1) / kTileRows * num_n;
+    if (offsets != nullptr) {
+        groups = load_groups(offsets, groups, total_rows, table, &g_fp4_gemm_error);
+        if (warp == 0) scan_chunks(groups, kTileRows, table, lane);
+        __syncthreads();
+        num_tiles = table.chunk0[groups] * num_n;
+    } else {
+        groups = 0;
+    }
 
     if (warp == 0) {
         if (lane == 0) {
@@ -232,7 +248,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
             uint32_t issued_mask = 0, issued_phase = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-                const ProductTile p = product_tile(tile, groups, num_n, table);
+                const ProductTile p = product_tile(tile, groups, total_rows, num_n, table);
                 const int half = ((p.rows + 31) & ~31) >> 1;  // rows this CTA loads
                 const int x_row = p.row0 + (int)rank * half;
                 // One box a k-block, of 128, 64 or 32 rows: a request costs more than the rows nobody uses.
@@ -284,7 +300,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
             bool ok = true;
             int t_local = 0;
             for (int tile = pair; ok && tile < num_tiles; tile += num_pairs, ++t_local) {
-                const ProductTile p = product_tile(tile, groups, num_n, table);
+                const ProductTile p = product_tile(tile, groups, total_rows, num_n, table);
                 const uint32_t idesc = idesc_n(make_idesc(256), (p.rows + 31) & ~31);
                 // The epilogue takes the tiles in order: with the last tile's shared columns, all of the one before.
                 if (t_local > 0 && !mbar_wait(smem_u32(&acce_bar), (uint32_t)(t_local - 1) & 1u, &abort_flag)) {
@@ -301,22 +317,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
                         break;
                     }
                     tc_fence_after();
+                    const int left = K - s * kStageK;
+                    if (elected) {
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint32_t slot = 2 * stage + b;
-                        const uint64_t w = w_desc0 + (uint64_t)((slot * kWBlock) >> 4);
-                        const uint64_t x = x_desc0 + (uint64_t)((slot * kXBlock) >> 4);
-                        const uint32_t scales = tmem_base + (uint32_t)(kTmemScales + (scale_slot + b) * kScaleCols);
+                        for (int b = 0; b < 2; ++b) {
+                            const uint32_t slot = 2 * stage + b;
+                            const uint64_t w = w_desc0 + (uint64_t)((slot * kWBlock) >> 4);
+                            const uint64_t x = x_desc0 + (uint64_t)((slot * kXBlock) >> 4);
+                            const uint32_t scales = tmem_base + (uint32_t)(kTmemScales + (scale_slot + b) * kScaleCols);
 #pragma unroll
-                        for (int i = 0; i < kBK / 64; ++i) {  // 64 k: 32 bytes of a k-block's 128, half of a scale word
-                            if (s * kStageK + b * kBK + i * 64 >= K) break;
-                            const uint32_t t = scales + (uint32_t)((i >> 1) * (kScaleCols / 2));
-                            if (elected) mma_pair_mxf4(d_tmem, w + (uint64_t)((i * 32) >> 4), x + (uint64_t)((i * 32) >> 4),
-                                          (i & 1) ? idesc | kSecondHalf : idesc, t, t + 4,
-                                          (s != 0 || b != 0 || i != 0) ? 1u : 0u);
+                            for (int i = 0; i < kBK / 64; ++i) {  // 64 k: 32 bytes of a k-block's 128, half of a scale word
+                                const uint32_t t = scales + (uint32_t)((i >> 1) * (kScaleCols / 2));
+                                if (b * kBK + i * 64 < left)
+                                    mma_pair_mxf4(d_tmem, w + (uint64_t)((i * 32) >> 4), x + (uint64_t)((i * 32) >> 4),
+                                                  (i & 1) ? idesc | kSecondHalf : idesc, t, t + 4,
+                                                  (s != 0 || b != 0 || i != 0) ? 1u : 0u);
+                            }
+                            tc_commit_pair_multicast(smem_u32(&empty_bar[slot]), 0x3);
                         }
-                        if (elected) tc_commit_pair_multicast(smem_u32(&empty_bar[slot]), 0x3);
                     }
+                    __syncwarp();
                     scale_slot ^= 2;
                     if (++stage == kStages) {
                         stage = 0;
@@ -341,7 +361,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         const bool whole = N % 8 == 0;  // rows of out begin at 16 bytes
         int t_local = 0;
         for (int tile = pair; tile < num_tiles; tile += num_pairs, ++t_local) {
-            const ProductTile p = product_tile(tile, groups, num_n, table);
+            const ProductTile p = product_tile(tile, groups, total_rows, num_n, table);
             const bool odd = t_local & 1;
             bool ok = mbar_wait(smem_u32(&accf_bar), (uint32_t)t_local & 1u, &abort_flag);
             ok = __all_sync(0xffffffffu, ok);
@@ -427,7 +447,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         uint32_t parity = 0;        // of the empty barrier's phase that ends with that k-block
         bool ok = true;
         for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-            const bool second = product_tile(tile, groups, num_n, table).rows > 128;
+            const bool second = product_tile(tile, groups, total_rows, num_n, table).rows > 128;
             for (int s = 0; s < num_stages; ++s) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&scalef_bar[buffer]), phase, &abort_flag));
                 const uint32_t rows = sScale + buffer * kScaleStage + lane * 16;
@@ -492,7 +512,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         int issued = 0;
         bool ok = true;
         for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-            const ProductTile p = product_tile(tile, groups, num_n, table);
+            const ProductTile p = product_tile(tile, groups, total_rows, num_n, table);
             const uint32_t bytes = (p.rows > 128 ? 3 : 2) * 128 * 16;
             for (int s = 0; s < num_stages; ++s) {
                 if (!mbar_wait(smem_u32(&scalee_bar[buffer]), phase ^ 1u, &abort_flag)) {
@@ -535,51 +555,421 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
     }
 }
 
+// ------------------------------------------------------------------ few tiles: K split over a cluster
+// The same transposed product with single CTAs, 128 columns of out x up to R rows, when the tiles of pairs are too few to
+// occupy the GPU: the CL CTAs of a cluster take a tile's K in CL parts, each streaming its own share of the weights.  CTA
+// r owns columns [128 r / CL, ...) of the tile: the others send it their fp32 parts through distributed shared memory,
+// and it adds them in the order of K, so the result does not depend on timing.  One tile a cluster.  Four warps bring the
+// scales to TMEM, a stage ahead of the products, and read the results afterwards.
+constexpr int kSplitThreads = 224;  // producer warp, MMA warp, 4 warps for scales and results, producer of the scales
+constexpr int kSplitN = 128;
+constexpr int kWStage = 2 * kWBlock;
+template <int R>
+struct SplitCfg {
+    static constexpr int kStages = R == 64 ? 3 : 2;
+    static constexpr int kX = 2 * R * 128;                 // a stage's rows of a
+    static constexpr int kScales = (128 + R) * 16;
+    static constexpr int kScaleCols = 16;                  // of a k-block in TMEM: 128 k of b and of a take 4 each
+    static constexpr int kAcc = R < 32 ? 32 : R;
+    static constexpr int kTmem = kAcc + kStages * 2 * kScaleCols <= 128 ? 128 : 256;
+    static constexpr int kReceive = R * kSplitN * 4;
+    static constexpr size_t kSmem = (size_t)kStages * (kWStage + kX + kScales) + kReceive + 1024;
+    static constexpr int kPerSm = R == 64 ? 1 : 2;
+};
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+template <int DT>
+__device__ __forceinline__ uint16_t round16(float v) {
+    if constexpr (DT == TRB_FLOAT16) return __half_as_ushort(__float2half_rn(v));
+    else return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+template <int DT, int R>
+__global__ void __launch_bounds__(kSplitThreads, SplitCfg<R>::kPerSm)
+    gemm_fp4_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                          const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmXS,
+                          const int* offsets, uint16_t* out, int groups, int total_rows, int N, int K, int log2_cl) {
+    using Cfg = SplitCfg<R>;
+    constexpr int kRing = Cfg::kStages;
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int group_words[3 * kMaxGroups + 1];
+    __shared__ __align__(8) uint64_t full_bar[kRing];    // operands have landed, and the four warps stored their scales
+    __shared__ __align__(8) uint64_t scalef_bar[kRing];  // scales have landed as rows
+    __shared__ __align__(8) uint64_t empty_bar[kRing];   // the products that read the stage are done
+    __shared__ __align__(8) uint64_t done_bar;           // all products of the tile
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+
+    const uint32_t sW = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sX = sW + kRing * kWStage;
+    const uint32_t sScale = sX + kRing * Cfg::kX;
+    const uint32_t receive = sScale + kRing * Cfg::kScales;
+
+    const uint32_t rank = cluster_ctarank();
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const int num_n = (N + kSplitN - 1) / kSplitN;
+    const int num_stages = (K + kStageK - 1) / kStageK;
+    const GroupTable table = {group_words, group_words + kMaxGroups, group_words + 2 * kMaxGroups};
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kRing; ++s) {
+            mbar_init(smem_u32(&full_bar[s]), 1 + 4);
+            mbar_init(smem_u32(&scalef_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        mbar_init(smem_u32(&done_bar), 1);
+        abort_flag = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmX);
+        tma_prefetch_desc(&tmWS);
+        tma_prefetch_desc(&tmXS);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_slot), Cfg::kTmem);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_slot;
+    grid_launch_dependents();  // after the allocation, as above
+    grid_dependency_wait();
+    const int tile = blockIdx.x >> log2_cl, chunk = tile / num_n;
+    int e = 0, row0 = chunk * R, rows = min(R, total_rows - row0);
+    bool some = rows > 0;
+    if (offsets != nullptr) {
+        groups = load_groups(offsets, groups, total_rows, table, &g_fp4_gemm_error);
+        if (warp == 0) scan_chunks(groups, R, table, lane);
+        __syncthreads();
+        some = chunk < table.chunk0[groups];
+        if (some) {
+            e = group_of_chunk(chunk, groups, table);
+            const int first = (chunk - table.chunk0[e]) * R;
+            row0 = table.start[e] + first;
+            rows = min(R, table.rows[e] - first);
+        }
+    }
+    if (!some) {  // the whole cluster: the grid covers the most tiles there can be
+        __syncthreads();
+        if (warp == 1) tmem_dealloc(tmem_base, Cfg::kTmem);
+        return;
+    }
+
+    const int cl = 1 << log2_cl;
+    const int padded = (rows + 15) & ~15;
+    const int n0 = (tile - chunk * num_n) * kSplitN;
+    const int s0 = (num_stages * (int)rank) >> log2_cl, s1 = (num_stages * ((int)rank + 1)) >> log2_cl;
+
+    cluster_arrive();  // peers may not write here before this CTA runs; the wait is before the first such write
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer
+            uint32_t stage = 0, phase = 0;
+            int issued = 0;
+            for (int s = s0; s < s1; ++s) {
+                if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
+                    atomicCAS(&g_fp4_gemm_error, 0, kErrProducerWait);
+                    abort_flag = 1;
+                    break;
+                }
+                const int blocks = s * kStageK + kBK < K ? 2 : 1;
+                const uint32_t bar = smem_u32(&full_bar[stage]);
+                const uint32_t w = sW + stage * kWStage, x = sX + stage * Cfg::kX;
+                mbar_arrive_expect_tx(bar, blocks * (kWBlock + Cfg::kX / 2));
+                for (int i = 0; i < blocks; ++i) {
+                    tma_load_3d(w + i * kWBlock, &tmW, bar, (2 * s + i) * 128, n0, e);
+                    tma_load_2d(x + i * (Cfg::kX / 2), &tmX, bar, (2 * s + i) * 128, row0);
+                }
+                ++issued;
+                if (++stage == kRing) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            for (int i = min(issued, kRing); i > 0; --i) {  // no copy in flight when this CTA ends
+                if (stage == 0) {
+                    stage = kRing;
+                    phase ^= 1u;
+                }
+                --stage;
+                if (!mbar_wait(smem_u32(&full_bar[stage]), phase, nullptr))
+                    atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer
+        const bool elected = elect_one();
+        const uint64_t w_desc0 = make_sdesc(sW, 16, 1024), x_desc0 = make_sdesc(sX, 16, 1024);
+        const uint32_t idesc = idesc_n(make_idesc(128), padded);
+        uint32_t stage = 0, phase = 0;
+        for (int s = s0; s < s1; ++s) {
+            if (!mbar_wait(smem_u32(&full_bar[stage]), phase, &abort_flag)) {
+                if (elected) atomicCAS(&g_fp4_gemm_error, 0, kErrMmaWait);
+                abort_flag = 1;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t scales = tmem_base + Cfg::kAcc + stage * 2 * Cfg::kScaleCols;
+            const int left = K - s * kStageK;
+            if (elected) {
+#pragma unroll
+                for (int i = 0; i < kStageK / 64; ++i) {  // 64 k: 32 bytes of a k-block's 128, half of a scale word
+                    const uint32_t t = scales + (uint32_t)((i >> 1) * (Cfg::kScaleCols / 2));
+                    if (i * 64 < left)
+                        mma_mxf4(tmem_base,
+                                 w_desc0 + (uint64_t)((stage * kWStage + (i >> 2) * kWBlock + (i & 3) * 32) >> 4),
+                                 x_desc0 + (uint64_t)((stage * Cfg::kX + (i >> 2) * (Cfg::kX / 2) + (i & 3) * 32) >> 4),
+                                 (i & 1) ? idesc | kSecondHalf : idesc, t, t + 4, (s != s0 || i != 0) ? 1u : 0u);
+                }
+                tc_commit(smem_u32(&empty_bar[stage]));
+            }
+            __syncwarp();
+            if (++stage == kRing) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        if (elected) tc_commit(smem_u32(&done_bar));
+        if (!mbar_wait(smem_u32(&done_bar), 0, nullptr) && elected) atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
+    } else if (warp == 6) {
+        if (lane == 0) {
+            // ---------------- TMA producer of the scales
+            uint32_t stage = 0, phase = 0;
+            int issued = 0;
+            for (int s = s0; s < s1; ++s) {
+                if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, &abort_flag)) {
+                    atomicCAS(&g_fp4_gemm_error, 0, kErrProducerWait);
+                    abort_flag = 1;
+                    break;
+                }
+                const uint32_t bar = smem_u32(&scalef_bar[stage]), scale = sScale + stage * Cfg::kScales;
+                mbar_arrive_expect_tx(bar, Cfg::kScales);
+                tma_load_3d(scale, &tmWS, bar, s * 16, n0, e);
+                tma_load_2d(scale + 128 * 16, &tmXS, bar, s * 16, row0);
+                ++issued;
+                if (++stage == kRing) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            for (int i = min(issued, kRing); i > 0; --i) {
+                if (stage == 0) {
+                    stage = kRing;
+                    phase ^= 1u;
+                }
+                --stage;
+                if (!mbar_wait(smem_u32(&scalef_bar[stage]), phase, nullptr))
+                    atomicCAS(&g_fp4_gemm_error, 0, kErrDrainWait);
+            }
+        }
+    } else {
+        // ---------------- scales, to this warp's quarter of the TMEM lanes.  Rows that have landed mean that the stage's
+        // last products are done: the producer waited for them.
+        const uint32_t t_quarter = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + Cfg::kAcc;
+        uint32_t stage = 0, phase = 0;
+        for (int s = s0; s < s1; ++s) {
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&scalef_bar[stage]), phase, &abort_flag))) {
+                if (lane == 0) {
+                    atomicCAS(&g_fp4_gemm_error, 0, kErrProducerWait);
+                    abort_flag = 1;
+                }
+                break;
+            }
+            tc_fence_after();
+            const uint32_t scale = sScale + stage * Cfg::kScales + lane * 16;
+            const int valid = K / kBlock - s * (kStageK / kBlock);
+            uint4 v[2][4];  // of b, of a
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[0][j] = first_bytes(ld_shared_v4(scale + (uint32_t)(32 * j * 16)), valid);
+                v[1][j] = make_uint4(0, 0, 0, 0);
+                // Past the tile's rows: what meets the products nobody takes.
+                if (32 * j + lane < R) v[1][j] = first_bytes(ld_shared_v4(scale + (uint32_t)((128 + 32 * j) * 16)), valid);
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t cols[16];  // 128 k: 4 columns of b, 4 of a; then the other 128 k
+#pragma unroll
+                for (int c = 0; c < 16; ++c) cols[c] = word(v[c % 8 / 4][c % 4], 2 * b + c / 8);
+                tmem_st_32x32b_x16(t_quarter + (uint32_t)((stage * 2 + b) * Cfg::kScaleCols), cols);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&full_bar[stage]));
+            if (++stage == kRing) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+    }
+    __syncwarp();
+    cluster_wait();  // every CTA of the cluster runs
+    const int log2_own = 7 - log2_cl, own = 1 << log2_own;  // columns this CTA owns
+    const bool results = warp >= 2 && warp < 6;
+    if (results) {
+        // ---------------- lane = column of out, TMEM column = row
+        const int n = (warp & 3) * 32 + lane;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&done_bar), 0, &abort_flag));
+        if (!ok && lane == 0) {
+            atomicCAS(&g_fp4_gemm_error, 0, kErrEpilogueWait);
+            abort_flag = 1;
+        }
+        if (ok) {
+            tc_fence_after();
+            const uint32_t owner = mapa_shared(receive, (uint32_t)(n >> log2_own)) +
+                                   (uint32_t)((((int)rank * R << log2_own) + (n & (own - 1))) * 4);
+            for (int c = 0; c < padded; c += 16) {
+                uint32_t v[16];
+                tmem_ld_32x32b_x16(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (c + i < rows) st_cluster_f32(owner + (uint32_t)(((c + i) << log2_own) * 4), __uint_as_float(v[i]));
+            }
+            tc_fence_before();
+        }
+    }
+    // The parts have arrived, and no CTA leaves while a peer may still write into it.
+    __syncwarp();
+    cluster_sync_all();
+    if (results && ok) {  // four columns of a row a thread
+        const int log2_quads = log2_own - 2;
+        for (int i = threadIdx.x - 64; i < rows << log2_quads; i += 128) {
+            const int r = i >> log2_quads, c = (i & ((1 << log2_quads) - 1)) * 4;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int src = 0; src < 8; ++src) {
+                if (src >= cl) break;
+                const uint4 p = ld_shared_v4(receive + (uint32_t)((((src * R + r) << log2_own) + c) * 4));
+                v[0] += __uint_as_float(p.x);
+                v[1] += __uint_as_float(p.y);
+                v[2] += __uint_as_float(p.z);
+                v[3] += __uint_as_float(p.w);
+            }
+            const int n = n0 + ((int)rank << log2_own) + c;
+            uint16_t* const to = out + (size_t)(row0 + r) * N + n;
+            if (N % 4 == 0) {
+                const uint2 w = {pack2<DT>(__float_as_uint(v[0]), __float_as_uint(v[1])),
+                                 pack2<DT>(__float_as_uint(v[2]), __float_as_uint(v[3]))};
+                if (n < N) *reinterpret_cast<uint2*>(to) = w;
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (n + x < N) to[x] = round16<DT>(v[x]);
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, Cfg::kTmem);
+    }
+}
+
 // ------------------------------------------------------------------ host side
 static int pairs_for(int64_t tiles, int dev) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count(dev) / 2));
 }
 
+// The tensor maps of one call: b's rows and scales by group, a's scales; those of a's rows are the kernels'.
+struct Operands {
+    const void *a, *a_scales, *b, *b_scales;
+    int groups, rows, n, k;
+    int map_w(CUtensorMap* m) const {
+        const uint64_t extent[3] = {(uint64_t)k / 2, (uint64_t)n, (uint64_t)groups};
+        const uint32_t box[3] = {128, 128, 1};
+        return gemm::encode_tiled(m, b, 1, 3, extent, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    int map_w_scales(CUtensorMap* m) const {
+        const uint64_t extent[3] = {(uint64_t)scale_pitch(k), (uint64_t)n, (uint64_t)groups};
+        const uint32_t box[3] = {16, 128, 1};
+        return gemm::encode_tiled(m, b_scales, 1, 3, extent, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+    }
+    int map_x(CUtensorMap* m, uint32_t box_rows) const {
+        const uint64_t extent[2] = {(uint64_t)k / 2, (uint64_t)rows};
+        const uint32_t box[2] = {128, box_rows};
+        return gemm::encode_tiled(m, a, 1, 2, extent, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    int map_x_scales(CUtensorMap* m, uint32_t box_rows) const {
+        const uint64_t extent[2] = {(uint64_t)scale_pitch(k), (uint64_t)rows};
+        const uint32_t box[2] = {16, box_rows};
+        return gemm::encode_tiled(m, a_scales, 1, 2, extent, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+    }
+    // The most tiles of `tile_rows` rows and `tile_n` columns that there can be.
+    int64_t tiles(int tile_rows, int tile_n, bool grouped) const {
+        const int64_t chunks = grouped ? (int64_t)rows / tile_rows + std::min(groups, rows)
+                                       : ((int64_t)rows + tile_rows - 1) / tile_rows;
+        return chunks * ((n + tile_n - 1) / tile_n);
+    }
+};
+
+template <int DT, int R>
+static int launch_split(const Operands& op, const int* offsets, void* out, int log2_cl, int dev, cudaStream_t stream) {
+    static bool attr_set[64] = {};
+    CUtensorMap tmW, tmX, tmWS, tmXS;
+    int rc = op.map_w(&tmW);
+    if (rc == TRB_OK) rc = op.map_x(&tmX, R);
+    if (rc == TRB_OK) rc = op.map_w_scales(&tmWS);
+    if (rc == TRB_OK) rc = op.map_x_scales(&tmXS, R);
+    if (rc != TRB_OK) return rc;
+    return launch_kernel(gemm_fp4_split_kernel<DT, R>, (int)op.tiles(R, kSplitN, offsets != nullptr) << log2_cl, kSplitThreads,
+                         1 << log2_cl, SplitCfg<R>::kSmem, dev, attr_set, stream, tmW, tmX, tmWS, tmXS, offsets,
+                         static_cast<uint16_t*>(out), op.groups, op.rows, op.n, op.k, log2_cl);
+}
+
 template <int DT>
-static int launch_product(int groups, int rows, int n, int k, const void* a, const void* a_scales, const void* b,
-                          const void* b_scales, const int* offsets, void* out, int dev, cudaStream_t stream) {
+static int launch_product(const Operands& op, const int* offsets, void* out, int dev, cudaStream_t stream) {
+    const bool grouped = offsets != nullptr;
+    const int num_stages = (op.k + kStageK - 1) / kStageK;
+    const int64_t num_n = (op.n + kSplitN - 1) / kSplitN, active = std::min(op.groups, op.rows);
+    // Single CTAs with K split over clusters as far as every cluster has a place at once (16 rows, 4096 x 4096: 5.5 us
+    // in clusters of 4, 6.1 of 8, of which 30 have places, and the pairs' 9.0).  Few rows take tiles of 16 of them, two CTAs
+    // an SM, more take tiles of 64 (17 rows as above: 5.9 us, with tiles of 16 6.1; 128 rows: 7.2, the pairs 9.7).  How the
+    // rows are dealt out to the groups is not known here: up to 8 a group on average count as one tile of 16 each, and are
+    // worth it even without places for all (16 groups of 8 rows, 4096 x 2048: 19.6 us, the pairs 22.3; of 16 rows 24.8 and
+    // 20.6); up to 32 count as one tile of 64 (8 groups of 24 rows, 2048 x 2048: 8.6 us, the pairs 9.6; of 48 11.9 and 9.5).
+    const bool few = grouped ? op.rows <= 8 * active : op.rows <= 16;
+    if (few || !grouped || op.rows <= 32 * active) {
+        const int64_t tiles = num_n * (grouped ? active : ((int64_t)op.rows + 63) / 64);
+        const auto fits = [&](int log2_cl) {
+            static int places[4][64] = {};
+            const int at_once = clusters_at_once(gemm_fp4_split_kernel<DT, 64>, kSplitThreads, SplitCfg<64>::kSmem,
+                                                 1 << log2_cl, dev, places[log2_cl]);
+            return tiles <= (few ? SplitCfg<16>::kPerSm : SplitCfg<64>::kPerSm) * at_once;
+        };
+        int log2_cl = -1;
+        while (log2_cl < 3 && 1 << (log2_cl + 1) <= num_stages && fits(log2_cl + 1)) ++log2_cl;
+        if (few && grouped && log2_cl < 0) log2_cl = 0;
+        if (log2_cl >= 0 && op.tiles(few ? 16 : 64, kSplitN, grouped) << log2_cl <= INT32_MAX)
+            return few ? launch_split<DT, 16>(op, offsets, out, log2_cl, dev, stream)
+                       : launch_split<DT, 64>(op, offsets, out, log2_cl, dev, stream);
+    }
     static bool attr_set[64] = {};
     CUtensorMap tmW, tmX128, tmX64, tmX32, tmWS, tmXS;
-    const uint64_t we[3] = {(uint64_t)k / 2, (uint64_t)n, (uint64_t)groups}, xe[2] = {(uint64_t)k / 2, (uint64_t)rows};
-    const uint32_t wb[3] = {128, 128, 1}, xb128[2] = {128, 128}, xb64[2] = {128, 64}, xb32[2] = {128, 32};
-    int rc = gemm::encode_tiled(&tmW, b, 1, 3, we, wb, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX128, a, 1, 2, xe, xb128, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX64, a, 1, 2, xe, xb64, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmX32, a, 1, 2, xe, xb32, CU_TENSOR_MAP_SWIZZLE_128B);
-    const uint64_t wse[3] = {(uint64_t)scale_pitch(k), (uint64_t)n, (uint64_t)groups};
-    const uint64_t xse[2] = {(uint64_t)scale_pitch(k), (uint64_t)rows};
-    const uint32_t scale_box[3] = {16, 128, 1};
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmWS, b_scales, 1, 3, wse, scale_box, CU_TENSOR_MAP_SWIZZLE_NONE);
-    if (rc == TRB_OK) rc = gemm::encode_tiled(&tmXS, a_scales, 1, 2, xse, scale_box, CU_TENSOR_MAP_SWIZZLE_NONE);
+    int rc = op.map_w(&tmW);
+    if (rc == TRB_OK) rc = op.map_x(&tmX128, 128);
+    if (rc == TRB_OK) rc = op.map_x(&tmX64, 64);
+    if (rc == TRB_OK) rc = op.map_x(&tmX32, 32);
+    if (rc == TRB_OK) rc = op.map_w_scales(&tmWS);
+    if (rc == TRB_OK) rc = op.map_x_scales(&tmXS, 128);
     if (rc != TRB_OK) return rc;
-    const int64_t num_n = (n + kTileN - 1) / kTileN;
-    const int64_t tiles = num_n * ((int64_t)rows / kTileRows + std::min(groups, rows));
+    const int64_t tiles = op.tiles(kTileRows, kTileN, grouped);
     if (tiles > INT32_MAX) {
-        set_error("trb_gemm_fp4_launch: too many tiles (rows=%d n=%d groups=%d)", rows, n, groups);
+        set_error("trb_gemm_fp4_launch: too many tiles (rows=%d n=%d groups=%d)", op.rows, op.n, op.groups);
         return TRB_SKIPPED;
     }
-    if (dev >= 64 || !attr_set[dev]) {
-        TRB_CUDA(cudaFuncSetAttribute(gemm_fp4_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kProductSmem));
-        if (dev < 64) attr_set[dev] = true;
-    }
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)(2 * pairs_for(tiles, dev)));
-    cfg.blockDim = dim3(kProductThreads);
-    cfg.dynamicSmemBytes = kProductSmem;
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    TRB_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp4_kernel<DT>, tmW, tmX128, tmX64, tmX32, tmWS, tmXS, offsets,
-                                static_cast<uint16_t*>(out), groups, rows, n, k));
-    return TRB_OK;
+    return launch_kernel(gemm_fp4_kernel<DT>, 2 * pairs_for(tiles, dev), kProductThreads, 0, kProductSmem, dev, attr_set,
+                         stream, tmW, tmX128, tmX64, tmX32, tmWS, tmXS, offsets, static_cast<uint16_t*>(out), op.groups,
+                         op.rows, op.n, op.k);
 }
 
 int read_product_error(bool clear) {
@@ -637,7 +1027,7 @@ extern "C" int trb_gemm_fp4_launch(int dtype, int groups, int rows, int n, int k
     int dev = 0;
     TRB_CUDA(cudaGetDevice(&dev));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return dtype == TRB_BFLOAT16
-               ? fp4::launch_product<TRB_BFLOAT16>(groups, rows, n, k, a, a_scales, b, b_scales, offsets, out, dev, s)
-               : fp4::launch_product<TRB_FLOAT16>(groups, rows, n, k, a, a_scales, b, b_scales, offsets, out, dev, s);
+    const fp4::Operands op = {a, a_scales, b, b_scales, groups, rows, n, k};
+    return dtype == TRB_BFLOAT16 ? fp4::launch_product<TRB_BFLOAT16>(op, offsets, out, dev, s)
+                                 : fp4::launch_product<TRB_FLOAT16>(op, offsets, out, dev, s);
 }

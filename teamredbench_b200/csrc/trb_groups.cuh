@@ -37,18 +37,6 @@ __device__ __forceinline__ int load_groups(const int* offsets, int groups, int t
     return 0;
 }
 
-// The same with one group of all rows where there are no offsets.
-__device__ __forceinline__ int load_groups_or_all(const int* offsets, int groups, int total_rows, const GroupTable& g,
-                                                  int* error) {
-    if (offsets != nullptr) return load_groups(offsets, groups, total_rows, g, error);
-    if (threadIdx.x == 0) {
-        g.start[0] = 0;
-        g.rows[0] = total_rows;
-    }
-    __syncthreads();
-    return 1;
-}
-
 // The check alone.
 __device__ __forceinline__ int check_groups(const int* offsets, int groups, int total_rows, int* error) {
     bool bad = false;

@@ -162,19 +162,45 @@ def test_product(dtype, rows, n, k):
     check(out, *product(values(a, a_scales), values(b, b_scales).unsqueeze(0), [(0, rows)]), k)
 
 
+# More tiles than the GPU has CTA pairs, so that a pair works through several with its two accumulators; K in one part.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows, n, k", [(700, 4100, 288), (1300, 4096, 32), (4100, 4100, 1056), (4095, 4608, 544),
+                                        (20000, 264, 1056)])
+def test_product_of_many_tiles(dtype, rows, n, k):
+    a, a_scales = operand((rows, k), 5)
+    b, b_scales = operand((n, k), 6, 115, 126)
+    out = torch.full((rows, n), NAN, device="cuda", dtype=dtype)
+    gemm_fp4(a, a_scales, b, b_scales, out)
+    check(out, *product(values(a, a_scales), values(b, b_scales).unsqueeze(0), [(0, rows)]), k)
+
+
+# K over clusters of 1, 2, 4 and 8 CTAs (as many as have places at once), tiles of 16 and 64 rows, uneven parts of K.
+@pytest.mark.parametrize("rows", [1, 16, 17, 64, 130])
+@pytest.mark.parametrize("n, k", [(384, 4640), (2056, 4640), (4096, 1568), (9000, 2080), (18944, 544)])
+def test_product_split_over_clusters(rows, n, k):
+    a, a_scales = operand((rows, k), 7)
+    b, b_scales = operand((n, k), 8, 115, 126)
+    out = torch.full((rows, n), NAN, device="cuda", dtype=torch.float16)
+    gemm_fp4(a, a_scales, b, b_scales, out)
+    check(out, *product(values(a, a_scales), values(b, b_scales).unsqueeze(0), [(0, rows)]), k)
+
+
 COUNTS = {
     "one_row": [1],
     "one_row_of_many": [0, 0, 1, 0],
     "edges": [31, 32, 33, 0, 191, 192, 193],
     "chunks": [513, 0, 769, 96, 1],
     "many": [(7 * i * i) % 41 for i in range(97)],
+    "few_each": [(5 * i) % 12 for i in range(40)],
+    "some_each": [(11 * i) % 60 for i in range(9)],
+    "uneven": [0, 300, 1, 0, 2, 0, 0, 1],
     "none": [0, 0, 0],
 }
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("counts", COUNTS)
-@pytest.mark.parametrize("n, k", [(8, 32), (136, 544), (264, 1024), (777, 352)])
+@pytest.mark.parametrize("n, k", [(8, 32), (136, 544), (264, 1024), (777, 352), (1030, 2080)])
 def test_product_grouped(dtype, counts, n, k):
     counts = COUNTS[counts]
     rows = sum(counts)
