@@ -12,6 +12,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_DIR = PKG / "lib"
 LIBRARY_PATH = LIB_DIR / "libtrb_b200.so"
+TORCH_BINDING_PATH = LIB_DIR / "trb_torch.so"
 HBM_EXECUTABLE = LIB_DIR / "trb_hbm"
 MFU_EXECUTABLE = LIB_DIR / "trb_mfu"
 
@@ -204,6 +205,21 @@ def load() -> ctypes.CDLL:
     lib.trb_selftest_bounded_wait.restype = i32
     _lib = lib
     return lib
+
+
+def load_torch_binding():
+    """The extension module trb_torch (csrc/trb_torch.cpp), or None where it is not
+    built or was built for another torch."""
+    import importlib.util
+
+    try:
+        load()  # its library
+        spec = importlib.util.spec_from_file_location("trb_torch", TORCH_BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except (ImportError, NativeLibraryMissing):
+        return None
+    return module
 
 
 def last_error() -> str:

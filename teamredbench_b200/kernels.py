@@ -277,6 +277,19 @@ def gemv_w4(x: Any, q: Any, scales: Any, out: Any, *, zeros: Any | None = None, 
     return out
 
 
+_SHORT: Any = None  # the compiled way from tensors to the library (csrc/trb_torch.cpp), False without it; found on first use
+
+
+def _find_short() -> Any:
+    """The functions of lib/trb_torch.so, each for the front end of its name: it
+    makes the call and returns True where all arguments are as they have to be
+    and the tensors' device is the current one, and does nothing and returns
+    False otherwise.  The checks below are the same ones, with the words."""
+    global _SHORT
+    _SHORT = _native.load_torch_binding() or False
+    return _SHORT
+
+
 _ID_BYTES: Any = None  # {torch.int32: 4, torch.int64: 8}, found on first use
 
 
@@ -290,6 +303,9 @@ def expert_sort(experts: Any, offsets: Any, slots: Any, *, stream: Any | None = 
     inside an expert.  A choice outside [0, experts) -- another rank's expert,
     or -1 for a token left out -- gets the slot -1 and no row.  One launch,
     nothing allocated, the same result at every call."""
+    short = _SHORT if _SHORT is not None else _find_short()
+    if stream is None and short and short.expert_sort(experts, offsets, slots):
+        return offsets, slots
     global _ID_BYTES
     device = _check_operands(experts, offsets, slots)
     if _ID_BYTES is None:
@@ -350,6 +366,9 @@ def expert_dispatch(x: Any, slots: Any, out: Any, *, weights: Any | None = None,
     (``_native.device_error``), which the host does not wait for here.  The
     gradient of x is expert_combine on the gradient of out, with the same
     weights."""
+    short = _SHORT if _SHORT is not None else _find_short()
+    if stream is None and short and short.expert_dispatch(x, slots, out, weights):
+        return out
     device = _check_operands(x, slots, out, weights)
     tokens, choices, rows, width = _check_rows(x, out, slots, weights, "x and out")
     dtype = trb_dtype(x)
@@ -367,6 +386,9 @@ def expert_combine(y: Any, slots: Any, out: Any, *, weights: Any | None = None, 
     zeros.  fp32 sums in the order of the choices, rounded once.  Types, slots and
     errors as in expert_dispatch, whose gradient for x this is; its own
     gradient is expert_combine_grad."""
+    short = _SHORT if _SHORT is not None else _find_short()
+    if stream is None and short and short.expert_combine(y, slots, out, weights):
+        return out
     device = _check_operands(y, slots, out, weights)
     tokens, choices, rows, width = _check_rows(out, y, slots, weights, "out and y")
     dtype = trb_dtype(y)
@@ -386,6 +408,9 @@ def expert_combine_grad(grad: Any, y: Any, slots: Any, weights: Any, grad_y: Any
     y[slots[t, j]] over the width (tokens x choices, 0 for a negative slot), of
     the weights' dtype, summed in fp32.  Types, slots and errors as in
     expert_dispatch."""
+    short = _SHORT if _SHORT is not None else _find_short()
+    if stream is None and short and short.expert_combine_grad(grad, y, slots, weights, grad_y, grad_weights):
+        return grad_y, grad_weights
     device = _check_operands(grad, y, slots, weights, grad_y, grad_weights)
     tokens, choices, rows, width = _check_rows(grad, y, slots, weights, "grad and y")
     if grad_y.shape != y.shape or grad_y.dtype is not y.dtype:
@@ -433,6 +458,9 @@ def quantize_fp4(x: Any, q: Any, scales: Any, *, slots: Any | None = None, strea
     slots[t, j] of q and scales, quantised once: expert_dispatch in 4 bits, with
     its rules for slots and other rows.  A matrix of weights (n x k) is
     quantised the same way, and a stack of them as its rows."""
+    short = _SHORT if _SHORT is not None else _find_short()
+    if stream is None and short and short.quantize_fp4(x, q, scales, slots):
+        return q, scales
     device = _check_operands(x, q, scales, slots)
     if x.dim() != 2 or q.dim() != 2 or scales.dim() != 2:
         raise ValueError(f"quantize_fp4 takes a 2-D x, q and scales, got {tuple(x.shape)}, {tuple(q.shape)} and "
@@ -451,6 +479,9 @@ def quantize_fp4(x: Any, q: Any, scales: Any, *, slots: Any | None = None, strea
 def dequantize_fp4(q: Any, scales: Any, out: Any, *, stream: Any | None = None) -> Any:
     """out (rows x k, bf16, f16 or float32) = the values of quantize_fp4's q and
     scales: exact in bf16 and float32."""
+    short = _SHORT if _SHORT is not None else _find_short()
+    if stream is None and short and short.dequantize_fp4(q, scales, out):
+        return out
     device = _check_operands(q, scales, out)
     if q.dim() != 2 or scales.dim() != 2 or out.dim() != 2:
         raise ValueError(f"dequantize_fp4 takes a 2-D q, scales and out, got {tuple(q.shape)}, {tuple(scales.shape)} and "
@@ -475,6 +506,9 @@ def gemm_fp4(a: Any, a_scales: Any, b: Any, b_scales: Any, out: Any, *, offsets:
     fp32 sums, rounded once.  k is a multiple of 32, n is free.  What stands
     behind the last scale of a row does not matter.  Rows outside every group
     and wrong offsets as in grouped_gemm."""
+    short = _SHORT if _SHORT is not None else _find_short()
+    if stream is None and short and short.gemm_fp4(a, a_scales, b, b_scales, out, offsets):
+        return out
     device = _check_operands(a, a_scales, b, b_scales, out, offsets)
     if a.dim() != 2 or b.dim() not in (2, 3) or out.dim() != 2:
         raise ValueError(f"gemm_fp4 takes a 2-D a, a 2-D or 3-D b and a 2-D out, got {tuple(a.shape)}, {tuple(b.shape)} "
