@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kSortThreads)
 }
 
 // ------------------------------------------------------------------ rows there and back
-// V values of a row that move together: 16 bytes, or one value where the rows are not 16-byte aligned.
+// V values of a row that move together, in one access.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
     T v[V];
@@ -204,7 +204,7 @@ __device__ __forceinline__ RowWalk row_walk(int log2_lanes) {
     return w;
 }
 
-// Each row of x is read once, whatever the number of its choices.  U packs of it move at the same time.
+// Each row of x is read once, whatever the number of its choices.
 template <typename T, typename W, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
     expert_dispatch_kernel(const T* x, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
@@ -214,25 +214,24 @@ __global__ void __launch_bounds__(kRowThreads)
     const RowWalk w = row_walk(log2_lanes);
     const int packs = width / V;
     for (int64_t t = w.token; t < tokens; t += w.token_step) {
-        for (int p0 = w.pack; p0 < packs; p0 += U * w.pack_step) {
+        for (int p = w.pack; p < packs; p += U * w.pack_step) {
             Pack<T, V> v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (p0 + u * w.pack_step < packs) v[u] = load<T, V>(x + t * width + (int64_t)(p0 + u * w.pack_step) * V);
+                if (p + u * w.pack_step < packs) v[u] = load<T, V>(x + t * width + (int64_t)(p + u * w.pack_step) * V);
             for (int j = 0; j < choices; ++j) {
                 const int row = row_of(slots, t * choices + j, rows);
                 if (row < 0) continue;
                 const float f = weights != nullptr ? to_f32(weights[t * choices + j]) : 1.0f;
-                T* const to = out + (int64_t)row * width;
+                T* const to = out + (int64_t)row * width + (int64_t)p * V;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int p = p0 + u * w.pack_step;
-                    if (p >= packs) break;
+                    if (p + u * w.pack_step >= packs) break;
                     Pack<T, V> o = v[u];
                     if (weights != nullptr)
 #pragma unroll
                         for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(f * to_f32(v[u].v[i]));
-                    store<T, V>(to + (int64_t)p * V, o);
+                    store<T, V>(to + (int64_t)u * w.pack_step * V, o);
                 }
             }
         }
@@ -242,7 +241,8 @@ __global__ void __launch_bounds__(kRowThreads)
 // Choices whose rows are on their way at the same time, in the gradient.
 constexpr int kAtOnce = 4;
 
-// Sums in fp32, in the order of the choices, rounded once.  For rows that are not 16-byte aligned: single values.
+// Sums in fp32, in the order of the choices, rounded once.  This is for rows that are not 16-byte aligned: V values, 8
+// bytes or less, an access, U of them of each row on their way.
 template <typename T, typename W, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
     expert_combine_kernel(const T* y, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kRowThreads)
     const RowWalk w = row_walk(log2_lanes);
     const int packs = width / V;
     for (int64_t t = w.token; t < tokens; t += w.token_step) {
-        for (int p0 = w.pack; p0 < packs; p0 += U * w.pack_step) {
+        for (int p = w.pack; p < packs; p += U * w.pack_step) {
             float sum[U][V];
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -270,10 +270,10 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) {
                     if (row[j] < 0) continue;
-                    const T* const from = y + (int64_t)row[j] * width;
+                    const T* const from = y + (int64_t)row[j] * width + (int64_t)p * V;
 #pragma unroll
                     for (int u = 0; u < U; ++u)
-                        if (p0 + u * w.pack_step < packs) v[j][u] = load<T, V>(from + (int64_t)(p0 + u * w.pack_step) * V);
+                        if (p + u * w.pack_step < packs) v[j][u] = load<T, V>(from + (int64_t)u * w.pack_step * V);
                 }
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) {
@@ -286,28 +286,32 @@ __global__ void __launch_bounds__(kRowThreads)
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (p0 + u * w.pack_step >= packs) break;
+                if (p + u * w.pack_step >= packs) break;
                 Pack<T, V> o;
 #pragma unroll
                 for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(sum[u][i]);
-                store<T, V>(out + t * width + (int64_t)(p0 + u * w.pack_step) * V, o);
+                store<T, V>(out + t * width + (int64_t)(p + u * w.pack_step) * V, o);
             }
         }
     }
 }
 
-// The same where rows move 16 bytes at a time.  The kernel above keeps too few bytes in flight there, for a slot has to be
-// read before its row can be and registers are few (16384 tokens of 2 rows of 4096 bf16: 119 us).  Here a thread copies
-// its 16 bytes of J rows to shared memory (cp.async) kDeep - 1 steps before it adds them up; nobody else reads them, so
-// there is no barrier.  A lane reads the slot and weight of one of a step's choices a step before the rows are asked for,
-// and shuffles pass them round.  Four CTAs an SM and 96 bytes a thread on their way: 70 us; three CTAs and 112 bytes 78,
-// five and 64 83.  Rows through a ring of bulk copies of 4 KB with a producer warp took 73 us and two waits a row.
+// The same for rows that are 16-byte aligned.  Loads into registers keep too few bytes in flight, for a slot
+// has to be read before its row can be (16384 tokens of 2 rows of 4096 bf16: 119 us).  Here a thread copies its 16 bytes
+// of J rows to shared memory (cp.async) kDeep - 1 steps before it adds them up; nobody else reads them, so there is no
+// barrier.  A lane reads the slot and weight of one of a step's choices a step before the rows are asked for, and shuffles
+// pass them round.  Four CTAs an SM and 96 bytes a thread on their way: 70 us; three CTAs and 112 bytes 78, five and 64
+// 83.  Rows through a ring of bulk copies of 4 KB with a producer warp took 73 us and two waits a row.
 constexpr int kRingCtas = 4;  // of an SM
 template <int J>
 struct Ring {
     static constexpr int kDeep = J == 2 ? 6 : 3;
     static constexpr size_t kSmem = (size_t)kDeep * J * kRowThreads * 16;
 };
+
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
 
 // A warp's way through its tokens, 32 packs of their rows and J choices at a time.
 struct Step {
@@ -358,9 +362,7 @@ __global__ void __launch_bounds__(kRowThreads, kRingCtas)
         for (int j = 0; j < J; ++j) {
             const int row = __shfl_sync(0xffffffffu, c.row, j);
             if (row >= 0 && s.pack0 + lane < packs)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(deep, j)),
-                             "l"(y + (int64_t)row * width + (int64_t)(s.pack0 + lane) * V)
-                             : "memory");
+                copy_async(at(deep, j), y + (int64_t)row * width + (int64_t)(s.pack0 + lane) * V);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         next(s);
@@ -387,12 +389,7 @@ __global__ void __launch_bounds__(kRowThreads, kRingCtas)
             for (int j = 0; j < J; ++j) {
                 const float f = __shfl_sync(0xffffffffu, weight[i], j);
                 if (!(present[i] >> j & 1)) continue;
-                Pack<T, V> v;
-                uint4* const raw = reinterpret_cast<uint4*>(&v);
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(raw->x), "=r"(raw->y), "=r"(raw->z), "=r"(raw->w)
-                             : "r"(at(i, j))
-                             : "memory");
+                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(ring + ((i * J + j) * kRowThreads + threadIdx.x) * 16);
 #pragma unroll
                 for (int x = 0; x < V; ++x) sum[x] = fmaf(f, to_f32(v.v[x]), sum[x]);
             }
@@ -410,9 +407,29 @@ __global__ void __launch_bounds__(kRowThreads, kRingCtas)
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// One pass over a token's rows for both gradients.  The products of a weight's gradient are added in fp32: in a
-// thread, in its warp, then over the row's warps, always in the same order.
-template <typename T, typename W, int V>
+// The sums of the weights' gradients over a row's lanes: in a thread, in its warp, then over the row's warps, always in
+// the same order.  All threads of the CTA.
+template <typename W>
+__device__ __forceinline__ void store_dots(float (&dot)[kAtOnce], float (&part)[kRowThreads / 32][kAtOnce], W* grad_weights,
+                                           int64_t t, int64_t tokens, int j0, int choices, int log2_lanes) {
+    const int warps = (1 << log2_lanes) / 32, own = threadIdx.x >> log2_lanes, l = threadIdx.x & ((1 << log2_lanes) - 1);
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot[j];
+    }
+    __syncthreads();
+    if (l < kAtOnce && j0 + l < choices && t < tokens) {
+        float sum = 0.0f;
+        for (int w = 0; w < warps; ++w) sum += part[own * warps + w][l];
+        grad_weights[t * choices + j0 + l] = round_to<W>(sum);
+    }
+    __syncthreads();
+}
+
+// One pass over a token's rows for both gradients.
+template <typename T, typename W, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
     expert_combine_grad_kernel(const T* grad, const T* y, const int* slots, const W* weights, T* grad_y, W* grad_weights,
                                int64_t tokens, int choices, int rows, int width, int log2_lanes) {
@@ -435,40 +452,36 @@ __global__ void __launch_bounds__(kRowThreads)
                 if (row[j] >= 0) f[j] = to_f32(weights[t * choices + j0 + j]);
             }
             if (t < tokens) {
-                for (int p = l; p < packs; p += lanes) {
-                    const int64_t at = (int64_t)p * V;
-                    const Pack<T, V> g = load<T, V>(grad + t * width + at);
-                    Pack<T, V> v[kAtOnce];
+                for (int p = l; p < packs; p += U * lanes) {
+                    Pack<T, V> g[U], v[kAtOnce][U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (p + u * lanes < packs) g[u] = load<T, V>(grad + t * width + (int64_t)(p + u * lanes) * V);
 #pragma unroll
                     for (int j = 0; j < kAtOnce; ++j)
-                        if (row[j] >= 0) v[j] = load<T, V>(y + (int64_t)row[j] * width + at);
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (row[j] >= 0 && p + u * lanes < packs)
+                                v[j][u] = load<T, V>(y + (int64_t)row[j] * width + (int64_t)(p + u * lanes) * V);
 #pragma unroll
                     for (int j = 0; j < kAtOnce; ++j) {
                         if (row[j] < 0) continue;
-                        Pack<T, V> o;
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            const float gi = to_f32(g.v[i]);
-                            dot[j] = fmaf(gi, to_f32(v[j].v[i]), dot[j]);
-                            o.v[i] = round_to<T>(f[j] * gi);
+                        for (int u = 0; u < U; ++u) {
+                            if (p + u * lanes >= packs) continue;
+                            Pack<T, V> o;
+#pragma unroll
+                            for (int i = 0; i < V; ++i) {
+                                const float gi = to_f32(g[u].v[i]);
+                                dot[j] = fmaf(gi, to_f32(v[j][u].v[i]), dot[j]);
+                                o.v[i] = round_to<T>(f[j] * gi);
+                            }
+                            store<T, V>(grad_y + (int64_t)row[j] * width + (int64_t)(p + u * lanes) * V, o);
                         }
-                        store<T, V>(grad_y + (int64_t)row[j] * width + at, o);
                     }
                 }
             }
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) {
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
-                if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot[j];
-            }
-            __syncthreads();
-            if (l < kAtOnce && j0 + l < choices && t < tokens) {
-                float sum = 0.0f;
-                for (int w = 0; w < lanes / 32; ++w) sum += part[own * (lanes / 32) + w][l];
-                grad_weights[t * choices + j0 + l] = round_to<W>(sum);
-            }
-            __syncthreads();
+            store_dots<W>(dot, part, grad_weights, t, tokens, j0, choices, log2_lanes);
         }
     }
 }
@@ -516,14 +529,11 @@ struct RowShape {
     dim3 grid;
     int log2_lanes;
 };
-// As many lanes a token as its row has packs for each to take `at_once` of, between a warp and a CTA, and more while the
-// GPU is not full; then a row is shared among CTAs.
+// As many lanes a token as its row has packs, at_once each, between a warp and a CTA; a row is shared among CTAs while the GPU is not full.
 static RowShape row_shape(int64_t tokens, int packs, int at_once, bool whole_rows, int dev) {
     RowShape s;
     s.log2_lanes = 5;
-    while (s.log2_lanes < 8 && (1 << s.log2_lanes) < packs &&
-           ((at_once << s.log2_lanes) < packs || tokens << s.log2_lanes < (int64_t)kRowThreads * 4 * device_sm_count(dev)))
-        ++s.log2_lanes;
+    while (s.log2_lanes < 8 && at_once << s.log2_lanes < packs) ++s.log2_lanes;
     const int64_t side = kRowThreads >> s.log2_lanes, blocks = (tokens + side - 1) / side;
     const int64_t full = 8 * (int64_t)device_sm_count(dev);  // CTAs of 256 threads that the GPU holds
     const int64_t share = whole_rows ? 1 : std::max<int64_t>(1, std::min<int64_t>((packs + kRowThreads - 1) / kRowThreads,
@@ -568,53 +578,65 @@ static int check_align(const char* what, int dtype, int weight_dtype, uintptr_t 
     return TRB_OK;
 }
 
+// The widest access, 16, 8, 4 or 2 bytes, that all rows are made of, aligned.
+static int access_bytes(size_t size, int width, uintptr_t pointers) {
+    const uint64_t all = (uint64_t)width * size | pointers | 16;
+    return (int)std::min<uint64_t>(all & (~all + 1), 16);
+}
+
 template <typename T, typename W, int J>
 static int launch_ring(const void* y, const int* slots, const void* weights, void* out, int tokens, int choices, int rows,
                        int width, int dev, cudaStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    constexpr size_t smem = Ring<J>::kSmem;
     static bool attr_set[64] = {};
     if (dev >= 64 || !attr_set[dev]) {
         TRB_CUDA(cudaFuncSetAttribute(expert_combine_ring_kernel<T, W, J>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)Ring<J>::kSmem));
+                                      (int)smem));
         if (dev < 64) attr_set[dev] = true;
     }
-    RowShape s = row_shape(tokens, width * (int)sizeof(T) / 16, 1, false, dev);
+    RowShape s = row_shape(tokens, width / V, 1, false, dev);
     // No more CTAs than the GPU holds, each for several tokens.
     const unsigned places = (unsigned)(device_sm_count(dev) * kRingCtas);
     s.grid.x = std::max(1u, std::min(s.grid.x, places / s.grid.y));
-    return launch(expert_combine_ring_kernel<T, W, J>, s.grid, kRowThreads, 0, Ring<J>::kSmem, stream,
-                  static_cast<const T*>(y), slots, static_cast<const W*>(weights), static_cast<T*>(out), (int64_t)tokens,
-                  choices, rows, width, s.log2_lanes);
+    return launch(expert_combine_ring_kernel<T, W, J>, s.grid, kRowThreads, 0, smem, stream, static_cast<const T*>(y),
+                  slots, static_cast<const W*>(weights), static_cast<T*>(out), (int64_t)tokens, choices, rows, width,
+                  s.log2_lanes);
 }
 
+// One of the two moves with V values an access.
 template <typename T, typename W, int V>
 static int launch_move(bool back, const void* src, const int* slots, const void* weights, void* dst, int tokens,
                        int choices, int rows, int width, int dev, cudaStream_t stream) {
-    constexpr int kWide = V > 1 ? 1 : 4;  // single values: four times as many packs, each a fraction of 16 bytes
+    constexpr int B = V * sizeof(T);
+    if constexpr (B == 16)
+        if (back)
+            return choices <= 2 ? launch_ring<T, W, 2>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
+                                : launch_ring<T, W, 4>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
     const auto run = [&](auto kernel, int at_once) {
         const RowShape s = row_shape(tokens, width / V, at_once, false, dev);
         return launch(kernel, s.grid, kRowThreads, 0, 0, stream, static_cast<const T*>(src), slots,
                       static_cast<const W*>(weights), static_cast<T*>(dst), (int64_t)tokens, choices, rows, width,
                       s.log2_lanes);
     };
-    if (!back) return run(expert_dispatch_kernel<T, W, V, kWide>, kWide);
-    if constexpr (V > 1) {
-        return choices <= 2
-                   ? launch_ring<T, W, 2>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
-                   : launch_ring<T, W, 4>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
-    }
-    else return run(expert_combine_kernel<T, W, V, kWide>, kWide);
+    // Accesses of a lane on their way: 4109 tokens of 8 rows of 2047 bf16, dispatch with 2, 4 and 8 of them 49, 43 and 43
+    // us, combine 61, 53 and 73.
+    if constexpr (B < 16)
+        if (back) return run(expert_combine_kernel<T, W, V, B == 2 ? 4 : 2>, B == 2 ? 4 : 2);
+    constexpr int U = B == 16 ? 1 : B == 8 ? 2 : 4;
+    return run(expert_dispatch_kernel<T, W, V, U>, U);
 }
 
-template <typename T>
-static int move_rows(bool back, bool weights_f32, const void* src, const int* slots, const void* weights, void* dst,
-                     int tokens, int choices, int rows, int width, int dev, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = width % V == 0 && (bits(src) | bits(dst)) % 16 == 0;
-    if (weights_f32)
-        return wide ? launch_move<T, float, V>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
-                    : launch_move<T, float, 1>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
-    return wide ? launch_move<T, T, V>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
-                : launch_move<T, T, 1>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+template <typename T, typename W>
+static int move_rows(bool back, const void* src, const int* slots, const void* weights, void* dst, int tokens, int choices,
+                     int rows, int width, int dev, cudaStream_t stream) {
+    constexpr int S = sizeof(T);
+    switch (access_bytes(S, width, bits(src) | bits(dst))) {
+        case 16: return launch_move<T, W, 16 / S>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+        case 8: return launch_move<T, W, 8 / S>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+        case 4: return launch_move<T, W, 4 / S>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+        default: return launch_move<T, W, 1>(back, src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+    }
 }
 
 static int move(const char* what, bool back, int dtype, int weight_dtype, int tokens, int choices, int rows, int width,
@@ -635,23 +657,29 @@ static int move(const char* what, bool back, int dtype, int weight_dtype, int to
     TRB_CUDA(cudaGetDevice(&dev));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool f32 = weight_dtype == TRB_FLOAT32;
+    const auto call = [&](auto f) { return f(back, src, slots, weights, dst, tokens, choices, rows, width, dev, s); };
     if (dtype == TRB_BFLOAT16)
-        return move_rows<__nv_bfloat16>(back, f32, src, slots, weights, dst, tokens, choices, rows, width, dev, s);
-    if (dtype == TRB_FLOAT16)
-        return move_rows<__half>(back, f32, src, slots, weights, dst, tokens, choices, rows, width, dev, s);
-    return move_rows<float>(back, true, src, slots, weights, dst, tokens, choices, rows, width, dev, s);
+        return f32 ? call(move_rows<__nv_bfloat16, float>) : call(move_rows<__nv_bfloat16, __nv_bfloat16>);
+    if (dtype == TRB_FLOAT16) return f32 ? call(move_rows<__half, float>) : call(move_rows<__half, __half>);
+    return call(move_rows<float, float>);
 }
 
 template <typename T, typename W>
 static int launch_grad(const void* grad, const void* y, const int* slots, const void* weights, void* grad_y,
                        void* grad_weights, int tokens, int choices, int rows, int width, int dev, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = width % V == 0 && (bits(grad) | bits(y) | bits(grad_y)) % 16 == 0;
-    const RowShape s = row_shape(tokens, wide ? width / V : width, 1, true, dev);
-    return launch(wide ? expert_combine_grad_kernel<T, W, V> : expert_combine_grad_kernel<T, W, 1>, s.grid, kRowThreads,
-                  0, 0, stream, static_cast<const T*>(grad), static_cast<const T*>(y), slots,
-                  static_cast<const W*>(weights), static_cast<T*>(grad_y), static_cast<W*>(grad_weights), (int64_t)tokens,
-                  choices, rows, width, s.log2_lanes);
+    constexpr int S = sizeof(T);
+    const auto run = [&](auto kernel, int values, int at_once) {
+        const RowShape s = row_shape(tokens, width / values, at_once, true, dev);
+        return launch(kernel, s.grid, kRowThreads, 0, 0, stream, static_cast<const T*>(grad), static_cast<const T*>(y),
+                      slots, static_cast<const W*>(weights), static_cast<T*>(grad_y), static_cast<W*>(grad_weights),
+                      (int64_t)tokens, choices, rows, width, s.log2_lanes);
+    };
+    switch (access_bytes(S, width, bits(grad) | bits(y) | bits(grad_y))) {
+        case 16: return run(expert_combine_grad_kernel<T, W, 16 / S, 1>, 16 / S, 1);
+        case 8: return run(expert_combine_grad_kernel<T, W, 8 / S, 2>, 8 / S, 2);
+        case 4: return run(expert_combine_grad_kernel<T, W, 4 / S, 2>, 4 / S, 2);
+        default: return run(expert_combine_grad_kernel<T, W, 1, 2>, 1, 2);
+    }
 }
 
 int read_error(bool clear) {

@@ -104,8 +104,9 @@ def _plan(tokens, choices, experts=6, outside=0.25, seed=3):
     return offsets, slots, (slots >= 0)
 
 
-# widths: one value, no vector, one vector of 16 bytes and one value more, whole rows of vectors, more than a CTA's
-WIDTHS = [1, 7, 8, 9, 1001, 2048, 4104]
+# widths: one value, no vector, one vector of 16 bytes and one value more, rows of 2-, 4-, 8- and 16-byte accesses, more
+# than a CTA takes at once
+WIDTHS = [1, 7, 8, 9, 1001, 1002, 1004, 2048, 4104]
 TOKENS = [(1, 1), (1, 9), (3, 2), (130, 4), (1201, 5)]
 
 
