@@ -1,4 +1,4 @@
-"""Matrix products of an expert (mixture-of-experts) layer, in process through
+"""Matrix products of an expert (mixture-of-experts) layer, and the layer around them, in process through
 libtrb_b200 (no reference counterpart; records, metrics and skipping follow
 src/teamredbench/benchmarks/mfu.py).
 
@@ -9,6 +9,16 @@ expert.
   train      forward, then the gradients of the rows and of the weights
   decode_w4  the forward product with 4-bit weights, a scale and a zero point
              per `group` k
+  layer      the rows are the choices of tokens, `choices` each: sorted by
+             expert, the tokens' rows dispatched, the forward product, and the
+             results combined with the router's weights
+  layer_train  layer, then all its gradients: of the experts' rows and the
+             router's weights, of the dispatched rows and the matrices, and of
+             the tokens' rows
+  layer_fp4  layer in microscaled 4-bit floating point: the tokens are
+             quantised into their experts' rows, against quantised matrices; its
+             MFU is of the hardware profile's float4_e2m1 peak
+The first three are the default.
 
 The calls of a case take several sets of operands in turn, which together move
 three times what the L2 holds, so that the bytes come from the memory whose
@@ -23,11 +33,15 @@ from typing import Any
 from teamredbench_b200 import _native
 from teamredbench_b200.benchmarks.base import Benchmark, BenchmarkRecord
 from teamredbench_b200.device import cuda_device_available
-from teamredbench_b200.kernels import gemv_w4, grouped_gemm, grouped_gemm_wgrad
+from teamredbench_b200.kernels import (expert_combine, expert_combine_grad, expert_dispatch, expert_sort,
+                                        fp4_scale_pitch, gemm_fp4, gemv_w4, grouped_gemm, grouped_gemm_wgrad,
+                                        quantize_fp4)
 from teamredbench_b200.registry import register_benchmark
 from teamredbench_b200.utils import timed_iterations
 
-MODES = ("forward", "train", "decode_w4")
+DEFAULT_MODES = ("forward", "train", "decode_w4")
+LAYER_MODES = ("layer", "layer_train", "layer_fp4")
+MODES = DEFAULT_MODES + LAYER_MODES
 DTYPES = ("bfloat16", "float16")
 
 
@@ -39,6 +53,18 @@ def expert_counts(torch_module: Any, rows: int, experts: int, skew: float, seed:
     if rows == 0:
         return torch.zeros(experts, dtype=torch.int64)
     return torch.bincount(torch.multinomial(share, rows, replacement=True, generator=gen), minlength=experts)
+
+
+def expert_choices(torch_module: Any, counts: Any, choices: int, seed: int):
+    """The experts (tokens x choices, int64) of as many tokens as the rows take, each expert as often as `counts` says,
+    in any order; -1 where the last token has fewer choices."""
+    torch = torch_module
+    rows = int(counts.sum())
+    tokens = -(-rows // choices)
+    ids = torch.full((tokens * choices,), -1, dtype=torch.int64)
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(seed))
+    ids[:rows] = torch.repeat_interleave(torch.arange(counts.numel()), counts)[order]
+    return ids.view(tokens, choices)
 
 
 def operand_sets(moved: int, held: int, l2_bytes: int, free_bytes: int) -> tuple[int, bool]:
@@ -75,6 +101,8 @@ class ExpertsBenchmark(Benchmark):
         def randn(*shape, scale=1.0):
             return (torch.randn(shape, device=dev, generator=gen) * scale).to(dtype)
 
+        if mode in LAYER_MODES:
+            return self._layer(mode, dtype, counts, k, n, randn, held)
         a, out = randn(rows, k), torch.empty((rows, n), device=dev, dtype=dtype)
         if mode == "decode_w4":
             q = torch.randint(0, 256, (experts, n, k // 2), device=dev, dtype=torch.uint8, generator=gen)
@@ -95,6 +123,63 @@ class ExpertsBenchmark(Benchmark):
 
         return (train, 3 * flops, 3 * row_bytes + (2 * active + experts) * weight_bytes,
                 held(a, out, b, grad, grad_a, grad_b))
+
+    def _layer(self, mode: str, dtype: Any, counts: Any, k: int, n: int, randn: Any, held: Any):
+        """_step for the whole layer."""
+        torch, dev = self.torch, self.device
+        rows, experts = int(counts.sum()), counts.numel()
+        active = int((counts > 0).sum())
+        ids = expert_choices(torch, counts, int(self.params.get("choices", 2)), int(self.params.get("seed", 0))).to(dev)
+        tokens = ids.shape[0]
+
+        def empty(*shape, dtype=dtype):
+            return torch.empty(shape, device=dev, dtype=dtype)
+
+        offsets, slots = empty(experts + 1, dtype=torch.int32), empty(*ids.shape, dtype=torch.int32)
+        weights = torch.softmax(randn(*ids.shape).float(), 1)
+        x, y, out = randn(tokens, k), empty(rows, n), empty(tokens, n)
+        plan = held(ids, slots, weights) + held(slots)  # written, then read
+        flops, moved = 2 * rows * k * n, plan + 2 * (tokens * k + tokens * n + 2 * rows * n)
+        if mode == "layer_fp4":
+            block = k // 2 + k // 32  # codes and scales of a row
+            a, a_scales = empty(rows, k // 2, dtype=torch.uint8), empty(rows, fp4_scale_pitch(k), dtype=torch.uint8)
+            b, b_scales = empty(experts, n, k // 2, dtype=torch.uint8), empty(experts, n, fp4_scale_pitch(k),
+                                                                              dtype=torch.uint8)
+            for e in range(experts):
+                quantize_fp4(randn(n, k, scale=k ** -0.5), b[e], b_scales[e])
+
+            def layer_fp4() -> None:
+                expert_sort(ids, offsets, slots)
+                quantize_fp4(x, a, a_scales, slots=slots)
+                gemm_fp4(a, a_scales, b, b_scales, y, offsets=offsets)
+                expert_combine(y, slots, out, weights=weights)
+
+            return layer_fp4, flops, moved + 2 * rows * block + active * n * block, held(x, y, out, a, a_scales, b, b_scales)
+        xs, b = empty(rows, k), randn(experts, k, n, scale=k ** -0.5)
+
+        def layer() -> None:
+            expert_sort(ids, offsets, slots)
+            expert_dispatch(x, slots, xs)
+            grouped_gemm(xs, b, offsets, y)
+            expert_combine(y, slots, out, weights=weights)
+
+        moved += 4 * rows * k + 2 * active * k * n
+        if mode == "layer":
+            return layer, flops, moved, held(x, y, out, xs, b)
+        grad, grad_y, grad_weights = randn(tokens, n), empty(rows, n), torch.empty_like(weights)
+        grad_xs, grad_x, grad_b = empty(rows, k), empty(tokens, k), torch.empty_like(b)
+
+        def layer_train() -> None:
+            layer()
+            expert_combine_grad(grad, y, slots, weights, grad_y, grad_weights)
+            grouped_gemm(grad_y, b, offsets, grad_xs, b_transposed=True)
+            grouped_gemm_wgrad(xs, grad_y, offsets, grad_b)
+            expert_combine(grad_xs, slots, grad_x)
+
+        moved += (held(slots, weights, grad_weights, slots) + 2 * (tokens * n + 4 * rows * n)
+                  + 2 * (3 * rows * k + tokens * k) + 2 * (active + experts) * k * n)
+        return (layer_train, 3 * flops, moved,
+                held(x, y, out, xs, b, grad, grad_y, grad_weights, grad_xs, grad_x, grad_b))
 
     def _measure(self, metadata: dict[str, Any], mode: str, dtype: Any, counts: Any, k: int, n: int,
                  group: int) -> dict[str, Any]:
@@ -123,7 +208,7 @@ class ExpertsBenchmark(Benchmark):
             return [self.emit_record(self.skipped_record(case="global", dtype="n/a",
                                                          error="No CUDA device visible to PyTorch."))]
         self.set_device()
-        modes = list(p.get("modes", MODES))
+        modes = list(p.get("modes", DEFAULT_MODES))
         for mode in modes:
             if mode not in MODES:
                 raise KeyError(f"Unknown experts mode: {mode}")
@@ -140,6 +225,8 @@ class ExpertsBenchmark(Benchmark):
                                                 "most_rows": int(counts.max())}
                     if mode == "decode_w4":
                         metadata["group"] = group
+                    if mode in LAYER_MODES:
+                        metadata["choices"] = int(p.get("choices", 2))
                     if spec.name not in DTYPES:
                         records.append(self.emit_record(self.skipped_record(
                             case=case, dtype=spec.name, error="The expert products take bfloat16 and float16.",
@@ -154,7 +241,8 @@ class ExpertsBenchmark(Benchmark):
                     records.append(self.emit_record(BenchmarkRecord(
                         benchmark=self.name, case=case, dtype=spec.name,
                         raw_metrics={**raw,
-                                     "peak_tops": profile.peak_compute_tops.get(spec.name),
+                                     "peak_tops": profile.peak_compute_tops.get(
+                                         "float4_e2m1" if mode == "layer_fp4" else spec.name),
                                      "peak_bandwidth_gbps": profile.peak_hbm_bandwidth_gbps},
                         metadata=metadata)))
         return records

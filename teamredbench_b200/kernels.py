@@ -440,6 +440,8 @@ def _check_fp4(q: Any, scales: Any, name: str) -> None:
     if q.dtype is not _UINT8 or scales.dtype is not _UINT8:
         raise ValueError(f"{name} and its scales must be uint8")
     shape = q.shape
+    if shape[-1] % 16:
+        raise ValueError(f"k must be a multiple of 32, got {2 * shape[-1]}")
     if scales.shape[:-1] != shape[:-1] or scales.shape[-1] != (shape[-1] // 16 + 15) // 16 * 16:
         raise ValueError(f"the scales of {name} must be {(*shape[:-1], fp4_scale_pitch(2 * shape[-1]))}, got "
                          f"{tuple(scales.shape)}")

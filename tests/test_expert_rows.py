@@ -206,6 +206,7 @@ def test_launches_on_the_tensors_device_and_refuses_another_stream(machine, call
     (lambda: kernels.quantize_fp4(ROWS, Stub(8, 32), SCALES), "uint8"),
     (lambda: kernels.quantize_fp4(ROWS, Q, Stub(8, 2, dtype=U8)), "scales of q must be"),
     (lambda: kernels.quantize_fp4(Stub(8, 64, 1), Q, SCALES), "2-D"),
+    (lambda: kernels.quantize_fp4(Stub(8, 48), Stub(8, 24, dtype=U8), SCALES), "multiple of 32"),
     (lambda: kernels.quantize_fp4(ROWS, Q, SCALES, slots=SLOTS), "slots must be 8"),
     (lambda: kernels.dequantize_fp4(Q, SCALES, X), "out must be"),
     (lambda: kernels.gemm_fp4(Q, SCALES, Stub(5, 16, dtype=U8), Stub(5, 16, dtype=U8), Stub(8, 5)), "incompatible"),
