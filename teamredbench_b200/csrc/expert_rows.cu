@@ -30,6 +30,7 @@ __device__ int g_rows_error;
 // then summed over the warps before, the CTAs before (distributed shared memory) and the experts before, and added.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortCtas = 16;  // the largest cluster
 constexpr int kBatch = 8;  // groups of 32 choices that a warp loads at once
 
 template <typename Id>
@@ -42,11 +43,12 @@ __device__ __forceinline__ int expert_of(const Id* ids, int i, int end, int expe
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
     expert_sort_kernel(const Id* ids, int entries, int experts, int* offsets, int* slots) {
-    extern __shared__ int counts[];  // [warps][experts], then the CTA's totals, where its places begin, the cluster's totals
+    extern __shared__ int counts[];  // [warps][experts], then the CTA's totals, where its places begin, where the expert's do
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int* const totals = counts + warps * experts;
     int* const begin = totals + experts;
-    int* const alls = begin + experts;
+    int* const offset = begin + experts;
+    __shared__ int group_total[32];  // at most kMaxGroups experts
     const int ctas = gridDim.x, rank = blockIdx.x;  // the grid is one cluster
     int* const mine = counts + warp * experts;
 
@@ -94,42 +96,59 @@ __global__ void __launch_bounds__(kSortThreads)
     }
     if (ctas > 1) cluster_sync_all();
     else __syncthreads();
-    for (int x = threadIdx.x; x < experts; x += blockDim.x) {
+    // begin[x] = what the CTAs before have of expert x, and the experts of its group of 32 before it have in all.
+    for (int x0 = warp * 32; x0 < experts; x0 += warps * 32) {
+        const int x = x0 + lane;
         int before = 0, all = 0;
-        if (ctas == 1) {
-            all = totals[x];
-        } else {
-#pragma unroll 4
-            for (int r = 0; r < ctas; ++r) {
-                int c;
-                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c) : "r"(mapa_shared(smem_u32(totals + x), r)));
-                before += r < rank ? c : 0;
-                all += c;
+        if (x < experts) {
+            if (ctas == 1) {
+                all = totals[x];
+            } else {
+                const uint32_t at = smem_u32(totals + x);
+                int c[kSortCtas];
+#pragma unroll
+                for (int r = 0; r < kSortCtas; ++r) {
+                    c[r] = 0;
+                    if (r < ctas) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c[r]) : "r"(mapa_shared(at, r)));
+                }
+#pragma unroll
+                for (int r = 0; r < kSortCtas; ++r) {
+                    before += r < rank ? c[r] : 0;
+                    all += c[r];
+                }
             }
         }
-        begin[x] = before;
-        alls[x] = all;
+        int sum = all;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += up;
+        }
+        if (x < experts) {
+            begin[x] = before;
+            offset[x] = sum - all;
+        }
+        if (lane == 31) group_total[x0 >> 5] = sum;
     }
     __syncthreads();
     if (ctas > 1) cluster_arrive();  // the other CTAs' totals have been read
     if (warp == 0) {
-        int base = 0;
-        for (int x0 = 0; x0 < experts; x0 += 32) {
-            const int x = x0 + lane;
-            const int all = x < experts ? alls[x] : 0;
-            int sum = all;
+        const int groups_of_32 = (experts + 31) >> 5;
+        int sum = lane < groups_of_32 ? group_total[lane] : 0;
+        const int own = sum;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, sum, d);
-                if (lane >= d) sum += up;
-            }
-            if (x < experts) {
-                begin[x] += base + sum - all;
-                if (rank == 0) offsets[x] = base + sum - all;
-            }
-            base += __shfl_sync(0xffffffffu, sum, 31);
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += up;
         }
-        if (lane == 0 && rank == 0) offsets[experts] = base;
+        group_total[lane] = sum - own;
+        if (lane == 31 && rank == 0) offsets[experts] = sum;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < experts; x += blockDim.x) {
+        const int at = offset[x] + group_total[x >> 5];
+        if (rank == 0) offsets[x] = at;
+        begin[x] += at;
     }
     __syncthreads();
     for (int i = first; i < end; i += 32 * kBatch) {
