@@ -329,7 +329,7 @@ int trb_expert_sort_launch(int id_bytes, int tokens, int choices, int experts, c
  * choices in float32 or that type (weight_dtype), or NULL.  A negative slot is
  * a choice without a row; a slot of `rows` or more is skipped and sets the
  * device error word to 8.  Rows of out that no slot names are left as they are;
- * one that two slots name gets either.  Products are made in fp32 and rounded
+ * one that two slots name gets values of both.  Products are made in fp32 and rounded
  * once.  Any width; rows move 16 bytes at a time where width and pointers are
  * multiples of 16 bytes.  rows, width and tokens * choices at most 2130706432. */
 int trb_expert_dispatch_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width, const void* x,

@@ -9,6 +9,9 @@
 // With slots, row t of x goes to the rows slots[t, j] of the result: tokens on their way to their experts are quantised
 // once and written in 4 bits, instead of moved in 16 and quantised after.
 //
+// The bytes of the rows bound both ways: 16384 x 8192 bf16 to 4 bits in 49.6 us, 6.85 TB/s (two bytes read for 0.53
+// written, a copy of as many bytes measures 6.55), and back in 52.6 us; 8192 x 8192 float32 in 46 us.
+//
 // No counterpart in the reference.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -360,7 +360,8 @@ def expert_dispatch(x: Any, slots: Any, out: Any, *, weights: Any | None = None,
     tokens to the rows of their experts.
 
     x is (tokens x width) and out (rows x width), bf16, f16 or float32; slots are
-    expert_sort's; weights (tokens x choices) are float32 or of x's dtype.  Rows
+    expert_sort's, which differ (a row that two slots name gets values of both);
+    weights (tokens x choices) are float32 or of x's dtype.  Rows
     of out that no slot names stay as they are, a negative slot is skipped, and
     one behind the last row is skipped and sets the device error word to 8
     (``_native.device_error``), which the host does not wait for here.  The
