@@ -319,6 +319,7 @@ int trb_gemv_w4_launch(int dtype, int groups, int rows, int n, int k, int group_
  * in the order of the choices inside an expert; -1 for an id outside [0,
  * experts), which no expert here takes (another rank's, a token left out).
  * At most 1024 experts; tokens * choices at most 2130706432; tokens may be 0.
+ * Here and below results must not overlap operands or each other (refused).
  * Asynchronous on `stream`, on the calling thread's current device, as all
  * entries of this section.  No reference counterpart. */
 int trb_expert_sort_launch(int id_bytes, int tokens, int choices, int experts, const void* ids, int32_t* offsets,
@@ -346,8 +347,8 @@ int trb_expert_combine_launch(int dtype, int weight_dtype, int tokens, int choic
  * width): grad_y[slots[t, j]] = weights[t, j] * grad[t] (rows x width; other
  * rows are left as they are) and grad_weights[t, j] = the sum over the width of
  * grad[t] * y[slots[t, j]] (tokens x choices, the weights' type; 0 for a
- * negative slot), in fp32 and in the same order at every call.  Types, slots and
- * limits as above. */
+ * negative slot), in fp32 and in the same order at every call.  grad_y may be y
+ * itself.  Types, slots and limits as above. */
 int trb_expert_combine_grad_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width,
                                    const void* grad, const void* y, const int32_t* slots, const void* weights,
                                    void* grad_y, void* grad_weights, void* stream);

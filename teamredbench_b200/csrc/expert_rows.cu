@@ -684,6 +684,12 @@ static int move(const char* what, bool back, int dtype, int weight_dtype, int to
     }
     rc = check_align(what, dtype, weight_dtype, bits(src) | bits(dst), weights, nullptr, slots);
     if (rc != TRB_OK) return rc;
+    const uint64_t size = dtype_size(dtype), entries = (uint64_t)tokens * choices;
+    rc = check_apart(what, {{dst, size, (uint64_t)(back ? tokens : rows), (uint64_t)width}},
+                     {{src, size, (uint64_t)(back ? rows : tokens), (uint64_t)width},
+                      {slots, 4, entries},
+                      {weights, dtype_size(weight_dtype), entries}});
+    if (rc != TRB_OK) return rc;
     int dev = 0;
     TRB_CUDA(cudaGetDevice(&dev));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -752,6 +758,10 @@ extern "C" int trb_expert_sort_launch(int id_bytes, int tokens, int choices, int
         set_error("trb_expert_sort_launch: pointers must be aligned to their elements");
         return TRB_ERR_ALIGN;
     }
+    const uint64_t entries = (uint64_t)tokens * choices;
+    const int rc = check_apart("trb_expert_sort_launch", {{offsets, 4, (uint64_t)experts + 1}, {slots, 4, entries}},
+                               {{ids, (uint64_t)id_bytes, entries}});
+    if (rc != TRB_OK) return rc;
     int dev = 0;
     TRB_CUDA(cudaGetDevice(&dev));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -789,6 +799,14 @@ extern "C" int trb_expert_combine_grad_launch(int dtype, int weight_dtype, int t
     }
     rc = rows::check_align(what, dtype, weight_dtype, rows::bits(grad) | rows::bits(y) | rows::bits(grad_y), weights,
                            grad_weights, slots);
+    if (rc != TRB_OK) return rc;
+    const uint64_t size = dtype_size(dtype), weight_size = dtype_size(weight_dtype), entries = (uint64_t)tokens * choices;
+    rc = check_apart(what, {{grad_y, size, (uint64_t)rows, (uint64_t)width}, {grad_weights, weight_size, entries}},
+                     {{grad, size, (uint64_t)tokens, (uint64_t)width},
+                      // The thread that writes a value of grad_y has read the one of y in its place, and nobody else does.
+                      {y == grad_y ? nullptr : y, size, (uint64_t)rows, (uint64_t)width},
+                      {slots, 4, entries},
+                      {weights, weight_size, entries}});
     if (rc != TRB_OK) return rc;
     int dev = 0;
     TRB_CUDA(cudaGetDevice(&dev));

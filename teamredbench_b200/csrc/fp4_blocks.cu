@@ -356,6 +356,11 @@ extern "C" int trb_quantize_fp4_launch(int dtype, int rows, int k, const void* x
         return TRB_SKIPPED;
     }
     if (rows == 0) return TRB_OK;
+    const uint64_t to = (uint64_t)(slots != nullptr ? out_rows : rows);
+    rc = check_apart(what, {{q, 1, to, (uint64_t)k / 2}, {scales, 1, to, (uint64_t)fp4::scale_pitch(k)}},
+                     {{x, dtype_size(dtype), (uint64_t)rows, (uint64_t)k},
+                      {slots, 4, (uint64_t)rows, (uint64_t)(slots != nullptr ? choices : 0)}});
+    if (rc != TRB_OK) return rc;
     int dev = 0;
     TRB_CUDA(cudaGetDevice(&dev));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -369,8 +374,12 @@ extern "C" int trb_dequantize_fp4_launch(int dtype, int rows, int k, const void*
                                          void* stream) {
     using namespace trb;
     clear_error();
-    const int rc = fp4::check("trb_dequantize_fp4_launch", dtype, rows, k, out, q, scales);
+    const char* const what = "trb_dequantize_fp4_launch";
+    int rc = fp4::check(what, dtype, rows, k, out, q, scales);
     if (rc != TRB_OK || rows == 0) return rc;
+    rc = check_apart(what, {{out, dtype_size(dtype), (uint64_t)rows, (uint64_t)k}},
+                     {{q, 1, (uint64_t)rows, (uint64_t)k / 2}, {scales, 1, (uint64_t)rows, (uint64_t)fp4::scale_pitch(k)}});
+    if (rc != TRB_OK) return rc;
     int dev = 0;
     TRB_CUDA(cudaGetDevice(&dev));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

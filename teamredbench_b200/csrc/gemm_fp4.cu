@@ -1031,6 +1031,14 @@ extern "C" int trb_gemm_fp4_launch(int dtype, int groups, int rows, int n, int k
         set_error("%s: matrices must be 16-byte aligned and offsets 4-byte aligned", what);
         return TRB_ERR_ALIGN;
     }
+    const uint64_t codes = (uint64_t)k / 2, pitch = (uint64_t)fp4::scale_pitch(k);
+    const int rc = check_apart(what, {{out, 2, (uint64_t)rows, (uint64_t)n}},
+                               {{a, 1, (uint64_t)rows, codes},
+                                {a_scales, 1, (uint64_t)rows, pitch},
+                                {b, 1, (uint64_t)n, codes, (uint64_t)groups},
+                                {b_scales, 1, (uint64_t)n, pitch, (uint64_t)groups},
+                                {offsets, 4, (uint64_t)groups + 1}});
+    if (rc != TRB_OK) return rc;
     int dev = 0;
     TRB_CUDA(cudaGetDevice(&dev));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -1,6 +1,8 @@
 // trb_groups.cuh -- rows sorted by group (expert) with offsets on the device.
 #pragma once
 
+#include <initializer_list>
+
 #include "trb_common.cuh"
 
 namespace trb {
@@ -9,6 +11,33 @@ constexpr int kMaxGroups = 1024;
 // Largest rows, n and k.  The kernels round sizes up to whole tiles and stages (a chunk's rows: up to one part in 256
 // above them) and step past the end by a stage in 32-bit integers, so sizes near 2^31 would wrap.
 constexpr int kMaxExtent = 0x7F000000;
+
+// Memory that a call reads or writes.
+struct Span {
+    const void* at;
+    uint64_t bytes;
+    Span(const void* p, uint64_t size, uint64_t rows, uint64_t width = 1, uint64_t groups = 1) : at(p) {
+        const unsigned __int128 all = (unsigned __int128)(size * groups) * rows * width;
+        bytes = p == nullptr ? 0 : all > UINT64_MAX ? UINT64_MAX : (uint64_t)all;
+    }
+};
+// CTAs read what others write where the two overlap, in any order, so such a call is refused.
+inline int check_apart(const char* what, std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    const auto overlap = [](const Span& a, const Span& b) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+        return a.bytes > 0 && b.bytes > 0 && (x <= y ? y - x < a.bytes : x - y < b.bytes);
+    };
+    for (auto w = written.begin(); w != written.end(); ++w) {
+        bool bad = false;
+        for (const Span& r : read) bad = bad || overlap(*w, r);
+        for (auto other = w + 1; other != written.end(); ++other) bad = bad || overlap(*w, *other);
+        if (bad) {
+            set_error("%s: results must not overlap operands or each other", what);
+            return TRB_ERR_ARGS;
+        }
+    }
+    return TRB_OK;
+}
 
 #if defined(__CUDACC__)
 

@@ -302,7 +302,8 @@ def expert_sort(experts: Any, offsets: Any, slots: Any, *, stream: Any | None = 
     of each choice among the rows sorted by expert, in the order of the tokens
     inside an expert.  A choice outside [0, experts) -- another rank's expert,
     or -1 for a token left out -- gets the slot -1 and no row.  One launch,
-    nothing allocated, the same result at every call."""
+    nothing allocated, the same result at every call.  As for the functions
+    below, results must not share memory with operands or each other."""
     short = _SHORT if _SHORT is not None else _find_short()
     if stream is None and short and short.expert_sort(experts, offsets, slots):
         return offsets, slots
@@ -407,7 +408,8 @@ def expert_combine_grad(grad: Any, y: Any, slots: Any, weights: Any, grad_y: Any
     grad_y[slots[t, j]] = weights[t, j] * grad[t] (rows x width; rows that no
     slot names stay as they are), grad_weights[t, j] = the sum of grad[t] *
     y[slots[t, j]] over the width (tokens x choices, 0 for a negative slot), of
-    the weights' dtype, summed in fp32.  Types, slots and errors as in
+    the weights' dtype, summed in fp32.  grad_y may be y itself, which saves a
+    matrix where y is not needed any more.  Types, slots and errors as in
     expert_dispatch."""
     short = _SHORT if _SHORT is not None else _find_short()
     if stream is None and short and short.expert_combine_grad(grad, y, slots, weights, grad_y, grad_weights):

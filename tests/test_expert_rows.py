@@ -222,3 +222,40 @@ def test_front_ends_refuse(machine, call, message):
 
 def test_scale_pitch():
     assert [kernels.fp4_scale_pitch(k) for k in (32, 512, 544, 4096, 16384)] == [16, 16, 32, 128, 512]
+
+
+A = [P + 2 ** 24 * i for i in range(7)]  # far from each other, and never read
+
+
+@pytest.mark.parametrize("entry, sizes, spans, written", [
+    ("trb_expert_sort_launch", (4, 64, 8, 16), [64 * 8 * 4, 17 * 4, 64 * 8 * 4], (1, 2)),
+    ("trb_expert_sort_launch", (8, 64, 8, 16), [64 * 8 * 8, 17 * 4, 64 * 8 * 4], (1, 2)),
+    ("trb_expert_dispatch_launch", (BF16, F32, 16, 2, 32, 24), [16 * 48, 16 * 8, 16 * 8, 32 * 48], (3,)),
+    ("trb_expert_combine_launch", (F32, F32, 16, 2, 32, 24), [32 * 96, 16 * 8, 16 * 8, 16 * 96], (3,)),
+    ("trb_expert_combine_grad_launch", (BF16, BF16, 16, 2, 32, 24),
+     [16 * 48, 32 * 48, 16 * 8, 16 * 4, 32 * 48, 16 * 4], (4, 5)),
+    ("trb_dequantize_fp4_launch", (F16, 16, 64), [16 * 32, 16 * 16, 16 * 128], (2,)),
+    ("trb_gemm_fp4_launch", (BF16, 4, 16, 24, 64), [16 * 32, 16 * 16, 4 * 24 * 32, 4 * 24 * 16, 5 * 4, 16 * 48], (5,)),
+])
+def test_results_that_overlap(entry, sizes, spans, written):
+    """The same memory, its first bytes and its last ones, for each result and every other tensor."""
+    for w in written:
+        for other in range(len(spans)):
+            for back in {0, 16, spans[other] // 16 * 16 - 16 if spans[other] % 16 == 0 else 0}:
+                if other == w or back >= spans[other]:
+                    continue
+                if entry == "trb_expert_combine_grad_launch" and (w, other, back) == (4, 1, 0):
+                    continue  # grad_y may be y itself
+                at = A[:len(spans)]
+                at[w] = at[other] + back
+                assert getattr(_native.load(), entry)(*sizes, *at, None) == -1, (w, other, back)
+                assert "must not overlap" in _native.last_error()
+
+
+@pytest.mark.parametrize("slots, rows", [(None, 16), (P + 2 ** 20, 32)])
+def test_quantised_results_that_overlap(slots, rows):
+    x, q, scales = A[1:4]
+    for over in ((x, x, scales), (x, x + 16 * 128 - 16, scales), (x, q, x), (x, q, q), (x, q, q + rows * 32 - 16),
+                 *(((x, slots, scales), (x, q, slots)) if slots else ())):
+        assert _native.load().trb_quantize_fp4_launch(BF16, 16, 64, over[0], 2, slots, rows, over[1], over[2], None) == -1
+        assert "must not overlap" in _native.last_error()

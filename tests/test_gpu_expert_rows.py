@@ -234,6 +234,29 @@ def test_a_slot_behind_the_last_row_is_skipped_and_reported(width):
     assert rows[0].eq(1).all() and rows[1].eq(1).all() and not whole[2:].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width, choices", [(264, 6), (263, 6), (2048, 4), (8, 1), (1, 2), (6, 9)])
+def test_gradient_into_y_itself(dtype, width, choices):
+    _, slots, here = _plan(300, choices)
+    g = torch.Generator(device="cuda").manual_seed(width)
+    grad, y = (torch.randn(n, width, generator=g, device="cuda").to(dtype) for n in (300, int(here.sum()) + 3))
+    w = torch.randn(300, choices, generator=g, device="cuda")
+    apart, weights_apart, weights_same = y.clone(), torch.empty_like(w), torch.empty_like(w)
+    expert_combine_grad(grad, y, slots, w, apart, weights_apart)
+    expert_combine_grad(grad, y, slots, w, y, weights_same)
+    assert torch.equal(y, apart) and torch.equal(weights_same, weights_apart)
+
+
+def test_sort_into_the_choices_themselves_is_refused():
+    ids = torch.zeros(50, 2, device="cuda", dtype=torch.int32)
+    with pytest.raises(_native.NativeError, match="must not overlap"):
+        expert_sort(ids, torch.empty(9, device="cuda", dtype=torch.int32), ids)
+    x = torch.ones(4, 32, device="cuda")
+    with pytest.raises(_native.NativeError, match="must not overlap"):
+        expert_dispatch(x, torch.zeros(4, 1, device="cuda", dtype=torch.int32), x)
+    assert not ids.any() and x.eq(1).all()
+
+
 def test_nothing_to_do():
     empty = torch.empty(0, 2, device="cuda", dtype=torch.int32)
     x = torch.empty(0, 16, device="cuda", dtype=torch.bfloat16)
