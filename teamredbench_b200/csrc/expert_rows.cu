@@ -266,76 +266,94 @@ __global__ void __launch_bounds__(kRowThreads)
 // Choices whose rows are on their way at the same time, in the gradient.
 constexpr int kAtOnce = 4;
 
-// Sums in fp32, in the order of the choices, rounded once.  This is for rows that are not 16-byte aligned: V values, 8
-// bytes or less, an access, U of them of each row on their way.
-template <typename T, typename W, int V, int U>
-__global__ void __launch_bounds__(kRowThreads)
-    expert_combine_kernel(const T* y, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
-                          int width, int log2_lanes) {
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const RowWalk w = row_walk(log2_lanes);
-    const int packs = width / V;
-    for (int64_t t = w.token; t < tokens; t += w.token_step) {
-        for (int p = w.pack; p < packs; p += U * w.pack_step) {
-            float sum[U][V];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int i = 0; i < V; ++i) sum[u][i] = 0.0f;
-            for (int j0 = 0; j0 < choices; j0 += kAtOnce) {
-                int row[kAtOnce];
-                float f[kAtOnce];
-                Pack<T, V> v[kAtOnce][U];
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    row[j] = j0 + j < choices ? row_of(slots, t * choices + j0 + j, rows) : -1;
-                    f[j] = weights != nullptr && row[j] >= 0 ? to_f32(weights[t * choices + j0 + j]) : 1.0f;
-                }
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    if (row[j] < 0) continue;
-                    const T* const from = y + (int64_t)row[j] * width + (int64_t)p * V;
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (p + u * w.pack_step < packs) v[j][u] = load<T, V>(from + (int64_t)u * w.pack_step * V);
-                }
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    if (row[j] < 0) continue;
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) sum[u][i] = fmaf(f[j], to_f32(v[j][u].v[i]), sum[u][i]);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (p + u * w.pack_step >= packs) break;
-                Pack<T, V> o;
-#pragma unroll
-                for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(sum[u][i]);
-                store<T, V>(out + t * width + (int64_t)(p + u * w.pack_step) * V, o);
-            }
-        }
-    }
-}
-
-// The same for rows that are 16-byte aligned.  Loads into registers keep too few bytes in flight, for a slot
-// has to be read before its row can be (16384 tokens of 2 rows of 4096 bf16: 119 us).  Here a thread copies its 16 bytes
-// of J rows to shared memory (cp.async) kDeep - 1 steps before it adds them up; nobody else reads them, so there is no
+// Combine: sums in fp32, in the order of the choices, rounded once.  Loads into registers keep too few bytes in flight, for
+// a slot has to be read before its row can be (16384 tokens of 2 rows of 4096 bf16: 119 us).  Here a thread copies its 16
+// bytes of J rows to shared memory (cp.async) kDeep - 1 steps before it adds them up; nobody else reads them, so there is no
 // barrier.  A lane reads the slot and weight of one of a step's choices a step before the rows are asked for, and shuffles
 // pass them round.  Four CTAs an SM and 96 bytes a thread on their way: 70 us; three CTAs and 112 bytes 78, five and 64
 // 83.  Rows through a ring of bulk copies of 4 KB with a producer warp took 73 us and two waits a row.
+//
+// Rows that begin anywhere (kAny) go the same way in the aligned pieces around them: 4109 tokens of 8 rows of 2047 and 2046
+// bf16 35 and 34 us, where accesses of 2 and 4 bytes straight to registers took 55 and 82, and of 2046 float32, 4 rows, 32.
 constexpr int kRingCtas = 4;  // of an SM
 template <int J>
 struct Ring {
     static constexpr int kDeep = J == 2 ? 6 : 3;
-    static constexpr size_t kSmem = (size_t)kDeep * J * kRowThreads * 16;
+    static constexpr size_t smem(int pieces) { return (size_t)kDeep * J * (kRowThreads / 32) * pieces * 16; }
 };
 
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// The first `bytes` of the 16, zeros behind them; no more than these are read.
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+// A row that begins at any value's place, in the 16-byte pieces that memory has: its values from e0 on stand `shift`
+// bytes behind the beginning of the first piece.
+template <typename T>
+__device__ __forceinline__ int row_shift(const T* rows, int row, int width, int e0) {
+    constexpr uint32_t S = sizeof(T);
+    return (int)(((uint32_t)reinterpret_cast<uintptr_t>(rows) + S * ((uint32_t)row * (uint32_t)width + (uint32_t)e0)) & 15u);
+}
+// Copies a piece, which begins with value `first` of its row, as far as it is the row's.  The one that begins before the
+// matrix goes value by value.
+template <typename T>
+__device__ __forceinline__ void copy_piece(uint32_t to, const T* from, int first, int width, const T* rows) {
+    constexpr int S = sizeof(T), V = 16 / S;
+    if (first + V <= 0 || first >= width) return;
+    if (first >= 0 || from >= rows) {
+        copy_async(to, from, min(16, (width - first) * S));
+    } else {
+        for (int x = -first; x < V && first + x < width; ++x) {
+            if constexpr (S == 2)
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + x * S),
+                             "h"(reinterpret_cast<const unsigned short*>(from)[x]) : "memory");
+            else
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + x * S),
+                             "r"(reinterpret_cast<const uint32_t*>(from)[x]) : "memory");
+        }
+    }
+}
+// Four words of shared memory, 128 bytes apart, from any value's place on.
+template <int S>
+__device__ __forceinline__ void load_words(uint32_t (&words)[4], uint32_t at) {
+    const uint32_t even = at & ~3u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(words[u]) : "r"(even + 128 * u) : "memory");
+    if (S == 2 && (at & 2u)) {  // all of the warp or none
+        uint32_t high[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(high[u]) : "r"(even + 128 * u + 4) : "memory");
+#pragma unroll
+        for (int u = 0; u < 4; ++u) words[u] = __byte_perm(words[u], high[u], 0x5432);
+    }
+}
+// The values of a word.
+template <typename T>
+struct alignas(4) Word {
+    static constexpr int kValues = 4 / sizeof(T);
+    T v[kValues];
+};
+template <typename T>
+__device__ __forceinline__ Word<T> as_word(uint32_t bits) {
+    Word<T> w;
+    memcpy(&w, &bits, 4);
+    return w;
+}
+// Values e, e + 1 of a row (or e alone), which stand in one word there, as far as they are the row's.
+template <typename T>
+__device__ __forceinline__ void store_word(T* row, int e, int width, const Word<T>& w) {
+    constexpr int N = Word<T>::kValues;
+    if (e >= 0 && e + N <= width) {
+        *reinterpret_cast<Word<T>*>(row + e) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (e + i >= 0 && e + i < width) row[e + i] = w.v[i];
+    }
 }
 
 // A warp's way through its tokens, 32 packs of their rows and J choices at a time.
@@ -343,19 +361,27 @@ struct Step {
     int64_t token;
     int pack0, chunk;
 };
+// What a warp has of a row in a step: 32 packs of 16 bytes, and one more piece where they stand anywhere.
+constexpr int kPieces = 33;
 
-template <typename T, typename W, int J>
+// kAny: the rows and the tokens' rows begin at any value's place.  The warp's 512 bytes of a row are then copied as the 33
+// pieces around them, and its lanes read words out of them, as the words of the token's row want them.
+template <typename T, typename W, int J, bool kAny>
 __global__ void __launch_bounds__(kRowThreads, kRingCtas)
     expert_combine_ring_kernel(const T* y, const int* slots, const W* weights, T* out, int64_t tokens, int choices,
                                int rows, int width, int log2_lanes) {
-    constexpr int V = 16 / sizeof(T), kDeep = Ring<J>::kDeep;
+    constexpr int S = sizeof(T), V = 16 / S, kDeep = Ring<J>::kDeep, N = Word<T>::kValues;
+    // Shared memory for a warp's part of a row, and from one row of a step to the next.
+    constexpr int kRow = kAny ? kPieces * 16 : 32 * 16, kNext = kAny ? kRow : kRow * (kRowThreads / 32);
     extern __shared__ __align__(16) uint8_t ring[];
     grid_launch_dependents();
     grid_dependency_wait();
     const RowWalk w = row_walk(log2_lanes);
-    const int packs = width / V, lane = threadIdx.x & 31, chunks = (choices + J - 1) / J;
-    const uint32_t own = smem_u32(ring) + threadIdx.x * 16;
-    const auto at = [&](int deep, int j) { return own + (uint32_t)((deep * J + j) * kRowThreads * 16); };
+    const int packs = kAny ? (width + N - 1 + V - 1) / V : width / V;
+    const int lane = threadIdx.x & 31, chunks = (choices + J - 1) / J;
+    const T* const y_end = y + (int64_t)rows * width;
+    const uint32_t own = smem_u32(ring) + (threadIdx.x >> 5) * (kAny ? kDeep * J * kRow : kRow);
+    const auto at = [&](int deep, int j) { return own + (uint32_t)((deep * J + j) * kNext); };
     const auto next = [&](Step& s) {
         if (++s.chunk < chunks) return;
         s.chunk = 0;
@@ -364,30 +390,70 @@ __global__ void __launch_bounds__(kRowThreads, kRingCtas)
         s.pack0 = w.pack - lane;
         s.token += w.token_step;
     };
+    // The value that a step's packs begin with: one before the row's pack where its words begin there.
+    const auto first_value = [&](const Step& s) {
+        const int e0 = s.pack0 * V;
+        if constexpr (S == 4 || !kAny) return e0;
+        else return e0 - (int)(((uint32_t)(reinterpret_cast<uintptr_t>(out) >> 1) + (uint32_t)s.token * (uint32_t)width) & 1u);
+    };
     struct Choice {
         int row;
         float weight;
+        int shift;      // kAny: where the row's part stands in its pieces, and the first of them
+        const T* from;
+        bool inside;    // all pieces are the matrix's
     };
     const auto choice = [&](Step& s) {
-        Choice c = {-1, 1.0f};
+        Choice c = {-1, 1.0f, -1, nullptr, true};
         const int j = s.chunk * J + lane;
         if (lane < J && j < choices && s.token < tokens) {
             c.row = row_of(slots, s.token * choices + j, rows);
+            if (kAny && c.row >= 0) {
+                const int e0 = first_value(s);
+                c.shift = row_shift(y, c.row, width, e0);
+                c.from = y + (int64_t)c.row * width + (e0 - c.shift / S);
+                c.inside = c.from >= y && c.from + kPieces * V <= y_end;
+            }
             if (weights != nullptr) c.weight = to_f32(weights[s.token * choices + j]);
         }
         next(s);
         return c;
     };
-    uint32_t present[kDeep];  // which of a step's choices have a row, and (lane j) the weight of choice j
-    float weight[kDeep];
+    uint32_t present[kDeep];  // which of a step's choices have a row
+    float weight[kDeep];      // (lane j) the weight of choice j
+    int shift[kDeep];         // kAny, in place of present: (lane j) that of choice j, negative without a row
     const auto ask = [&](int deep, Step& s, const Choice& c) {
-        present[deep] = __ballot_sync(0xffffffffu, c.row >= 0);
+        if constexpr (!kAny) present[deep] = __ballot_sync(0xffffffffu, c.row >= 0);
         weight[deep] = c.weight;
+        if constexpr (kAny) {
+            shift[deep] = c.shift;
+            const int e0 = first_value(s);
+            if (__all_sync(0xffffffffu, c.inside)) {
+                // What stands before and behind the row in the pieces is read along and left out of the results.
+                const bool needed = e0 + V * (lane - 1) < width;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int row = __shfl_sync(0xffffffffu, c.row, j);
-            if (row >= 0 && s.pack0 + lane < packs)
-                copy_async(at(deep, j), y + (int64_t)row * width + (int64_t)(s.pack0 + lane) * V);
+                for (int j = 0; j < J; ++j) {
+                    const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(c.from), j);
+                    if (from != 0 && needed) copy_async(at(deep, j) + lane * 16, reinterpret_cast<const T*>(from) + lane * V);
+                }
+                if (c.shift >= 0 && e0 + V * 31 < width) copy_async(at(deep, lane) + 32 * 16, c.from + 32 * V);  // the last
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < J; ++j) {
+                    const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(c.from), j);
+                    const int first = e0 - __shfl_sync(0xffffffffu, c.shift, j) / S + V * lane;
+                    if (from != 0)
+                        copy_piece(at(deep, j) + lane * 16, reinterpret_cast<const T*>(from) + lane * V, first, width, y);
+                }
+                if (c.shift >= 0) copy_piece(at(deep, lane) + 32 * 16, c.from + 32 * V, e0 - c.shift / S + 32 * V, width, y);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int row = __shfl_sync(0xffffffffu, c.row, j);
+                if (row >= 0 && s.pack0 + lane < packs)
+                    copy_async(at(deep, j) + lane * 16, y + (int64_t)row * width + (int64_t)(s.pack0 + lane) * V);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         next(s);
@@ -407,22 +473,47 @@ __global__ void __launch_bounds__(kRowThreads, kRingCtas)
         for (int i = 0; i < kDeep; ++i) {
             if (now.token >= tokens) break;
             asm volatile("cp.async.wait_group %0;" ::"n"(kDeep - 2) : "memory");
+            if constexpr (kAny) __syncwarp();  // the other lanes' pieces; and all have read what the next request overwrites
             if (now.chunk == 0)
 #pragma unroll
                 for (int x = 0; x < V; ++x) sum[x] = 0.0f;
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 const float f = __shfl_sync(0xffffffffu, weight[i], j);
-                if (!(present[i] >> j & 1)) continue;
-                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(ring + ((i * J + j) * kRowThreads + threadIdx.x) * 16);
+                const int sh = kAny ? __shfl_sync(0xffffffffu, shift[i], j) : 0;
+                if (kAny ? sh < 0 : !(present[i] >> j & 1)) continue;
+                if constexpr (kAny) {
+                    const uint32_t from = at(i, j) + sh + 4 * lane;
+                    uint32_t words[4];
+                    load_words<S>(words, from);
 #pragma unroll
-                for (int x = 0; x < V; ++x) sum[x] = fmaf(f, to_f32(v.v[x]), sum[x]);
+                    for (int u = 0; u < 4; ++u) {
+                        const Word<T> v = as_word<T>(words[u]);
+#pragma unroll
+                        for (int x = 0; x < N; ++x) sum[u * N + x] = fmaf(f, to_f32(v.v[x]), sum[u * N + x]);
+                    }
+                } else {
+                    const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(ring + (i * J + j) * kNext + threadIdx.x * 16);
+#pragma unroll
+                    for (int x = 0; x < V; ++x) sum[x] = fmaf(f, to_f32(v.v[x]), sum[x]);
+                }
             }
-            if (now.chunk == chunks - 1 && now.pack0 + lane < packs) {
-                Pack<T, V> o;
+            if (now.chunk == chunks - 1) {
+                if constexpr (kAny) {
+                    const int e0 = first_value(now);
 #pragma unroll
-                for (int x = 0; x < V; ++x) o.v[x] = round_to<T>(sum[x]);
-                store<T, V>(out + now.token * width + (int64_t)(now.pack0 + lane) * V, o);
+                    for (int u = 0; u < 4; ++u) {
+                        Word<T> o;
+#pragma unroll
+                        for (int x = 0; x < N; ++x) o.v[x] = round_to<T>(sum[u * N + x]);
+                        store_word(out + now.token * width, e0 + N * (lane + 32 * u), width, o);
+                    }
+                } else if (now.pack0 + lane < packs) {
+                    Pack<T, V> o;
+#pragma unroll
+                    for (int x = 0; x < V; ++x) o.v[x] = round_to<T>(sum[x]);
+                    store<T, V>(out + now.token * width + (int64_t)(now.pack0 + lane) * V, o);
+                }
             }
             next(now);
             ask((i + kDeep - 1) % kDeep, asked, known);
@@ -615,22 +706,22 @@ static int access_bytes(size_t size, int width, uintptr_t pointers) {
     return (int)std::min<uint64_t>(all & (~all + 1), 16);
 }
 
-template <typename T, typename W, int J>
+template <typename T, typename W, int J, bool kAny>
 static int launch_ring(const void* y, const int* slots, const void* weights, void* out, int tokens, int choices, int rows,
                        int width, int dev, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    constexpr size_t smem = Ring<J>::kSmem;
+    constexpr size_t smem = Ring<J>::smem(kAny ? kPieces : 32);
     static bool attr_set[64] = {};
     if (dev >= 64 || !attr_set[dev]) {
-        TRB_CUDA(cudaFuncSetAttribute(expert_combine_ring_kernel<T, W, J>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        TRB_CUDA(cudaFuncSetAttribute(expert_combine_ring_kernel<T, W, J, kAny>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)smem));
         if (dev < 64) attr_set[dev] = true;
     }
-    RowShape s = row_shape(tokens, width / V, 1, false, dev);
+    RowShape s = row_shape(tokens, kAny ? (width + Word<T>::kValues + V - 2) / V : width / V, 1, false, dev);
     // No more CTAs than the GPU holds, each for several tokens.
     const unsigned places = (unsigned)(device_sm_count(dev) * kRingCtas);
     s.grid.x = std::max(1u, std::min(s.grid.x, places / s.grid.y));
-    return launch(expert_combine_ring_kernel<T, W, J>, s.grid, kRowThreads, 0, smem, stream, static_cast<const T*>(y),
+    return launch(expert_combine_ring_kernel<T, W, J, kAny>, s.grid, kRowThreads, 0, smem, stream, static_cast<const T*>(y),
                   slots, static_cast<const W*>(weights), static_cast<T*>(out), (int64_t)tokens, choices, rows, width,
                   s.log2_lanes);
 }
@@ -640,20 +731,17 @@ template <typename T, typename W, int V>
 static int launch_move(bool back, const void* src, const int* slots, const void* weights, void* dst, int tokens,
                        int choices, int rows, int width, int dev, cudaStream_t stream) {
     constexpr int B = V * sizeof(T);
-    if constexpr (B == 16)
-        if (back)
-            return choices <= 2 ? launch_ring<T, W, 2>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
-                                : launch_ring<T, W, 4>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+    if (back)
+        return choices <= 2
+                   ? launch_ring<T, W, 2, B != 16>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
+                   : launch_ring<T, W, 4, B != 16>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
     const auto run = [&](auto kernel, int at_once) {
         const RowShape s = row_shape(tokens, width / V, at_once, false, dev);
         return launch(kernel, s.grid, kRowThreads, 0, 0, stream, static_cast<const T*>(src), slots,
                       static_cast<const W*>(weights), static_cast<T*>(dst), (int64_t)tokens, choices, rows, width,
                       s.log2_lanes);
     };
-    // Accesses of a lane on their way: 4109 tokens of 8 rows of 2047 bf16, dispatch with 2, 4 and 8 of them 49, 43 and 43
-    // us, combine 61, 53 and 73.
-    if constexpr (B < 16)
-        if (back) return run(expert_combine_kernel<T, W, V, B == 2 ? 4 : 2>, B == 2 ? 4 : 2);
+    // Accesses of a lane on their way: 4109 tokens of 8 rows of 2047 bf16 with 2, 4 and 8 of them 49, 43 and 43 us.
     constexpr int U = B == 16 ? 1 : B == 8 ? 2 : 4;
     return run(expert_dispatch_kernel<T, W, V, U>, U);
 }

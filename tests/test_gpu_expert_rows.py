@@ -234,6 +234,55 @@ def test_a_slot_behind_the_last_row_is_skipped_and_reported(width):
     assert rows[0].eq(1).all() and rows[1].eq(1).all() and not whole[2:].any()
 
 
+def _at(t, offset):
+    """A copy of t that begins `offset` values behind an aligned address, with NaN around it."""
+    whole = torch.full((t.numel() + 32,), float("nan"), device="cuda", dtype=t.dtype)
+    there = whole[offset:offset + t.numel()].view(t.shape)
+    there.copy_(t)
+    return whole, there
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [1, 2, 3, 7, 8, 255, 256, 257, 510, 2046, 2048])
+@pytest.mark.parametrize("offsets", [(0, 1), (1, 0), (1, 1), (2, 1), (3, 2), (4, 7), (5, 3), (6, 6), (7, 4)])
+def test_rows_that_begin_anywhere(dtype, width, offsets):
+    """Every place of a row in 16 bytes; rows that no slot names, and all around the matrices, are NaN and stay so."""
+    tokens, choices = 37, 5
+    _, slots, here = _plan(tokens, choices)
+    count = int(here.sum())
+    slots = torch.where(here, 2 * slots, -1)  # every other row of 2 * count - 1
+    g = torch.Generator(device="cuda").manual_seed(width)
+    rows = torch.full((2 * count - 1, width), float("nan"), device="cuda", dtype=dtype)
+    rows[::2] = torch.randn(count, width, generator=g, device="cuda").to(dtype)
+    x = torch.randn(tokens, width, generator=g, device="cuda").to(dtype)
+    w = torch.randn(tokens, choices, generator=g, device="cuda")
+    around_y, y = _at(rows, offsets[0])
+    around_out, out = _at(torch.zeros_like(x), offsets[1])
+    expert_combine(y, slots, out, weights=w)
+    want = torch.zeros_like(x, dtype=torch.float32)
+    for j in range(choices):  # fp32, in the order of the choices: fma's one rounding less is what differs
+        want += torch.where(here[:, j:j + 1], w[:, j:j + 1] * rows[slots[:, j].clamp_min(0).long()].float(), 0.0)
+    size = torch.stack([torch.where(here[:, j:j + 1], (w[:, j:j + 1] * rows[slots[:, j].clamp_min(0).long()].float()).abs(),
+                                    0.0) for j in range(choices)]).sum(0)
+    eps = torch.finfo(dtype).eps / 2
+    assert ((out.double() - want.double()).abs() <= eps * want.double().abs() + 4 * choices * 2.0 ** -24 * size.double()).all()
+    assert around_out.isnan().sum() == 32
+    around_x, xs = _at(x, offsets[0])
+    around_rows, ys = _at(torch.full_like(rows, float("nan")), offsets[1])
+    expert_dispatch(xs, slots, ys)
+    assert torch.equal(ys[slots[here].long()], x.unsqueeze(1).expand(-1, choices, -1)[here])
+    assert ys[1::2].isnan().all() and around_rows.isnan().sum() == 32 + (count - 1) * width
+    grad_w = torch.empty_like(w)
+    around_rows, gy = _at(torch.full_like(rows, float("nan")), offsets[1])
+    expert_combine_grad(xs, y, slots, w, gy, grad_w)
+    assert torch.equal(gy[slots[here].long()], (w.unsqueeze(-1) * x.float().unsqueeze(1))[here].to(dtype))
+    assert gy[1::2].isnan().all() and around_rows.isnan().sum() == 32 + (count - 1) * width
+    products = x.double().unsqueeze(1) * rows[slots.clamp_min(0).long()].double()
+    want_w = torch.where(here, products.sum(-1), 0.0)
+    slack = torch.where(here, products.abs().sum(-1), 0.0) * width * 2.0 ** -24
+    assert ((grad_w.double() - want_w).abs() <= slack + 2.0 ** -24 * want_w.abs()).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("width, choices", [(264, 6), (263, 6), (2048, 4), (8, 1), (1, 2), (6, 9)])
 def test_gradient_into_y_itself(dtype, width, choices):
