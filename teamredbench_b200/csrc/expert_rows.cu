@@ -602,6 +602,147 @@ __global__ void __launch_bounds__(kRowThreads)
     }
 }
 
+// The same for many tokens and rows that are 16-byte aligned: the parts of up to four rows and of the token's own come
+// through a ring as in combine, a thread's 16 bytes of each, a step ahead.  A token is a CTA's (kWhole), whose warps add up
+// the sums of the weights' gradients in order, or a warp's.  4109 tokens of 8 rows of 2048 bf16 47.7 us (the kernel above
+// 57), 16384 of 2 rows of 4096 116 (146); two steps ahead with three CTAs an SM 50.4 and 115.6, and 77 where this takes 67.
+constexpr int kGradRows = 4, kGradDeep = 2;
+constexpr int kGradCtas = 4;  // of an SM
+constexpr size_t kGradSmem = (size_t)kGradDeep * (kGradRows + 1) * kRowThreads * 16;
+
+template <typename T, typename W, bool kWhole>
+__global__ void __launch_bounds__(kRowThreads, kGradCtas)
+    expert_combine_grad_ring_kernel(const T* grad, const T* y, const int* slots, const W* weights, T* grad_y,
+                                    W* grad_weights, int64_t tokens, int choices, int rows, int width) {
+    constexpr int V = 16 / sizeof(T), J = kGradRows, D = kGradDeep, kWarps = kRowThreads / 32;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ float part[2][kWarps][J];
+    // The next kernel does not start before the end.  Started early into this one's division of the SM's memory, a combine
+    // found room for three CTAs an SM instead of four, and its fourth part came after the others (a training step's two
+    // calls: 354 us instead of 303; the largest division for both kernels took 331 and slowed combine down).
+    grid_dependency_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int packs = width / V, chunks = (choices + J - 1) / J;
+    const int pack_first = kWhole ? warp * 32 : 0, pack_step = kWhole ? kRowThreads : 32;
+    const int64_t token_first = kWhole ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarps + warp;
+    const int64_t token_step = kWhole ? (int64_t)gridDim.x : (int64_t)gridDim.x * kWarps;
+    uint8_t* const own = ring + threadIdx.x * 16;
+    const auto at = [&](int deep, int j) { return own + (deep * (J + 1) + j) * (kRowThreads * 16); };
+    const auto next_row = [&](Step& s) {
+        s.pack0 = pack_first;
+        if (++s.chunk < chunks) return;
+        s.chunk = 0;
+        s.token += token_step;
+    };
+    // True at the end of a row's packs.  A warp behind them goes through every row once, too, with nothing to do.
+    const auto next = [&](Step& s) {
+        s.pack0 += pack_step;
+        if (s.pack0 < packs) return false;
+        next_row(s);
+        return true;
+    };
+    // Lane j has a step's choice j, lane J the token's own row: where the warp's next packs of them are, if there are any.
+    struct Part {
+        int row;
+        float weight;
+        const T* from;
+    };
+    const auto part_of = [&](const Step& s) {
+        Part c = {-1, 0.0f, nullptr};
+        const int j = s.chunk * J + lane;
+        if (s.token >= tokens) return c;
+        if (lane < J && j < choices) {
+            c.row = row_of(slots, s.token * choices + j, rows);
+            if (c.row >= 0) {
+                c.weight = to_f32(weights[s.token * choices + j]);
+                c.from = y + (int64_t)c.row * width + s.pack0 * V;
+            }
+        } else if (lane == J) {
+            c.from = grad + s.token * width + s.pack0 * V;
+        }
+        return c;
+    };
+    Step now = {token_first, pack_first, 0};
+    Step asked = now, read = now;
+    Part known = part_of(read);  // of the rows that are asked for, and of those after them
+    next_row(read);
+    Part then = part_of(read);
+    int row[D];  // (lane j) of a step's choice j
+    float weight[D];
+    const auto ask = [&](int deep) {
+        row[deep] = known.row;
+        weight[deep] = known.weight;
+#pragma unroll
+        for (int j = 0; j <= J; ++j) {
+            const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(known.from), j);
+            if (from != 0 && asked.pack0 + lane < packs)
+                copy_async(smem_u32(at(deep, j)), reinterpret_cast<const T*>(from) + lane * V);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (known.from != nullptr) known.from += pack_step * V;
+        if (next(asked)) {
+            known = then;
+            next_row(read);
+            then = part_of(read);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i) ask(i);
+    float dot[J] = {};
+    int turn = 0;
+    while (now.token < tokens) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            if (now.token >= tokens) break;
+            asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+            const int pack = now.pack0 + lane;
+            const bool inside = pack < packs;
+            Pack<T, V> g;
+            if (inside) g = *reinterpret_cast<const Pack<T, V>*>(at(i, J));
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int r = __shfl_sync(0xffffffffu, row[i], j);
+                const float f = __shfl_sync(0xffffffffu, weight[i], j);
+                if (r < 0 || !inside) continue;
+                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(at(i, j));
+                Pack<T, V> o;
+#pragma unroll
+                for (int x = 0; x < V; ++x) {
+                    const float gx = to_f32(g.v[x]);
+                    dot[j] = fmaf(gx, to_f32(v.v[x]), dot[j]);
+                    o.v[x] = round_to<T>(f * gx);
+                }
+                store<T, V>(grad_y + (int64_t)r * width + (int64_t)pack * V, o);
+            }
+            const int64_t entry = now.token * choices + now.chunk * J;
+            const int left = choices - now.chunk * J;
+            if (next(now)) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
+                    if (kWhole && lane == 0) part[turn][warp][j] = dot[j];
+                    if (!kWhole && lane == j) sum = dot[j];
+                    dot[j] = 0.0f;
+                }
+                if constexpr (kWhole) {
+                    // The warps come here after different numbers of steps.  The first one has read the turn before last
+                    // before it came here the last time.
+                    asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory");
+                    if (warp == 0 && lane < J)
+#pragma unroll
+                        for (int x = 0; x < kWarps; ++x) sum += part[turn][x][lane];
+                    turn ^= 1;
+                }
+                if ((!kWhole || warp == 0) && lane < J && lane < left) grad_weights[entry + lane] = round_to<W>(sum);
+            }
+            ask((i + D - 1) % D);
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 // ------------------------------------------------------------------ host side
 template <typename Kernel, typename... Args>
 static int launch(Kernel kernel, dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream, Args... args) {
@@ -789,6 +930,24 @@ static int move(const char* what, bool back, int dtype, int weight_dtype, int to
     return call(move_rows<float, float>);
 }
 
+template <typename T, typename W, bool kWhole>
+static int launch_grad_ring(const void* grad, const void* y, const int* slots, const void* weights, void* grad_y,
+                            void* grad_weights, int tokens, int choices, int rows, int width, int dev,
+                            cudaStream_t stream) {
+    static bool attr_set[64] = {};
+    if (dev >= 64 || !attr_set[dev]) {
+        TRB_CUDA(cudaFuncSetAttribute(expert_combine_grad_ring_kernel<T, W, kWhole>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGradSmem));
+        if (dev < 64) attr_set[dev] = true;
+    }
+    const int64_t side = kWhole ? 1 : kRowThreads / 32, blocks = (tokens + side - 1) / side;
+    const int64_t places = (int64_t)device_sm_count(dev) * kGradCtas;
+    return launch(expert_combine_grad_ring_kernel<T, W, kWhole>, dim3((unsigned)std::min(blocks, places)), kRowThreads, 0,
+                  kGradSmem, stream, static_cast<const T*>(grad), static_cast<const T*>(y), slots,
+                  static_cast<const W*>(weights), static_cast<T*>(grad_y), static_cast<W*>(grad_weights), (int64_t)tokens,
+                  choices, rows, width);
+}
+
 template <typename T, typename W>
 static int launch_grad(const void* grad, const void* y, const int* slots, const void* weights, void* grad_y,
                        void* grad_weights, int tokens, int choices, int rows, int width, int dev, cudaStream_t stream) {
@@ -799,7 +958,21 @@ static int launch_grad(const void* grad, const void* y, const int* slots, const 
                       slots, static_cast<const W*>(weights), static_cast<T*>(grad_y), static_cast<W*>(grad_weights),
                       (int64_t)tokens, choices, rows, width, s.log2_lanes);
     };
-    switch (access_bytes(S, width, bits(grad) | bits(y) | bits(grad_y))) {
+    const int access = access_bytes(S, width, bits(grad) | bits(y) | bits(grad_y)), packs = width / (16 / S);
+    // The ring has a CTA a token where its row keeps all threads busy (16384 tokens of 4 rows of 1024 and 2048 bf16: a CTA 67
+    // and 95 us, a warp 57 and 110, without the ring 64 and 124), and is for tokens enough for all CTAs, or warps, of it to
+    // be worth their start (a CTA: 64 and 500 tokens of 4 rows of 4096 bf16 4.0 and 8.6 us, without the ring 3.6 and 10.2;
+    // a warp: 500 and 16384 of 4 rows of 512 4.0 and 28.7, without 3.2 and 34.4).
+    if (access == 16) {
+        const int64_t sms = device_sm_count(dev);
+        if (packs >= kRowThreads && tokens >= sms)
+            return launch_grad_ring<T, W, true>(grad, y, slots, weights, grad_y, grad_weights, tokens, choices, rows, width,
+                                                dev, stream);
+        if (packs < kRowThreads && tokens >= sms * kGradCtas * (kRowThreads / 32))
+            return launch_grad_ring<T, W, false>(grad, y, slots, weights, grad_y, grad_weights, tokens, choices, rows, width,
+                                                 dev, stream);
+    }
+    switch (access) {
         case 16: return run(expert_combine_grad_kernel<T, W, 16 / S, 1>, 16 / S, 1);
         case 8: return run(expert_combine_grad_kernel<T, W, 8 / S, 2>, 8 / S, 2);
         case 4: return run(expert_combine_grad_kernel<T, W, 4 / S, 2>, 4 / S, 2);

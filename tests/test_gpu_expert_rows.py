@@ -174,6 +174,32 @@ def test_combine_grad(dtype, weights, tokens, choices, width):
     assert grad_y[int(here.sum()):].isnan().all() and not grad_w[~here].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bfloat16", "float32"])
+@pytest.mark.parametrize("tokens, choices, packs", [(4737, 1, 1), (4800, 3, 31), (9600, 5, 33), (5003, 9, 255), (4736, 2, 64),
+                                                   (148, 4, 256), (700, 9, 257), (593, 1, 511), (1300, 2, 512),
+                                                   (1185, 7, 300)])
+def test_combine_grad_of_many_tokens(dtype, tokens, choices, packs):
+    """A warp's and a CTA's tokens: rows of 16-byte packs around a warp's, a CTA's and a ring's, tokens in one go and more."""
+    width = packs * (16 // dtype.itemsize)
+    _, slots, here = _plan(tokens, choices)
+    rows = int(here.sum()) + 2
+    y, grad = _randn((rows, width), dtype, 1), _randn((tokens, width), dtype, 2)
+    y[-2:] = NAN
+    w = _randn((tokens, choices), torch.float32, 3)
+    w[~here] = NAN
+    grad_y, grad_w, in_place, again = torch.full_like(y, NAN), torch.full_like(w, NAN), y.clone(), torch.empty_like(w)
+    expert_combine_grad(grad, y, slots, w, grad_y, grad_w)
+    for lo in range(0, tokens, 1000):
+        part = slice(lo, lo + 1000)
+        ref_y, ref_w, magnitude = _grad_reference(grad[part], y, slots[part], here[part], w[part])
+        at = here[part]
+        _close(grad_y[slots[part][at].long()], ref_y[at], ref_y[at].abs(), 1)
+        _close(grad_w[part], ref_w, magnitude, width)
+    assert grad_y[-2:].isnan().all() and not grad_w[~here].any()
+    expert_combine_grad(grad, in_place, slots, w, in_place, again)
+    assert torch.equal(in_place[:-2], grad_y[:-2]) and torch.equal(again, grad_w)
+
+
 def test_gradients_agree_with_differences():
     """<combine_grad, direction> against the difference of two 64-bit combines along it; combine is linear in each."""
     tokens, choices, width = 7, 3, 40
