@@ -10,8 +10,8 @@
 //
 // What bounds all of it is the rows' bytes (the sort: launch and latency).  Measured in CUDA graphs of calls on several
 // sets of inputs, floors at 6551 GB/s, a measured copy: dispatch of 4109 tokens to 8 rows of 2048 bf16 25.2 us (floor
-// 23.1), of 16384 to 2 of 4096 62 to 65 (61.5); combine of the same 26.8 (23.2) and 69.5 (61.5); gradient, 16384 tokens of
-// 4 rows of 4096 bf16, 204 us (184); the sort of 2, 32872 and 131072 choices 2.4, 6.8 and 14.2 us.
+// 23.1), of 16384 to 2 of 4096 62 to 65 (61.5); combine of the same 26.8 (23.2) and 69.5 (61.5); gradient of the same 48
+// (43.7) and 116 (102); the sort of 2, 32872 and 131072 choices 2.4, 6.8 and 14.2 us.
 //
 // No counterpart in the reference.
 #include <cuda_bf16.h>
@@ -550,7 +550,8 @@ __global__ void __launch_bounds__(kRowThreads)
     expert_combine_grad_kernel(const T* grad, const T* y, const int* slots, const W* weights, T* grad_y, W* grad_weights,
                                int64_t tokens, int choices, int rows, int width, int log2_lanes) {
     __shared__ float part[kRowThreads / 32][kAtOnce];
-    grid_launch_dependents();
+    // The next kernel does not start before the end: a combine, which divides the SM's memory otherwise, gained nothing from
+    // an early start (both, 64 tokens of 4 rows of 4096 and 500 of 512 bf16: 7.4 and 6.9 us with it, 7.1 and 6.4 without).
     grid_dependency_wait();
     const int lanes = 1 << log2_lanes;  // 32 or more
     const int side = kRowThreads >> log2_lanes, own = threadIdx.x >> log2_lanes, l = threadIdx.x & (lanes - 1);
@@ -974,8 +975,11 @@ static int launch_grad(const void* grad, const void* y, const int* slots, const 
     }
     switch (access) {
         case 16: return run(expert_combine_grad_kernel<T, W, 16 / S, 1>, 16 / S, 1);
-        case 8: return run(expert_combine_grad_kernel<T, W, 8 / S, 2>, 8 / S, 2);
-        case 4: return run(expert_combine_grad_kernel<T, W, 4 / S, 2>, 4 / S, 2);
+        // Accesses of each row on their way: two of single values, one of more.  4109 tokens of 8 rows of 2047, 2046 and 2044
+        // bf16 with one, two and four: 104, 91 and 87 us; 79, 97 and 255; 72, 75 and 146.  509 of 8 of 1001 float32: 11.6,
+        // 10.1 and 11.9.
+        case 8: return run(expert_combine_grad_kernel<T, W, 8 / S, 1>, 8 / S, 1);
+        case 4: return run(expert_combine_grad_kernel<T, W, 4 / S, S == 4 ? 2 : 1>, 4 / S, S == 4 ? 2 : 1);
         default: return run(expert_combine_grad_kernel<T, W, 1, 2>, 1, 2);
     }
 }
