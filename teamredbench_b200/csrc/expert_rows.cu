@@ -10,7 +10,7 @@
 //
 // What bounds all of it is the rows' bytes (the sort: launch and latency).  Measured in CUDA graphs of calls on several
 // sets of inputs, floors at 6551 GB/s, a measured copy: dispatch of 4109 tokens to 8 rows of 2048 bf16 25.2 us (floor
-// 23.1), of 16384 to 2 of 4096 62 to 65 (61.5); combine of the same 26.8 (23.2) and 69.5 (61.5); gradient of the same 48
+// 23.1), of 16384 to 2 of 4096 62 to 65 (61.5); combine of the same 25.2 (23.2) and 64 to 66 (61.5); gradient of the same 48
 // (43.7) and 116 (102); the sort of 2, 32872 and 131072 choices 2.4, 6.8 and 14.2 us.
 //
 // No counterpart in the reference.
@@ -201,9 +201,9 @@ __device__ __forceinline__ void store(T* p, const Pack<T, V>& v) {
     *reinterpret_cast<Pack<T, V>*>(p) = v;
 }
 
-// The row of a slot, or -1 where there is none.  A slot behind the last row is an error of the caller's.
-__device__ __forceinline__ int row_of(const int* slots, int64_t i, int rows) {
-    const int s = slots[i];
+// The row of a slot, or -1 where there is none.  A slot behind the last row is an error of the caller's.  This waits for
+// the slot, so slots are read well before they are looked at.
+__device__ __forceinline__ int row_of(int s, int rows) {
     if (s >= rows) {
         atomicCAS(&g_rows_error, 0, kErrSlots);
         return -1;
@@ -234,6 +234,9 @@ template <typename T, typename W, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
     expert_dispatch_kernel(const T* x, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
                            int width, int log2_lanes) {
+    // Slots read at once: single 16-bit values 40.5 us (4109 tokens of 8 rows of 2047) with four, 42.9 with one; pairs of them
+    // (2046) 31.5 and 30.8, 16 bytes (16384 of 2 of 4096) 68 and 65.
+    constexpr int kSlotsAtOnce = V * sizeof(T) == 2 ? 4 : 1;
     grid_launch_dependents();
     grid_dependency_wait();
     const RowWalk w = row_walk(log2_lanes);
@@ -244,19 +247,28 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (p + u * w.pack_step < packs) v[u] = load<T, V>(x + t * width + (int64_t)(p + u * w.pack_step) * V);
-            for (int j = 0; j < choices; ++j) {
-                const int row = row_of(slots, t * choices + j, rows);
-                if (row < 0) continue;
-                const float f = weights != nullptr ? to_f32(weights[t * choices + j]) : 1.0f;
-                T* const to = out + (int64_t)row * width + (int64_t)p * V;
+            for (int j0 = 0; j0 < choices; j0 += kSlotsAtOnce) {
+                int slot[kSlotsAtOnce];
+                W weight[kSlotsAtOnce];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (p + u * w.pack_step >= packs) break;
-                    Pack<T, V> o = v[u];
-                    if (weights != nullptr)
+                for (int j = 0; j < kSlotsAtOnce; ++j) {
+                    slot[j] = j0 + j < choices ? slots[t * choices + j0 + j] : -1;
+                    if (weights != nullptr && j0 + j < choices) weight[j] = weights[t * choices + j0 + j];
+                }
 #pragma unroll
-                        for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(f * to_f32(v[u].v[i]));
-                    store<T, V>(to + (int64_t)u * w.pack_step * V, o);
+                for (int j = 0; j < kSlotsAtOnce; ++j) {
+                    const int row = row_of(slot[j], rows);
+                    if (row < 0) continue;
+                    T* const to = out + (int64_t)row * width + (int64_t)p * V;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (p + u * w.pack_step >= packs) break;
+                        Pack<T, V> o = v[u];
+                        if (weights != nullptr)
+#pragma unroll
+                            for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(to_f32(weight[j]) * to_f32(v[u].v[i]));
+                        store<T, V>(to + (int64_t)u * w.pack_step * V, o);
+                    }
                 }
             }
         }
@@ -269,16 +281,17 @@ constexpr int kAtOnce = 4;
 // Combine: sums in fp32, in the order of the choices, rounded once.  Loads into registers keep too few bytes in flight, for
 // a slot has to be read before its row can be (16384 tokens of 2 rows of 4096 bf16: 119 us).  Here a thread copies its 16
 // bytes of J rows to shared memory (cp.async) kDeep - 1 steps before it adds them up; nobody else reads them, so there is no
-// barrier.  A lane reads the slot and weight of one of a step's choices a step before the rows are asked for, and shuffles
-// pass them round.  Four CTAs an SM and 96 bytes a thread on their way: 70 us; three CTAs and 112 bytes 78, five and 64
-// 83.  Rows through a ring of bulk copies of 4 KB with a producer warp took 73 us and two waits a row.
+// barrier.  A lane reads the slot and weight of one of a step's choices a step before the rows are asked for and looks at
+// them then (70 us if it does at once, which waits for them), and shuffles pass them round.  Four CTAs an SM and 96 bytes a
+// thread on their way: 64 to 66 us.  Before the late look three CTAs and 112 bytes took 78, five and 64 83, and rows through a
+// ring of bulk copies of 4 KB with a producer warp 73 and two waits a row.
 //
 // Rows that begin anywhere (kAny) go the same way in the aligned pieces around them: 4109 tokens of 8 rows of 2047 and 2046
-// bf16 35 and 34 us, where accesses of 2 and 4 bytes straight to registers took 55 and 82, and of 2046 float32, 4 rows, 32.
-constexpr int kRingCtas = 4;  // of an SM
+// bf16 31 and 30 us, where accesses of 2 and 4 bytes straight to registers took 55 and 82, and of 2046 float32, 4 rows, 32.
 template <int J>
 struct Ring {
-    static constexpr int kDeep = J == 2 ? 6 : 3;
+    static constexpr int kDeep = J == 2 ? 6 : J == 4 ? 3 : 2;
+    static constexpr int kCtas = J == 8 ? 3 : 4;  // of an SM
     static constexpr size_t smem(int pieces) { return (size_t)kDeep * J * (kRowThreads / 32) * pieces * 16; }
 };
 
@@ -367,7 +380,7 @@ constexpr int kPieces = 33;
 // kAny: the rows and the tokens' rows begin at any value's place.  The warp's 512 bytes of a row are then copied as the 33
 // pieces around them, and its lanes read words out of them, as the words of the token's row want them.
 template <typename T, typename W, int J, bool kAny>
-__global__ void __launch_bounds__(kRowThreads, kRingCtas)
+__global__ void __launch_bounds__(kRowThreads, Ring<J>::kCtas)
     expert_combine_ring_kernel(const T* y, const int* slots, const W* weights, T* out, int64_t tokens, int choices,
                                int rows, int width, int log2_lanes) {
     constexpr int S = sizeof(T), V = 16 / S, kDeep = Ring<J>::kDeep, N = Word<T>::kValues;
@@ -396,25 +409,18 @@ __global__ void __launch_bounds__(kRowThreads, kRingCtas)
         if constexpr (S == 4 || !kAny) return e0;
         else return e0 - (int)(((uint32_t)(reinterpret_cast<uintptr_t>(out) >> 1) + (uint32_t)s.token * (uint32_t)width) & 1u);
     };
+    // Lane j has choice j of a step, as it was read.
     struct Choice {
-        int row;
-        float weight;
-        int shift;      // kAny: where the row's part stands in its pieces, and the first of them
-        const T* from;
-        bool inside;    // all pieces are the matrix's
+        int slot;
+        W weight;
     };
     const auto choice = [&](Step& s) {
-        Choice c = {-1, 1.0f, -1, nullptr, true};
+        Choice c;
+        c.slot = -1;
         const int j = s.chunk * J + lane;
         if (lane < J && j < choices && s.token < tokens) {
-            c.row = row_of(slots, s.token * choices + j, rows);
-            if (kAny && c.row >= 0) {
-                const int e0 = first_value(s);
-                c.shift = row_shift(y, c.row, width, e0);
-                c.from = y + (int64_t)c.row * width + (e0 - c.shift / S);
-                c.inside = c.from >= y && c.from + kPieces * V <= y_end;
-            }
-            if (weights != nullptr) c.weight = to_f32(weights[s.token * choices + j]);
+            c.slot = slots[s.token * choices + j];
+            if (weights != nullptr) c.weight = weights[s.token * choices + j];
         }
         next(s);
         return c;
@@ -423,34 +429,38 @@ __global__ void __launch_bounds__(kRowThreads, kRingCtas)
     float weight[kDeep];      // (lane j) the weight of choice j
     int shift[kDeep];         // kAny, in place of present: (lane j) that of choice j, negative without a row
     const auto ask = [&](int deep, Step& s, const Choice& c) {
-        if constexpr (!kAny) present[deep] = __ballot_sync(0xffffffffu, c.row >= 0);
-        weight[deep] = c.weight;
+        const int own_row = row_of(c.slot, rows);
+        if constexpr (!kAny) present[deep] = __ballot_sync(0xffffffffu, own_row >= 0);
+        weight[deep] = weights != nullptr && c.slot >= 0 ? to_f32(c.weight) : 1.0f;
         if constexpr (kAny) {
-            shift[deep] = c.shift;
+            // Where the row's part stands in its pieces, the first of them, and whether all are the matrix's.
             const int e0 = first_value(s);
-            if (__all_sync(0xffffffffu, c.inside)) {
+            const int own_shift = own_row < 0 ? -1 : row_shift(y, own_row, width, e0);
+            const T* const own_from = own_row < 0 ? nullptr : y + (int64_t)own_row * width + (e0 - own_shift / S);
+            shift[deep] = own_shift;
+            if (__all_sync(0xffffffffu, own_row < 0 || (own_from >= y && own_from + kPieces * V <= y_end))) {
                 // What stands before and behind the row in the pieces is read along and left out of the results.
                 const bool needed = e0 + V * (lane - 1) < width;
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(c.from), j);
+                    const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(own_from), j);
                     if (from != 0 && needed) copy_async(at(deep, j) + lane * 16, reinterpret_cast<const T*>(from) + lane * V);
                 }
-                if (c.shift >= 0 && e0 + V * 31 < width) copy_async(at(deep, lane) + 32 * 16, c.from + 32 * V);  // the last
+                if (own_shift >= 0 && e0 + V * 31 < width) copy_async(at(deep, lane) + 32 * 16, own_from + 32 * V);  // the last
             } else {
 #pragma unroll 1
                 for (int j = 0; j < J; ++j) {
-                    const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(c.from), j);
-                    const int first = e0 - __shfl_sync(0xffffffffu, c.shift, j) / S + V * lane;
+                    const uint64_t from = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(own_from), j);
+                    const int first = e0 - __shfl_sync(0xffffffffu, own_shift, j) / S + V * lane;
                     if (from != 0)
                         copy_piece(at(deep, j) + lane * 16, reinterpret_cast<const T*>(from) + lane * V, first, width, y);
                 }
-                if (c.shift >= 0) copy_piece(at(deep, lane) + 32 * 16, c.from + 32 * V, e0 - c.shift / S + 32 * V, width, y);
+                if (own_shift >= 0) copy_piece(at(deep, lane) + 32 * 16, own_from + 32 * V, e0 - own_shift / S + 32 * V, width, y);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                const int row = __shfl_sync(0xffffffffu, c.row, j);
+                const int row = __shfl_sync(0xffffffffu, own_row, j);
                 if (row >= 0 && s.pack0 + lane < packs)
                     copy_async(at(deep, j) + lane * 16, y + (int64_t)row * width + (int64_t)(s.pack0 + lane) * V);
             }
@@ -560,13 +570,20 @@ __global__ void __launch_bounds__(kRowThreads)
         const int64_t t = t0 + own;
         for (int j0 = 0; j0 < choices; j0 += kAtOnce) {
             int row[kAtOnce];
+            W weight[kAtOnce];
             float f[kAtOnce], dot[kAtOnce];
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j) {
+                row[j] = -1;
+                if (t >= tokens || j0 + j >= choices) continue;
+                row[j] = slots[t * choices + j0 + j];
+                weight[j] = weights[t * choices + j0 + j];
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
                 dot[j] = 0.0f;
-                f[j] = 0.0f;
-                row[j] = t < tokens && j0 + j < choices ? row_of(slots, t * choices + j0 + j, rows) : -1;
-                if (row[j] >= 0) f[j] = to_f32(weights[t * choices + j0 + j]);
+                row[j] = row_of(row[j], rows);
+                f[j] = row[j] >= 0 ? to_f32(weight[j]) : 0.0f;
             }
             if (t < tokens) {
                 for (int p = l; p < packs; p += U * lanes) {
@@ -642,32 +659,46 @@ __global__ void __launch_bounds__(kRowThreads, kGradCtas)
         next_row(s);
         return true;
     };
-    // Lane j has a step's choice j, lane J the token's own row: where the warp's next packs of them are, if there are any.
+    // Lane j has choice j of a token's row, as it was read; lane J has the token's own row.
+    struct Choice {
+        int slot;
+        W weight;
+        int64_t token;
+    };
+    const auto choice = [&](const Step& s) {
+        Choice c;
+        c.slot = -1;
+        c.token = s.token;
+        const int j = s.chunk * J + lane;
+        if (lane < J && j < choices && s.token < tokens) {
+            c.slot = slots[s.token * choices + j];
+            c.weight = weights[s.token * choices + j];
+        }
+        return c;
+    };
+    // Where the warp's next packs of them are, if there are any.
     struct Part {
         int row;
         float weight;
         const T* from;
     };
-    const auto part_of = [&](const Step& s) {
-        Part c = {-1, 0.0f, nullptr};
-        const int j = s.chunk * J + lane;
-        if (s.token >= tokens) return c;
-        if (lane < J && j < choices) {
-            c.row = row_of(slots, s.token * choices + j, rows);
-            if (c.row >= 0) {
-                c.weight = to_f32(weights[s.token * choices + j]);
-                c.from = y + (int64_t)c.row * width + s.pack0 * V;
-            }
-        } else if (lane == J) {
-            c.from = grad + s.token * width + s.pack0 * V;
-        }
+    const auto part_of = [&](const Choice& choice) {
+        Part c;
+        c.row = row_of(choice.slot, rows);
+        c.weight = c.row >= 0 ? to_f32(choice.weight) : 0.0f;
+        c.from = c.row >= 0 ? y + (int64_t)c.row * width + pack_first * V : nullptr;
+        if (lane == J && choice.token < tokens) c.from = grad + choice.token * width + pack_first * V;
         return c;
     };
     Step now = {token_first, pack_first, 0};
     Step asked = now, read = now;
-    Part known = part_of(read);  // of the rows that are asked for, and of those after them
+    // The rows that are asked for, and the choices after them: a warp's tokens change often, and it looks at their slots when
+    // it comes to them (16384 tokens of 4 rows of 256 and 1024 bf16 15.0 and 55.3 us, at once 15.7 and 56.2); a CTA's change
+    // seldom, and it looks at them at once (of 2048 and 4096 95 and 201 us, later 100 and 204).
+    Part known = part_of(choice(read)), then;
     next_row(read);
-    Part then = part_of(read);
+    Choice after = choice(read);
+    if constexpr (kWhole) then = part_of(after);
     int row[D];  // (lane j) of a step's choice j
     float weight[D];
     const auto ask = [&](int deep) {
@@ -682,9 +713,10 @@ __global__ void __launch_bounds__(kRowThreads, kGradCtas)
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (known.from != nullptr) known.from += pack_step * V;
         if (next(asked)) {
-            known = then;
+            known = kWhole ? then : part_of(after);
             next_row(read);
-            then = part_of(read);
+            after = choice(read);
+            if constexpr (kWhole) then = part_of(after);
         }
     };
 #pragma unroll
@@ -861,7 +893,7 @@ static int launch_ring(const void* y, const int* slots, const void* weights, voi
     }
     RowShape s = row_shape(tokens, kAny ? (width + Word<T>::kValues + V - 2) / V : width / V, 1, false, dev);
     // No more CTAs than the GPU holds, each for several tokens.
-    const unsigned places = (unsigned)(device_sm_count(dev) * kRingCtas);
+    const unsigned places = (unsigned)(device_sm_count(dev) * Ring<J>::kCtas);
     s.grid.x = std::max(1u, std::min(s.grid.x, places / s.grid.y));
     return launch(expert_combine_ring_kernel<T, W, J, kAny>, s.grid, kRowThreads, 0, smem, stream, static_cast<const T*>(y),
                   slots, static_cast<const W*>(weights), static_cast<T*>(out), (int64_t)tokens, choices, rows, width,
@@ -873,10 +905,17 @@ template <typename T, typename W, int V>
 static int launch_move(bool back, const void* src, const int* slots, const void* weights, void* dst, int tokens,
                        int choices, int rows, int width, int dev, cudaStream_t stream) {
     constexpr int B = V * sizeof(T);
-    if (back)
+    if (back) {
+        // Eight rows a step where each has shifting to do and there are as many: 4109 tokens of 8 rows of 2047 and 2048 bf16
+        // 30.6 and 26.1 us, four rows 34.2 and 25.2.
+        constexpr bool kAny = B != 16;
+        if constexpr (kAny)
+            if (choices > 4)
+                return launch_ring<T, W, 8, kAny>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
         return choices <= 2
-                   ? launch_ring<T, W, 2, B != 16>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
-                   : launch_ring<T, W, 4, B != 16>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+                   ? launch_ring<T, W, 2, kAny>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream)
+                   : launch_ring<T, W, 4, kAny>(src, slots, weights, dst, tokens, choices, rows, width, dev, stream);
+    }
     const auto run = [&](auto kernel, int at_once) {
         const RowShape s = row_shape(tokens, width / V, at_once, false, dev);
         return launch(kernel, s.grid, kRowThreads, 0, 0, stream, static_cast<const T*>(src), slots,
