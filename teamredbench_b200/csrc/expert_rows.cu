@@ -10,7 +10,7 @@
 //
 // What bounds all of it is the rows' bytes (the sort: launch and latency).  Measured in CUDA graphs of calls on several
 // sets of inputs, floors at 6551 GB/s, a measured copy: dispatch of 4109 tokens to 8 rows of 2048 bf16 25.2 us (floor
-// 23.1), of 16384 to 2 of 4096 62 to 65 (61.5); combine of the same 25.2 (23.2) and 64 to 66 (61.5); gradient of the same 48
+// 23.1), of 16384 to 2 of 4096 62 to 65 (61.5); combine of the same 25.2 (23.2) and 60.7 (61.5); gradient of the same 48
 // (43.7) and 116 (102); the sort of 2, 32872 and 131072 choices 2.4, 6.8 and 14.2 us.
 //
 // No counterpart in the reference.
@@ -282,15 +282,17 @@ constexpr int kAtOnce = 4;
 // a slot has to be read before its row can be (16384 tokens of 2 rows of 4096 bf16: 119 us).  Here a thread copies its 16
 // bytes of J rows to shared memory (cp.async) kDeep - 1 steps before it adds them up; nobody else reads them, so there is no
 // barrier.  A lane reads the slot and weight of one of a step's choices a step before the rows are asked for and looks at
-// them then (70 us if it does at once, which waits for them), and shuffles pass them round.  Four CTAs an SM and 96 bytes a
-// thread on their way: 64 to 66 us.  Before the late look three CTAs and 112 bytes took 78, five and 64 83, and rows through a
-// ring of bulk copies of 4 KB with a producer warp 73 and two waits a row.
+// them then, for a check behind the load would wait for it, and shuffles pass them round.  J = 2: 60.7 us three steps deep
+// with four CTAs an SM; two, four and six steps 74, 60.7 and 65.8, three CTAs 71, five 67 (four steps), six 78; 64 tokens
+// 1.9 us, with six steps 2.6.  J = 4: four steps and three CTAs are 3 to 4% faster where every choice has a row (16384
+// tokens of 4 rows of 4096 99 us) and 6% slower where half have none.  Rows through a ring of bulk copies of 4 KB with a
+// producer warp took two waits a row and, when slots were still checked at once, 73 us to this ring's 70.
 //
 // Rows that begin anywhere (kAny) go the same way in the aligned pieces around them: 4109 tokens of 8 rows of 2047 and 2046
 // bf16 31 and 30 us, where accesses of 2 and 4 bytes straight to registers took 55 and 82, and of 2046 float32, 4 rows, 32.
 template <int J>
 struct Ring {
-    static constexpr int kDeep = J == 2 ? 6 : J == 4 ? 3 : 2;
+    static constexpr int kDeep = J == 8 ? 2 : 3;
     static constexpr int kCtas = J == 8 ? 3 : 4;  // of an SM
     static constexpr size_t smem(int pieces) { return (size_t)kDeep * J * (kRowThreads / 32) * pieces * 16; }
 };
