@@ -319,7 +319,7 @@ __device__ __forceinline__ void copy_piece(uint32_t to, const T* from, int first
     constexpr int S = sizeof(T), V = 16 / S;
     if (first + V <= 0 || first >= width) return;
     if (first >= 0 || from >= rows) {
-        copy_async(to, from, min(16, (width - first) * S));
+        copy_async(to, from, min(V, width - first) * S);
     } else {
         for (int x = -first; x < V && first + x < width; ++x) {
             if constexpr (S == 2)

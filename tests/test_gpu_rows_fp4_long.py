@@ -129,6 +129,31 @@ def test_rows_as_wide_as_they_come():
     assert ((out[0].double() - total).abs() <= 2.0 ** -8 * total.abs() + 42 * 2.0 ** -23 * magnitude + 2.0 ** -133).all()
 
 
+@pytest.mark.parametrize("dtype, width", [(BF16, 2 ** 30 + 9), (torch.float32, 2 ** 29 + 9), (BF16, 2 ** 30 + 8)])
+def test_rows_behind_2_31_bytes_in_one(dtype, width):
+    """Rows of more than 2^31 bytes each, one of them the matrix's first and one its last."""
+    y = torch.zeros(2, width, device="cuda", dtype=dtype)
+    places = torch.tensor([0, 1, 255, 256, width // 2, width // 2 + 1, width - 9, width - 2, width - 1], device="cuda")
+    some = _randn((2, places.numel()), 3, dtype)
+    y[:, places] = some
+    slots, w = torch.tensor([[1, 0]], device="cuda", dtype=torch.int32), torch.tensor([[0.5, 2.0]], device="cuda")
+    out = torch.full((1, width), float("nan"), device="cuda", dtype=dtype)
+    expert_combine(y, slots, out, weights=w)
+    want = (0.5 * some[1].float() + 2.0 * some[0].float()).to(dtype)  # powers of two: one rounding of fp32 sums each way
+    assert torch.equal(out[0, places], want)
+    assert int(torch.count_nonzero(out)) == int(torch.count_nonzero(want))
+    grad_w = torch.empty_like(w)
+    del want
+    expert_combine_grad(out, y, slots, w, y, grad_w)  # over y: at most nine products that are not 0
+    ref = (out[0, places].double() * some.double()).sum(1).flip(0)
+    size = (out[0, places].double() * some.double()).abs().sum(1).flip(0)
+    assert ((grad_w[0].double() - ref).abs() <= 18 * 2.0 ** -24 * size).all()
+    assert torch.equal(y[1, places], (0.5 * out[0, places].float()).to(dtype)) and torch.equal(y[0, places], 2 * out[0, places])
+    expert_dispatch(out, slots, y)
+    assert torch.equal(y[0, places], out[0, places]) and torch.equal(y[1, places], out[0, places])
+    assert int(torch.count_nonzero(y)) == 2 * int(torch.count_nonzero(out))
+
+
 @pytest.mark.parametrize("k", [2 ** 20, 2 ** 20 + 32])
 def test_product_of_a_long_k(k):
     a, a_scales = operand((3, k), 1, 120, 124)
