@@ -7,12 +7,12 @@ library fallback: if the shared library is missing, every call raises
 from __future__ import annotations
 
 import ctypes
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 LIB_DIR = PKG / "lib"
 LIBRARY_PATH = LIB_DIR / "libtrb_b200.so"
-TORCH_BINDING_PATH = LIB_DIR / "trb_torch.so"
 HBM_EXECUTABLE = LIB_DIR / "trb_hbm"
 MFU_EXECUTABLE = LIB_DIR / "trb_mfu"
 
@@ -207,14 +207,30 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+def torch_binding_path() -> Path | None:
+    """Where the extension module trb_torch (csrc/trb_torch.cpp) is for the torch
+    and the Python that run, or None without torch.  Their names are part of the
+    file's: another torch's tensors may be laid out otherwise than those that the
+    module was compiled for, and it would be loaded all the same where its
+    symbols resolve."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    return LIB_DIR / f"trb_torch.{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so"
+
+
 def load_torch_binding():
-    """The extension module trb_torch (csrc/trb_torch.cpp), or None where it is not
-    built or was built for another torch."""
+    """The extension module trb_torch, or None where it is not built for the torch
+    and the Python that run."""
     import importlib.util
 
+    path = torch_binding_path()
+    if path is None or not path.exists():
+        return None
     try:
         load()  # its library
-        spec = importlib.util.spec_from_file_location("trb_torch", TORCH_BINDING_PATH)
+        spec = importlib.util.spec_from_file_location("trb_torch", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
     except (ImportError, NativeLibraryMissing):

@@ -4,8 +4,9 @@ Produces, in-tree under ``teamredbench_b200/lib/``:
     libtrb_b200.so  -- the C-ABI library (include/trb_b200.h)
     trb_hbm, trb_mfu -- launcher executables that keep the reference's
                         argv / last-line-JSON contract
-    trb_torch.so    -- where torch is installed: the short way from its tensors
-                       to the library (csrc/trb_torch.cpp)
+    trb_torch.*.so  -- where torch is installed: the short way from its tensors
+                       to the library (csrc/trb_torch.cpp), one file for each
+                       torch and Python that it was built with
 
 ``python -m teamredbench_b200.build`` or ``build()`` from Python.  nvcc
 cross-compiles without a GPU.  Objects are rebuilt only when a source or
@@ -38,7 +39,6 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompil
               f"-I{INCLUDE}", "-Xptxas", "-warn-spills"]
 
 LIBRARY = LIB_DIR / "libtrb_b200.so"
-TORCH_BINDING = LIB_DIR / "trb_torch.so"
 EXECUTABLES = {"trb_hbm": "TRB_BENCH_HBM", "trb_mfu": "TRB_BENCH_MFU"}
 
 
@@ -65,7 +65,7 @@ def _run(cmd: list[str], verbose: bool) -> str:
     return completed.stdout + completed.stderr
 
 
-def _torch_binding_command(cxx: str) -> list[str]:
+def _torch_binding_command(cxx: str, target: Path) -> list[str]:
     import torch
 
     root = Path(torch.__file__).resolve().parent
@@ -74,7 +74,7 @@ def _torch_binding_command(cxx: str) -> list[str]:
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
             f"-I{sysconfig.get_paths()['include']}", "-isystem", str(root / "include"), "-isystem",
             str(root / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda / "include"),
-            str(CSRC / "trb_torch.cpp"), "-o", str(TORCH_BINDING), f"-L{LIB_DIR}", "-ltrb_b200",
+            str(CSRC / "trb_torch.cpp"), "-o", str(target), f"-L{LIB_DIR}", "-ltrb_b200",
             f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
 
 
@@ -104,8 +104,12 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
         if _stale(target, [main_src, INCLUDE / "trb_b200.h", LIBRARY]):
             _run([cxx, "-O2", "-std=c++17", f"-D{define}", f"-I{INCLUDE}", str(main_src), "-o", str(target),
                   f"-L{LIB_DIR}", "-ltrb_b200", "-Wl,-rpath,$ORIGIN"], verbose)
-    if importlib.util.find_spec("torch") and _stale(TORCH_BINDING, [CSRC / "trb_torch.cpp", INCLUDE / "trb_b200.h"]):
-        _run(_torch_binding_command(cxx), verbose)
+    if importlib.util.find_spec("torch"):
+        from teamredbench_b200 import _native
+
+        target = _native.torch_binding_path()
+        if _stale(target, [CSRC / "trb_torch.cpp", INCLUDE / "trb_b200.h"]):
+            _run(_torch_binding_command(cxx, target), verbose)
     return LIBRARY
 
 

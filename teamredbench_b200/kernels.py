@@ -281,7 +281,7 @@ _SHORT: Any = None  # the compiled way from tensors to the library (csrc/trb_tor
 
 
 def _find_short() -> Any:
-    """The functions of lib/trb_torch.so, each for the front end of its name: it
+    """The functions of lib/trb_torch.*.so, each for the front end of its name: it
     makes the call and returns True where all arguments are as they have to be
     and the tensors' device is the current one, and does nothing and returns
     False otherwise.  The checks below are the same ones, with the words."""
