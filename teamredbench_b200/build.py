@@ -4,9 +4,11 @@ Produces, in-tree under ``teamredbench_b200/lib/``:
     libtrb_b200.so  -- the C-ABI library (include/trb_b200.h)
     trb_hbm, trb_mfu -- launcher executables that keep the reference's
                         argv / last-line-JSON contract
-    trb_torch.*.so  -- where torch is installed: the short way from its tensors
-                       to the library (csrc/trb_torch.cpp), one file for each
-                       torch and Python that it was built with
+    trb_torch.*.so  -- where torch is installed with CUDA: the short way from its
+                       tensors to the library (csrc/trb_torch.cpp), one file for
+                       each torch and Python that it was built with; without it
+                       everything works, too, only slower by a few microseconds
+                       a call
 
 ``python -m teamredbench_b200.build`` or ``build()`` from Python.  nvcc
 cross-compiles without a GPU.  Objects are rebuilt only when a source or
@@ -20,6 +22,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -78,6 +81,32 @@ def _torch_binding_command(cxx: str, target: Path) -> list[str]:
             f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
 
 
+def _build_torch_binding(cxx: str, verbose: bool) -> None:
+    """The binding is a short cut: where there is none, the front ends reach the
+    library through ctypes.  So what keeps it from being built (a torch without
+    CUDA, which has no tensors for it; a Python without headers) is at most a
+    warning, and no older one is left that was made for another header."""
+    if not importlib.util.find_spec("torch"):
+        return
+    target = None
+    try:
+        import torch
+
+        from teamredbench_b200 import _native
+
+        if torch.version.cuda is None:
+            return
+        target = _native.torch_binding_path()
+        if _stale(target, [CSRC / "trb_torch.cpp", INCLUDE / "trb_b200.h"]):
+            target.unlink(missing_ok=True)
+            _run(_torch_binding_command(cxx, target), verbose)
+    except Exception as error:  # noqa: BLE001 - a broken torch fails in many ways
+        if target is not None:
+            target.unlink(missing_ok=True)
+        warnings.warn(f"the binding to torch's tensors was not built, calls will take a few microseconds longer: {error}",
+                      RuntimeWarning, stacklevel=3)
+
+
 def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
     nvcc = find_nvcc()
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
@@ -104,12 +133,7 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
         if _stale(target, [main_src, INCLUDE / "trb_b200.h", LIBRARY]):
             _run([cxx, "-O2", "-std=c++17", f"-D{define}", f"-I{INCLUDE}", str(main_src), "-o", str(target),
                   f"-L{LIB_DIR}", "-ltrb_b200", "-Wl,-rpath,$ORIGIN"], verbose)
-    if importlib.util.find_spec("torch"):
-        from teamredbench_b200 import _native
-
-        target = _native.torch_binding_path()
-        if _stale(target, [CSRC / "trb_torch.cpp", INCLUDE / "trb_b200.h"]):
-            _run(_torch_binding_command(cxx, target), verbose)
+    _build_torch_binding(cxx, verbose)
     return LIBRARY
 
 

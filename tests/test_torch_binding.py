@@ -46,3 +46,45 @@ def test_another_torch_gets_a_binding_of_its_own(monkeypatch, nothing_else_stale
     (command,) = nothing_else_stale
     target = command[command.index("-o") + 1]
     assert target == str(_native.torch_binding_path()) and "1.0.0+other" in target
+
+
+@pytest.fixture
+def elsewhere(monkeypatch, tmp_path, nothing_else_stale):
+    """The binding's file is another one, which an older source has left."""
+    monkeypatch.setattr(_native, "LIB_DIR", tmp_path)
+    left = _native.torch_binding_path()
+    left.touch()
+    monkeypatch.setattr(build, "_stale", lambda target, deps: "torch" in target.name)
+    return left
+
+
+@pytest.mark.parametrize("error", [RuntimeError("Python.h: No such file"), ImportError("libc10"), OSError("libcudart")])
+@pytest.mark.parametrize("where", ["_run", "_torch_binding_command"])
+def test_a_binding_that_cannot_be_built_is_a_warning(monkeypatch, elsewhere, where, error):
+    """The library and the executables are there, and the front ends work without the binding."""
+    def fail(*_):
+        raise error
+
+    monkeypatch.setattr(build, where, fail)
+    with pytest.warns(RuntimeWarning, match=str(error)):
+        assert build.build() == build.LIBRARY
+    assert not elsewhere.exists()  # made for another header, maybe
+    monkeypatch.setattr(_native, "load", lambda: None)
+    assert _native.load_torch_binding() is None
+
+
+def test_a_compiler_that_fails_is_a_warning(monkeypatch, elsewhere):
+    monkeypatch.undo()
+    monkeypatch.setenv("CXX", "/bin/false")
+    monkeypatch.setattr(_native, "LIB_DIR", elsewhere.parent)
+    monkeypatch.setattr(build, "find_nvcc", lambda: "/usr/local/cuda/bin/nvcc")
+    monkeypatch.setattr(build, "_stale", lambda target, deps: "torch" in target.name)
+    with pytest.warns(RuntimeWarning, match="command failed"):
+        build.build()
+    assert not elsewhere.exists()
+
+
+def test_a_torch_without_cuda_needs_no_binding(monkeypatch, elsewhere, nothing_else_stale, recwarn):
+    monkeypatch.setattr(torch.version, "cuda", None)
+    assert build.build() == build.LIBRARY
+    assert nothing_else_stale == [] and not recwarn.list
