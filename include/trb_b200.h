@@ -332,7 +332,10 @@ int trb_expert_sort_launch(int id_bytes, int tokens, int choices, int experts, c
  * device error word to 8.  Rows of out that no slot names are left as they are;
  * one that two slots name gets values of both.  Products are made in fp32 and rounded
  * once.  Any width; rows move 16 bytes at a time where width and pointers are
- * multiples of 16 bytes.  rows, width and tokens * choices at most 2130706432. */
+ * multiples of 16 bytes.  rows, width and tokens * choices at most 2130706432.
+ * Gradients, from that of out: of x by trb_expert_combine_launch with the same
+ * weights; of the weights by trb_expert_combine_grad_launch with x in place of
+ * grad and the gradient of out in place of y. */
 int trb_expert_dispatch_launch(int dtype, int weight_dtype, int tokens, int choices, int rows, int width, const void* x,
                                const int32_t* slots, const void* weights, void* out, void* stream);
 

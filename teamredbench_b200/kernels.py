@@ -367,7 +367,10 @@ def expert_dispatch(x: Any, slots: Any, out: Any, *, weights: Any | None = None,
     one behind the last row is skipped and sets the device error word to 8
     (``_native.device_error``), which the host does not wait for here.  The
     gradient of x is expert_combine on the gradient of out, with the same
-    weights."""
+    weights.  That of the weights is grad_weights of expert_combine_grad(x,
+    grad_out, slots, weights, grad_y, grad_weights), where grad_y, which gets
+    dispatch's own result again, may be grad_out itself once x's gradient is
+    made."""
     short = _SHORT if _SHORT is not None else _find_short()
     if stream is None and short and short.expert_dispatch(x, slots, out, weights):
         return out
