@@ -378,8 +378,9 @@ int trb_quantize_fp4_launch(int dtype, int rows, int k, const void* x, int choic
                             void* q, void* scales, void* stream);
 
 /* out (rows x k, bfloat16, float16 or float32) = the values of q and scales;
- * exact in bfloat16 and float32, rounded in float16 where they are too small
- * for it (or infinite, where too large). */
+ * exact in bfloat16 and float32, but infinite from 2^128 on, which the scale
+ * bytes 253 and 254 can give (trb_quantize_fp4_launch writes neither); in
+ * float16 rounded where they are too small for it, infinite where too large. */
 int trb_dequantize_fp4_launch(int dtype, int rows, int k, const void* q, const void* scales, void* out, void* stream);
 
 /* out[r, n] = the sum over k of a[r, k] * b[e, n, k], both 4-bit floating point

@@ -486,7 +486,10 @@ def quantize_fp4(x: Any, q: Any, scales: Any, *, slots: Any | None = None, strea
 
 def dequantize_fp4(q: Any, scales: Any, out: Any, *, stream: Any | None = None) -> Any:
     """out (rows x k, bf16, f16 or float32) = the values of quantize_fp4's q and
-    scales: exact in bf16 and float32."""
+    scales: exact in bf16 and float32, except that values of 2^128 or more, which
+    the scale bytes 253 and 254 can give and quantize_fp4 never writes, are
+    infinite there.  f16 rounds what is too small for it, and what is too large
+    is infinite."""
     short = _SHORT if _SHORT is not None else _find_short()
     if stream is None and short and short.dequantize_fp4(q, scales, out):
         return out
