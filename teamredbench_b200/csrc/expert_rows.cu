@@ -234,9 +234,10 @@ template <typename T, typename W, int V, int U>
 __global__ void __launch_bounds__(kRowThreads)
     expert_dispatch_kernel(const T* x, const int* slots, const W* weights, T* out, int64_t tokens, int choices, int rows,
                            int width, int log2_lanes) {
-    // Slots read at once: single 16-bit values 40.5 us (4109 tokens of 8 rows of 2047) with four, 42.9 with one; pairs of them
-    // (2046) 31.5 and 30.8, 16 bytes (16384 of 2 of 4096) 68 and 65.
-    constexpr int kSlotsAtOnce = V * sizeof(T) == 2 ? 4 : 1;
+    // A slot is looked at as it is read, and then its weight is read.  Rows that begin anywhere lost by reading them ahead: with
+    // four slots of single 16-bit values at once one row of 4095 for each of 16384 tokens took 108 us, two of them 126 (here
+    // 75 and 103), 8 rows of 2047 for 4109 tokens 40 (42.5); with the weight ahead of the look 8 rows of 2046 36 (31), but 30
+    // where weights are given (33).  Aligned rows do not mind.
     grid_launch_dependents();
     grid_dependency_wait();
     const RowWalk w = row_walk(log2_lanes);
@@ -247,28 +248,19 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (p + u * w.pack_step < packs) v[u] = load<T, V>(x + t * width + (int64_t)(p + u * w.pack_step) * V);
-            for (int j0 = 0; j0 < choices; j0 += kSlotsAtOnce) {
-                int slot[kSlotsAtOnce];
-                W weight[kSlotsAtOnce];
+            for (int j = 0; j < choices; ++j) {
+                const int row = row_of(slots[t * choices + j], rows);
+                if (row < 0) continue;
+                const float f = weights != nullptr ? to_f32(weights[t * choices + j]) : 1.0f;
+                T* const to = out + (int64_t)row * width + (int64_t)p * V;
 #pragma unroll
-                for (int j = 0; j < kSlotsAtOnce; ++j) {
-                    slot[j] = j0 + j < choices ? slots[t * choices + j0 + j] : -1;
-                    if (weights != nullptr && j0 + j < choices) weight[j] = weights[t * choices + j0 + j];
-                }
+                for (int u = 0; u < U; ++u) {
+                    if (p + u * w.pack_step >= packs) break;
+                    Pack<T, V> o = v[u];
+                    if (weights != nullptr)
 #pragma unroll
-                for (int j = 0; j < kSlotsAtOnce; ++j) {
-                    const int row = row_of(slot[j], rows);
-                    if (row < 0) continue;
-                    T* const to = out + (int64_t)row * width + (int64_t)p * V;
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        if (p + u * w.pack_step >= packs) break;
-                        Pack<T, V> o = v[u];
-                        if (weights != nullptr)
-#pragma unroll
-                            for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(to_f32(weight[j]) * to_f32(v[u].v[i]));
-                        store<T, V>(to + (int64_t)u * w.pack_step * V, o);
-                    }
+                        for (int i = 0; i < V; ++i) o.v[i] = round_to<T>(f * to_f32(v[u].v[i]));
+                    store<T, V>(to + (int64_t)u * w.pack_step * V, o);
                 }
             }
         }
