@@ -856,7 +856,7 @@ static int check(const char* what, int dtype, int weight_dtype, int tokens, int 
 
 static uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-// Pointers of values are aligned to a value, and those of rows that move 16 bytes at a time to 16 bytes.
+// Pointers are aligned to their elements.  Wider accesses are chosen where they are aligned to more (access_bytes).
 static int check_align(const char* what, int dtype, int weight_dtype, uintptr_t values, const void* weights,
                        const void* grad_weights, const void* slots) {
     const size_t size = dtype_size(dtype), weight_size = dtype_size(weight_dtype);
@@ -996,7 +996,9 @@ static int launch_grad(const void* grad, const void* y, const int* slots, const 
     // The ring has a CTA a token where its row keeps all threads busy (16384 tokens of 4 rows of 1024 and 2048 bf16: a CTA 67
     // and 95 us, a warp 57 and 110, without the ring 64 and 124), and is for tokens enough for all CTAs, or warps, of it to
     // be worth their start (a CTA: 64 and 500 tokens of 4 rows of 4096 bf16 4.0 and 8.6 us, without the ring 3.6 and 10.2;
-    // a warp: 500 and 16384 of 4 rows of 512 4.0 and 28.7, without 3.2 and 34.4).
+    // a warp: 500 and 16384 of 4 rows of 512 4.0 and 28.7, without 3.2 and 34.4).  Rows a little wider than a CTA were
+    // not measured with a warp a token; with a CTA 16384 tokens of 4 rows of 2056 and 2400 bf16 take 113 and 128 us (floors
+    // 93 and 108).
     if (access == 16) {
         const int64_t sms = device_sm_count(dev);
         if (packs >= kRowThreads && tokens >= sms)

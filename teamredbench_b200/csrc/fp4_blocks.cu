@@ -78,8 +78,8 @@ __device__ __forceinline__ void halves_of(uint32_t codes, uint32_t (&h)[4]) {
         : "r"(codes));
 }
 
-// Threads of a CTA: 1 << log2_lanes of them, 32 or more, for one row, several rows side by side; blockIdx.y shares a
-// row among CTAs where there are few.  
+// Threads of a CTA: 1 << log2_lanes of them, 32 or more, for one row, several rows side by side; blockIdx.y shares a row
+// among CTAs where there are few.
 struct Walk {
     int first, step;  // octets
     int64_t row, row_step;
@@ -175,8 +175,7 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// 32-bit values: eight a thread, four threads a block.  Threads of a CTA: 1 << log2_lanes of them, 32 or more, for one row,
-// several rows side by side; blockIdx.y shares a row among CTAs where there are few.
+// 32-bit values: eight a thread, four threads a block.
 __global__ void __launch_bounds__(kThreads)
     quantize_fp4_f32_kernel(const float* x, const int* slots, uint8_t* q, uint8_t* scales, int64_t rows, int choices,
                             int out_rows, int k, int log2_lanes) {

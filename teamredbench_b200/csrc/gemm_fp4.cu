@@ -11,7 +11,9 @@
 // 16-bit rates would be 164 and 195 us); the tensor pipe is busy in 83% of the cycles, 6% go to the change from tile to
 // tile, the rest to instructions of 140 cycles instead of 128.  16436 rows of 16 experts, 4096 x 2048: 76 us (89
 // sustained), a sixth of it the change of tiles of only four stages.  16 rows, 4096 x 4096: 5.5 us, launch and one round
-// of loads; 256 rows of 32 experts, 2047 x 4096: 31.5 us, 4.6 TB/s, 30.3 with the products left out.
+// of loads; 256 rows of 32 experts, 2047 x 4096: 31.5 us, 4.6 TB/s, 30.3 with the products left out: the order and depth of
+// the loads.  Where n is no multiple of 8 the pair kernel's results leave two bytes at a time: the case of 16 experts above
+// with n = 4095 takes 329 us.
 //
 // No counterpart in the reference.
 #include <cuda_bf16.h>
